@@ -2,9 +2,10 @@
 
 Four operators in the order in which a serving loop runs them: block tables and slot maps from the
 requests' lengths, the projection's rows normalised, rotated and written into the pages, attention of
-one new token per request over its pages, and a token drawn from the logits.  Head layouts, vocabulary
-and context lengths are the PLaMo-3 0.8B model's (16 query heads on one KV head of 128, 107,520 tokens,
-a 2,048-key window), beside generic ones (grouped heads, a head of 64 or 256, FP16, odd vocabularies).
+one new token per request over its pages, and a token drawn from the logits, counted from the
+likeliest on.  Head layouts, vocabulary and context lengths are the PLaMo-3 0.8B model's (16 query heads
+on one KV head of 128, 107,520 tokens, a 2,048-key window), beside generic ones (grouped heads, a head
+of 64 or 256, FP16, odd vocabularies).
 """
 import math
 import os
@@ -296,13 +297,13 @@ def _plain_sample(s):
     p = s["top_p"].double()[:, None]
     keep = (rank == 0) | (sums - weight < p * sums[:, -1:]) | (p >= 1)
     keep &= weight >= s["min_p"].double()[:, None].clamp(max=1)
-    weight = torch.zeros_like(weight).scatter_(1, token, torch.where(keep, weight, 0.0))
+    weight = torch.where(keep, weight, 0.0)
     sums = weight.cumsum(1)
     total = sums[:, -1:]
-    last = torch.where(weight > 0, rank, -1).amax(1)
-    chosen = torch.minimum((sums <= s["uniform"].double()[:, None].clamp(0, 1) * total).sum(1), last)
-    s["token"].copy_(chosen)
-    s["prob"].copy_((weight.gather(1, chosen.clamp(min=0)[:, None]) / total)[:, 0])
+    last = torch.where(weight > 0, rank, 0).amax(1)
+    at = torch.minimum((sums <= s["uniform"].double()[:, None].clamp(0, 1) * total).sum(1), last)[:, None]
+    s["token"].copy_(token.gather(1, at)[:, 0])
+    s["prob"].copy_((weight.gather(1, at) / total)[:, 0])
     return {"token": s["token"], "prob": s["prob"]}
 
 
@@ -485,7 +486,7 @@ def _exact_attend(s):
 
 
 def _exact_sample(s):
-    """Row by row on the host, the kept tokens listed one after the other."""
+    """Row by row on the host, the kept tokens listed from the likeliest on."""
     logits = s["logits"].double().cpu().numpy()
     host = lambda name: s[name].double().cpu().numpy()  # noqa: E731
     temperature, top_k, top_p, min_p, uniform = (host(n) for n in ("temperature", "top_k", "top_p", "min_p", "uniform"))
@@ -505,10 +506,8 @@ def _exact_sample(s):
             order = order[: max(1, int(cut[0]) if len(cut) else len(order))]
             w = w[: len(order)]
         order, w = order[w >= min_p[r]], w[w >= min_p[r]]
-        ids = np.sort(order)
-        w = w[np.argsort(order)]
         sums = np.cumsum(w)
-        at = min(int(np.searchsorted(sums, uniform[r] * sums[-1], side="right")), len(ids) - 1)
-        tokens.append(int(ids[at]))
+        at = min(int(np.searchsorted(sums, uniform[r] * sums[-1], side="right")), len(order) - 1)
+        tokens.append(int(order[at]))
         probs.append(float(w[at] / sums[-1]))
     return {"token": torch.tensor(tokens, dtype=torch.int32), "prob": torch.tensor(probs, dtype=torch.float64)}
