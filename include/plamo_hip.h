@@ -368,6 +368,90 @@ int plamo_kernel_attention_decode_static(uint64_t qkv, uint64_t q_norm, uint64_t
                                          int32_t full, uint64_t local_rope, uint64_t global_rope, uint64_t out16,
                                          uint64_t stream, char* err, size_t errlen);
 
+/* ---- Many requests over one pool of pages -------------------------------------------
+ * No counterpart in the reference, which keeps one contiguous cache per sequence and at most four of
+ * them.  A step of a serving loop: plamo_kernel_paged_tables gives every request the pages its new
+ * tokens need and says where each token goes, plamo_kernel_paged_qkv writes the projection's keys and
+ * values there, plamo_kernel_attention_paged attends, plamo_kernel_sample draws the next tokens.  The
+ * calls launch on `stream` (and its device, which all memory has to belong to), allocate nothing, keep
+ * nothing between calls and can be captured into graphs.  What lengths, tables and positions hold is
+ * read on the device: out-of-range values are skipped as described, and never lead outside the cache. */
+#define PLAMO_BF16 0
+#define PLAMO_F16 1
+#define PLAMO_F32 2
+
+/* One layer's pages.  Token t of a request lies in slot t % page_size of the page that entry
+ * t / page_size of the request's table names; element d of KV head h is at
+ *   page * page_stride + slot * slot_stride + h * head_stride + d
+ * from `keys` and from `values` (strides in elements, multiples of 8: any order of the dimensions
+ * before the last, and keys and values may be interleaved).  16-byte aligned addresses, type
+ * PLAMO_BF16 or PLAMO_F16, head_dim 64, 128 or 256.  Pages of a multiple of 16 tokens are read fastest. */
+typedef struct plamo_paged_cache {
+    uint64_t keys, values; /* device addresses */
+    int64_t page_stride, slot_stride, head_stride;
+    int32_t pages, page_size, kv_heads, head_dim, type;
+} plamo_paged_cache;
+
+/* Block tables and the slot map of a step.  Request r holds lengths[r] tokens in the first
+ * ceil(lengths[r] / page_size) pages of tables[r][width].  counts[r] > 0: so many new tokens; 0: none;
+ * -1: the request has ended, its pages go back and its length becomes 0.  free_pages[0 .. free_count)
+ * is a stack: pages given back are pushed in the order of requests and table entries, then new ones
+ * popped in the same order (free_pages has room for all `pages`).  Written: the new entries of `tables`
+ * (others are left), lengths_out and free_out (which may be lengths and free_count themselves),
+ * offsets[rows + 1] (request r's new tokens are offsets[r] .. offsets[r + 1] - 1), and for each of them
+ * its position and slot (page * page_size + place in the page) in positions and slots [capacity], -1
+ * behind the last.  All int32, on the device.  All or nothing: with `status` (a sum of 1: too few free
+ * pages, 2: a request needs more than `width` pages, 4: more than `capacity` tokens, 8: invalid lengths,
+ * counts or free_count) other than 0 no length, table or free page changes and offsets are 0, slots and
+ * positions -1. */
+int plamo_kernel_paged_tables(uint64_t lengths, uint64_t counts, int32_t rows, uint64_t tables, int32_t width,
+                              int32_t page_size, uint64_t free_pages, uint64_t free_count, int32_t pages,
+                              uint64_t lengths_out, uint64_t free_out, uint64_t offsets, uint64_t slots,
+                              uint64_t positions, int32_t capacity, uint64_t status, uint64_t stream, char* err,
+                              size_t errlen);
+
+/* Rows of a qkv projection into the cache: qkv [tokens] rows of heads + 2 * kv_heads heads (queries,
+ * keys, values; `type` PLAMO_F32 or the cache's, qkv_stride elements between rows).  q_norm, k_norm
+ * ([head_dim], the cache's type; 0: none): x / sqrt(mean(x^2) + 1e-6) * (1 + gain).  rope (0: none;
+ * [rope_rows][head_dim / 2] words as plamo_rope_table makes them): pairs (d, d + head_dim / 2) turned by
+ * row positions[token].  FP32 inside, rounded once.  Queries go to q [tokens][heads * head_dim] (the
+ * cache's type; rows of that type may be overwritten in place), keys and values to slots[token].  A token
+ * with a position below 0 or from rope_rows on is skipped, and one with a slot outside the cache leaves
+ * the cache as it is.  Slots that are not skipped have to differ. */
+int plamo_kernel_paged_qkv(const plamo_paged_cache* cache, uint64_t qkv, int32_t type, int64_t qkv_stride, int32_t heads,
+                           uint64_t q_norm, uint64_t k_norm, uint64_t rope, int32_t rope_rows, uint64_t positions,
+                           uint64_t slots, int32_t tokens, uint64_t q, int64_t q_stride, uint64_t stream, char* err,
+                           size_t errlen);
+
+/* Attention of one token per request: out[r] = softmax(scale * q[r] . k) v over keys 0 .. lengths[r] - 1
+ * of tables[r][width], or the last `window` of them (window > 0); query head h reads KV head
+ * h / (heads / kv_heads).  q and out: rows of heads * head_dim of the cache's type.  lse (0: none): FP32
+ * [rows][heads], the logarithm of each sum of exponents.  Keys of a table entry outside 0 .. pages - 1 are
+ * not seen, lengths past the table end with it, and a row that sees nothing gives zeros and minus
+ * infinity.  `workspace` (16-byte aligned, plamo_kernel_attention_paged_workspace bytes, uninitialised) is the
+ * call's own until it has run: calls that may overlap need one each.  Results do not depend on timing;
+ * how a row's keys are divided depends on all rows' lengths. */
+int64_t plamo_kernel_attention_paged_workspace(int32_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim);
+int plamo_kernel_attention_paged(const plamo_paged_cache* cache, uint64_t q, int64_t q_stride, int32_t heads,
+                                 uint64_t tables, int32_t width, uint64_t lengths, int32_t rows, float scale,
+                                 int32_t window, uint64_t out, int64_t out_stride, uint64_t lse, uint64_t workspace,
+                                 int64_t workspace_bytes, uint64_t stream, char* err, size_t errlen);
+
+/* Tokens drawn from `rows` rows of n logits (`type`, `stride` elements apart, any alignment).  Per row
+ * (device arrays [rows], 0: off for all): temperature FP32 (0 or less: the first largest logit),
+ * top_k int32 (0 or less: off), top_p FP32 (1 or more: off), min_p FP32 (0 or less: off), uniform FP32 in
+ * [0, 1).  Tokens are ordered by descending logit, equal ones by ascending id, with weights
+ * exp((x - max x) / temperature).  Of these the first top_k stay, of them those before which less than
+ * top_p of the weight lies (at least one), of them those of at least min_p of the largest weight; `token`
+ * (int32) is the first up to which more than `uniform` of the weight that is left lies, and prob (FP32, 0:
+ * none) its share of it.  NaN counts as minus infinity, which is never drawn; a row of nothing else gives
+ * -1 and 0.  Tokens below 2^-46 of the largest weight are not drawn (n > 2^17: 2^-43).  n <= 2^20.  The
+ * result depends on the row and its controls alone.  Workspace as for plamo_kernel_attention_paged. */
+int64_t plamo_kernel_sample_workspace(int32_t rows, int32_t n);
+int plamo_kernel_sample(uint64_t logits, int32_t type, int64_t stride, int32_t n, int32_t rows, uint64_t temperature,
+                        uint64_t top_k, uint64_t top_p, uint64_t min_p, uint64_t uniform, uint64_t token, uint64_t prob,
+                        uint64_t workspace, int64_t workspace_bytes, uint64_t stream, char* err, size_t errlen);
+
 /* The host RoPE table builder the runtime uploads (`init_rope`, Kernels.metal:212-219; global
  * factors of `rotated`, Kernels.metal:264-267): `rows` x 64 entries of BF16 cos | sin << 16
  * from 64 inverse frequencies (config-mlx.json plamo_rope_inv_freq, Runtime.swift:268-274).

@@ -2,6 +2,7 @@
 #include <atomic>
 #include <algorithm>
 #include <chrono>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <map>
@@ -11,6 +12,7 @@
 
 #include "../../include/plamo_hip.h"
 #include "formats.h"
+#include "paged.h"
 #include "runtime.h"
 #include "tokenizer.h"
 
@@ -845,6 +847,231 @@ int plamo_kernel_attention_decode_static(uint64_t qkv, uint64_t q_norm, uint64_t
                                                    " visible keys per row");
         attn_workspace_bind(plamo::static_attn_scratch(), parts, a, reinterpret_cast<hipStream_t>(stream));
         attn_decode_launch(a, rows, full != 0, reinterpret_cast<hipStream_t>(stream));
+        PLAMO_HIP(hipGetLastError());
+    });
+}
+
+}  // extern "C"
+
+namespace {
+// The stream's device is current for the length of a call: kernels go where their stream is, whatever
+// device the thread had chosen.
+struct OnDeviceOf {
+    int before = -1;
+    explicit OnDeviceOf(hipStream_t s) {
+        if (!s) return;  // the current device's default stream
+        hipDevice_t of = 0;
+        int now = 0;
+        PLAMO_HIP(hipStreamGetDevice(s, &of));
+        PLAMO_HIP(hipGetDevice(&now));
+        if (now == of) return;
+        PLAMO_HIP(hipSetDevice(of));
+        before = now;
+    }
+    ~OnDeviceOf() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+    OnDeviceOf(const OnDeviceOf&) = delete;
+    OnDeviceOf& operator=(const OnDeviceOf&) = delete;
+};
+
+void require(bool ok, const char* message) {
+    if (!ok) throw plamo::Error(plamo::E_INVAL, message);
+}
+bool aligned(uint64_t address, uint64_t to) { return address % to == 0; }
+
+// The pages of a cache as every paged call checks them.
+void check_cache(const plamo_paged_cache* c) {
+    require(c != nullptr, "null paged cache");
+    require(c->type == PLAMO_BF16 || c->type == PLAMO_F16, "paged cache: type must be PLAMO_BF16 or PLAMO_F16");
+    require(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, "paged cache: head_dim must be 64, 128 or 256");
+    require(c->kv_heads >= 1 && c->kv_heads <= 256, "paged cache: kv_heads must be 1...256");
+    require(c->pages >= 1 && c->page_size >= 1 && int64_t(c->pages) * c->page_size <= INT32_MAX,
+            "paged cache: pages and page_size must be at least 1, and hold less than 2^31 tokens");
+    require(c->keys && c->values && aligned(c->keys, 16) && aligned(c->values, 16),
+            "paged cache: keys and values must be 16-byte aligned");
+    require(c->page_stride % 8 == 0 && c->slot_stride % 8 == 0 && c->head_stride % 8 == 0 && c->page_stride >= 0 &&
+                c->head_stride >= 0 && c->slot_stride >= 0 && c->slot_stride <= (1 << 24) &&
+                c->page_stride <= (int64_t(1) << 40) && c->head_stride <= (int64_t(1) << 40),
+            "paged cache: strides must be non-negative multiples of 8 elements, slot_stride at most 2^24");
+}
+}  // namespace
+
+extern "C" {
+
+int plamo_kernel_paged_tables(uint64_t lengths, uint64_t counts, int32_t rows, uint64_t tables, int32_t width,
+                              int32_t page_size, uint64_t free_pages, uint64_t free_count, int32_t pages,
+                              uint64_t lengths_out, uint64_t free_out, uint64_t offsets, uint64_t slots,
+                              uint64_t positions, int32_t capacity, uint64_t status, uint64_t stream, char* err,
+                              size_t errlen) {
+    return guard(err, errlen, [&] {
+        require(rows >= 1 && width >= 1 && capacity >= 0, "paged tables: rows and width must be at least 1");
+        require(page_size >= 1 && pages >= 1 && int64_t(pages) * page_size <= INT32_MAX,
+                "paged tables: pages and page_size must be at least 1, and hold less than 2^31 tokens");
+        require(lengths && counts && tables && free_pages && free_count && lengths_out && free_out && offsets && status &&
+                    (capacity == 0 || (slots && positions)),
+                "paged tables: null argument");
+        const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+        const OnDeviceOf device(s);
+        plamo::PagedTablesParams p{};
+        p.lengths = reinterpret_cast<const int32_t*>(lengths);
+        p.counts = reinterpret_cast<const int32_t*>(counts);
+        p.rows = rows;
+        p.tables = reinterpret_cast<int32_t*>(tables);
+        p.width = width;
+        p.page_size = page_size;
+        p.free_pages = reinterpret_cast<int32_t*>(free_pages);
+        p.free_count = reinterpret_cast<const int32_t*>(free_count);
+        p.pages = pages;
+        p.lengths_out = reinterpret_cast<int32_t*>(lengths_out);
+        p.free_out = reinterpret_cast<int32_t*>(free_out);
+        p.offsets = reinterpret_cast<int32_t*>(offsets);
+        p.slots = reinterpret_cast<int32_t*>(slots);
+        p.positions = reinterpret_cast<int32_t*>(positions);
+        p.capacity = capacity;
+        p.status = reinterpret_cast<int32_t*>(status);
+        p.div = plamo::divider(uint32_t(page_size));
+        plamo::launch_paged_tables(p, s);
+        PLAMO_HIP(hipGetLastError());
+    });
+}
+
+int plamo_kernel_paged_qkv(const plamo_paged_cache* cache, uint64_t qkv, int32_t type, int64_t qkv_stride, int32_t heads,
+                           uint64_t q_norm, uint64_t k_norm, uint64_t rope, int32_t rope_rows, uint64_t positions,
+                           uint64_t slots, int32_t tokens, uint64_t q, int64_t q_stride, uint64_t stream, char* err,
+                           size_t errlen) {
+    return guard(err, errlen, [&] {
+        check_cache(cache);
+        require(type == PLAMO_F32 || type == cache->type, "paged qkv: rows must be FP32 or of the cache's type");
+        require(heads >= 1 && heads <= 4096 && heads % cache->kv_heads == 0,
+                "paged qkv: heads must be a multiple of kv_heads, at most 4096");
+        require(tokens >= 0, "paged qkv: negative token count");
+        const int64_t wide = int64_t(heads + 2 * cache->kv_heads) * cache->head_dim, size = type == PLAMO_F32 ? 4 : 2;
+        require(qkv_stride >= wide && qkv_stride * size % 16 == 0 && q_stride >= int64_t(heads) * cache->head_dim &&
+                    q_stride % 8 == 0,
+                "paged qkv: row strides must hold a row and be multiples of 16 bytes");
+        require(int64_t(tokens) * wide / 8 <= INT32_MAX, "paged qkv: too many rows");
+        require((tokens == 0 || (qkv && q && slots)) && aligned(qkv, 16) && aligned(q, 16) && aligned(q_norm, 8) && aligned(k_norm, 8) &&
+                    aligned(rope, 16),
+                "paged qkv: rows and rope must be 16-byte aligned, gains 8-byte");
+        require(!rope || ((positions || tokens == 0) && rope_rows >= 1), "paged qkv: a rotation needs positions and rope_rows");
+        const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+        const OnDeviceOf device(s);
+        plamo::PagedQkvParams p{};
+        p.qkv = reinterpret_cast<const void*>(qkv);
+        p.stride = qkv_stride;
+        p.heads = heads;
+        p.kv_heads = cache->kv_heads;
+        p.q_norm = reinterpret_cast<const uint16_t*>(q_norm);
+        p.k_norm = reinterpret_cast<const uint16_t*>(k_norm);
+        p.rope = reinterpret_cast<const uint32_t*>(rope);
+        p.rope_rows = rope_rows;
+        p.positions = reinterpret_cast<const int32_t*>(positions);
+        p.slots = reinterpret_cast<const int32_t*>(slots);
+        p.tokens = tokens;
+        p.q = reinterpret_cast<uint16_t*>(q);
+        p.q_stride = q_stride;
+        p.keys = reinterpret_cast<uint16_t*>(cache->keys);
+        p.values = reinterpret_cast<uint16_t*>(cache->values);
+        p.page_stride = cache->page_stride;
+        p.slot_stride = cache->slot_stride;
+        p.head_stride = cache->head_stride;
+        p.pages = cache->pages;
+        p.page_size = cache->page_size;
+        p.div = plamo::divider(uint32_t(cache->page_size));
+        plamo::launch_paged_qkv(p, type, cache->type, cache->head_dim, s);
+        PLAMO_HIP(hipGetLastError());
+    });
+}
+
+int64_t plamo_kernel_attention_paged_workspace(int32_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim) {
+    if (rows < 1 || heads < 1 || heads > 4096 || kv_heads < 1 || heads % kv_heads != 0 || head_dim < 1 || head_dim > 256)
+        return -1;
+    return int64_t(plamo::paged_attn_workspace(rows, heads, kv_heads, head_dim));
+}
+
+int plamo_kernel_attention_paged(const plamo_paged_cache* cache, uint64_t q, int64_t q_stride, int32_t heads,
+                                 uint64_t tables, int32_t width, uint64_t lengths, int32_t rows, float scale,
+                                 int32_t window, uint64_t out, int64_t out_stride, uint64_t lse, uint64_t workspace,
+                                 int64_t workspace_bytes, uint64_t stream, char* err, size_t errlen) {
+    return guard(err, errlen, [&] {
+        check_cache(cache);
+        require(heads >= 1 && heads <= 4096 && heads % cache->kv_heads == 0,
+                "paged attention: heads must be a multiple of kv_heads, at most 4096");
+        require(rows >= 1 && rows <= (1 << 20) && width >= 1 && int64_t(width) * cache->page_size <= (1 << 30),
+                "paged attention: rows must be 1...2^20, width at least 1, and a row's pages hold at most 2^30 tokens");
+        require(window >= 0 && std::isfinite(scale), "paged attention: window must not be negative, scale finite");
+        const int64_t wide = int64_t(heads) * cache->head_dim;
+        require(q_stride >= wide && out_stride >= wide && q_stride % 8 == 0 && out_stride % 8 == 0,
+                "paged attention: row strides must hold a row and be multiples of 16 bytes");
+        require(q && out && tables && lengths && aligned(q, 16) && aligned(out, 16),
+                "paged attention: q and out must be 16-byte aligned");
+        require(workspace && aligned(workspace, 16) &&
+                    workspace_bytes >= plamo_kernel_attention_paged_workspace(rows, heads, cache->kv_heads, cache->head_dim),
+                "paged attention: workspace too small or not 16-byte aligned");
+        const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+        const OnDeviceOf device(s);
+        plamo::PagedAttnParams p{};
+        p.keys = reinterpret_cast<const char*>(cache->keys);
+        p.values = reinterpret_cast<const char*>(cache->values);
+        p.page_stride = cache->page_stride * 2;
+        p.slot_stride = cache->slot_stride * 2;
+        p.head_stride = cache->head_stride * 2;
+        p.pages = cache->pages;
+        p.page_size = cache->page_size;
+        p.div = plamo::divider(uint32_t(cache->page_size));
+        p.kv_heads = cache->kv_heads;
+        p.group = heads / cache->kv_heads;
+        p.q = reinterpret_cast<const uint16_t*>(q);
+        p.q_stride = q_stride;
+        p.tables = reinterpret_cast<const int32_t*>(tables);
+        p.width = width;
+        p.lengths = reinterpret_cast<const int32_t*>(lengths);
+        p.rows = rows;
+        p.most = width * cache->page_size;
+        p.window = window;
+        p.scale = scale * 1.4426950408889634f;
+        p.out = reinterpret_cast<uint16_t*>(out);
+        p.out_stride = out_stride;
+        p.lse = reinterpret_cast<float*>(lse);
+        plamo::paged_attn_bind(p, reinterpret_cast<void*>(workspace), cache->head_dim);
+        plamo::launch_paged_attention(p, cache->type, cache->head_dim, s);
+        PLAMO_HIP(hipGetLastError());
+    });
+}
+
+int64_t plamo_kernel_sample_workspace(int32_t rows, int32_t n) {
+    if (rows < 1 || n < 1 || n > plamo::SAMPLE_MAX_VOCAB) return -1;
+    return int64_t(plamo::sample_workspace(rows, n));
+}
+
+int plamo_kernel_sample(uint64_t logits, int32_t type, int64_t stride, int32_t n, int32_t rows, uint64_t temperature,
+                        uint64_t top_k, uint64_t top_p, uint64_t min_p, uint64_t uniform, uint64_t token, uint64_t prob,
+                        uint64_t workspace, int64_t workspace_bytes, uint64_t stream, char* err, size_t errlen) {
+    return guard(err, errlen, [&] {
+        require(type == PLAMO_BF16 || type == PLAMO_F16 || type == PLAMO_F32, "sample: unknown logits type");
+        require(n >= 1 && n <= plamo::SAMPLE_MAX_VOCAB && rows >= 1 && rows <= (1 << 20), "sample: n and rows must be 1...2^20");
+        require(stride >= n || rows == 1, "sample: rows overlap");
+        require(logits && uniform && token && aligned(logits, type == PLAMO_F32 ? 4 : 2), "sample: null or unaligned argument");
+        const int64_t need = plamo_kernel_sample_workspace(rows, n);
+        require(workspace_bytes >= need && (need == 0 || (workspace && aligned(workspace, 16))),
+                "sample: workspace too small or not 16-byte aligned");
+        const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+        const OnDeviceOf device(s);
+        plamo::SampleParams p{};
+        p.logits = reinterpret_cast<const void*>(logits);
+        p.stride = stride;
+        p.n = n;
+        p.rows = rows;
+        p.temperature = reinterpret_cast<const float*>(temperature);
+        p.top_k = reinterpret_cast<const int32_t*>(top_k);
+        p.top_p = reinterpret_cast<const float*>(top_p);
+        p.min_p = reinterpret_cast<const float*>(min_p);
+        p.uniform = reinterpret_cast<const float*>(uniform);
+        p.token = reinterpret_cast<int32_t*>(token);
+        p.prob = reinterpret_cast<float*>(prob);
+        p.workspace = reinterpret_cast<void*>(workspace);
+        plamo::launch_sample(p, type, s);
         PLAMO_HIP(hipGetLastError());
     });
 }

@@ -1,0 +1,757 @@
+// Serving many requests from one pool of KV pages on gfx950.
+//
+//   paged_tables_kernel     pages taken from and given back to the free list, block tables, offsets
+//   paged_slots_kernel      slot and position of each new token
+//   paged_qkv_kernel        q and k RMS-normalised and rotated, k and v written to their slots
+//   paged_attention_kernel  attention of one token per request over its pages, split over the keys
+//   paged_merge_kernel      parts of a row joined
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "common.h"
+#include "device.h"
+#include "paged.h"
+
+namespace plamo {
+using namespace dev;
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ uint32_t divide(uint32_t x, Divider d) { return uint32_t((uint64_t(x) * d.mul) >> d.shift); }
+
+// ------------------------------------------------------------------------------------ tables
+// One workgroup: prefix sums over the requests of pages given back, pages taken and tokens, then the
+// moves flattened over pages so that a long request's are not one thread's.  Latency-bound: at 64
+// requests the few KB move in the time of the dependent loads and barriers.
+constexpr int TABLE_THREADS = 1024;
+
+struct Scan3 {
+    int back, take, fresh;
+};
+
+// Inclusive sums over the workgroup; `total` in every thread.
+__device__ Scan3 block_scan3(Scan3 v, Scan3* waves, Scan3& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int a = __shfl_up(v.back, o, 64), b = __shfl_up(v.take, o, 64), c = __shfl_up(v.fresh, o, 64);
+        if (lane >= o) {
+            v.back += a;
+            v.take += b;
+            v.fresh += c;
+        }
+    }
+    __syncthreads();  // the sums of a scan before this one have been read
+    if (lane == 63) waves[wave] = v;
+    __syncthreads();
+    total = {0, 0, 0};
+    for (int w = 0; w < TABLE_THREADS / 64; ++w) {
+        if (w == wave) {
+            v.back += total.back;
+            v.take += total.take;
+            v.fresh += total.fresh;
+        }
+        total.back += waves[w].back;
+        total.take += waves[w].take;
+        total.fresh += waves[w].fresh;
+    }
+    return v;
+}
+
+// What row r asks for, from its length and count (both checked).
+__device__ __forceinline__ Scan3 row_moves(const PagedTablesParams& p, int r, int& held) {
+    held = 0;
+    if (r >= p.rows) return {0, 0, 0};
+    const int64_t length = p.lengths[r], count = p.counts[r];
+    held = int((length + p.page_size - 1) / p.page_size);
+    if (count < 0) return {held, 0, 0};
+    return {0, int((length + count + p.page_size - 1) / p.page_size) - held, int(count)};
+}
+
+// The first of `n` ascending inclusive sums above x.
+__device__ __forceinline__ int first_above(const int* sums, int n, int x) {
+    int lo = 0;
+    while (n > 0) {
+        const int half = n >> 1;
+        if (sums[lo + half] > x) {
+            n = half;
+        } else {
+            lo += half + 1;
+            n -= half + 1;
+        }
+    }
+    return lo;
+}
+
+// Token j of the step: its request by the offsets, its position behind the request's old length, its slot.
+__device__ __forceinline__ void token_slot(const PagedTablesParams& p, int j, int total) {
+    int slot = -1, at = -1;
+    if (j < total) {
+        const int r = first_above(p.offsets + 1, p.rows, j);
+        at = p.lengths_out[r] - (p.offsets[r + 1] - j);
+        const uint32_t page = divide(uint32_t(at), p.div);
+        slot = p.tables[int64_t(r) * p.width + page] * p.page_size + (at - int(page) * p.page_size);
+    }
+    p.slots[j] = slot;
+    p.positions[j] = at;
+}
+
+template <bool SLOTS>
+__global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(PagedTablesParams p) {
+    __shared__ Scan3 s_waves[TABLE_THREADS / 64];
+    __shared__ unsigned long long s_back, s_take, s_fresh;
+    __shared__ int s_status;
+    __shared__ int s_sums[TABLE_THREADS], s_start[TABLE_THREADS], s_held[TABLE_THREADS];
+    const int tid = threadIdx.x;
+    if (tid == 0) {
+        s_back = s_take = s_fresh = 0;
+        s_status = 0;
+    }
+    const int64_t first = *p.free_count;
+    __syncthreads();
+    // totals and checks before anything is written
+    int bad = 0;
+    int64_t back = 0, take = 0, fresh = 0;
+    for (int r = tid; r < p.rows; r += TABLE_THREADS) {
+        const int64_t length = p.lengths[r], count = p.counts[r];
+        if (length < 0 || count < -1) {
+            bad |= 8;
+            continue;
+        }
+        const int64_t held = (length + p.page_size - 1) / p.page_size;
+        const int64_t after = count < 0 ? 0 : (length + count + p.page_size - 1) / p.page_size;
+        if (held > p.width || after > p.width || length + count > INT32_MAX) bad |= 2;
+        if (count < 0) back += held;
+        else take += after - held, fresh += count;
+    }
+    if (bad) atomicOr(&s_status, bad);
+    if (back) atomicAdd(&s_back, static_cast<unsigned long long>(back));
+    if (take) atomicAdd(&s_take, static_cast<unsigned long long>(take));
+    if (fresh) atomicAdd(&s_fresh, static_cast<unsigned long long>(fresh));
+    __syncthreads();
+    const int64_t full = first + int64_t(s_back);
+    int status = s_status;
+    if (first < 0 || full > p.pages) status |= 8;
+    else if (int64_t(s_take) > full) status |= 1;
+    if (int64_t(s_fresh) > p.capacity) status |= 4;
+    if (tid == 0) {
+        *p.status = status;
+        p.offsets[0] = 0;
+        *p.free_out = status ? int32_t(first) : int32_t(full - int64_t(s_take));
+    }
+    const int total = status ? 0 : int(s_fresh);
+    if (status) {
+        for (int r = tid; r < p.rows; r += TABLE_THREADS) {
+            p.offsets[r + 1] = 0;
+            p.lengths_out[r] = p.lengths[r];
+        }
+    } else {
+        // pages given back, on top of the free ones, in row order; lengths and offsets, unless the
+        // lengths are still read by the second pass
+        Scan3 run = {0, 0, 0}, sum;
+        for (int pass = 0; pass < 2; ++pass) {
+            run = {0, 0, 0};
+            for (int base = 0; base < p.rows; base += TABLE_THREADS) {
+                const int r = base + tid;
+                int held;
+                const Scan3 own = row_moves(p, r, held);
+                const Scan3 incl = block_scan3(own, s_waves, sum);
+                const int moved = pass ? own.take : own.back, chunk = pass ? sum.take : sum.back;
+                const int before = pass ? run.take : run.back;
+                s_sums[tid] = pass ? incl.take : incl.back;
+                s_start[tid] = s_sums[tid] - moved;
+                s_held[tid] = held;
+                __syncthreads();
+                for (int e = tid; e < chunk; e += TABLE_THREADS) {
+                    const int q = first_above(s_sums, TABLE_THREADS, e), i = e - s_start[q];
+                    int32_t* table = p.tables + int64_t(base + q) * p.width;
+                    if (pass) table[s_held[q] + i] = p.free_pages[full - 1 - (before + e)];
+                    else p.free_pages[first + before + e] = table[i];
+                }
+                if (pass && r < p.rows) {
+                    p.offsets[r + 1] = run.fresh + incl.fresh;
+                    p.lengths_out[r] = p.counts[r] < 0 ? 0 : p.lengths[r] + p.counts[r];
+                }
+                run = {run.back + sum.back, run.take + sum.take, run.fresh + sum.fresh};
+            }
+            __syncthreads();  // the pages given back are on the stack, the tables complete
+        }
+    }
+    if constexpr (SLOTS) {
+        __syncthreads();
+        for (int j = tid; j < p.capacity; j += TABLE_THREADS) token_slot(p, j, total);
+    }
+}
+
+__global__ __launch_bounds__(256) void paged_slots_kernel(PagedTablesParams p) {
+    const int j = int(blockIdx.x * 256 + threadIdx.x);
+    if (j < p.capacity) token_slot(p, j, p.offsets[p.rows]);
+}
+
+// ------------------------------------------------------------------------------------ qkv
+template <int TYPE>
+__device__ __forceinline__ float from16(uint32_t h) {
+    if constexpr (TYPE == TYPE_BF16) return bf(h & 0xffffu);
+    return float(__builtin_bit_cast(_Float16, uint16_t(h)));
+}
+// Two values rounded to nearest even and packed.
+template <int TYPE>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+    if constexpr (TYPE == TYPE_BF16) return pack_bf16(a, b);
+    const f16x2 h = {_Float16(a), _Float16(b)};
+    return __builtin_bit_cast(uint32_t, h);
+}
+template <int SOURCE>
+__device__ __forceinline__ void load4(const void* base, int64_t at, float (&v)[4]) {
+    if constexpr (SOURCE == TYPE_F32) {
+        const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
+        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + at);
+        v[0] = from16<SOURCE>(x.x), v[1] = from16<SOURCE>(x.x >> 16);
+        v[2] = from16<SOURCE>(x.y), v[3] = from16<SOURCE>(x.y >> 16);
+    }
+}
+
+// y = x / sqrt(mean(x^2) + 1e-6) (1 + g), (y_i, y_{i + D/2}) turned by the position's angle, rounded
+// once.  D / 8 lanes hold a head, each four dims of its first half and the same four of its second, so
+// that the rotation stays in a lane.  Bound by memory: each element is read and written once.
+template <int SOURCE, int TYPE, int D>
+__global__ __launch_bounds__(256) void paged_qkv_kernel(PagedQkvParams p) {
+    constexpr int LANES = D / 8;
+    const int wide = p.heads + 2 * p.kv_heads;
+    const int64_t item = (int64_t(blockIdx.x) * 256 + threadIdx.x) / LANES;
+    if (item >= int64_t(p.tokens) * wide) return;  // whole groups of lanes
+    const int t = int(item / wide), h = int(item - int64_t(t) * wide), d = int(threadIdx.x % LANES) * 4;
+    const int pos = p.positions ? p.positions[t] : 0;
+    if (p.rope ? uint32_t(pos) >= uint32_t(p.rope_rows) : pos < 0) return;  // a padding row
+    float a[4], b[4];
+    const int64_t at = t * p.stride + int64_t(h) * D + d;
+    load4<SOURCE>(p.qkv, at, a);
+    load4<SOURCE>(p.qkv, at + D / 2, b);
+    const bool query = h < p.heads, value = h >= p.heads + p.kv_heads;
+    const uint16_t* gain = value ? nullptr : query ? p.q_norm : p.k_norm;
+    if (gain) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ss += a[i] * a[i] + b[i] * b[i];
+        if constexpr (LANES > 16) ss += xor_lane<16>(ss);
+        if constexpr (LANES > 8) ss += xor_lane<8>(ss);
+        ss += xor_lane<4>(ss);
+        ss += xor_lane<2>(ss);
+        ss += xor_lane<1>(ss);
+        const float r = 1.0f / sqrtf(ss / float(D) + 1e-6f);
+        float ga[4], gb[4];
+        load4<TYPE>(gain, d, ga);
+        load4<TYPE>(gain, d + D / 2, gb);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            a[i] = a[i] * r * (1.0f + ga[i]);
+            b[i] = b[i] * r * (1.0f + gb[i]);
+        }
+    }
+    if (p.rope && !value) {
+        const uint4 w = *reinterpret_cast<const uint4*>(p.rope + int64_t(pos) * (D / 2) + d);
+        const uint32_t cs[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float c = lo(cs[i]), s = hi(cs[i]), x = a[i], y = b[i];
+            a[i] = x * c - y * s;
+            b[i] = y * c + x * s;
+        }
+    }
+    uint16_t* to;
+    if (query) {
+        to = p.q + t * p.q_stride + int64_t(h) * D;
+    } else {
+        const int slot = p.slots[t];
+        const uint32_t page = divide(uint32_t(slot) & 0x7fffffffu, p.div);
+        if (slot < 0 || page >= uint32_t(p.pages)) return;
+        to = (value ? p.values : p.keys) + int64_t(page) * p.page_stride +
+             int64_t(slot - int(page) * p.page_size) * p.slot_stride +
+             int64_t(h - p.heads - (value ? p.kv_heads : 0)) * p.head_stride;
+    }
+    *reinterpret_cast<uint2*>(to + d) = make_uint2(pack16<TYPE>(a[0], a[1]), pack16<TYPE>(a[2], a[3]));
+    *reinterpret_cast<uint2*>(to + d + D / 2) = make_uint2(pack16<TYPE>(b[0], b[1]), pack16<TYPE>(b[2], b[3]));
+}
+
+// ------------------------------------------------------------------------------------ attention
+// o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m) over the visible keys of a row, one pass with the
+// running maximum and sum.  A wave holds 16 query heads (one per column) and takes 32 keys at a time:
+//   S^T = K Q^T   v_mfma_f32_16x16x32 with the keys as rows: lane l gets head l % 16 and the keys
+//                 4 (l / 16) + i of both halves of the tile, so the softmax of a head is within four
+//                 lanes and its weights are already the operand of the next product;
+//   O^T += V^T P^T  the same four keys of both halves are the depth: lane l reads rows of V (whole
+//                 lines: 16 lanes side by side) and transposes its 8 keys x 8 dims in registers.
+// Nothing passes through LDS until the four waves of a part are joined.  The bound is the pages'
+// bytes: 16 heads on one KV head cost 2 x 16 x 128 products for 512 bytes, a fifth of what the matrix
+// units do in that time.
+// The weights are kept in two halves of the type (p = hi + lo, 2^-17 off for BF16, 2^-23 for FP16): one
+// rounding of them would be as large an error as the output's own.
+constexpr int ATTN_WAVES = 4;
+constexpr int ATTN_THREADS = ATTN_WAVES * 64;
+constexpr int PART_KEYS = 32 * ATTN_WAVES;  // fewest keys of a part: a tile for each wave
+// Parts aimed at over all rows and KV heads: four workgroups for each of 256 CUs.
+constexpr int ATTN_TARGET = 1024;
+
+inline int attn_tiles(int heads, int kv_heads) { return (heads / kv_heads + 15) / 16; }
+inline int attn_target(int heads, int kv_heads) {
+    return std::max(1, ATTN_TARGET / (kv_heads * attn_tiles(heads, kv_heads)));
+}
+
+struct Row {
+    int len;    // keys 0 .. len - 1
+    int first;  // the first visible one
+    int span;   // keys from `first` rounded down to 16 on
+};
+__device__ __forceinline__ Row row_keys(const PagedAttnParams& p, int r) {
+    Row k;
+    k.len = min(max(p.lengths[r], 0), p.most);
+    k.first = p.window > 0 ? max(0, k.len - p.window) : 0;
+    k.span = k.len - (k.first & ~15);
+    return k;
+}
+__device__ __forceinline__ int row_parts(int span, int chunk) { return max(1, (span + chunk - 1) / chunk); }
+
+// Keys of a part: all rows' keys divided by the parts aimed at (the same in every wave of the launch).
+__device__ __forceinline__ int part_chunk(const PagedAttnParams& p) {
+    const int lane = threadIdx.x & 63;
+    long long sum = 0;
+    for (int r = lane; r < p.rows; r += 64) sum += row_keys(p, r).span;
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    const long long each = (sum + p.target - 1) / p.target;  // at most the longest table's keys per row
+    return each <= PART_KEYS ? PART_KEYS : int((each + PART_KEYS - 1) / PART_KEYS * PART_KEYS);
+}
+
+// The row that part `item` belongs to and the row's first part; false past the last part.
+__device__ __forceinline__ bool find_part(const PagedAttnParams& p, int chunk, int item, int& row, int& first, int& parts) {
+    const int lane = threadIdx.x & 63;
+    int run = 0;
+    for (int base = 0; base < p.rows; base += 64) {
+        const int r = base + lane;
+        const int own = r < p.rows ? row_parts(row_keys(p, r).span, chunk) : 0;
+        int incl = own;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(incl, o, 64);
+            if (lane >= o) incl += v;
+        }
+        const unsigned long long past = __ballot(run + incl > item);
+        if (past) {
+            const int l = __ffsll(past) - 1;
+            row = __builtin_amdgcn_readfirstlane(base + l);
+            parts = __builtin_amdgcn_readlane(own, l);
+            first = run + __builtin_amdgcn_readlane(incl, l) - parts;
+            return true;
+        }
+        run += __builtin_amdgcn_readlane(incl, 63);
+    }
+    return false;
+}
+
+template <int TYPE>
+__device__ __forceinline__ floatx4 mfma16(uint4 a, uint4 b, floatx4 c) {
+    if constexpr (TYPE == TYPE_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// FP16 weights are held times 2^12: their smallest normal value is then 2^-26 of the largest weight's.
+template <int TYPE>
+constexpr float weight_shift() { return TYPE == TYPE_F16 ? 12.0f : 0.0f; }
+
+template <int TYPE, int D>
+struct Tile {
+    static constexpr int STEPS = D / 32;             // products over a head's dims
+    static constexpr int CHUNK = D < 128 ? D / 16 : 8;  // dims of V that a lane takes of a key, at once
+    static constexpr int SLABS = D < 128 ? 1 : D / 128;
+    uint4 k[2][STEPS];
+    uint32_t v[8][SLABS][CHUNK / 2];
+    uint32_t seen;  // bit i: key 4 (l / 16) + i % 4 of half i / 4 is visible
+    bool whole;     // all keys of the tile are
+};
+
+// EVEN: pages of whole half tiles (a multiple of 16 tokens), so that a half tile is one page's and
+// its page and addresses are the wave's, not the lane's.
+template <int TYPE, int D, bool EVEN>
+__device__ __forceinline__ void load_tile(Tile<TYPE, D>& t, const PagedAttnParams& p, const int32_t* table,
+                                          int64_t head, int pos, int lo_key, int hi_key) {
+    typedef Tile<TYPE, D> X;
+    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    t.whole = pos >= lo_key && pos + 32 <= hi_key;
+    t.seen = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int j = pos + 16 * (i >> 2) + 4 * g + (i & 3);
+        t.seen |= uint32_t(j >= lo_key && j < hi_key) << i;
+    }
+    if constexpr (EVEN) {
+        __amdgpu_buffer_rsrc_t kr[2], vr[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            // a half past the last key, or of a page that is none, reads nothing: its view is empty
+            const int at = pos + 16 * h;
+            int page = -1;
+            const uint32_t index = divide(uint32_t(at), p.div);
+            if (at < hi_key) page = table[index];
+            const bool there = uint32_t(page) < uint32_t(p.pages);
+            if (at < hi_key && !there) {
+                t.whole = false;
+                t.seen &= ~(0xfu << (4 * h));
+            }
+            const int64_t off = there ? page * p.page_stride + (at - int(index) * p.page_size) * p.slot_stride + head : 0;
+            const uint32_t bytes = there ? uint32_t(15 * p.slot_stride + D * 2) : 0u;
+            kr[h] = buffer_view(p.keys + off, bytes);
+            vr[h] = buffer_view(p.values + off, bytes);
+        }
+        const uint32_t ks = uint32_t(col * int(p.slot_stride) + g * 16);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int s = 0; s < X::STEPS; ++s) t.k[h][s] = buffer_prefetch16(kr[h], ks + s * 64);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int s = 0; s < X::SLABS; ++s) {
+                const uint32_t at = uint32_t((4 * g + (i & 3)) * int(p.slot_stride) + col * X::CHUNK * 2 + s * 256);
+                if constexpr (X::CHUNK == 8) {
+                    const uint4 w = buffer_prefetch16(vr[i >> 2], at);
+                    t.v[i][s][0] = w.x, t.v[i][s][1] = w.y, t.v[i][s][2] = w.z, t.v[i][s][3] = w.w;
+                } else {
+                    const uint2 w = buffer_load8(vr[i >> 2], at);
+                    t.v[i][s][0] = w.x, t.v[i][s][1] = w.y;
+                }
+            }
+    } else {
+        auto place = [&](int j, bool& there) {
+            int page = -1;
+            const uint32_t index = divide(uint32_t(j), p.div);
+            if (j >= lo_key && j < hi_key) page = table[index];
+            there = uint32_t(page) < uint32_t(p.pages);
+            return there ? page * p.page_stride + (j - int(index) * p.page_size) * p.slot_stride + head : int64_t(0);
+        };
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            bool there;
+            const int64_t off = place(pos + 16 * h + col, there) + g * 16;
+#pragma unroll
+            for (int s = 0; s < X::STEPS; ++s)
+                t.k[h][s] = there ? *reinterpret_cast<const uint4*>(p.keys + off + s * 64) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            bool there;
+            const int64_t off = place(pos + 16 * (i >> 2) + 4 * g + (i & 3), there) + col * X::CHUNK * 2;
+            if (!there) t.seen &= ~(1u << i);
+#pragma unroll
+            for (int s = 0; s < X::SLABS; ++s)
+#pragma unroll
+                for (int w = 0; w < X::CHUNK / 2; w += 2) {
+                    const uint2 x = there ? *reinterpret_cast<const uint2*>(p.values + off + s * 256 + w * 4) : make_uint2(0, 0);
+                    t.v[i][s][w] = x.x;
+                    t.v[i][s][w + 1] = x.y;
+                }
+        }
+        t.whole = __all(t.seen == 0xffu);
+    }
+}
+
+template <int TYPE, int D>
+struct Running {
+    typedef Tile<TYPE, D> X;
+    float m = NEG_INF, l = 0.f;               // of the lane's head; l over the lane's own keys
+    floatx4 o[X::SLABS][X::CHUNK];            // dims slab * 128 + (4 (l / 16) + i) CHUNK + j
+};
+
+template <int TYPE, int D>
+__device__ __forceinline__ void take_tile(Running<TYPE, D>& run, Tile<TYPE, D>& t, const uint4 (&q)[D / 32], float scale) {
+    typedef Tile<TYPE, D> X;
+    floatx4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int c = 0; c < X::STEPS; ++c) {
+        s[0] = mfma16<TYPE>(t.k[0][c], q[c], s[0]);
+        s[1] = mfma16<TYPE>(t.k[1][c], q[c], s[1]);
+    }
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = s[i >> 2][i & 3] * scale;
+    if (!t.whole) {
+        // what a hidden key's row holds (NaN among it) reaches neither the scores nor the sums
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool seen = (t.seen >> i) & 1u;
+            x[i] = seen ? x[i] : NEG_INF;
+#pragma unroll
+            for (int b = 0; b < X::SLABS; ++b)
+#pragma unroll
+                for (int w = 0; w < X::CHUNK / 2; ++w) t.v[i][b][w] = seen ? t.v[i][b][w] : 0u;
+        }
+    }
+    float most = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) most = fmaxf(most, x[i]);
+    most = fmaxf(most, xor_lane<16>(most));
+    most = fmaxf(most, xor_lane<32>(most));
+    const float before = run.m;
+    run.m = fmaxf(before, most);
+    // exponents are taken from `from`: the maximum, or any number while that is minus infinity
+    const float from = (run.m == NEG_INF ? 0.f : run.m) - weight_shift<TYPE>();
+    if (__any(run.m > before)) {
+        const float shrink = __builtin_amdgcn_exp2f(before - weight_shift<TYPE>() - from);
+        run.l *= shrink;
+#pragma unroll
+        for (int b = 0; b < X::SLABS; ++b)
+#pragma unroll
+            for (int j = 0; j < X::CHUNK; ++j) run.o[b][j] *= shrink;
+    }
+    float e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        e[i] = __builtin_amdgcn_exp2f(x[i] - from);
+        run.l += e[i];
+    }
+    uint32_t high[4], low[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        high[i] = pack16<TYPE>(e[2 * i], e[2 * i + 1]);
+        low[i] = pack16<TYPE>(e[2 * i] - from16<TYPE>(high[i]), e[2 * i + 1] - from16<TYPE>(high[i] >> 16));
+    }
+    const uint4 ph = make_uint4(high[0], high[1], high[2], high[3]), pl = make_uint4(low[0], low[1], low[2], low[3]);
+#pragma unroll
+    for (int b = 0; b < X::SLABS; ++b)
+#pragma unroll
+        for (int j = 0; j < X::CHUNK; ++j) {
+            // dim j of the lane's eight keys, two keys a word
+            const uint32_t pick = j & 1 ? 0x07060302u : 0x05040100u;
+            uint32_t a[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] = __builtin_amdgcn_perm(t.v[2 * i + 1][b][j >> 1], t.v[2 * i][b][j >> 1], pick);
+            const uint4 column = make_uint4(a[0], a[1], a[2], a[3]);
+            run.o[b][j] = mfma16<TYPE>(column, ph, run.o[b][j]);
+            run.o[b][j] = mfma16<TYPE>(column, pl, run.o[b][j]);
+        }
+}
+
+template <int TYPE, int D, bool EVEN>
+__global__ __launch_bounds__(ATTN_THREADS, 2) void paged_attention_kernel(PagedAttnParams p) {
+    typedef Tile<TYPE, D> X;
+    constexpr int PITCH = D + 4;
+    __shared__ __align__(16) float s_o[ATTN_WAVES][16][PITCH];
+    __shared__ float s_m[ATTN_WAVES][16], s_l[ATTN_WAVES][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, g = lane >> 4;
+    const int item = blockIdx.x, kv = blockIdx.y / p.tiles, tile = blockIdx.y - kv * p.tiles;
+    const int chunk = __builtin_amdgcn_readfirstlane(part_chunk(p));
+    int row, first_part, parts;
+    if (!find_part(p, chunk, item, row, first_part, parts)) return;  // every wave of the workgroup
+    const Row keys = row_keys(p, row);
+    const int len = __builtin_amdgcn_readfirstlane(keys.len), first = __builtin_amdgcn_readfirstlane(keys.first);
+    const int part = item - first_part;
+    const int each = __builtin_amdgcn_readfirstlane(((len - (first & ~15) + parts - 1) / parts + 31) & ~31);
+    const int begin = (first & ~15) + part * each, end = min(len, begin + each);
+    const int heads = p.kv_heads * p.group, head0 = kv * p.group + tile * 16, live = min(16, p.group - tile * 16);
+    if (blockIdx.y == 0 && threadIdx.x == 0 && part == 0) p.row_parts[row] = make_int2(first_part, parts);
+
+    uint4 q[X::STEPS];
+    const uint16_t* qrow = p.q + row * p.q_stride + int64_t(head0 + min(col, live - 1)) * D;
+#pragma unroll
+    for (int c = 0; c < X::STEPS; ++c) q[c] = *reinterpret_cast<const uint4*>(qrow + c * 32 + g * 8);
+
+    const int32_t* table = p.tables + int64_t(row) * p.width;
+    const int64_t head = kv * p.head_stride;
+    Running<TYPE, D> run;
+#pragma unroll
+    for (int b = 0; b < X::SLABS; ++b)
+#pragma unroll
+        for (int j = 0; j < X::CHUNK; ++j) run.o[b][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int pos = begin + 32 * wave; pos < end; pos += PART_KEYS) {
+        Tile<TYPE, D> t;
+        load_tile<TYPE, D, EVEN>(t, p, table, head, pos, first, end);
+        take_tile<TYPE, D>(run, t, q, p.scale);
+    }
+    run.l += xor_lane<16>(run.l);
+    run.l += xor_lane<32>(run.l);
+
+    // the four waves joined
+    if (lane < 16) s_m[wave][lane] = run.m;
+    __syncthreads();
+    float most = s_m[0][col];
+#pragma unroll
+    for (int w = 1; w < ATTN_WAVES; ++w) most = fmaxf(most, s_m[w][col]);
+    const float share = run.m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(run.m - most);
+    if (lane < 16) s_l[wave][lane] = run.l * share;
+#pragma unroll
+    for (int b = 0; b < X::SLABS; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < X::CHUNK; j += 4) {
+                const float4 v = make_float4(run.o[b][j][i] * share, run.o[b][j + 1][i] * share, run.o[b][j + 2][i] * share,
+                                             run.o[b][j + 3][i] * share);
+                *reinterpret_cast<float4*>(&s_o[wave][col][b * 128 + (4 * g + i) * X::CHUNK + j]) = v;
+            }
+    __syncthreads();
+    for (int e = threadIdx.x; e < live * (D / 4); e += ATTN_THREADS) {
+        const int h = e / (D / 4), d = (e - h * (D / 4)) * 4;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.f;
+#pragma unroll
+        for (int w = 0; w < ATTN_WAVES; ++w) {
+            const float4 v = *reinterpret_cast<const float4*>(&s_o[w][h][d]);
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+            l += s_l[w][h];
+        }
+        float m = s_m[0][h];
+#pragma unroll
+        for (int w = 1; w < ATTN_WAVES; ++w) m = fmaxf(m, s_m[w][h]);
+        if (parts == 1) {
+            // nothing visible: zeros
+            const float r = l == 0.f ? 0.f : 1.0f / l;
+            *reinterpret_cast<uint2*>(p.out + row * p.out_stride + int64_t(head0 + h) * D + d) =
+                make_uint2(pack16<TYPE>(sum.x * r, sum.y * r), pack16<TYPE>(sum.z * r, sum.w * r));
+            if (p.lse && d == 0)
+                p.lse[int64_t(row) * heads + head0 + h] =
+                    l == 0.f ? NEG_INF : (m - weight_shift<TYPE>() + log2f(l)) * 0.69314718055994531f;
+        } else {
+            const int64_t at = int64_t(item) * heads + head0 + h;
+            *reinterpret_cast<float4*>(p.part_o + at * D + d) = sum;
+            if (d == 0) p.part_ml[at] = make_float2(m, l);
+        }
+    }
+}
+
+// A head of a row from its parts, in a fixed order: D / 4 lanes hold the dims, the groups of lanes
+// take every GROUPS-th part.
+constexpr int MERGE_THREADS = 512;
+
+template <int TYPE, int D>
+__global__ __launch_bounds__(MERGE_THREADS) void paged_merge_kernel(PagedAttnParams p) {
+    constexpr int LANES = D / 4, GROUPS = MERGE_THREADS / LANES;
+    __shared__ __align__(16) float s_o[GROUPS][D];
+    __shared__ float s_m[MERGE_THREADS / 64], s_l[MERGE_THREADS / 64];
+    const int row = blockIdx.x, h = blockIdx.y, heads = p.kv_heads * p.group;
+    const int2 parts = p.row_parts[row];
+    if (parts.y == 1) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const float2* ml = p.part_ml + int64_t(parts.x) * heads + h;
+    float m = NEG_INF;
+    for (int i = tid; i < parts.y; i += MERGE_THREADS) m = fmaxf(m, ml[int64_t(i) * heads].x);
+    m = wave_max(m);
+    if (lane == 0) s_m[wave] = m;
+    __syncthreads();
+    for (int w = 0; w < MERGE_THREADS / 64; ++w) m = fmaxf(m, s_m[w]);
+    const float from = m == NEG_INF ? 0.f : m;
+    float l = 0.f;
+    for (int i = tid; i < parts.y; i += MERGE_THREADS) {
+        const float2 v = ml[int64_t(i) * heads];
+        l += v.y * __builtin_amdgcn_exp2f(v.x - from);
+    }
+    l = wave_sum(l);
+    if (lane == 0) s_l[wave] = l;
+    const int group = tid / LANES, d = (tid % LANES) * 4;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float* o = p.part_o + (int64_t(parts.x) * heads + h) * D + d;
+#pragma unroll 4
+    for (int i = group; i < parts.y; i += GROUPS) {
+        const float share = __builtin_amdgcn_exp2f(ml[int64_t(i) * heads].x - from);
+        const float4 v = *reinterpret_cast<const float4*>(o + int64_t(i) * heads * D);
+        sum.x += v.x * share, sum.y += v.y * share, sum.z += v.z * share, sum.w += v.w * share;
+    }
+    *reinterpret_cast<float4*>(&s_o[group][d]) = sum;
+    __syncthreads();
+    l = 0.f;
+    for (int w = 0; w < MERGE_THREADS / 64; ++w) l += s_l[w];
+    if (tid < LANES) {
+        sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < GROUPS; ++k) {
+            const float4 v = *reinterpret_cast<const float4*>(&s_o[k][d]);
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        }
+        const float r = l == 0.f ? 0.f : 1.0f / l;
+        *reinterpret_cast<uint2*>(p.out + row * p.out_stride + int64_t(h) * D + d) =
+            make_uint2(pack16<TYPE>(sum.x * r, sum.y * r), pack16<TYPE>(sum.z * r, sum.w * r));
+        if (p.lse && tid == 0)
+            p.lse[int64_t(row) * heads + h] = l == 0.f ? NEG_INF : (m - weight_shift<TYPE>() + log2f(l)) * 0.69314718055994531f;
+    }
+}
+
+template <int TYPE, int D>
+void run_attention(const PagedAttnParams& p, hipStream_t s) {
+    // parts: at most one more than its share of the aimed ones for each row, and none of less than PART_KEYS
+    const int64_t most = int64_t(p.rows) * std::max<int64_t>(1, (int64_t(p.most) + 15 + PART_KEYS - 1) / PART_KEYS);
+    const unsigned parts = unsigned(std::min<int64_t>(most, int64_t(p.rows) + p.target));
+    const dim3 grid(parts, unsigned(p.kv_heads * p.tiles));
+    if (p.page_size % 16 == 0)
+        hipLaunchKernelGGL((paged_attention_kernel<TYPE, D, true>), grid, dim3(ATTN_THREADS), 0, s, p);
+    else
+        hipLaunchKernelGGL((paged_attention_kernel<TYPE, D, false>), grid, dim3(ATTN_THREADS), 0, s, p);
+    if (int64_t(parts) > p.rows)  // else no row has two
+        hipLaunchKernelGGL((paged_merge_kernel<TYPE, D>), dim3(unsigned(p.rows), unsigned(p.kv_heads * p.group)),
+                           dim3(MERGE_THREADS), 0, s, p);
+}
+
+template <int SOURCE, int TYPE>
+void run_qkv(const PagedQkvParams& p, int head_dim, hipStream_t s) {
+    const int64_t threads = int64_t(p.tokens) * (p.heads + 2 * p.kv_heads) * (head_dim / 8);
+    const dim3 grid(unsigned((threads + 255) / 256));
+    if (head_dim == 64) hipLaunchKernelGGL((paged_qkv_kernel<SOURCE, TYPE, 64>), grid, dim3(256), 0, s, p);
+    else if (head_dim == 128) hipLaunchKernelGGL((paged_qkv_kernel<SOURCE, TYPE, 128>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((paged_qkv_kernel<SOURCE, TYPE, 256>), grid, dim3(256), 0, s, p);
+}
+
+}  // namespace
+
+void launch_paged_tables(const PagedTablesParams& p, hipStream_t s) {
+    hipLaunchKernelGGL((paged_tables_kernel<false>), dim3(1), dim3(TABLE_THREADS), 0, s, p);
+    if (p.capacity > 0)
+        hipLaunchKernelGGL(paged_slots_kernel, dim3(unsigned((p.capacity + 255) / 256)), dim3(256), 0, s, p);
+}
+
+void launch_paged_qkv(const PagedQkvParams& p, int source, int type, int head_dim, hipStream_t s) {
+    if (p.tokens == 0) return;
+    if (type == TYPE_BF16) {
+        if (source == TYPE_F32) run_qkv<TYPE_F32, TYPE_BF16>(p, head_dim, s);
+        else run_qkv<TYPE_BF16, TYPE_BF16>(p, head_dim, s);
+    } else {
+        if (source == TYPE_F32) run_qkv<TYPE_F32, TYPE_F16>(p, head_dim, s);
+        else run_qkv<TYPE_F16, TYPE_F16>(p, head_dim, s);
+    }
+}
+
+size_t paged_attn_workspace(int rows, int heads, int kv_heads, int head_dim) {
+    const size_t parts = size_t(rows) + size_t(attn_target(heads, kv_heads));
+    const size_t lists = (size_t(rows) * sizeof(int2) + 15) / 16 * 16 + (parts * size_t(heads) * sizeof(float2) + 15) / 16 * 16;
+    return lists + parts * size_t(heads) * size_t(head_dim) * sizeof(float);
+}
+
+void paged_attn_bind(PagedAttnParams& p, void* workspace, int head_dim) {
+    const int heads = p.kv_heads * p.group;
+    p.tiles = attn_tiles(heads, p.kv_heads);
+    p.target = attn_target(heads, p.kv_heads);
+    const size_t parts = size_t(p.rows) + size_t(p.target);
+    char* at = static_cast<char*>(workspace);
+    p.row_parts = reinterpret_cast<int2*>(at);
+    at += (size_t(p.rows) * sizeof(int2) + 15) / 16 * 16;
+    p.part_ml = reinterpret_cast<float2*>(at);
+    at += (parts * size_t(heads) * sizeof(float2) + 15) / 16 * 16;
+    p.part_o = reinterpret_cast<float*>(at);
+}
+
+void launch_paged_attention(const PagedAttnParams& p, int type, int head_dim, hipStream_t s) {
+    if (type == TYPE_BF16) {
+        if (head_dim == 64) run_attention<TYPE_BF16, 64>(p, s);
+        else if (head_dim == 128) run_attention<TYPE_BF16, 128>(p, s);
+        else run_attention<TYPE_BF16, 256>(p, s);
+    } else {
+        if (head_dim == 64) run_attention<TYPE_F16, 64>(p, s);
+        else if (head_dim == 128) run_attention<TYPE_F16, 128>(p, s);
+        else run_attention<TYPE_F16, 256>(p, s);
+    }
+}
+
+}  // namespace plamo

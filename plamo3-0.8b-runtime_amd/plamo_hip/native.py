@@ -36,6 +36,18 @@ class PackReport(ctypes.Structure):
                 ("blocks", ctypes.c_int64)]
 
 
+# value types of the paged and sampling kernels (PLAMO_BF16, PLAMO_F16, PLAMO_F32)
+TYPES = {"bf16": 0, "fp16": 1, "fp32": 2}
+
+
+class PagedCache(ctypes.Structure):
+    """plamo_paged_cache: one layer's pages, addresses and strides (in elements)."""
+    _fields_ = [("keys", ctypes.c_uint64), ("values", ctypes.c_uint64), ("page_stride", ctypes.c_int64),
+                ("slot_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("pages", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("type", ctypes.c_int32)]
+
+
 STEP_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, c_i32p, ctypes.c_int32, c_i32p)
 EMIT_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32)
 FINISH_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_int32, c_i32p, ctypes.c_int32, ctypes.c_int32)
@@ -124,6 +136,25 @@ _SIGNATURES = {
     "plamo_kernel_attention_decode_static": (ctypes.c_int, [ctypes.c_uint64] * 5 +
                                              [ctypes.c_int32, c_i32p, ctypes.c_int32, ctypes.c_int32] +
                                              [ctypes.c_uint64] * 4 + [ctypes.c_char_p, ctypes.c_size_t]),
+    "plamo_kernel_paged_tables": (ctypes.c_int, [ctypes.c_uint64] * 2 + [ctypes.c_int32, ctypes.c_uint64] +
+                                  [ctypes.c_int32] * 2 + [ctypes.c_uint64] * 2 + [ctypes.c_int32] +
+                                  [ctypes.c_uint64] * 5 + [ctypes.c_int32] + [ctypes.c_uint64] * 2 +
+                                  [ctypes.c_char_p, ctypes.c_size_t]),
+    "plamo_kernel_paged_qkv": (ctypes.c_int, [ctypes.POINTER(PagedCache), ctypes.c_uint64, ctypes.c_int32,
+                                              ctypes.c_int64, ctypes.c_int32] + [ctypes.c_uint64] * 3 +
+                               [ctypes.c_int32] + [ctypes.c_uint64] * 2 +
+                               [ctypes.c_int32, ctypes.c_uint64, ctypes.c_int64, ctypes.c_uint64, ctypes.c_char_p,
+                                ctypes.c_size_t]),
+    "plamo_kernel_attention_paged_workspace": (ctypes.c_int64, [ctypes.c_int32] * 4),
+    "plamo_kernel_attention_paged": (ctypes.c_int, [ctypes.POINTER(PagedCache), ctypes.c_uint64, ctypes.c_int64,
+                                                    ctypes.c_int32, ctypes.c_uint64, ctypes.c_int32, ctypes.c_uint64,
+                                                    ctypes.c_int32, ctypes.c_float, ctypes.c_int32, ctypes.c_uint64,
+                                                    ctypes.c_int64, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_int64,
+                                                    ctypes.c_uint64, ctypes.c_char_p, ctypes.c_size_t]),
+    "plamo_kernel_sample_workspace": (ctypes.c_int64, [ctypes.c_int32] * 2),
+    "plamo_kernel_sample": (ctypes.c_int, [ctypes.c_uint64, ctypes.c_int32, ctypes.c_int64] + [ctypes.c_int32] * 2 +
+                            [ctypes.c_uint64] * 8 + [ctypes.c_int64, ctypes.c_uint64, ctypes.c_char_p,
+                                                     ctypes.c_size_t]),
     "plamo_rope_table": (ctypes.c_int, [ctypes.POINTER(ctypes.c_double), ctypes.c_int32, ctypes.c_int32,
                                         ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t]),
     "plamo_version": (ctypes.c_char_p, []),
