@@ -6,11 +6,13 @@
 // keep a beginning of the order.  The token is the first one up to which more than u of the kept weight
 // lies.  Nothing is sorted but the few tokens around a border:
 //   1. the largest logit;
-//   2. a histogram of the weights over bins of the exponent (32 bins for a factor of two), counts and
-//      sums, from one pass over the row;
+//   2. a histogram over bins of the exponent (16 bins for a factor of two) in LDS: sums of the weights,
+//      or, for a top-k of at most 1024, numbers of tokens, for which no exponential is taken;
 //   3. prefix sums over the bins give the bin of each border; the tokens of that bin (or of all bins
 //      up to it) are gathered, sorted in LDS and searched.  A bin of more tokens than the list holds
 //      is divided again by the bits of the logits until it is small enough or one value.
+// Steps 1 and 2 are spread over segments of a row (a launch each), as one row's 107,520 logits are 40 us
+// of one CU's LDS atomics and FP64; the third is one workgroup's.
 // Weights are whole multiples of 2^-S of the largest (S = 63 - log2 of the vocabulary, at most 46), so
 // that all sums are exact whatever their order: the token depends on the row alone, not on how it was
 // split, and sums of unsigned 64-bit atomics are the same in every run.  A token of less than 2^-(S+1)
@@ -29,11 +31,13 @@ using namespace dev;
 
 namespace {
 
-constexpr int THREADS = 1024, WAVES = THREADS / 64;
+constexpr int THREADS = 1024, WAVES = THREADS / 64;  // of the workgroup that ends a row
+constexpr int PART_THREADS = 256;    // of a segment's workgroup
 constexpr int STEPS = 1024;          // table entries for a factor of two
-constexpr int BIN_SHIFT = 5;         // table steps of a bin
-constexpr int BINS = 1536;           // 32 (S + 1) <= 1504 are used
+constexpr int BIN_SHIFT = 6;         // log2 of a bin's table steps
+constexpr int BINS = 768;            // 16 (S + 1) <= 752 are used
 constexpr int LIST = 2048;           // tokens that are sorted at once
+constexpr int LIST_TOP_K = 1024;     // a top-k up to which its tokens' weights are summed in the list
 constexpr int SUB = 1024;            // parts that a bin is divided into again
 
 typedef unsigned long long u64;
@@ -58,9 +62,9 @@ struct Element<TYPE_F32> {
 };
 __device__ __forceinline__ float plain(float v) { return v == v ? v + 0.0f : NEG_INF; }
 
-// f(id, value) for a row's elements, a thread's in ascending order; 16 bytes a load behind the
-// first aligned element.
-template <int TYPE, typename F>
+// f(id, value) for n elements, a thread's in ascending order; 16 bytes a load behind the first
+// aligned element.
+template <int TYPE, int NT, typename F>
 __device__ __forceinline__ void for_row(const void* base, int n, F f) {
     typedef typename Element<TYPE>::T T;
     constexpr int PER = 16 / sizeof(T), AHEAD = 4;
@@ -70,15 +74,15 @@ __device__ __forceinline__ void for_row(const void* base, int n, F f) {
     if (tid < head) f(tid, plain(Element<TYPE>::value(row[tid])));
     const int vectors = (n - head) / PER;
     const uint4* body = reinterpret_cast<const uint4*>(row + head);
-    for (int i = tid; i < vectors; i += THREADS * AHEAD) {
+    for (int i = tid; i < vectors; i += NT * AHEAD) {
         uint4 w[AHEAD];
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a)
-            if (i + a * THREADS < vectors) w[a] = body[i + a * THREADS];
+            if (i + a * NT < vectors) w[a] = body[i + a * NT];
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) {
-            if (i + a * THREADS >= vectors) break;
-            const int id = head + (i + a * THREADS) * PER;
+            if (i + a * NT >= vectors) break;
+            const int id = head + (i + a * NT) * PER;
             const uint32_t words[4] = {w[a].x, w[a].y, w[a].z, w[a].w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -95,6 +99,40 @@ __device__ __forceinline__ void for_row(const void* base, int n, F f) {
     if (tail < n) f(tail, plain(Element<TYPE>::value(row[tail])));
 }
 
+// The largest of a workgroup's values and its lowest id, in every thread (id 0xffffffff: minus infinity).
+template <int NT>
+__device__ __forceinline__ void block_best(float& best, uint32_t& id, float* values, uint32_t* ids) {
+    for (int o = 32; o > 0; o >>= 1) {
+        const float v = __shfl_xor(best, o, 64);
+        const uint32_t i = __shfl_xor(id, o, 64);
+        if (v > best || (v == best && i < id)) {
+            best = v;
+            id = i;
+        }
+    }
+    if ((threadIdx.x & 63) == 0) {
+        values[threadIdx.x >> 6] = best;
+        ids[threadIdx.x >> 6] = id;
+    }
+    __syncthreads();
+    for (int w = 0; w < NT / 64; ++w)
+        if (values[w] > best || (values[w] == best && ids[w] < id)) {
+            best = values[w];
+            id = ids[w];
+        }
+}
+template <int TYPE, int NT>
+__device__ __forceinline__ void find_best(const void* base, int n, float& best, uint32_t& id) {
+    best = NEG_INF;
+    id = 0xffffffffu;
+    for_row<TYPE, NT>(base, n, [&](int i, float v) {
+        if (v > best) {
+            best = v;
+            id = uint32_t(i);
+        }
+    });
+}
+
 struct Sum {
     uint32_t count;
     u64 mass;
@@ -105,7 +143,7 @@ struct Shared {
     u64 bin_mass[BINS];    // then inclusive sums
     uint32_t bin_count[BINS];
     u64 order[LIST];       // descending logit, ascending id
-    u64 weight[LIST];      // then inclusive sums
+    u64 weight[LIST];      // inclusive sums of the list's weights
     Sum waves[WAVES];
     float wave_value[WAVES];
     uint32_t wave_id[WAVES];
@@ -114,8 +152,7 @@ struct Shared {
     uint32_t found_id;
     u64 found_weight;
     int found_bin;
-    uint32_t min_count;    // tokens of at least min_p
-    u64 min_mass;
+    u64 min_mass;          // of the tokens of at least min_p
 };
 
 // Inclusive sums over the workgroup.
@@ -150,6 +187,10 @@ __device__ __forceinline__ uint32_t sort_key(float v) {
     return u & 0x80000000u ? u : ~(u | 0x80000000u);
 }
 
+__device__ __forceinline__ float key_value(uint32_t key) {
+    return __uint_as_float(key & 0x80000000u ? key : ~key & 0x7fffffffu);
+}
+
 // A row's weights.
 struct Weights {
     float top;        // largest logit
@@ -157,21 +198,86 @@ struct Weights {
     double rate;      // STEPS log2(e) / T
     double limit;     // exponents from here on weigh nothing
     int scale;        // S
-    const double* table;
 
+    __device__ __forceinline__ void set(float best, float temperature, int n) {
+        scale = min(46, 31 + __clz(n));  // sums of n weights stay below 2^63
+        top = best;
+        infinite = best == -NEG_INF;
+        rate = STEPS * 1.44269504088896340736 / double(temperature);
+        limit = double((scale + 1) * STEPS) - 0.5;
+    }
     __device__ __forceinline__ bool exponent(float v, double& x) const {
         if (infinite) v = v == top ? 0.0f : NEG_INF;
         x = (double(infinite ? 0.0f : top) - double(v)) * rate;
         return x < limit;  // false for minus infinity
     }
     static __device__ __forceinline__ int steps(double x) { return int(__builtin_rint(x)); }
-    __device__ __forceinline__ u64 weight(double x, int n) const {
+    __device__ __forceinline__ u64 weight(const double* table, double x, int n) const {
         // 2^(-x / STEPS) = table[n % STEPS] 2^-(n / STEPS) exp(-f), |f| <= log(2) / (2 STEPS): the cubic
-        // is off by f^4 / 24 < 2^-50
+        // is off by f^4 / 24 < 2^-50.  Added to 2^52 a value below 2^47 is rounded to a whole number,
+        // which the low bits of the sum then hold.
         const double f = (x - double(n)) * (0.69314718055994530942 / STEPS);
         const double e = 1.0 - f * (1.0 - f * (0.5 - f * (1.0 / 6.0)));
-        return u64(__builtin_rint(ldexp(table[n & (STEPS - 1)] * e, scale - n / STEPS)));
+        const double w = ldexp(table[n & (STEPS - 1)] * e, scale - n / STEPS);
+        return u64(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
     }
+    __device__ __forceinline__ u64 weight_of(const double* table, float v) const {
+        double x;
+        return exponent(v, x) ? weight(table, x, steps(x)) : 0;
+    }
+};
+__device__ __forceinline__ double table_entry(int j) { return exp2(-double(j) / STEPS); }
+
+// A row's controls.
+struct Controls {
+    float temperature, top_p;
+    int top_k;
+    u64 least;        // smallest weight that min-p keeps; 0: off
+    bool counts, masses;  // which histograms the row needs
+
+    __device__ __forceinline__ Controls(const SampleParams& p, int r) {
+        temperature = p.temperature ? p.temperature[r] : 1.0f;
+        top_p = p.top_p ? p.top_p[r] : 1.0f;
+        top_k = p.top_k ? p.top_k[r] : 0;
+        const float min_p = p.min_p ? p.min_p[r] : 0.0f;
+        least = min_p > 0.0f ? u64(ceil(ldexp(double(fminf(min_p, 1.0f)), min(46, 31 + __clz(p.n))))) : 0;
+        counts = top_k > 0;
+        masses = !(top_k > 0 && top_k <= LIST_TOP_K);
+    }
+    __device__ __forceinline__ bool greedy() const { return !(temperature > 0.0f); }
+};
+
+// Histograms of n elements in LDS, and the sum of the weights of at least `least`.
+template <int TYPE, int NT>
+__device__ __forceinline__ u64 fill_bins(const void* base, int n, const Weights& w, const double* table, bool counts,
+                                         bool masses, u64 least, u64* bin_mass, uint32_t* bin_count) {
+    u64 kept = 0;
+    if (masses) {
+        for_row<TYPE, NT>(base, n, [&](int, float v) {
+            double x;
+            if (!w.exponent(v, x)) return;
+            const int step = Weights::steps(x);
+            const u64 weight = w.weight(table, x, step);
+            atomicAdd(&bin_mass[step >> BIN_SHIFT], weight);
+            if (counts) atomicAdd(&bin_count[step >> BIN_SHIFT], 1u);
+            if (weight >= least) kept += weight;
+        });
+    } else {
+        for_row<TYPE, NT>(base, n, [&](int, float v) {
+            double x;
+            if (w.exponent(v, x)) atomicAdd(&bin_count[Weights::steps(x) >> BIN_SHIFT], 1u);
+        });
+    }
+    return kept;
+}
+
+// A segment's results in the workspace.
+struct Segment {
+    u64 bin_mass[BINS];
+    u64 min_mass;
+    uint32_t bin_count[BINS];
+    float best;
+    uint32_t id;
 };
 
 enum Border { BORDER_COUNT, BORDER_MASS, BORDER_DRAW };
@@ -182,34 +288,57 @@ __device__ __forceinline__ bool reached(Sum upto, u64 target) {
     return KIND == BORDER_COUNT ? upto.count >= target : KIND == BORDER_MASS ? upto.mass >= target : upto.mass > target;
 }
 
-// The tokens of the list (s.listed of them, padded to LIST) in order, with inclusive sums of weights.
-__device__ void sort_list(Shared& s) {
-    const int tid = threadIdx.x;
-    const uint32_t count = s.listed;
-    uint32_t size = 2;
+template <int O>
+__device__ __forceinline__ void exchange(u64& x, uint32_t i, uint32_t k) {
+    const u64 y = u64(xor_lane<O>(uint32_t(x >> 32))) << 32 | xor_lane<O>(uint32_t(x));
+    // the lower place of an ascending run keeps the smaller one
+    const bool smaller = ((i & k) == 0) == ((i & O) == 0);
+    x = (y < x) == smaller ? y : x;
+}
+
+// The list's tokens (s.listed of them) in order, bitonic: strides of a wave and more through LDS, shorter
+// ones between lanes.  Then inclusive sums of the weights.
+__device__ void sort_list(Shared& s, const Weights& w) {
+    const uint32_t tid = threadIdx.x, count = s.listed;
+    uint32_t size = 64;
     while (size < count) size <<= 1;
-    for (uint32_t i = count + tid; i < size; i += THREADS) {
-        s.order[i] = ~u64(0);
-        s.weight[i] = 0;
+    for (uint32_t i = count + tid; i < size; i += THREADS) s.order[i] = ~u64(0);
+    __syncthreads();
+    for (uint32_t i = tid; i < size; i += THREADS) {
+        u64 x = s.order[i];
+        exchange<1>(x, i, 2);
+        exchange<2>(x, i, 4), exchange<1>(x, i, 4);
+        exchange<4>(x, i, 8), exchange<2>(x, i, 8), exchange<1>(x, i, 8);
+        exchange<8>(x, i, 16), exchange<4>(x, i, 16), exchange<2>(x, i, 16), exchange<1>(x, i, 16);
+        exchange<16>(x, i, 32), exchange<8>(x, i, 32), exchange<4>(x, i, 32), exchange<2>(x, i, 32), exchange<1>(x, i, 32);
+        exchange<32>(x, i, 64), exchange<16>(x, i, 64), exchange<8>(x, i, 64), exchange<4>(x, i, 64);
+        exchange<2>(x, i, 64), exchange<1>(x, i, 64);
+        s.order[i] = x;
     }
     __syncthreads();
-    for (uint32_t k = 2; k <= size; k <<= 1)
-        for (uint32_t j = k >> 1; j > 0; j >>= 1) {
+    for (uint32_t k = 128; k <= size; k <<= 1) {
+        for (uint32_t j = k >> 1; j >= 64; j >>= 1) {
             for (uint32_t t = tid; t < size / 2; t += THREADS) {
-                const uint32_t a = (t / j) * 2 * j + t % j, b = a + j;
+                const uint32_t a = (t & ~(j - 1)) * 2 + (t & (j - 1)), b = a + j;
                 const u64 x = s.order[a], y = s.order[b];
                 if ((x > y) == ((a & k) == 0)) {
                     s.order[a] = y;
                     s.order[b] = x;
-                    const u64 w = s.weight[a];
-                    s.weight[a] = s.weight[b];
-                    s.weight[b] = w;
                 }
             }
             __syncthreads();
         }
+        for (uint32_t i = tid; i < size; i += THREADS) {
+            u64 x = s.order[i];
+            exchange<32>(x, i, k), exchange<16>(x, i, k), exchange<8>(x, i, k);
+            exchange<4>(x, i, k), exchange<2>(x, i, k), exchange<1>(x, i, k);
+            s.order[i] = x;
+        }
+        __syncthreads();
+    }
     const uint32_t i = 2 * tid;
-    const u64 w0 = i < size ? s.weight[i] : 0, w1 = i < size ? s.weight[i + 1] : 0;
+    const u64 w0 = i < count ? w.weight_of(s.table, key_value(uint32_t(s.order[i] >> 32))) : 0;
+    const u64 w1 = i + 1 < count ? w.weight_of(s.table, key_value(uint32_t(s.order[i + 1] >> 32))) : 0;
     Sum total;
     const Sum incl = block_scan({0, w0 + w1}, s.waves, total);
     if (i < size) {
@@ -242,24 +371,37 @@ struct Row {
     Weights w;
 };
 
+// The tokens with a value from `low` to `high` for which `inside` says so; sorted if the list holds them.
 template <int TYPE, typename P>
-__device__ void gather(Shared& s, const Row<TYPE>& row, P inside) {
+__device__ void gather(Shared& s, const Row<TYPE>& row, float low, float high, P inside) {
     __syncthreads();
     if (threadIdx.x == 0) s.listed = 0;
     __syncthreads();
-    for_row<TYPE>(row.base, row.n, [&](int id, float v) {
-        double x;
-        if (!row.w.exponent(v, x)) return;
-        const int n = Weights::steps(x);
-        if (!inside(n, v)) return;
+    for_row<TYPE, THREADS>(row.base, row.n, [&](int id, float v) {
+        if (v < low || v > high || !inside(v)) return;
         const uint32_t at = atomicAdd(&s.listed, 1u);
-        if (at < LIST) {
-            s.order[at] = u64(sort_key(v)) << 32 | uint32_t(id);
-            s.weight[at] = row.w.weight(x, n);
-        }
+        if (at < LIST) s.order[at] = u64(sort_key(v)) << 32 | uint32_t(id);
     });
     __syncthreads();
-    sort_list(s);
+    if (s.listed <= LIST) sort_list(s, row.w);
+}
+
+// The tokens of bins first .. last.
+template <int TYPE>
+__device__ void gather_bins(Shared& s, const Row<TYPE>& row, int first, int last) {
+    // values that may lie there, by a table step more at each end
+    float low = NEG_INF, high = -NEG_INF;
+    if (!row.w.infinite) {
+        low = __double2float_rd(double(row.w.top) - double(((last + 1) << BIN_SHIFT) + 1) / row.w.rate);
+        high = __double2float_ru(double(row.w.top) - double((first << BIN_SHIFT) - 1) / row.w.rate);
+    }
+    const Weights w = row.w;
+    gather(s, row, low, high, [=](float v) {
+        double x;
+        if (!w.exponent(v, x)) return false;
+        const int bin = Weights::steps(x) >> BIN_SHIFT;
+        return bin >= first && bin <= last;
+    });
 }
 
 // The token that is the `index`-th, by id, of those of one logit (`key`).
@@ -306,7 +448,7 @@ __device__ void divide_bin(Shared& s, const Row<TYPE>& row, int bin, Sum base, u
     }
     __syncthreads();
     uint32_t low = 0xffffffffu, high = 0;
-    for_row<TYPE>(row.base, row.n, [&](int, float v) {
+    for_row<TYPE, THREADS>(row.base, row.n, [&](int, float v) {
         double x;
         if (!row.w.exponent(v, x) || Weights::steps(x) >> BIN_SHIFT != bin) return;
         low = min(low, sort_key(v));
@@ -320,10 +462,7 @@ __device__ void divide_bin(Shared& s, const Row<TYPE>& row, int bin, Sum base, u
     while (true) {
         if (low == high) {
             // one logit: every token has the same weight
-            double x;
-            const uint32_t bits = low & 0x80000000u ? low : ~low & 0x7fffffffu;
-            row.w.exponent(__uint_as_float(bits), x);
-            const u64 w = row.w.weight(x, Weights::steps(x));
+            const u64 w = row.w.weight_of(s.table, key_value(low));
             u64 index;
             if (KIND == BORDER_COUNT) index = target - base.count - 1;
             else if (KIND == BORDER_MASS) index = (target - base.mass + w - 1) / w - 1;
@@ -344,13 +483,11 @@ __device__ void divide_bin(Shared& s, const Row<TYPE>& row, int bin, Sum base, u
             count[i] = 0;
         }
         __syncthreads();
-        for_row<TYPE>(row.base, row.n, [&](int, float v) {
+        for_row<TYPE, THREADS>(row.base, row.n, [&](int, float v) {
             const uint32_t key = sort_key(v);
             if (key < low || key > high) return;
-            double x;
-            if (!row.w.exponent(v, x)) return;
             atomicAdd(&count[(key - low) >> shift], 1u);
-            atomicAdd(&mass[(key - low) >> shift], row.w.weight(x, Weights::steps(x)));
+            atomicAdd(&mass[(key - low) >> shift], row.w.weight_of(s.table, v));
         });
         __syncthreads();
         static_assert(SUB == THREADS, "one part for each thread");
@@ -371,8 +508,7 @@ __device__ void divide_bin(Shared& s, const Row<TYPE>& row, int bin, Sum base, u
         low += part << shift;
         __syncthreads();
         if (held <= LIST) {
-            const uint32_t from = low, to = high;
-            gather(s, row, [=](int, float v) { return sort_key(v) >= from && sort_key(v) <= to; });
+            gather(s, row, key_value(high), key_value(low), [](float) { return true; });
             search_list<KIND>(s, base, target);
             return;
         }
@@ -380,15 +516,20 @@ __device__ void divide_bin(Shared& s, const Row<TYPE>& row, int bin, Sum base, u
     }
 }
 
-// The bins whose tokens are in the list; none: first > last.
+// The bins whose tokens are in the list; none: first > last.  `whole`: all tokens that may be kept are.
 struct Listed {
     int first, last;
+    bool whole;
 };
 
 // Finds a border by the bins' sums; the result is in s.found, s.found_id and s.found_weight.
 template <Border KIND, int TYPE>
 __device__ void find_border(Shared& s, const Row<TYPE>& row, Listed& list, u64 target) {
     __syncthreads();
+    if (list.whole) {
+        search_list<KIND>(s, {0, 0}, target);
+        return;
+    }
     for (int b = threadIdx.x; b < BINS; b += THREADS) {
         const Sum upto = {s.bin_count[b], s.bin_mass[b]};
         const Sum before = {b ? s.bin_count[b - 1] : 0, b ? s.bin_mass[b - 1] : 0};
@@ -397,38 +538,81 @@ __device__ void find_border(Shared& s, const Row<TYPE>& row, Listed& list, u64 t
     __syncthreads();
     const int bin = s.found_bin;
     __syncthreads();
+    auto before = [&](int b) -> Sum { return {b ? s.bin_count[b - 1] : 0, b ? s.bin_mass[b - 1] : 0}; };
     if (bin < list.first || bin > list.last) {
         // all tokens up to the bin if they fit, so that further borders need no pass; else the bin's
-        const int first = s.bin_count[bin] <= uint32_t(LIST) ? 0 : bin;
-        const Sum base = {first ? s.bin_count[first - 1] : 0, first ? s.bin_mass[first - 1] : 0};
-        if (s.bin_count[bin] - base.count > uint32_t(LIST)) {
-            divide_bin<KIND>(s, row, bin, base, target);
-            list = {1, 0};
+        list = {s.bin_count[bin] <= uint32_t(LIST) ? 0 : bin, bin, false};
+        gather_bins(s, row, list.first, bin);
+        if (s.listed > uint32_t(LIST) && list.first < bin) {  // the numbers of tokens were estimates
+            list.first = bin;
+            gather_bins(s, row, bin, bin);
+        }
+        if (s.listed > uint32_t(LIST)) {
+            divide_bin<KIND>(s, row, bin, before(bin), target);
+            list = {1, 0, false};
             return;
         }
-        gather(s, row, [=](int n, float) { return n >> BIN_SHIFT >= first && n >> BIN_SHIFT <= bin; });
-        list = {first, bin};
     }
-    const Sum base = {list.first ? s.bin_count[list.first - 1] : 0, list.first ? s.bin_mass[list.first - 1] : 0};
-    search_list<KIND>(s, base, target);
+    search_list<KIND>(s, before(list.first), target);
+}
+
+// Inclusive sums of the histograms -> all tokens' count and mass.  Where tokens were not counted, their
+// number in a bin is estimated by the bin's smallest weight.
+__device__ Sum sum_bins(Shared& s, const Weights& w, bool counts, bool masses) {
+    __syncthreads();
+    const int b = threadIdx.x;
+    static_assert(BINS <= THREADS, "one bin for each thread");
+    Sum own = {0, 0}, total;
+    if (b < BINS) {
+        own = {counts ? s.bin_count[b] : 0, masses ? s.bin_mass[b] : 0};
+        if (!counts && own.mass) {
+            const int step = ((b + 1) << BIN_SHIFT) - 1;
+            const u64 least = w.weight(s.table, double(step), step);
+            own.count = uint32_t(least ? min(own.mass / least + 1, u64(1) << 21) : u64(1) << 21);
+        }
+    }
+    const Sum incl = block_scan(own, s.waves, total);
+    if (b < BINS) {
+        s.bin_count[b] = incl.count;
+        s.bin_mass[b] = incl.mass;
+    }
+    __syncthreads();
+    return total;
 }
 
 template <int TYPE>
-__global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
-    __shared__ Shared s;
-    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    Row<TYPE> row;
-    row.base = static_cast<const typename Element<TYPE>::T*>(p.logits) + r * p.stride;
-    row.n = p.n;
-    // the largest logit and its first token
-    float best = NEG_INF;
-    uint32_t id = 0xffffffffu;
-    for_row<TYPE>(row.base, p.n, [&](int i, float v) {
-        if (v > best) {
-            best = v;
-            id = uint32_t(i);
+__device__ __forceinline__ const void* row_base(const SampleParams& p, int r) {
+    return static_cast<const typename Element<TYPE>::T*>(p.logits) + r * p.stride;
+}
+
+// The largest logit of a segment.
+template <int TYPE>
+__global__ __launch_bounds__(PART_THREADS) void sample_best_kernel(SampleParams p, int each) {
+    __shared__ float s_values[PART_THREADS / 64];
+    __shared__ uint32_t s_ids[PART_THREADS / 64];
+    const int begin = blockIdx.x * each, n = min(each, p.n - begin);
+    float best;
+    uint32_t id;
+    find_best<TYPE, PART_THREADS>(static_cast<const typename Element<TYPE>::T*>(row_base<TYPE>(p, blockIdx.y)) + begin, n,
+                                  best, id);
+    block_best<PART_THREADS>(best, id, s_values, s_ids);
+    if (threadIdx.x == 0) {
+        Segment& out = static_cast<Segment*>(p.workspace)[int64_t(blockIdx.y) * gridDim.x + blockIdx.x];
+        out.best = best;
+        out.id = id == 0xffffffffu ? id : id + uint32_t(begin);
+    }
+}
+
+// The row's largest logit from its segments', in every thread (a wave's lanes take a segment each).
+__device__ __forceinline__ void segments_best(const Segment* segments, int count, float& best, uint32_t& id) {
+    best = NEG_INF;
+    id = 0xffffffffu;
+    for (int i = threadIdx.x & 63; i < count; i += 64) {
+        if (segments[i].best > best) {
+            best = segments[i].best;
+            id = segments[i].id;
         }
-    });
+    }
     for (int o = 32; o > 0; o >>= 1) {
         const float v = __shfl_xor(best, o, 64);
         const uint32_t i = __shfl_xor(id, o, 64);
@@ -437,89 +621,145 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
             id = i;
         }
     }
-    if (lane == 0) {
-        s.wave_value[wave] = best;
-        s.wave_id[wave] = id;
+}
+
+// A segment's histograms.
+template <int TYPE>
+__global__ __launch_bounds__(PART_THREADS) void sample_bins_kernel(SampleParams p, int each) {
+    __shared__ double s_table[STEPS];
+    __shared__ u64 s_mass[BINS];
+    __shared__ uint32_t s_count[BINS];
+    __shared__ u64 s_kept;
+    const int r = blockIdx.y, tid = threadIdx.x;
+    Segment* segments = static_cast<Segment*>(p.workspace) + int64_t(r) * gridDim.x;
+    const Controls c(p, r);
+    if (c.greedy()) return;
+    for (int i = tid; i < STEPS; i += PART_THREADS) s_table[i] = table_entry(i);
+    for (int i = tid; i < BINS; i += PART_THREADS) {
+        s_mass[i] = 0;
+        s_count[i] = 0;
     }
-    for (int b = tid; b < BINS; b += THREADS) {
-        s.bin_mass[b] = 0;
-        s.bin_count[b] = 0;
-    }
-    if (tid == 0) {
-        s.min_count = 0;
-        s.min_mass = 0;
-    }
-    static_assert(STEPS == THREADS, "one entry for each thread");
-    s.table[tid] = exp2(-double(tid) / STEPS);
+    if (tid == 0) s_kept = 0;
+    float best;
+    uint32_t id;
+    segments_best(segments, gridDim.x, best, id);
+    if (id == 0xffffffffu) return;
+    Weights w;
+    w.set(best, c.temperature, p.n);
     __syncthreads();
-    for (int w = 0; w < WAVES; ++w)
-        if (s.wave_value[w] > best || (s.wave_value[w] == best && s.wave_id[w] < id)) {
-            best = s.wave_value[w];
-            id = s.wave_id[w];
-        }
-    const float temperature = p.temperature ? p.temperature[r] : 1.0f;
-    if (id == 0xffffffffu || !(temperature > 0.0f)) {
+    const int begin = blockIdx.x * each, n = min(each, p.n - begin);
+    const u64 kept = fill_bins<TYPE, PART_THREADS>(
+        static_cast<const typename Element<TYPE>::T*>(row_base<TYPE>(p, r)) + begin, n, w, s_table, c.counts, c.masses,
+        c.least, s_mass, s_count);
+    if (c.least && kept) atomicAdd(&s_kept, kept);
+    __syncthreads();
+    Segment& out = segments[blockIdx.x];
+    for (int i = tid; i < BINS; i += PART_THREADS) {
+        if (c.masses) out.bin_mass[i] = s_mass[i];
+        if (c.counts) out.bin_count[i] = s_count[i];
+    }
+    if (tid == 0) out.min_mass = s_kept;
+}
+
+// SEGMENTS: the first two steps are done, in `segments` parts; else they are this workgroup's too.
+template <int TYPE, bool SEGMENTS>
+__global__ __launch_bounds__(THREADS) void sample_pick_kernel(SampleParams p, int segments) {
+    __shared__ Shared s;
+    const int r = blockIdx.x, tid = threadIdx.x;
+    Row<TYPE> row;
+    row.base = row_base<TYPE>(p, r);
+    row.n = p.n;
+    const Controls c(p, r);
+    const Segment* parts = static_cast<const Segment*>(p.workspace) + int64_t(r) * segments;
+    float best;
+    uint32_t id;
+    if constexpr (SEGMENTS) {
+        segments_best(parts, segments, best, id);
+    } else {
+        find_best<TYPE, THREADS>(row.base, p.n, best, id);
+        block_best<THREADS>(best, id, s.wave_value, s.wave_id);
+    }
+    if (id == 0xffffffffu || c.greedy()) {
         if (tid == 0) {
             p.token[r] = int32_t(id);  // -1 where nothing can be drawn
             if (p.prob) p.prob[r] = id == 0xffffffffu ? 0.0f : 1.0f;
         }
         return;
     }
-    const int scale = min(46, 31 + __clz(p.n));  // sums of n weights stay below 2^63
-    row.w.top = best;
-    row.w.infinite = best == -NEG_INF;
-    row.w.rate = STEPS * 1.44269504088896340736 / double(temperature);
-    row.w.limit = double((scale + 1) * STEPS) - 0.5;
-    row.w.scale = scale;
-    row.w.table = s.table;
-
-    const float min_p = p.min_p ? p.min_p[r] : 0.0f, top_p = p.top_p ? p.top_p[r] : 1.0f;
-    const int top_k = p.top_k ? p.top_k[r] : 0;
-    const u64 least = min_p > 0.0f ? u64(ceil(ldexp(double(fminf(min_p, 1.0f)), scale))) : 0;
-    uint32_t min_count = 0;
-    u64 min_mass = 0;
-    for_row<TYPE>(row.base, p.n, [&](int, float v) {
-        double x;
-        if (!row.w.exponent(v, x)) return;
-        const int n = Weights::steps(x);
-        const u64 w = row.w.weight(x, n);
-        atomicAdd(&s.bin_mass[n >> BIN_SHIFT], w);
-        atomicAdd(&s.bin_count[n >> BIN_SHIFT], 1u);
-        if (w >= least) {
-            ++min_count;
-            min_mass += w;
+    row.w.set(best, c.temperature, p.n);
+    static_assert(STEPS == THREADS, "one entry for each thread");
+    s.table[tid] = table_entry(tid);
+    if (tid == 0) s.min_mass = 0;
+    auto fill = [&](bool counts, bool masses) {
+        for (int b = tid; b < BINS; b += THREADS) {
+            s.bin_mass[b] = 0;
+            s.bin_count[b] = 0;
         }
-    });
-    if (least) {
-        atomicAdd(&s.min_count, min_count);
-        atomicAdd(&s.min_mass, min_mass);
+        __syncthreads();
+        const u64 kept = fill_bins<TYPE, THREADS>(row.base, p.n, row.w, s.table, counts, masses, c.least, s.bin_mass, s.bin_count);
+        if (c.least && kept) atomicAdd(&s.min_mass, kept);
+    };
+    if constexpr (SEGMENTS) {
+        if (tid < BINS) {
+            u64 mass = 0;
+            uint32_t count = 0;
+            if (c.masses) {
+#pragma unroll 4
+                for (int i = 0; i < segments; ++i) mass += parts[i].bin_mass[tid];
+            }
+            if (c.counts) {
+#pragma unroll 4
+                for (int i = 0; i < segments; ++i) count += parts[i].bin_count[tid];
+            }
+            s.bin_mass[tid] = mass;
+            s.bin_count[tid] = count;
+        }
+        __syncthreads();
+        if (c.masses && c.least && tid < segments) atomicAdd(&s.min_mass, parts[tid].min_mass);
+    } else {
+        fill(c.counts, c.masses);
     }
-    __syncthreads();
-    Sum kept;
-    {
-        const int b = 2 * tid;
-        const bool own = b < BINS;
-        const Sum first = {own ? s.bin_count[b] : 0, own ? s.bin_mass[b] : 0};
-        const Sum second = {own ? s.bin_count[b + 1] : 0, own ? s.bin_mass[b + 1] : 0};
-        const Sum incl = block_scan({first.count + second.count, first.mass + second.mass}, s.waves, kept);
-        if (own) {
-            s.bin_count[b] = incl.count - second.count;
-            s.bin_mass[b] = incl.mass - second.mass;
-            s.bin_count[b + 1] = incl.count;
-            s.bin_mass[b + 1] = incl.mass;
+    Sum kept = sum_bins(s, row.w, c.counts, c.masses);
+    Listed list = {1, 0, false};
+    if (!c.masses) {
+        // the top-k's tokens, and what shares the last one's bin
+        int last = BINS - 1;
+        if (uint32_t(c.top_k) < kept.count) {
+            if (tid < BINS && s.bin_count[tid] >= uint32_t(c.top_k) && (tid == 0 || s.bin_count[tid - 1] < uint32_t(c.top_k)))
+                s.found_bin = tid;
+            __syncthreads();
+            last = s.found_bin;
+        }
+        gather_bins(s, row, 0, last);
+        if (s.listed <= uint32_t(LIST)) {
+            list.whole = true;
+            kept = {s.listed, s.weight[s.listed - 1]};
+        } else {
+            // too many share it: weights of all tokens after all
+            fill(true, true);
+            kept = sum_bins(s, row.w, true, true);
         }
     }
-    Listed list = {1, 0};
-    if (top_k > 0 && uint32_t(top_k) < kept.count) {
-        find_border<BORDER_COUNT>(s, row, list, u64(top_k));
+    if (c.top_k > 0 && uint32_t(c.top_k) < kept.count) {
+        find_border<BORDER_COUNT>(s, row, list, u64(c.top_k));
         kept = s.found;
     }
-    if (top_p < 1.0f) {
-        const double target = ceil(double(top_p) * double(kept.mass));
+    if (c.top_p < 1.0f) {
+        const double target = ceil(double(c.top_p) * double(kept.mass));
         find_border<BORDER_MASS>(s, row, list, target > 1.0 ? u64(target) : u64(1));
         kept = s.found;
     }
-    if (least && s.min_count < kept.count) kept = {s.min_count, s.min_mass};
+    if (c.least) {
+        if (list.whole) {
+            __syncthreads();
+            for (uint32_t i = tid; i < s.listed; i += THREADS) {
+                const u64 own = s.weight[i] - (i ? s.weight[i - 1] : 0);
+                if (own >= c.least && (i + 1 == s.listed || s.weight[i + 1] - s.weight[i] < c.least)) s.min_mass = s.weight[i];
+            }
+            __syncthreads();
+        }
+        kept.mass = min(kept.mass, s.min_mass);  // both are beginnings of one order
+    }
     const float u = p.uniform[r];
     const u64 at = u > 0.0f ? u64(double(fminf(u, 1.0f)) * double(kept.mass)) : 0;
     find_border<BORDER_DRAW>(s, row, list, at < kept.mass ? at : kept.mass - 1);
@@ -529,15 +769,37 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     }
 }
 
+// Segments of a row: of 4,096 logits at least, and some 2,048 in all, which fill the CUs several times;
+// 1: a workgroup does the whole row.
+int row_segments(int rows, int n) { return std::max(1, std::min((n + 4095) / 4096, 2048 / rows)); }
+constexpr int FEWEST_SEGMENTS = 3;
+
+template <int TYPE>
+void run_sample(const SampleParams& p, hipStream_t s) {
+    int segments = row_segments(p.rows, p.n);
+    if (segments < FEWEST_SEGMENTS) {
+        hipLaunchKernelGGL((sample_pick_kernel<TYPE, false>), dim3(unsigned(p.rows)), dim3(THREADS), 0, s, p, 0);
+        return;
+    }
+    const int each = (p.n + segments * 64 - 1) / (segments * 64) * 64;
+    segments = (p.n + each - 1) / each;
+    const dim3 grid(unsigned(segments), unsigned(p.rows));
+    hipLaunchKernelGGL((sample_best_kernel<TYPE>), grid, dim3(PART_THREADS), 0, s, p, each);
+    hipLaunchKernelGGL((sample_bins_kernel<TYPE>), grid, dim3(PART_THREADS), 0, s, p, each);
+    hipLaunchKernelGGL((sample_pick_kernel<TYPE, true>), dim3(unsigned(p.rows)), dim3(THREADS), 0, s, p, segments);
+}
+
 }  // namespace
 
-size_t sample_workspace(int, int) { return 0; }
+size_t sample_workspace(int rows, int n) {
+    const int segments = row_segments(rows, n);
+    return segments < FEWEST_SEGMENTS ? 0 : size_t(rows) * size_t(segments) * sizeof(Segment);
+}
 
 void launch_sample(const SampleParams& p, int type, hipStream_t s) {
-    const dim3 grid{unsigned(p.rows)};
-    if (type == TYPE_BF16) hipLaunchKernelGGL((sample_kernel<TYPE_BF16>), grid, dim3(THREADS), 0, s, p);
-    else if (type == TYPE_F16) hipLaunchKernelGGL((sample_kernel<TYPE_F16>), grid, dim3(THREADS), 0, s, p);
-    else hipLaunchKernelGGL((sample_kernel<TYPE_F32>), grid, dim3(THREADS), 0, s, p);
+    if (type == TYPE_BF16) run_sample<TYPE_BF16>(p, s);
+    else if (type == TYPE_F16) run_sample<TYPE_F16>(p, s);
+    else run_sample<TYPE_F32>(p, s);
 }
 
 }  // namespace plamo
