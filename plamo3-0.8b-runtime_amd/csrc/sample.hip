@@ -33,8 +33,8 @@ namespace {
 
 constexpr int THREADS = 1024, WAVES = THREADS / 64;  // of the workgroup that ends a row
 constexpr int PART_THREADS = 256;    // of a segment's workgroup
-constexpr int STEPS = 1024;          // table entries for a factor of two
-constexpr int BIN_SHIFT = 6;         // log2 of a bin's table steps
+constexpr int STEPS = 256;           // table entries for a factor of two
+constexpr int BIN_SHIFT = 4;         // log2 of a bin's table steps
 constexpr int BINS = 768;            // 16 (S + 1) <= 752 are used
 constexpr int LIST = 2048;           // tokens that are sorted at once
 constexpr int LIST_TOP_K = 1024;     // a top-k up to which its tokens' weights are summed in the list
@@ -42,7 +42,7 @@ constexpr int SUB = 1024;            // parts that a bin is divided into again
 
 typedef unsigned long long u64;
 
-// Row values: NaN counts as minus infinity; minus zero equals zero.
+// Row values as they stand: NaN fails every comparison, as minus infinity does, and minus zero equals zero.
 template <int TYPE>
 struct Element;
 template <>
@@ -60,18 +60,17 @@ struct Element<TYPE_F32> {
     typedef uint32_t T;
     static __device__ __forceinline__ float value(uint32_t w) { return __uint_as_float(w); }
 };
-__device__ __forceinline__ float plain(float v) { return v == v ? v + 0.0f : NEG_INF; }
 
 // f(id, value) for n elements, a thread's in ascending order; 16 bytes a load behind the first
-// aligned element.
-template <int TYPE, int NT, typename F>
+// aligned element, AHEAD loads at once.
+template <int TYPE, int NT, int AHEAD = 4, typename F>
 __device__ __forceinline__ void for_row(const void* base, int n, F f) {
     typedef typename Element<TYPE>::T T;
-    constexpr int PER = 16 / sizeof(T), AHEAD = 4;
+    constexpr int PER = 16 / sizeof(T);
     const T* row = static_cast<const T*>(base);
     const int tid = threadIdx.x;
     const int head = min(n, int(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T)));
-    if (tid < head) f(tid, plain(Element<TYPE>::value(row[tid])));
+    if (tid < head) f(tid, Element<TYPE>::value(row[tid]));
     const int vectors = (n - head) / PER;
     const uint4* body = reinterpret_cast<const uint4*>(row + head);
     for (int i = tid; i < vectors; i += NT * AHEAD) {
@@ -87,16 +86,16 @@ __device__ __forceinline__ void for_row(const void* base, int n, F f) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if constexpr (PER == 4) {
-                    f(id + j, plain(Element<TYPE>::value(words[j])));
+                    f(id + j, Element<TYPE>::value(words[j]));
                 } else {
-                    f(id + 2 * j, plain(Element<TYPE>::value(words[j])));
-                    f(id + 2 * j + 1, plain(Element<TYPE>::value(words[j] >> 16)));
+                    f(id + 2 * j, Element<TYPE>::value(words[j]));
+                    f(id + 2 * j + 1, Element<TYPE>::value(words[j] >> 16));
                 }
             }
         }
     }
     const int tail = head + vectors * PER + tid;
-    if (tail < n) f(tail, plain(Element<TYPE>::value(row[tail])));
+    if (tail < n) f(tail, Element<TYPE>::value(row[tail]));
 }
 
 // The largest of a workgroup's values and its lowest id, in every thread (id 0xffffffff: minus infinity).
@@ -121,16 +120,22 @@ __device__ __forceinline__ void block_best(float& best, uint32_t& id, float* val
             id = ids[w];
         }
 }
+// The id is looked for where it is asked for: else it is 0, or 0xffffffff for minus infinity.
 template <int TYPE, int NT>
-__device__ __forceinline__ void find_best(const void* base, int n, float& best, uint32_t& id) {
+__device__ __forceinline__ void find_best(const void* base, int n, bool ids, float& best, uint32_t& id) {
     best = NEG_INF;
     id = 0xffffffffu;
-    for_row<TYPE, NT>(base, n, [&](int i, float v) {
-        if (v > best) {
-            best = v;
-            id = uint32_t(i);
-        }
-    });
+    if (ids) {
+        for_row<TYPE, NT>(base, n, [&](int i, float v) {
+            if (v > best) {
+                best = v;
+                id = uint32_t(i);
+            }
+        });
+    } else {
+        for_row<TYPE, NT, 8>(base, n, [&](int, float v) { best = v > best ? v : best; });  // a maximum of a signalling NaN is NaN
+        if (best > NEG_INF) id = 0;
+    }
 }
 
 struct Sum {
@@ -140,14 +145,14 @@ struct Sum {
 
 struct Shared {
     double table[STEPS];   // 2^(-j / STEPS)
-    u64 bin_mass[BINS];    // then inclusive sums
+    u64 bin_mass[2 * BINS];  // then inclusive sums in the first half
     uint32_t bin_count[BINS];
     u64 order[LIST];       // descending logit, ascending id
     u64 weight[LIST];      // inclusive sums of the list's weights
     Sum waves[WAVES];
     float wave_value[WAVES];
     uint32_t wave_id[WAVES];
-    uint32_t low, high, listed;
+    uint32_t low, high, listed, split;
     Sum found;             // a border's count and mass up to and with its token
     uint32_t found_id;
     u64 found_weight;
@@ -155,35 +160,48 @@ struct Shared {
     u64 min_mass;          // of the tokens of at least min_p
 };
 
-// Inclusive sums over the workgroup.
-__device__ Sum block_scan(Sum v, Sum* waves, Sum& total) {
+// v of the lane that a DPP control names, 0 where there is none (or the row is not in ROWS).
+template <int CONTROL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t shifted(uint32_t v) {
+    return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CONTROL, ROWS, 0xf, false));
+}
+template <int CONTROL, int ROWS = 0xf>
+__device__ __forceinline__ void add_shifted(Sum& v) {
+    const uint32_t low = uint32_t(v.mass), high = uint32_t(v.mass >> 32);
+    v.count += shifted<CONTROL, ROWS>(v.count);
+    v.mass += u64(shifted<CONTROL, ROWS>(high)) << 32 | shifted<CONTROL, ROWS>(low);
+}
+
+// Inclusive sums over the workgroup: rows of 16 lanes by shifts of 1, 2, 4 and 8, then the last lane of
+// the row, and of the half, before.
+__device__ __forceinline__ Sum block_scan(Sum v, Sum* waves, Sum& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t c = __shfl_up(v.count, o, 64);
-        const u64 m = __shfl_up(v.mass, o, 64);
-        if (lane >= o) {
-            v.count += c;
-            v.mass += m;
-        }
-    }
+    add_shifted<0x111>(v);
+    add_shifted<0x112>(v);
+    add_shifted<0x114>(v);
+    add_shifted<0x118>(v);
+    add_shifted<0x142, 0xa>(v);
+    add_shifted<0x143, 0xc>(v);
     __syncthreads();  // the sums of a scan before this one have been read
     if (lane == 63) waves[wave] = v;
     __syncthreads();
     total = {0, 0};
+#pragma unroll
     for (int w = 0; w < WAVES; ++w) {
+        const Sum own = waves[w];
         if (w == wave) {
             v.count += total.count;
             v.mass += total.mass;
         }
-        total.count += waves[w].count;
-        total.mass += waves[w].mass;
+        total.count += own.count;
+        total.mass += own.mass;
     }
     return v;
 }
 
-// Descending logits as ascending 32-bit keys.
+// Descending logits as ascending 32-bit keys; minus zero's is zero's.  (NaN's is any: no NaN is kept.)
 __device__ __forceinline__ uint32_t sort_key(float v) {
-    const uint32_t u = __float_as_uint(v);
+    const uint32_t u = __float_as_uint(v + 0.0f);
     return u & 0x80000000u ? u : ~(u | 0x80000000u);
 }
 
@@ -191,42 +209,72 @@ __device__ __forceinline__ float key_value(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key : ~key & 0x7fffffffu);
 }
 
-// A row's weights.
+// A row's weights: 2^S exp((x - top) / T), rounded.
 struct Weights {
+    static constexpr float MOST = 3.4028234663852886e38f;
+    static constexpr double ROUND = 6755399441055744.0;  // sums with it are whole numbers, in their low bits
     float top;        // largest logit
-    bool infinite;    // it is plus infinity: only such tokens have a weight
-    double rate;      // STEPS log2(e) / T
-    double limit;     // exponents from here on weigh nothing
+    bool infinite;    // the largest is plus infinity: only such tokens have a weight
     int scale;        // S
+    double rate;      // STEPS log2(e) / T
+    double end;       // ROUND and the table steps from which on nothing is weighed
+    double c1, c2, c3, c4;
 
     __device__ __forceinline__ void set(float best, float temperature, int n) {
         scale = min(46, 31 + __clz(n));  // sums of n weights stay below 2^63
-        top = best;
+        end = ROUND + (scale + 1) * STEPS;
         infinite = best == -NEG_INF;
-        rate = STEPS * 1.44269504088896340736 / double(temperature);
-        limit = double((scale + 1) * STEPS) - 0.5;
+        // plus infinity stands for the largest finite value, next to which the others weigh nothing
+        top = infinite ? MOST : best;
+        rate = infinite ? double(MOST) : STEPS * 1.44269504088896340736 / double(temperature);
+        constexpr double C = -0.69314718055994530942 / STEPS;
+        c1 = C, c2 = C * C / 2, c3 = C * C * C / 6, c4 = C * C * C * C / 24;
+        // in vector registers: an FP64 product takes one scalar operand, and its constants would be moved
+        // into place for every element
+        asm volatile("" : "+v"(c1), "+v"(c2), "+v"(c3), "+v"(c4));
     }
-    __device__ __forceinline__ bool exponent(float v, double& x) const {
-        if (infinite) v = v == top ? 0.0f : NEG_INF;
-        x = (double(infinite ? 0.0f : top) - double(v)) * rate;
-        return x < limit;  // false for minus infinity
+    // The logit's distance from the top in table steps, rounded; false where it weighs nothing, as minus
+    // infinity and NaN do (their distance is infinite, or compares with nothing).
+    __device__ __forceinline__ bool step(float v, uint32_t& n, double& below, double& whole) const {
+        below = double(top) - double(infinite && v > MOST ? MOST : v);
+        const double t = fma(below, rate, ROUND);
+        n = uint32_t(__double2loint(t));
+        whole = t - ROUND;
+        return t < end;
     }
-    static __device__ __forceinline__ int steps(double x) { return int(__builtin_rint(x)); }
-    __device__ __forceinline__ u64 weight(const double* table, double x, int n) const {
-        // 2^(-x / STEPS) = table[n % STEPS] 2^-(n / STEPS) exp(-f), |f| <= log(2) / (2 STEPS): the cubic
-        // is off by f^4 / 24 < 2^-50.  Added to 2^52 a value below 2^47 is rounded to a whole number,
-        // which the low bits of the sum then hold.
-        const double f = (x - double(n)) * (0.69314718055994530942 / STEPS);
-        const double e = 1.0 - f * (1.0 - f * (0.5 - f * (1.0 / 6.0)));
-        const double w = ldexp(table[n & (STEPS - 1)] * e, scale - n / STEPS);
+    __device__ __forceinline__ bool bin(float v, int& b) const {
+        uint32_t n;
+        double below, whole;
+        const bool any = step(v, n, below, whole);
+        b = int(n >> BIN_SHIFT);
+        return any;
+    }
+    // 2^(-x / STEPS) = table[n % STEPS] 2^-(n / STEPS) exp(-g log(2) / STEPS) for x = n + g, |g| <= 1/2: the
+    // fourth degree is off by (log(2) / 2 STEPS)^5 / 120 < 2^-54.  The powers of two go into the exponent;
+    // added to 2^52 a value below 2^47 is rounded to a whole number, which the low bits of the sum hold.
+    __device__ __forceinline__ u64 weight(const double* table, uint32_t n, double below, double whole) const {
+        const double g = fma(below, rate, -whole);
+        const double e = fma(g, fma(g, fma(g, fma(g, c4, c3), c2), c1), 1.0);
+        const double m = table[n & (STEPS - 1)] * e;
+        const double w = __hiloint2double(__double2hiint(m) + ((scale - int(n / STEPS)) << 20), __double2loint(m));
         return u64(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
     }
     __device__ __forceinline__ u64 weight_of(const double* table, float v) const {
-        double x;
-        return exponent(v, x) ? weight(table, x, steps(x)) : 0;
+        uint32_t n;
+        double below, whole;
+        return step(v, n, below, whole) ? weight(table, n, below, whole) : 0;
     }
 };
-__device__ __forceinline__ double table_entry(int j) { return exp2(-double(j) / STEPS); }
+// 2^(-j / STEPS) by the bits of j.
+__device__ __forceinline__ double table_entry(int j) {
+    constexpr double ROOT[8] = {0.99729605608547012, 0.99459942348363317, 0.98922801319397555, 0.97857206208770013,
+                                0.95760328069857365, 0.91700404320467123, 0.84089641525371454, 0.70710678118654752};
+    static_assert(STEPS == 256, "eight bits");
+    double v = 1.0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v *= (j >> k) & 1 ? ROOT[k] : 1.0;
+    return v;
+}
 
 // A row's controls.
 struct Controls {
@@ -247,28 +295,40 @@ struct Controls {
     __device__ __forceinline__ bool greedy() const { return !(temperature > 0.0f); }
 };
 
-// Histograms of n elements in LDS, and the sum of the weights of at least `least`.
+// Histograms of n elements in LDS, and the sum of the weights of at least `least`.  Even and odd lanes
+// have a histogram of their own (bin_mass[2][BINS]): half as many lanes of a wave meet at an address.
 template <int TYPE, int NT>
 __device__ __forceinline__ u64 fill_bins(const void* base, int n, const Weights& w, const double* table, bool counts,
                                          bool masses, u64 least, u64* bin_mass, uint32_t* bin_count) {
     u64 kept = 0;
     if (masses) {
+        u64* own = bin_mass + (threadIdx.x & 1) * BINS;
         for_row<TYPE, NT>(base, n, [&](int, float v) {
-            double x;
-            if (!w.exponent(v, x)) return;
-            const int step = Weights::steps(x);
-            const u64 weight = w.weight(table, x, step);
-            atomicAdd(&bin_mass[step >> BIN_SHIFT], weight);
-            if (counts) atomicAdd(&bin_count[step >> BIN_SHIFT], 1u);
-            if (weight >= least) kept += weight;
+            // what weighs nothing is computed along (from any table entry), not branched around
+            uint32_t n;
+            double below, whole;
+            const bool any = w.step(v, n, below, whole);
+            const u64 weight = w.weight(table, n, below, whole);
+            if (any) {
+                atomicAdd(&own[n >> BIN_SHIFT], weight);
+                if (counts) atomicAdd(&bin_count[n >> BIN_SHIFT], 1u);
+                kept += weight >= least ? weight : 0;
+            }
         });
     } else {
+        uint32_t* own = reinterpret_cast<uint32_t*>(bin_mass) + (threadIdx.x & 3) * BINS;
         for_row<TYPE, NT>(base, n, [&](int, float v) {
-            double x;
-            if (w.exponent(v, x)) atomicAdd(&bin_count[Weights::steps(x) >> BIN_SHIFT], 1u);
+            int b;
+            if (w.bin(v, b)) atomicAdd(&own[b], 1u);
         });
     }
     return kept;
+}
+// A bin's sums from the copies.
+__device__ __forceinline__ Sum copies_sum(int b, bool counts, bool masses, const u64* bin_mass, const uint32_t* bin_count) {
+    if (masses) return {counts ? bin_count[b] : 0, bin_mass[b] + bin_mass[BINS + b]};
+    const uint32_t* c = reinterpret_cast<const uint32_t*>(bin_mass);
+    return {c[b] + c[BINS + b] + c[2 * BINS + b] + c[3 * BINS + b], 0};
 }
 
 // A segment's results in the workspace.
@@ -348,14 +408,14 @@ __device__ void sort_list(Shared& s, const Weights& w) {
     __syncthreads();
 }
 
-// The border among the sorted list's tokens, `base` before them.
+// The border among the sorted list's tokens from `from` to before `to`, `base` before the first of them.
 template <Border KIND>
-__device__ void search_list(Shared& s, Sum base, u64 target) {
-    const uint32_t count = s.listed;
-    for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
+__device__ __forceinline__ void search_list(Shared& s, Sum base, u64 target, uint32_t from, uint32_t to) {
+    base.mass -= from ? s.weight[from - 1] : 0;
+    for (uint32_t i = from + threadIdx.x; i < to; i += THREADS) {
         const u64 before = i ? s.weight[i - 1] : 0;
-        const Sum upto = {base.count + i + 1, base.mass + s.weight[i]};
-        if (reached<KIND>(upto, target) && !reached<KIND>({base.count + i, base.mass + before}, target)) {
+        const Sum upto = {base.count + i - from + 1, base.mass + s.weight[i]};
+        if (reached<KIND>(upto, target) && !reached<KIND>({upto.count - 1, base.mass + before}, target)) {
             s.found = upto;
             s.found_id = uint32_t(s.order[i]);
             s.found_weight = s.weight[i] - before;
@@ -373,47 +433,106 @@ struct Row {
 
 // The tokens with a value from `low` to `high` for which `inside` says so; sorted if the list holds them.
 template <int TYPE, typename P>
-__device__ void gather(Shared& s, const Row<TYPE>& row, float low, float high, P inside) {
+__device__ __forceinline__ void gather(Shared& s, const Row<TYPE>& row, float low, float high, P inside) {
+    typedef typename Element<TYPE>::T T;
+    constexpr int PER = 16 / sizeof(T), AHEAD = 8;
     __syncthreads();
     if (threadIdx.x == 0) s.listed = 0;
     __syncthreads();
-    for_row<TYPE, THREADS>(row.base, row.n, [&](int id, float v) {
-        if (v < low || v > high || !inside(v)) return;
+    auto add = [&](int id, float v) {
+        if (!inside(v)) return;
         const uint32_t at = atomicAdd(&s.listed, 1u);
         if (at < LIST) s.order[at] = u64(sort_key(v)) << 32 | uint32_t(id);
-    });
+    };
+    const T* x = static_cast<const T*>(row.base);
+    const int tid = threadIdx.x, n = row.n;
+    const int head = min(n, int(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
+    const int vectors = (n - head) / PER, tail = head + vectors * PER + tid;
+    if (tid < head) {
+        const float v = Element<TYPE>::value(x[tid]);
+        if (v >= low && v <= high) add(tid, v);
+    }
+    if (tail < n) {
+        const float v = Element<TYPE>::value(x[tail]);
+        if (v >= low && v <= high) add(tail, v);
+    }
+    const uint4* body = reinterpret_cast<const uint4*>(x + head);
+    for (int i = tid; i < vectors; i += THREADS * AHEAD) {
+        uint4 w[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a)
+            if (i + a * THREADS < vectors) w[a] = body[i + a * THREADS];
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            if (i + a * THREADS >= vectors) break;
+            const uint32_t words[4] = {w[a].x, w[a].y, w[a].z, w[a].w};
+            // few are: first whether any is large enough, then which, then one after the other
+            float v[PER];
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                v[j] = Element<TYPE>::value(PER == 4 ? words[j % 4] : words[j / 2] >> (j & 1) * 16);
+                any |= v[j] >= low;
+            }
+            if (!any) continue;
+            uint32_t which = 0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) which |= (v[j] >= low && v[j] <= high ? 1u : 0u) << j;
+            while (which) {
+                const int j = __ffs(which) - 1;
+                which &= which - 1;
+                const uint32_t pick = PER == 4 ? uint32_t(j) : uint32_t(j) >> 1;
+                const uint32_t word = pick & 2 ? (pick & 1 ? words[3] : words[2]) : (pick & 1 ? words[1] : words[0]);
+                add(head + (i + a * THREADS) * PER + j, Element<TYPE>::value(PER == 4 ? word : word >> (j & 1) * 16));
+            }
+        }
+    }
     __syncthreads();
     if (s.listed <= LIST) sort_list(s, row.w);
 }
 
-// The tokens of bins first .. last.
+// The tokens of bins first .. last, and of bin `extra` (past `last`; below 0: none).
 template <int TYPE>
-__device__ void gather_bins(Shared& s, const Row<TYPE>& row, int first, int last) {
+__device__ __forceinline__ void gather_bins(Shared& s, const Row<TYPE>& row, int first, int last, int extra) {
     // values that may lie there, by a table step more at each end
-    float low = NEG_INF, high = -NEG_INF;
+    float low = -__builtin_inff(), high = __builtin_inff();
     if (!row.w.infinite) {
-        low = __double2float_rd(double(row.w.top) - double(((last + 1) << BIN_SHIFT) + 1) / row.w.rate);
+        low = __double2float_rd(double(row.w.top) - double(((max(last, extra) + 1) << BIN_SHIFT) + 1) / row.w.rate);
         high = __double2float_ru(double(row.w.top) - double((first << BIN_SHIFT) - 1) / row.w.rate);
     }
-    const Weights w = row.w;
-    gather(s, row, low, high, [=](float v) {
-        double x;
-        if (!w.exponent(v, x)) return false;
-        const int bin = Weights::steps(x) >> BIN_SHIFT;
-        return bin >= first && bin <= last;
+    gather(s, row, low, high, [&](float v) {
+        int bin;
+        return row.w.bin(v, bin) && ((bin >= first && bin <= last) || bin == extra);
     });
+    // where the extra bin's tokens begin
+    if (s.listed <= uint32_t(LIST)) {
+        if (threadIdx.x == 0) s.split = s.listed;
+        __syncthreads();
+        if (extra >= 0) {
+            auto bin = [&](uint32_t i) {
+                int b;
+                row.w.bin(key_value(uint32_t(s.order[i] >> 32)), b);
+                return b;
+            };
+            for (uint32_t i = threadIdx.x; i < s.listed; i += THREADS)
+                if (bin(i) == extra && (i == 0 || bin(i - 1) != extra)) s.split = i;
+        }
+        __syncthreads();
+    }
 }
 
 // The token that is the `index`-th, by id, of those of one logit (`key`).
 template <int TYPE>
-__device__ void find_equal(Shared& s, const Row<TYPE>& row, uint32_t key, uint32_t index) {
+__device__ __noinline__ void find_equal(Shared& s, Row<TYPE> row, uint32_t key, uint32_t index) {
     typedef typename Element<TYPE>::T T;
     const T* x = static_cast<const T*>(row.base);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int each = (row.n + WAVES * 64 - 1) / (WAVES * 64) * 64, begin = wave * each, end = min(row.n, begin + each);
+    const float logit = key_value(key);
+    auto equal = [&](T w) { return Element<TYPE>::value(w) == logit; };
     uint32_t own = 0;
     for (int i = begin; i < end; i += 64) {
-        const bool same = i + lane < end && sort_key(plain(Element<TYPE>::value(x[i + lane]))) == key;
+        const bool same = i + lane < end && equal(x[i + lane]);
         own += uint32_t(__popcll(__ballot(same)));
     }
     __syncthreads();
@@ -423,7 +542,7 @@ __device__ void find_equal(Shared& s, const Row<TYPE>& row, uint32_t key, uint32
     for (int w = 0; w < wave; ++w) before += s.wave_id[w];
     if (index >= before && index < before + own)
         for (int i = begin; i < end; i += 64) {
-            const bool same = i + lane < end && sort_key(plain(Element<TYPE>::value(x[i + lane]))) == key;
+            const bool same = i + lane < end && equal(x[i + lane]);
             const u64 mask = __ballot(same);
             const uint32_t here = uint32_t(__popcll(mask));
             if (index < before + here) {
@@ -437,7 +556,7 @@ __device__ void find_equal(Shared& s, const Row<TYPE>& row, uint32_t key, uint32
 
 // The border within a bin of more tokens than the list holds.
 template <Border KIND, int TYPE>
-__device__ void divide_bin(Shared& s, const Row<TYPE>& row, int bin, Sum base, u64 target) {
+__device__ __noinline__ void divide_bin(Shared& s, Row<TYPE> row, int bin, Sum base, u64 target) {
     const int tid = threadIdx.x;
     u64* mass = s.order;  // the list is not in use
     uint32_t* count = reinterpret_cast<uint32_t*>(s.weight);
@@ -449,8 +568,8 @@ __device__ void divide_bin(Shared& s, const Row<TYPE>& row, int bin, Sum base, u
     __syncthreads();
     uint32_t low = 0xffffffffu, high = 0;
     for_row<TYPE, THREADS>(row.base, row.n, [&](int, float v) {
-        double x;
-        if (!row.w.exponent(v, x) || Weights::steps(x) >> BIN_SHIFT != bin) return;
+        int b;
+        if (!row.w.bin(v, b) || b != bin) return;
         low = min(low, sort_key(v));
         high = max(high, sort_key(v));
     });
@@ -483,9 +602,10 @@ __device__ void divide_bin(Shared& s, const Row<TYPE>& row, int bin, Sum base, u
             count[i] = 0;
         }
         __syncthreads();
+        const float least = key_value(high), most = key_value(low);
         for_row<TYPE, THREADS>(row.base, row.n, [&](int, float v) {
+            if (!(v >= least && v <= most)) return;
             const uint32_t key = sort_key(v);
-            if (key < low || key > high) return;
             atomicAdd(&count[(key - low) >> shift], 1u);
             atomicAdd(&mass[(key - low) >> shift], row.w.weight_of(s.table, v));
         });
@@ -509,51 +629,83 @@ __device__ void divide_bin(Shared& s, const Row<TYPE>& row, int bin, Sum base, u
         __syncthreads();
         if (held <= LIST) {
             gather(s, row, key_value(high), key_value(low), [](float) { return true; });
-            search_list<KIND>(s, base, target);
+            search_list<KIND>(s, base, target, 0, s.listed);
             return;
         }
         if (shift == 0) high = low;
     }
 }
 
-// The bins whose tokens are in the list; none: first > last.  `whole`: all tokens that may be kept are.
+// The bins whose tokens are in the list: first .. last (none: first > last) and `extra`.  `whole`: all
+// tokens that may be kept are.
 struct Listed {
-    int first, last;
+    int first, last, extra;
     bool whole;
 };
 
-// Finds a border by the bins' sums; the result is in s.found, s.found_id and s.found_weight.
-template <Border KIND, int TYPE>
-__device__ void find_border(Shared& s, const Row<TYPE>& row, Listed& list, u64 target) {
+__device__ __forceinline__ Sum before_bin(const Shared& s, int b) {
+    return {b ? s.bin_count[b - 1] : 0, b ? s.bin_mass[b - 1] : 0};
+}
+
+// The bin of a border, in every thread.
+template <Border KIND>
+__device__ __forceinline__ int border_bin(Shared& s, u64 target) {
     __syncthreads();
+    for (int b = threadIdx.x; b < BINS; b += THREADS)
+        if (reached<KIND>({s.bin_count[b], s.bin_mass[b]}, target) && !reached<KIND>(before_bin(s, b), target)) s.found_bin = b;
+    __syncthreads();
+    return s.found_bin;
+}
+
+// Finds a border; the result is in s.found, s.found_id and s.found_weight.
+template <Border KIND, int TYPE>
+__device__ __forceinline__ void find_border(Shared& s, const Row<TYPE>& row, Listed& list, u64 target) {
     if (list.whole) {
-        search_list<KIND>(s, {0, 0}, target);
+        __syncthreads();
+        search_list<KIND>(s, {0, 0}, target, 0, s.listed);
         return;
     }
-    for (int b = threadIdx.x; b < BINS; b += THREADS) {
-        const Sum upto = {s.bin_count[b], s.bin_mass[b]};
-        const Sum before = {b ? s.bin_count[b - 1] : 0, b ? s.bin_mass[b - 1] : 0};
-        if (reached<KIND>(upto, target) && !reached<KIND>(before, target)) s.found_bin = b;
-    }
+    const int bin = border_bin<KIND>(s, target);
     __syncthreads();
-    const int bin = s.found_bin;
-    __syncthreads();
-    auto before = [&](int b) -> Sum { return {b ? s.bin_count[b - 1] : 0, b ? s.bin_mass[b - 1] : 0}; };
-    if (bin < list.first || bin > list.last) {
+    if (bin != list.extra && (bin < list.first || bin > list.last)) {
         // all tokens up to the bin if they fit, so that further borders need no pass; else the bin's
-        list = {s.bin_count[bin] <= uint32_t(LIST) ? 0 : bin, bin, false};
-        gather_bins(s, row, list.first, bin);
+        list = {s.bin_count[bin] <= uint32_t(LIST) ? 0 : bin, bin, -1, false};
+        gather_bins(s, row, list.first, bin, -1);
         if (s.listed > uint32_t(LIST) && list.first < bin) {  // the numbers of tokens were estimates
             list.first = bin;
-            gather_bins(s, row, bin, bin);
+            gather_bins(s, row, bin, bin, -1);
         }
         if (s.listed > uint32_t(LIST)) {
-            divide_bin<KIND>(s, row, bin, before(bin), target);
-            list = {1, 0, false};
+            divide_bin<KIND>(s, row, bin, before_bin(s, bin), target);
+            list = {1, 0, -1, false};
             return;
         }
     }
-    search_list<KIND>(s, before(list.first), target);
+    if (bin == list.extra) search_list<KIND>(s, before_bin(s, bin), target, s.split, s.listed);
+    else search_list<KIND>(s, before_bin(s, list.first), target, 0, s.split);
+}
+
+// The bins of the two borders of a row with a top-p, gathered in one pass: the draw's is known but for
+// what the top-p's bin adds to the weight, which moves it by a bin at most, as a rule.
+template <int TYPE>
+__device__ __forceinline__ void gather_both(Shared& s, const Row<TYPE>& row, Listed& list, u64 target, u64 most, float u) {
+    const int bin = border_bin<BORDER_MASS>(s, target);
+    if (s.bin_count[bin] <= uint32_t(LIST)) return;  // find_border takes all up to it
+    const double share = u > 0.0f ? double(fminf(u, 1.0f)) : 0.0;
+    const u64 least = min(before_bin(s, bin).mass, most), full = min(s.bin_mass[bin], most);
+    u64 low = u64(share * double(least)), high = u64(share * double(full));
+    if (low >= full) low = full - 1;
+    if (high >= full) high = full - 1;
+    const int first = border_bin<BORDER_DRAW>(s, low);
+    __syncthreads();
+    const int last = border_bin<BORDER_DRAW>(s, high);
+    __syncthreads();
+    uint32_t held = s.bin_count[last] - before_bin(s, first).count;
+    if (last < bin) held += s.bin_count[bin] - before_bin(s, bin).count;
+    if (held > uint32_t(LIST)) return;
+    list = {first, last, last < bin ? bin : -1, false};
+    gather_bins(s, row, first, last, list.extra);
+    if (s.listed > uint32_t(LIST)) list = {1, 0, -1, false};
 }
 
 // Inclusive sums of the histograms -> all tokens' count and mass.  Where tokens were not counted, their
@@ -566,9 +718,10 @@ __device__ Sum sum_bins(Shared& s, const Weights& w, bool counts, bool masses) {
     if (b < BINS) {
         own = {counts ? s.bin_count[b] : 0, masses ? s.bin_mass[b] : 0};
         if (!counts && own.mass) {
-            const int step = ((b + 1) << BIN_SHIFT) - 1;
-            const u64 least = w.weight(s.table, double(step), step);
-            own.count = uint32_t(least ? min(own.mass / least + 1, u64(1) << 21) : u64(1) << 21);
+            // the bin's end is 2^(S - (b + 1) / 16)
+            const double many = double(own.mass) / ldexp(s.table[((b + 1) << BIN_SHIFT) & (STEPS - 1)],
+                                                        w.scale - ((b + 1) << BIN_SHIFT) / STEPS);
+            own.count = uint32_t(many < 2097152.0 ? many : 2097152.0) + 1;
         }
     }
     const Sum incl = block_scan(own, s.waves, total);
@@ -593,8 +746,9 @@ __global__ __launch_bounds__(PART_THREADS) void sample_best_kernel(SampleParams 
     const int begin = blockIdx.x * each, n = min(each, p.n - begin);
     float best;
     uint32_t id;
+    const bool greedy = Controls(p, blockIdx.y).greedy();
     find_best<TYPE, PART_THREADS>(static_cast<const typename Element<TYPE>::T*>(row_base<TYPE>(p, blockIdx.y)) + begin, n,
-                                  best, id);
+                                  greedy, best, id);
     block_best<PART_THREADS>(best, id, s_values, s_ids);
     if (threadIdx.x == 0) {
         Segment& out = static_cast<Segment*>(p.workspace)[int64_t(blockIdx.y) * gridDim.x + blockIdx.x];
@@ -627,7 +781,7 @@ __device__ __forceinline__ void segments_best(const Segment* segments, int count
 template <int TYPE>
 __global__ __launch_bounds__(PART_THREADS) void sample_bins_kernel(SampleParams p, int each) {
     __shared__ double s_table[STEPS];
-    __shared__ u64 s_mass[BINS];
+    __shared__ u64 s_mass[2 * BINS];
     __shared__ uint32_t s_count[BINS];
     __shared__ u64 s_kept;
     const int r = blockIdx.y, tid = threadIdx.x;
@@ -635,10 +789,8 @@ __global__ __launch_bounds__(PART_THREADS) void sample_bins_kernel(SampleParams 
     const Controls c(p, r);
     if (c.greedy()) return;
     for (int i = tid; i < STEPS; i += PART_THREADS) s_table[i] = table_entry(i);
-    for (int i = tid; i < BINS; i += PART_THREADS) {
-        s_mass[i] = 0;
-        s_count[i] = 0;
-    }
+    for (int i = tid; i < 2 * BINS; i += PART_THREADS) s_mass[i] = 0;
+    for (int i = tid; i < BINS; i += PART_THREADS) s_count[i] = 0;
     if (tid == 0) s_kept = 0;
     float best;
     uint32_t id;
@@ -655,8 +807,9 @@ __global__ __launch_bounds__(PART_THREADS) void sample_bins_kernel(SampleParams 
     __syncthreads();
     Segment& out = segments[blockIdx.x];
     for (int i = tid; i < BINS; i += PART_THREADS) {
-        if (c.masses) out.bin_mass[i] = s_mass[i];
-        if (c.counts) out.bin_count[i] = s_count[i];
+        const Sum sum = copies_sum(i, c.counts, c.masses, s_mass, s_count);
+        if (c.masses) out.bin_mass[i] = sum.mass;
+        if (c.counts) out.bin_count[i] = sum.count;
     }
     if (tid == 0) out.min_mass = s_kept;
 }
@@ -676,7 +829,7 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(SampleParams p, in
     if constexpr (SEGMENTS) {
         segments_best(parts, segments, best, id);
     } else {
-        find_best<TYPE, THREADS>(row.base, p.n, best, id);
+        find_best<TYPE, THREADS>(row.base, p.n, c.greedy(), best, id);
         block_best<THREADS>(best, id, s.wave_value, s.wave_id);
     }
     if (id == 0xffffffffu || c.greedy()) {
@@ -687,29 +840,42 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(SampleParams p, in
         return;
     }
     row.w.set(best, c.temperature, p.n);
-    static_assert(STEPS == THREADS, "one entry for each thread");
-    s.table[tid] = table_entry(tid);
+    if (tid < STEPS) s.table[tid] = table_entry(tid);
     if (tid == 0) s.min_mass = 0;
     auto fill = [&](bool counts, bool masses) {
-        for (int b = tid; b < BINS; b += THREADS) {
-            s.bin_mass[b] = 0;
-            s.bin_count[b] = 0;
-        }
+        for (int b = tid; b < 2 * BINS; b += THREADS) s.bin_mass[b] = 0;
+        for (int b = tid; b < BINS; b += THREADS) s.bin_count[b] = 0;
         __syncthreads();
         const u64 kept = fill_bins<TYPE, THREADS>(row.base, p.n, row.w, s.table, counts, masses, c.least, s.bin_mass, s.bin_count);
         if (c.least && kept) atomicAdd(&s.min_mass, kept);
+        __syncthreads();
+        Sum sum = {0, 0};
+        if (tid < BINS) sum = copies_sum(tid, counts, masses, s.bin_mass, s.bin_count);
+        __syncthreads();
+        if (tid < BINS) {
+            s.bin_mass[tid] = sum.mass;
+            s.bin_count[tid] = sum.count;
+        }
     };
     if constexpr (SEGMENTS) {
         if (tid < BINS) {
+            // sixteen segments' loads at once
             u64 mass = 0;
             uint32_t count = 0;
-            if (c.masses) {
-#pragma unroll 4
-                for (int i = 0; i < segments; ++i) mass += parts[i].bin_mass[tid];
-            }
-            if (c.counts) {
-#pragma unroll 4
-                for (int i = 0; i < segments; ++i) count += parts[i].bin_count[tid];
+            for (int i = 0; i < segments; i += 16) {
+                u64 m[16];
+                uint32_t n[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const Segment& part = parts[min(i + j, segments - 1)];
+                    m[j] = c.masses ? part.bin_mass[tid] : 0;
+                    n[j] = c.counts ? part.bin_count[tid] : 0;
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    mass += i + j < segments ? m[j] : 0;
+                    count += i + j < segments ? n[j] : 0;
+                }
             }
             s.bin_mass[tid] = mass;
             s.bin_count[tid] = count;
@@ -720,7 +886,7 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(SampleParams p, in
         fill(c.counts, c.masses);
     }
     Sum kept = sum_bins(s, row.w, c.counts, c.masses);
-    Listed list = {1, 0, false};
+    Listed list = {1, 0, -1, false};
     if (!c.masses) {
         // the top-k's tokens, and what shares the last one's bin
         int last = BINS - 1;
@@ -730,7 +896,7 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(SampleParams p, in
             __syncthreads();
             last = s.found_bin;
         }
-        gather_bins(s, row, 0, last);
+        gather_bins(s, row, 0, last, -1);
         if (s.listed <= uint32_t(LIST)) {
             list.whole = true;
             kept = {s.listed, s.weight[s.listed - 1]};
@@ -744,9 +910,12 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(SampleParams p, in
         find_border<BORDER_COUNT>(s, row, list, u64(c.top_k));
         kept = s.found;
     }
+    const float u = p.uniform[r];
     if (c.top_p < 1.0f) {
-        const double target = ceil(double(c.top_p) * double(kept.mass));
-        find_border<BORDER_MASS>(s, row, list, target > 1.0 ? u64(target) : u64(1));
+        const double share = ceil(double(c.top_p) * double(kept.mass));
+        const u64 target = share > 1.0 ? u64(share) : u64(1);
+        if (!list.whole) gather_both(s, row, list, target, c.least ? s.min_mass : ~u64(0), u);
+        find_border<BORDER_MASS>(s, row, list, target);
         kept = s.found;
     }
     if (c.least) {
@@ -760,7 +929,6 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(SampleParams p, in
         }
         kept.mass = min(kept.mass, s.min_mass);  // both are beginnings of one order
     }
-    const float u = p.uniform[r];
     const u64 at = u > 0.0f ? u64(double(fminf(u, 1.0f)) * double(kept.mass)) : 0;
     find_border<BORDER_DRAW>(s, row, list, at < kept.mass ? at : kept.mass - 1);
     if (tid == 0) {

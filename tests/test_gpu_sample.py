@@ -201,3 +201,49 @@ def test_replayed_graph_and_another_stream():
         torch.cuda.synchronize()
         eager, share = check(x, u.cpu().numpy(), top_p=np.full(3, 0.9, np.float32))
         assert torch.equal(token[:3], eager) and torch.equal(prob[:3], share)
+
+
+@pytest.mark.parametrize("temperature", [1e-3, 1e-6, 1e-10, 3e-13, 1e-14, 2.2e-15, 1e-20, 1e-38])
+def test_temperatures_near_zero(temperature):
+    """Neighbouring logits are any number of the weights' steps apart; some share the largest."""
+    rng = np.random.default_rng(13)
+    for kind in ("bf16", "fp32"):
+        x = bell(rng, 4, 20000, kind)
+        top = x.amax(1)
+        x[0, 5] = x[0, 19000] = top[0]
+        x[1, 7] = torch.nextafter(top[1].float(), torch.tensor(-1.0, device="cuda"))
+        x[2] = torch.nextafter(top[2].float(), torch.tensor(-1.0, device="cuda"))
+        x[2, 11] = top[2]
+        check(x, rng.random(4), temperature=np.full(4, temperature, np.float32))
+        check(x, rng.random(4), temperature=np.full(4, temperature, np.float32), top_p=np.full(4, 0.5, np.float32))
+
+
+def test_borders_among_negative_logits():
+    """Packed pairs are looked over before they are taken apart: neighbours of every kind beside a border."""
+    rng = np.random.default_rng(14)
+    for kind in ("bf16", "fp16", "fp32"):
+        x = -(rng.random((12, 40001)) * 30 + 2)
+        x[:, 1::2] = -200 - rng.random((12, 20000))      # upper halves far lower than lower ones
+        x[6:] = x[6:][:, ::-1]
+        for r in range(12):
+            few = rng.integers(0, 40001, 90)
+            x[r, few] = -1.5 - rng.random(90) * 0.1
+            x[r, few + (few < 40000)] = rng.choice([-np.inf, np.nan, -1.53, -0.0 - 3, 1e-30])
+        x = torch.from_numpy(x.copy()).to(TYPES[kind]).cuda()
+        check(x, rng.random(12), top_k=rng.integers(1, 90, 12).astype(np.int32))
+        check(x, rng.random(12), top_p=rng.uniform(0.3, 0.999, 12).astype(np.float32))
+        inf = x.clone()
+        inf[:, ::7] = float("nan")
+        inf[:, 35001] = float("inf")
+        check(inf, rng.random(12), top_k=rng.integers(1, 90, 12).astype(np.int32))
+        raw = {2: (torch.int16, 0x7F81 if kind == "bf16" else 0x7C01), 4: (torch.int32, 0x7F800001)}[x.element_size()]
+        x.view(raw[0])[:, 3::5] = raw[1]                 # signalling NaN
+        assert torch.isnan(x[:, 3::5]).all()
+        check(x, rng.random(12), top_k=rng.integers(1, 90, 12).astype(np.int32))
+        check(x, rng.random(12), top_p=rng.uniform(0.3, 0.999, 12).astype(np.float32))
+        check(x, rng.random(12), temperature=np.zeros(12, np.float32))
+    alone = torch.full((2, 20000), float("nan"), dtype=torch.bfloat16, device="cuda")
+    alone[0, 12345] = float("inf")
+    alone[1, 12346] = -7.0
+    check(alone, [0.5, 0.5])
+    check(alone, [0.5, 0.5], top_k=np.full(2, 3, np.int32))
