@@ -21,6 +21,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cstddef>
 
 #include "common.h"
 #include "device.h"
@@ -62,40 +63,55 @@ struct Element<TYPE_F32> {
 };
 
 // f(id, value) for n elements, a thread's in ascending order; 16 bytes a load behind the first
-// aligned element, AHEAD loads at once.
-template <int TYPE, int NT, int AHEAD = 4, typename F>
+// aligned element, AHEAD loads at once.  ROLLED: one copy of f for each half of a word: these kernels run
+// through most of their code once, and its first fetch costs more than the loop.
+template <int TYPE, int NT, int AHEAD, bool ROLLED, typename F>
 __device__ __forceinline__ void for_row(const void* base, int n, F f) {
     typedef typename Element<TYPE>::T T;
     constexpr int PER = 16 / sizeof(T);
     const T* row = static_cast<const T*>(base);
     const int tid = threadIdx.x;
     const int head = min(n, int(((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T)));
-    if (tid < head) f(tid, Element<TYPE>::value(row[tid]));
-    const int vectors = (n - head) / PER;
+    const int vectors = (n - head) / PER, tail = head + vectors * PER;
     const uint4* body = reinterpret_cast<const uint4*>(row + head);
+    auto word = [&](int id, uint32_t w) {
+        f(id, Element<TYPE>::value(w));
+        if constexpr (PER == 8) f(id + 1, Element<TYPE>::value(w >> 16));
+    };
     for (int i = tid; i < vectors; i += NT * AHEAD) {
         uint4 w[AHEAD];
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a)
-            if (i + a * NT < vectors) w[a] = body[i + a * NT];
-#pragma unroll
-        for (int a = 0; a < AHEAD; ++a) {
-            if (i + a * NT >= vectors) break;
-            const int id = head + (i + a * NT) * PER;
-            const uint32_t words[4] = {w[a].x, w[a].y, w[a].z, w[a].w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if constexpr (PER == 4) {
-                    f(id + j, Element<TYPE>::value(words[j]));
-                } else {
-                    f(id + 2 * j, Element<TYPE>::value(words[j]));
-                    f(id + 2 * j + 1, Element<TYPE>::value(words[j] >> 16));
+        for (int a = 0; a < AHEAD; ++a) w[a] = body[min(i + a * NT, vectors - 1)];
+        if constexpr (ROLLED) {
+#pragma unroll 1
+            for (int a = 0; a < AHEAD && i + a * NT < vectors; ++a) {
+                int id = head + (i + a * NT) * PER;
+#pragma unroll 1
+                for (int j = 0; j < 4; ++j, id += PER / 4) {
+                    word(id, w[0].x);
+                    w[0] = make_uint4(w[0].y, w[0].z, w[0].w, 0);
                 }
+#pragma unroll
+                for (int k = 0; k + 1 < AHEAD; ++k) w[k] = w[k + 1];
+            }
+        } else {
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                if (i + a * NT >= vectors) break;
+                const int id = head + (i + a * NT) * PER;
+                word(id, w[a].x);
+                word(id + PER / 4, w[a].y);
+                word(id + PER / 2, w[a].z);
+                word(id + PER / 4 * 3, w[a].w);
             }
         }
     }
-    const int tail = head + vectors * PER + tid;
-    if (tail < n) f(tail, Element<TYPE>::value(row[tail]));
+    // what lies before the first aligned element and behind the last whole 16 bytes (fewer than a wave's)
+    const int rest = head + n - tail;
+    if (tid < rest) {
+        const int id = tid < head ? tid : tail + tid - head;
+        f(id, Element<TYPE>::value(row[id]));
+    }
 }
 
 // The largest of a workgroup's values and its lowest id, in every thread (id 0xffffffff: minus infinity).
@@ -126,14 +142,14 @@ __device__ __forceinline__ void find_best(const void* base, int n, bool ids, flo
     best = NEG_INF;
     id = 0xffffffffu;
     if (ids) {
-        for_row<TYPE, NT>(base, n, [&](int i, float v) {
-            if (v > best) {
+        for_row<TYPE, NT, 4, true>(base, n, [&](int i, float v) {
+            if (v > best || (v == best && uint32_t(i) < id)) {
                 best = v;
-                id = uint32_t(i);
+                id = v > NEG_INF ? uint32_t(i) : id;
             }
         });
     } else {
-        for_row<TYPE, NT, 8>(base, n, [&](int, float v) { best = v > best ? v : best; });  // a maximum of a signalling NaN is NaN
+        for_row<TYPE, NT, 4, false>(base, n, [&](int, float v) { best = v > best ? v : best; });  // a maximum of a signalling NaN is NaN
         if (best > NEG_INF) id = 0;
     }
 }
@@ -145,14 +161,14 @@ struct Sum {
 
 struct Shared {
     double table[STEPS];   // 2^(-j / STEPS)
-    u64 bin_mass[2 * BINS];  // then inclusive sums in the first half
+    __attribute__((aligned(16))) u64 bin_mass[2 * BINS];  // copies, then inclusive sums in the first half
     uint32_t bin_count[BINS];
     u64 order[LIST];       // descending logit, ascending id
     u64 weight[LIST];      // inclusive sums of the list's weights
     Sum waves[WAVES];
     float wave_value[WAVES];
     uint32_t wave_id[WAVES];
-    uint32_t low, high, listed, split;
+    uint32_t low, high, queued, listed, split;
     Sum found;             // a border's count and mass up to and with its token
     uint32_t found_id;
     u64 found_weight;
@@ -175,7 +191,7 @@ __device__ __forceinline__ void add_shifted(Sum& v) {
 // Inclusive sums over the workgroup: rows of 16 lanes by shifts of 1, 2, 4 and 8, then the last lane of
 // the row, and of the half, before.
 __device__ __forceinline__ Sum block_scan(Sum v, Sum* waves, Sum& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     add_shifted<0x111>(v);
     add_shifted<0x112>(v);
     add_shifted<0x114>(v);
@@ -185,16 +201,23 @@ __device__ __forceinline__ Sum block_scan(Sum v, Sum* waves, Sum& total) {
     __syncthreads();  // the sums of a scan before this one have been read
     if (lane == 63) waves[wave] = v;
     __syncthreads();
-    total = {0, 0};
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-        const Sum own = waves[w];
-        if (w == wave) {
-            v.count += total.count;
-            v.mass += total.mass;
-        }
-        total.count += own.count;
-        total.mass += own.mass;
+    // the waves' sums, in a row of 16 lanes
+    static_assert(WAVES == 16, "a row");
+    Sum sum = waves[lane & 15];
+    add_shifted<0x111>(sum);
+    add_shifted<0x112>(sum);
+    add_shifted<0x114>(sum);
+    add_shifted<0x118>(sum);
+    auto of = [&](int l) -> Sum {
+        return {uint32_t(__builtin_amdgcn_readlane(sum.count, l)),
+                u64(uint32_t(__builtin_amdgcn_readlane(uint32_t(sum.mass >> 32), l))) << 32 |
+                    uint32_t(__builtin_amdgcn_readlane(uint32_t(sum.mass), l))};
+    };
+    total = of(15);
+    if (wave > 0) {
+        const Sum before = of(wave - 1);
+        v.count += before.count;
+        v.mass += before.mass;
     }
     return v;
 }
@@ -209,6 +232,15 @@ __device__ __forceinline__ float key_value(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key : ~key & 0x7fffffffu);
 }
 
+// exp(-g log(2) / STEPS) = 1 + g (c1 + g (c2 + g (c3 + g c4))).
+struct Series {
+    static constexpr double C = -0.69314718055994530942 / STEPS;
+    double c1 = C, c2 = C * C / 2, c3 = C * C * C / 6, c4 = C * C * C * C / 24;
+    // In vector registers, for loops over many: an FP64 product takes one scalar operand, and its constants
+    // would be moved into place for every element.
+    __device__ __forceinline__ void hold() { asm volatile("" : "+v"(c1), "+v"(c2), "+v"(c3), "+v"(c4)); }
+};
+
 // A row's weights: 2^S exp((x - top) / T), rounded.
 struct Weights {
     static constexpr float MOST = 3.4028234663852886e38f;
@@ -218,7 +250,6 @@ struct Weights {
     int scale;        // S
     double rate;      // STEPS log2(e) / T
     double end;       // ROUND and the table steps from which on nothing is weighed
-    double c1, c2, c3, c4;
 
     __device__ __forceinline__ void set(float best, float temperature, int n) {
         scale = min(46, 31 + __clz(n));  // sums of n weights stay below 2^63
@@ -227,11 +258,6 @@ struct Weights {
         // plus infinity stands for the largest finite value, next to which the others weigh nothing
         top = infinite ? MOST : best;
         rate = infinite ? double(MOST) : STEPS * 1.44269504088896340736 / double(temperature);
-        constexpr double C = -0.69314718055994530942 / STEPS;
-        c1 = C, c2 = C * C / 2, c3 = C * C * C / 6, c4 = C * C * C * C / 24;
-        // in vector registers: an FP64 product takes one scalar operand, and its constants would be moved
-        // into place for every element
-        asm volatile("" : "+v"(c1), "+v"(c2), "+v"(c3), "+v"(c4));
     }
     // The logit's distance from the top in table steps, rounded; false where it weighs nothing, as minus
     // infinity and NaN do (their distance is infinite, or compares with nothing).
@@ -252,9 +278,9 @@ struct Weights {
     // 2^(-x / STEPS) = table[n % STEPS] 2^-(n / STEPS) exp(-g log(2) / STEPS) for x = n + g, |g| <= 1/2: the
     // fourth degree is off by (log(2) / 2 STEPS)^5 / 120 < 2^-54.  The powers of two go into the exponent;
     // added to 2^52 a value below 2^47 is rounded to a whole number, which the low bits of the sum hold.
-    __device__ __forceinline__ u64 weight(const double* table, uint32_t n, double below, double whole) const {
+    __device__ __forceinline__ u64 weight(const double* table, const Series& c, uint32_t n, double below, double whole) const {
         const double g = fma(below, rate, -whole);
-        const double e = fma(g, fma(g, fma(g, fma(g, c4, c3), c2), c1), 1.0);
+        const double e = fma(g, fma(g, fma(g, fma(g, c.c4, c.c3), c.c2), c.c1), 1.0);
         const double m = table[n & (STEPS - 1)] * e;
         const double w = __hiloint2double(__double2hiint(m) + ((scale - int(n / STEPS)) << 20), __double2loint(m));
         return u64(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
@@ -262,7 +288,7 @@ struct Weights {
     __device__ __forceinline__ u64 weight_of(const double* table, float v) const {
         uint32_t n;
         double below, whole;
-        return step(v, n, below, whole) ? weight(table, n, below, whole) : 0;
+        return step(v, n, below, whole) ? weight(table, Series(), n, below, whole) : 0;
     }
 };
 // 2^(-j / STEPS) by the bits of j.
@@ -303,12 +329,14 @@ __device__ __forceinline__ u64 fill_bins(const void* base, int n, const Weights&
     u64 kept = 0;
     if (masses) {
         u64* own = bin_mass + (threadIdx.x & 1) * BINS;
-        for_row<TYPE, NT>(base, n, [&](int, float v) {
+        Series series;
+        series.hold();
+        for_row<TYPE, NT, 2, true>(base, n, [&](int, float v) {
             // what weighs nothing is computed along (from any table entry), not branched around
             uint32_t n;
             double below, whole;
             const bool any = w.step(v, n, below, whole);
-            const u64 weight = w.weight(table, n, below, whole);
+            const u64 weight = w.weight(table, series, n, below, whole);
             if (any) {
                 atomicAdd(&own[n >> BIN_SHIFT], weight);
                 if (counts) atomicAdd(&bin_count[n >> BIN_SHIFT], 1u);
@@ -317,66 +345,52 @@ __device__ __forceinline__ u64 fill_bins(const void* base, int n, const Weights&
         });
     } else {
         uint32_t* own = reinterpret_cast<uint32_t*>(bin_mass) + (threadIdx.x & 3) * BINS;
-        for_row<TYPE, NT>(base, n, [&](int, float v) {
+        for_row<TYPE, NT, 2, true>(base, n, [&](int, float v) {
             int b;
             if (w.bin(v, b)) atomicAdd(&own[b], 1u);
         });
     }
     return kept;
 }
-// A bin's sums from the copies.
-__device__ __forceinline__ Sum copies_sum(int b, bool counts, bool masses, const u64* bin_mass, const uint32_t* bin_count) {
-    if (masses) return {counts ? bin_count[b] : 0, bin_mass[b] + bin_mass[BINS + b]};
-    const uint32_t* c = reinterpret_cast<const uint32_t*>(bin_mass);
-    return {c[b] + c[BINS + b] + c[2 * BINS + b] + c[3 * BINS + b], 0};
-}
-
 // A segment's results in the workspace.
 struct Segment {
-    u64 bin_mass[BINS];
+    u64 bins[BINS];        // sums of the weights, or numbers of tokens where no weights are summed
     u64 min_mass;
-    uint32_t bin_count[BINS];
+    uint32_t counts[BINS];  // numbers of tokens beside sums
     float best;
     uint32_t id;
 };
 
-enum Border { BORDER_COUNT, BORDER_MASS, BORDER_DRAW };
+// A border: the first token up to which so many tokens, or so much weight, lie.
+struct Goal {
+    bool counted;
+    u64 value;
+    __device__ __forceinline__ bool reached(Sum upto) const { return (counted ? u64(upto.count) : upto.mass) >= value; }
+};
 
-// Whether a token with these sums before it is the border, or lies behind it.
-template <Border KIND>
-__device__ __forceinline__ bool reached(Sum upto, u64 target) {
-    return KIND == BORDER_COUNT ? upto.count >= target : KIND == BORDER_MASS ? upto.mass >= target : upto.mass > target;
+// Bitonic steps of strides j, j / 2 .. 1 for place i of runs of k, between lanes.
+__device__ __forceinline__ u64 exchange(u64 x, uint32_t i, uint32_t k, uint32_t j) {
+#pragma unroll 1
+    for (; j > 0; j >>= 1) {
+        const u64 y = __shfl_xor(x, int(j), 64);
+        // the lower place of an ascending run keeps the smaller one
+        const bool smaller = ((i & k) == 0) == ((i & j) == 0);
+        x = (y < x) == smaller ? y : x;
+    }
+    return x;
 }
 
-template <int O>
-__device__ __forceinline__ void exchange(u64& x, uint32_t i, uint32_t k) {
-    const u64 y = u64(xor_lane<O>(uint32_t(x >> 32))) << 32 | xor_lane<O>(uint32_t(x));
-    // the lower place of an ascending run keeps the smaller one
-    const bool smaller = ((i & k) == 0) == ((i & O) == 0);
-    x = (y < x) == smaller ? y : x;
-}
-
-// The list's tokens (s.listed of them) in order, bitonic: strides of a wave and more through LDS, shorter
-// ones between lanes.  Then inclusive sums of the weights.
-__device__ void sort_list(Shared& s, const Weights& w) {
+// The list's tokens (s.listed of them) in order: strides of a wave and more through LDS, shorter ones
+// between lanes.  Then inclusive sums of the weights.
+__device__ __forceinline__ void sort_list(Shared& s, const Weights& w) {
     const uint32_t tid = threadIdx.x, count = s.listed;
     uint32_t size = 64;
     while (size < count) size <<= 1;
     for (uint32_t i = count + tid; i < size; i += THREADS) s.order[i] = ~u64(0);
     __syncthreads();
-    for (uint32_t i = tid; i < size; i += THREADS) {
-        u64 x = s.order[i];
-        exchange<1>(x, i, 2);
-        exchange<2>(x, i, 4), exchange<1>(x, i, 4);
-        exchange<4>(x, i, 8), exchange<2>(x, i, 8), exchange<1>(x, i, 8);
-        exchange<8>(x, i, 16), exchange<4>(x, i, 16), exchange<2>(x, i, 16), exchange<1>(x, i, 16);
-        exchange<16>(x, i, 32), exchange<8>(x, i, 32), exchange<4>(x, i, 32), exchange<2>(x, i, 32), exchange<1>(x, i, 32);
-        exchange<32>(x, i, 64), exchange<16>(x, i, 64), exchange<8>(x, i, 64), exchange<4>(x, i, 64);
-        exchange<2>(x, i, 64), exchange<1>(x, i, 64);
-        s.order[i] = x;
-    }
-    __syncthreads();
-    for (uint32_t k = 128; k <= size; k <<= 1) {
+#pragma unroll 1
+    for (uint32_t k = 64; k <= size; k <<= 1) {
+#pragma unroll 1
         for (uint32_t j = k >> 1; j >= 64; j >>= 1) {
             for (uint32_t t = tid; t < size / 2; t += THREADS) {
                 const uint32_t a = (t & ~(j - 1)) * 2 + (t & (j - 1)), b = a + j;
@@ -388,34 +402,40 @@ __device__ void sort_list(Shared& s, const Weights& w) {
             }
             __syncthreads();
         }
+#pragma unroll 1
         for (uint32_t i = tid; i < size; i += THREADS) {
             u64 x = s.order[i];
-            exchange<32>(x, i, k), exchange<16>(x, i, k), exchange<8>(x, i, k);
-            exchange<4>(x, i, k), exchange<2>(x, i, k), exchange<1>(x, i, k);
+            // the first time, all runs up to 64
+#pragma unroll 1
+            for (uint32_t run = k == 64 ? 2 : k; run <= k; run <<= 1) x = exchange(x, i, run, min(run >> 1, 32u));
             s.order[i] = x;
         }
         __syncthreads();
     }
     const uint32_t i = 2 * tid;
-    const u64 w0 = i < count ? w.weight_of(s.table, key_value(uint32_t(s.order[i] >> 32))) : 0;
-    const u64 w1 = i + 1 < count ? w.weight_of(s.table, key_value(uint32_t(s.order[i + 1] >> 32))) : 0;
+    u64 weight[2];
+#pragma unroll 1
+    for (uint32_t e = 0; e < 2; ++e) {
+        weight[1] = i + e < count ? w.weight_of(s.table, key_value(uint32_t(s.order[i + e] >> 32))) : 0;
+        if (e == 0) weight[0] = weight[1];
+    }
     Sum total;
-    const Sum incl = block_scan({0, w0 + w1}, s.waves, total);
+    const Sum incl = block_scan({0, weight[0] + weight[1]}, s.waves, total);
     if (i < size) {
-        s.weight[i] = incl.mass - w1;
+        s.weight[i] = incl.mass - weight[1];
         s.weight[i + 1] = incl.mass;
     }
     __syncthreads();
 }
 
-// The border among the sorted list's tokens from `from` to before `to`, `base` before the first of them.
-template <Border KIND>
-__device__ __forceinline__ void search_list(Shared& s, Sum base, u64 target, uint32_t from, uint32_t to) {
+// The border among the sorted list's tokens from `from` to before `to`, `base` before the first of them;
+// the result is in s.found, s.found_id and s.found_weight.
+__device__ __forceinline__ void search_list(Shared& s, Sum base, Goal goal, uint32_t from, uint32_t to) {
     base.mass -= from ? s.weight[from - 1] : 0;
     for (uint32_t i = from + threadIdx.x; i < to; i += THREADS) {
         const u64 before = i ? s.weight[i - 1] : 0;
         const Sum upto = {base.count + i - from + 1, base.mass + s.weight[i]};
-        if (reached<KIND>(upto, target) && !reached<KIND>({upto.count - 1, base.mass + before}, target)) {
+        if (goal.reached(upto) && !goal.reached({upto.count - 1, base.mass + before})) {
             s.found = upto;
             s.found_id = uint32_t(s.order[i]);
             s.found_weight = s.weight[i] - before;
@@ -431,99 +451,104 @@ struct Row {
     Weights w;
 };
 
-// The tokens with a value from `low` to `high` for which `inside` says so; sorted if the list holds them.
-template <int TYPE, typename P>
-__device__ __forceinline__ void gather(Shared& s, const Row<TYPE>& row, float low, float high, P inside) {
+// The least and largest value of bins first .. last, by a table step more at each end.
+struct Window {
+    float low, high;
+    __device__ __forceinline__ bool has(float v) const { return v >= low && v <= high; }
+};
+__device__ __forceinline__ Window bin_window(const Weights& w, int first, int last) {
+    if (w.infinite) return {NEG_INF, -NEG_INF};
+    return {__double2float_rd(double(w.top) - double(((last + 1) << BIN_SHIFT) + 1) / w.rate),
+            __double2float_ru(double(w.top) - double((first << BIN_SHIFT) - 1) / w.rate)};
+}
+
+// The tokens in either window, and of bins first .. last or `extra` where first <= last; sorted if the list
+// holds them.  First the 16 bytes that hold any are queued, then these are taken apart: few are, but in
+// most waves some lane's.
+template <int TYPE>
+__device__ __forceinline__ void gather(Shared& s, const Row<TYPE>& row, Window one, Window two, int first, int last, int extra) {
     typedef typename Element<TYPE>::T T;
-    constexpr int PER = 16 / sizeof(T), AHEAD = 8;
+    constexpr int PER = 16 / sizeof(T), AHEAD = 4;
+    constexpr uint32_t QUEUE = 2 * LIST;
+    uint32_t* queue = reinterpret_cast<uint32_t*>(s.weight);
     __syncthreads();
-    if (threadIdx.x == 0) s.listed = 0;
+    if (threadIdx.x == 0) s.listed = s.queued = 0;
     __syncthreads();
     auto add = [&](int id, float v) {
-        if (!inside(v)) return;
+        int bin = 0;
+        if (!one.has(v) && !two.has(v)) return;
+        if (first <= last && !(row.w.bin(v, bin) && ((bin >= first && bin <= last) || bin == extra))) return;
         const uint32_t at = atomicAdd(&s.listed, 1u);
         if (at < LIST) s.order[at] = u64(sort_key(v)) << 32 | uint32_t(id);
     };
     const T* x = static_cast<const T*>(row.base);
     const int tid = threadIdx.x, n = row.n;
     const int head = min(n, int(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
-    const int vectors = (n - head) / PER, tail = head + vectors * PER + tid;
-    if (tid < head) {
-        const float v = Element<TYPE>::value(x[tid]);
-        if (v >= low && v <= high) add(tid, v);
-    }
-    if (tail < n) {
-        const float v = Element<TYPE>::value(x[tail]);
-        if (v >= low && v <= high) add(tail, v);
-    }
+    const int vectors = (n - head) / PER, tail = head + vectors * PER, rest = head + n - tail;
     const uint4* body = reinterpret_cast<const uint4*>(x + head);
     for (int i = tid; i < vectors; i += THREADS * AHEAD) {
         uint4 w[AHEAD];
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a)
-            if (i + a * THREADS < vectors) w[a] = body[i + a * THREADS];
+        for (int a = 0; a < AHEAD; ++a) w[a] = body[min(i + a * THREADS, vectors - 1)];
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) {
-            if (i + a * THREADS >= vectors) break;
             const uint32_t words[4] = {w[a].x, w[a].y, w[a].z, w[a].w};
-            // few are: first whether any is large enough, then which, then one after the other
-            float v[PER];
             bool any = false;
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-                v[j] = Element<TYPE>::value(PER == 4 ? words[j % 4] : words[j / 2] >> (j & 1) * 16);
-                any |= v[j] >= low;
+                const float v = Element<TYPE>::value(PER == 4 ? words[j % 4] : words[j / 2] >> (j & 1) * 16);
+                any |= one.has(v) || two.has(v);
             }
-            if (!any) continue;
-            uint32_t which = 0;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) which |= (v[j] >= low && v[j] <= high ? 1u : 0u) << j;
-            while (which) {
-                const int j = __ffs(which) - 1;
-                which &= which - 1;
-                const uint32_t pick = PER == 4 ? uint32_t(j) : uint32_t(j) >> 1;
-                const uint32_t word = pick & 2 ? (pick & 1 ? words[3] : words[2]) : (pick & 1 ? words[1] : words[0]);
-                add(head + (i + a * THREADS) * PER + j, Element<TYPE>::value(PER == 4 ? word : word >> (j & 1) * 16));
+            if (any && i + a * THREADS < vectors) {
+                const uint32_t at = atomicAdd(&s.queued, 1u);
+                if (at < QUEUE) queue[at] = uint32_t(i + a * THREADS);
             }
         }
     }
     __syncthreads();
+    const uint32_t queued = s.queued;
+    for (uint32_t e = tid; e < min(queued, QUEUE); e += THREADS) {
+        uint4 w = body[queue[e]];
+        int id = head + int(queue[e]) * PER;
+#pragma unroll 1
+        for (int j = 0; j < 4; ++j) {
+            add(id++, Element<TYPE>::value(w.x));
+            if constexpr (PER == 8) add(id++, Element<TYPE>::value(w.x >> 16));
+            w = make_uint4(w.y, w.z, w.w, 0);
+        }
+    }
+    if (tid < rest) {
+        const int id = tid < head ? tid : tail + tid - head;
+        add(id, Element<TYPE>::value(x[id]));
+    }
+    __syncthreads();
+    if (queued > QUEUE) {  // 16 bytes each of which holds one: more than the list does
+        __syncthreads();
+        if (tid == 0) s.listed = LIST + 1;
+        __syncthreads();
+    }
     if (s.listed <= LIST) sort_list(s, row.w);
 }
 
-// The tokens of bins first .. last, and of bin `extra` (past `last`; below 0: none).
+// Where the extra bin's tokens begin in the list.
 template <int TYPE>
-__device__ __forceinline__ void gather_bins(Shared& s, const Row<TYPE>& row, int first, int last, int extra) {
-    // values that may lie there, by a table step more at each end
-    float low = -__builtin_inff(), high = __builtin_inff();
-    if (!row.w.infinite) {
-        low = __double2float_rd(double(row.w.top) - double(((max(last, extra) + 1) << BIN_SHIFT) + 1) / row.w.rate);
-        high = __double2float_ru(double(row.w.top) - double((first << BIN_SHIFT) - 1) / row.w.rate);
-    }
-    gather(s, row, low, high, [&](float v) {
-        int bin;
-        return row.w.bin(v, bin) && ((bin >= first && bin <= last) || bin == extra);
-    });
-    // where the extra bin's tokens begin
-    if (s.listed <= uint32_t(LIST)) {
-        if (threadIdx.x == 0) s.split = s.listed;
-        __syncthreads();
-        if (extra >= 0) {
-            auto bin = [&](uint32_t i) {
-                int b;
-                row.w.bin(key_value(uint32_t(s.order[i] >> 32)), b);
-                return b;
-            };
-            for (uint32_t i = threadIdx.x; i < s.listed; i += THREADS)
-                if (bin(i) == extra && (i == 0 || bin(i - 1) != extra)) s.split = i;
-        }
-        __syncthreads();
-    }
+__device__ __forceinline__ void split_list(Shared& s, const Row<TYPE>& row, int extra) {
+    if (threadIdx.x == 0) s.split = s.listed;
+    __syncthreads();
+    if (extra < 0) return;
+    auto bin = [&](uint32_t i) {
+        int b;
+        row.w.bin(key_value(uint32_t(s.order[i] >> 32)), b);
+        return b;
+    };
+    for (uint32_t i = threadIdx.x; i < s.listed; i += THREADS)
+        if (bin(i) == extra && (i == 0 || bin(i - 1) != extra)) s.split = i;
+    __syncthreads();
 }
 
 // The token that is the `index`-th, by id, of those of one logit (`key`).
 template <int TYPE>
-__device__ __noinline__ void find_equal(Shared& s, Row<TYPE> row, uint32_t key, uint32_t index) {
+__device__ __forceinline__ void find_equal(Shared& s, const Row<TYPE>& row, uint32_t key, uint32_t index) {
     typedef typename Element<TYPE>::T T;
     const T* x = static_cast<const T*>(row.base);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -554,9 +579,11 @@ __device__ __noinline__ void find_equal(Shared& s, Row<TYPE> row, uint32_t key, 
     __syncthreads();
 }
 
-// The border within a bin of more tokens than the list holds.
-template <Border KIND, int TYPE>
-__device__ __noinline__ void divide_bin(Shared& s, Row<TYPE> row, int bin, Sum base, u64 target) {
+// The border within a bin of more tokens than the list holds: narrows the bin's keys to low .. high, with
+// `base` before them, until the list holds them (true), or they are one logit's: then the border is found.
+template <int TYPE>
+__device__ __forceinline__ bool divide_bin(Shared& s, const Row<TYPE>& row, int bin, Sum& base, Goal goal, uint32_t& low,
+                                           uint32_t& high) {
     const int tid = threadIdx.x;
     u64* mass = s.order;  // the list is not in use
     uint32_t* count = reinterpret_cast<uint32_t*>(s.weight);
@@ -566,8 +593,9 @@ __device__ __noinline__ void divide_bin(Shared& s, Row<TYPE> row, int bin, Sum b
         s.high = 0;
     }
     __syncthreads();
-    uint32_t low = 0xffffffffu, high = 0;
-    for_row<TYPE, THREADS>(row.base, row.n, [&](int, float v) {
+    low = 0xffffffffu;
+    high = 0;
+    for_row<TYPE, THREADS, 1, true>(row.base, row.n, [&](int, float v) {
         int b;
         if (!row.w.bin(v, b) || b != bin) return;
         low = min(low, sort_key(v));
@@ -578,23 +606,8 @@ __device__ __noinline__ void divide_bin(Shared& s, Row<TYPE> row, int bin, Sum b
     __syncthreads();
     low = s.low;
     high = s.high;
-    while (true) {
-        if (low == high) {
-            // one logit: every token has the same weight
-            const u64 w = row.w.weight_of(s.table, key_value(low));
-            u64 index;
-            if (KIND == BORDER_COUNT) index = target - base.count - 1;
-            else if (KIND == BORDER_MASS) index = (target - base.mass + w - 1) / w - 1;
-            else index = (target - base.mass) / w;
-            if (KIND == BORDER_DRAW) find_equal(s, row, low, uint32_t(index));
-            __syncthreads();
-            if (tid == 0) {
-                s.found = {uint32_t(base.count + index + 1), base.mass + (index + 1) * w};
-                s.found_weight = w;
-            }
-            __syncthreads();
-            return;
-        }
+    uint32_t held = 0xffffffffu;
+    while (held > uint32_t(LIST) && low < high) {
         int shift = 0;
         while ((high - low) >> shift >= SUB) ++shift;
         for (int i = tid; i < SUB; i += THREADS) {
@@ -603,7 +616,7 @@ __device__ __noinline__ void divide_bin(Shared& s, Row<TYPE> row, int bin, Sum b
         }
         __syncthreads();
         const float least = key_value(high), most = key_value(low);
-        for_row<TYPE, THREADS>(row.base, row.n, [&](int, float v) {
+        for_row<TYPE, THREADS, 1, true>(row.base, row.n, [&](int, float v) {
             if (!(v >= least && v <= most)) return;
             const uint32_t key = sort_key(v);
             atomicAdd(&count[(key - low) >> shift], 1u);
@@ -615,7 +628,7 @@ __device__ __noinline__ void divide_bin(Shared& s, Row<TYPE> row, int bin, Sum b
         const Sum own = {count[tid], mass[tid]}, incl = block_scan(own, s.waves, total);
         const Sum upto = {base.count + incl.count, base.mass + incl.mass};
         const Sum before = {upto.count - own.count, upto.mass - own.mass};
-        if (reached<KIND>(upto, target) && !reached<KIND>(before, target)) {
+        if (goal.reached(upto) && !goal.reached(before)) {
             s.found_bin = tid;
             s.found = before;
             s.listed = own.count;
@@ -623,107 +636,45 @@ __device__ __noinline__ void divide_bin(Shared& s, Row<TYPE> row, int bin, Sum b
         __syncthreads();
         const uint32_t part = uint32_t(s.found_bin);
         base = s.found;
-        const uint32_t held = s.listed;
+        held = s.listed;
         high = min(high, low + (((part + 1) << shift) - 1));
         low += part << shift;
         __syncthreads();
-        if (held <= LIST) {
-            gather(s, row, key_value(high), key_value(low), [](float) { return true; });
-            search_list<KIND>(s, base, target, 0, s.listed);
-            return;
-        }
-        if (shift == 0) high = low;
     }
+    if (held <= uint32_t(LIST)) return true;
+    // one logit: every token has the same weight
+    const u64 w = row.w.weight_of(s.table, key_value(low));
+    const u64 index = goal.counted ? goal.value - base.count - 1 : (goal.value - base.mass + w - 1) / w - 1;
+    find_equal(s, row, low, uint32_t(index));
+    if (tid == 0) {
+        s.found = {uint32_t(base.count + index + 1), base.mass + (index + 1) * w};
+        s.found_weight = w;
+    }
+    __syncthreads();
+    return false;
 }
-
-// The bins whose tokens are in the list: first .. last (none: first > last) and `extra`.  `whole`: all
-// tokens that may be kept are.
-struct Listed {
-    int first, last, extra;
-    bool whole;
-};
 
 __device__ __forceinline__ Sum before_bin(const Shared& s, int b) {
     return {b ? s.bin_count[b - 1] : 0, b ? s.bin_mass[b - 1] : 0};
 }
 
 // The bin of a border, in every thread.
-template <Border KIND>
-__device__ __forceinline__ int border_bin(Shared& s, u64 target) {
+__device__ __forceinline__ int border_bin(Shared& s, Goal goal) {
     __syncthreads();
-    for (int b = threadIdx.x; b < BINS; b += THREADS)
-        if (reached<KIND>({s.bin_count[b], s.bin_mass[b]}, target) && !reached<KIND>(before_bin(s, b), target)) s.found_bin = b;
+    const int b = threadIdx.x;
+    if (b < BINS && goal.reached({s.bin_count[b], s.bin_mass[b]}) && !goal.reached(before_bin(s, b))) s.found_bin = b;
     __syncthreads();
     return s.found_bin;
 }
 
-// Finds a border; the result is in s.found, s.found_id and s.found_weight.
-template <Border KIND, int TYPE>
-__device__ __forceinline__ void find_border(Shared& s, const Row<TYPE>& row, Listed& list, u64 target) {
-    if (list.whole) {
-        __syncthreads();
-        search_list<KIND>(s, {0, 0}, target, 0, s.listed);
-        return;
-    }
-    const int bin = border_bin<KIND>(s, target);
-    __syncthreads();
-    if (bin != list.extra && (bin < list.first || bin > list.last)) {
-        // all tokens up to the bin if they fit, so that further borders need no pass; else the bin's
-        list = {s.bin_count[bin] <= uint32_t(LIST) ? 0 : bin, bin, -1, false};
-        gather_bins(s, row, list.first, bin, -1);
-        if (s.listed > uint32_t(LIST) && list.first < bin) {  // the numbers of tokens were estimates
-            list.first = bin;
-            gather_bins(s, row, bin, bin, -1);
-        }
-        if (s.listed > uint32_t(LIST)) {
-            divide_bin<KIND>(s, row, bin, before_bin(s, bin), target);
-            list = {1, 0, -1, false};
-            return;
-        }
-    }
-    if (bin == list.extra) search_list<KIND>(s, before_bin(s, bin), target, s.split, s.listed);
-    else search_list<KIND>(s, before_bin(s, list.first), target, 0, s.split);
-}
-
-// The bins of the two borders of a row with a top-p, gathered in one pass: the draw's is known but for
-// what the top-p's bin adds to the weight, which moves it by a bin at most, as a rule.
-template <int TYPE>
-__device__ __forceinline__ void gather_both(Shared& s, const Row<TYPE>& row, Listed& list, u64 target, u64 most, float u) {
-    const int bin = border_bin<BORDER_MASS>(s, target);
-    if (s.bin_count[bin] <= uint32_t(LIST)) return;  // find_border takes all up to it
-    const double share = u > 0.0f ? double(fminf(u, 1.0f)) : 0.0;
-    const u64 least = min(before_bin(s, bin).mass, most), full = min(s.bin_mass[bin], most);
-    u64 low = u64(share * double(least)), high = u64(share * double(full));
-    if (low >= full) low = full - 1;
-    if (high >= full) high = full - 1;
-    const int first = border_bin<BORDER_DRAW>(s, low);
-    __syncthreads();
-    const int last = border_bin<BORDER_DRAW>(s, high);
-    __syncthreads();
-    uint32_t held = s.bin_count[last] - before_bin(s, first).count;
-    if (last < bin) held += s.bin_count[bin] - before_bin(s, bin).count;
-    if (held > uint32_t(LIST)) return;
-    list = {first, last, last < bin ? bin : -1, false};
-    gather_bins(s, row, first, last, list.extra);
-    if (s.listed > uint32_t(LIST)) list = {1, 0, -1, false};
-}
-
-// Inclusive sums of the histograms -> all tokens' count and mass.  Where tokens were not counted, their
-// number in a bin is estimated by the bin's smallest weight.
-__device__ Sum sum_bins(Shared& s, const Weights& w, bool counts, bool masses) {
-    __syncthreads();
-    const int b = threadIdx.x;
+// Inclusive sums of the histograms (a bin's sum and count in thread b) -> all tokens' count and mass.  Where
+// tokens were not counted, twice their number at most is estimated by the power of two below the bin's
+// weights.
+__device__ __forceinline__ Sum sum_bins(Shared& s, int scale, bool counts, Sum own) {
     static_assert(BINS <= THREADS, "one bin for each thread");
-    Sum own = {0, 0}, total;
-    if (b < BINS) {
-        own = {counts ? s.bin_count[b] : 0, masses ? s.bin_mass[b] : 0};
-        if (!counts && own.mass) {
-            // the bin's end is 2^(S - (b + 1) / 16)
-            const double many = double(own.mass) / ldexp(s.table[((b + 1) << BIN_SHIFT) & (STEPS - 1)],
-                                                        w.scale - ((b + 1) << BIN_SHIFT) / STEPS);
-            own.count = uint32_t(many < 2097152.0 ? many : 2097152.0) + 1;
-        }
-    }
+    const int b = threadIdx.x;
+    Sum total;
+    if (!counts) own.count = uint32_t(min(own.mass >> max(scale - ((b + 1) * (1 << BIN_SHIFT) + STEPS - 1) / STEPS, 0), u64(1) << 21));
     const Sum incl = block_scan(own, s.waves, total);
     if (b < BINS) {
         s.bin_count[b] = incl.count;
@@ -731,6 +682,13 @@ __device__ Sum sum_bins(Shared& s, const Weights& w, bool counts, bool masses) {
     }
     __syncthreads();
     return total;
+}
+
+// Thread b's bin of the copies in LDS.
+__device__ __forceinline__ u64 copies_sum(const u64* bin_mass, bool masses, int b) {
+    if (masses) return bin_mass[b] + bin_mass[BINS + b];
+    const uint32_t* c = reinterpret_cast<const uint32_t*>(bin_mass);
+    return c[b] + c[BINS + b] + c[2 * BINS + b] + c[3 * BINS + b];
 }
 
 template <int TYPE>
@@ -807,9 +765,8 @@ __global__ __launch_bounds__(PART_THREADS) void sample_bins_kernel(SampleParams 
     __syncthreads();
     Segment& out = segments[blockIdx.x];
     for (int i = tid; i < BINS; i += PART_THREADS) {
-        const Sum sum = copies_sum(i, c.counts, c.masses, s_mass, s_count);
-        if (c.masses) out.bin_mass[i] = sum.mass;
-        if (c.counts) out.bin_count[i] = sum.count;
+        out.bins[i] = copies_sum(s_mass, c.masses, i);
+        if (c.masses && c.counts) out.counts[i] = s_count[i];
     }
     if (tid == 0) out.min_mass = s_kept;
 }
@@ -839,98 +796,145 @@ __global__ __launch_bounds__(THREADS) void sample_pick_kernel(SampleParams p, in
         }
         return;
     }
-    row.w.set(best, c.temperature, p.n);
+    row.w.set(__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(best))), c.temperature, p.n);
     if (tid < STEPS) s.table[tid] = table_entry(tid);
     if (tid == 0) s.min_mass = 0;
-    auto fill = [&](bool counts, bool masses) {
-        for (int b = tid; b < 2 * BINS; b += THREADS) s.bin_mass[b] = 0;
-        for (int b = tid; b < BINS; b += THREADS) s.bin_count[b] = 0;
-        __syncthreads();
-        const u64 kept = fill_bins<TYPE, THREADS>(row.base, p.n, row.w, s.table, counts, masses, c.least, s.bin_mass, s.bin_count);
-        if (c.least && kept) atomicAdd(&s.min_mass, kept);
-        __syncthreads();
-        Sum sum = {0, 0};
-        if (tid < BINS) sum = copies_sum(tid, counts, masses, s.bin_mass, s.bin_count);
-        __syncthreads();
-        if (tid < BINS) {
-            s.bin_mass[tid] = sum.mass;
-            s.bin_count[tid] = sum.count;
-        }
-    };
-    if constexpr (SEGMENTS) {
-        if (tid < BINS) {
+    const float u = p.uniform[r], share = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
+
+    // The borders one after the other: of the top-k, of the top-p, the drawn token's.  A small top-k's
+    // tokens are listed first of all, with what shares the last one's bin; should too many do, weights are
+    // summed after all and all begins again.
+    enum Stage { LIST_ALL, TOP_K, TOP_P, DRAW, DONE };
+    bool counts = c.counts, masses = c.masses;
+    Sum kept;
+    int stage;
+    do {
+        Sum own = {0, 0};
+        u64 bin = 0;
+        if (SEGMENTS && masses == c.masses) {
             // sixteen segments' loads at once
-            u64 mass = 0;
-            uint32_t count = 0;
-            for (int i = 0; i < segments; i += 16) {
-                u64 m[16];
-                uint32_t n[16];
+            if (tid < BINS)
+                for (int i = 0; i < segments; i += 16) {
+                    u64 m[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const Segment& part = parts[min(i + j, segments - 1)];
-                    m[j] = c.masses ? part.bin_mass[tid] : 0;
-                    n[j] = c.counts ? part.bin_count[tid] : 0;
-                }
+                    for (int j = 0; j < 16; ++j) m[j] = parts[min(i + j, segments - 1)].bins[tid];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    mass += i + j < segments ? m[j] : 0;
-                    count += i + j < segments ? n[j] : 0;
+                    for (int j = 0; j < 16; ++j) bin += i + j < segments ? m[j] : 0;
                 }
+            if (masses && counts && tid < BINS) {
+#pragma unroll 1
+                for (int i = 0; i < segments; ++i) own.count += parts[i].counts[tid];
             }
-            s.bin_mass[tid] = mass;
-            s.bin_count[tid] = count;
-        }
-        __syncthreads();
-        if (c.masses && c.least && tid < segments) atomicAdd(&s.min_mass, parts[tid].min_mass);
-    } else {
-        fill(c.counts, c.masses);
-    }
-    Sum kept = sum_bins(s, row.w, c.counts, c.masses);
-    Listed list = {1, 0, -1, false};
-    if (!c.masses) {
-        // the top-k's tokens, and what shares the last one's bin
-        int last = BINS - 1;
-        if (uint32_t(c.top_k) < kept.count) {
-            if (tid < BINS && s.bin_count[tid] >= uint32_t(c.top_k) && (tid == 0 || s.bin_count[tid - 1] < uint32_t(c.top_k)))
-                s.found_bin = tid;
+            if (masses && c.least && tid < segments) atomicAdd(&s.min_mass, parts[tid].min_mass);
             __syncthreads();
-            last = s.found_bin;
-        }
-        gather_bins(s, row, 0, last, -1);
-        if (s.listed <= uint32_t(LIST)) {
-            list.whole = true;
-            kept = {s.listed, s.weight[s.listed - 1]};
         } else {
-            // too many share it: weights of all tokens after all
-            fill(true, true);
-            kept = sum_bins(s, row.w, true, true);
-        }
-    }
-    if (c.top_k > 0 && uint32_t(c.top_k) < kept.count) {
-        find_border<BORDER_COUNT>(s, row, list, u64(c.top_k));
-        kept = s.found;
-    }
-    const float u = p.uniform[r];
-    if (c.top_p < 1.0f) {
-        const double share = ceil(double(c.top_p) * double(kept.mass));
-        const u64 target = share > 1.0 ? u64(share) : u64(1);
-        if (!list.whole) gather_both(s, row, list, target, c.least ? s.min_mass : ~u64(0), u);
-        find_border<BORDER_MASS>(s, row, list, target);
-        kept = s.found;
-    }
-    if (c.least) {
-        if (list.whole) {
+            for (int b = tid; b < 2 * BINS; b += THREADS) s.bin_mass[b] = 0;
+            for (int b = tid; b < BINS; b += THREADS) s.bin_count[b] = 0;
             __syncthreads();
-            for (uint32_t i = tid; i < s.listed; i += THREADS) {
-                const u64 own = s.weight[i] - (i ? s.weight[i - 1] : 0);
-                if (own >= c.least && (i + 1 == s.listed || s.weight[i + 1] - s.weight[i] < c.least)) s.min_mass = s.weight[i];
+            const u64 enough = fill_bins<TYPE, THREADS>(row.base, p.n, row.w, s.table, counts, masses, c.least, s.bin_mass, s.bin_count);
+            if (c.least && enough) atomicAdd(&s.min_mass, enough);
+            __syncthreads();
+            if (tid < BINS) {
+                bin = copies_sum(s.bin_mass, masses, tid);
+                if (masses && counts) own.count = s.bin_count[tid];
             }
             __syncthreads();
         }
-        kept.mass = min(kept.mass, s.min_mass);  // both are beginnings of one order
-    }
-    const u64 at = u > 0.0f ? u64(double(fminf(u, 1.0f)) * double(kept.mass)) : 0;
-    find_border<BORDER_DRAW>(s, row, list, at < kept.mass ? at : kept.mass - 1);
+        if (masses) own.mass = bin;
+        else own.count = uint32_t(bin);
+        kept = sum_bins(s, row.w.scale, counts, own);
+        // the list holds bins first .. last (none: first > last) and `extra`, or all tokens that may be kept
+        int first = 1, last = 0, extra = -1;
+        bool whole = false;
+        for (stage = masses ? TOP_K : LIST_ALL; stage < DONE; ++stage) {
+            Goal goal = {false, 1};
+            if (stage == LIST_ALL) {
+                goal = {true, min(u64(c.top_k), u64(kept.count))};
+            } else if (stage == TOP_K) {
+                if (c.top_k <= 0 || uint32_t(c.top_k) >= kept.count) continue;
+                goal = {true, u64(c.top_k)};
+            } else if (stage == TOP_P) {
+                if (!(c.top_p < 1.0f)) continue;
+                const double part = ceil(double(c.top_p) * double(kept.mass));
+                if (part > 1.0) goal.value = u64(part);
+            } else {
+                if (c.least) kept.mass = min(kept.mass, s.min_mass);  // both are beginnings of one order
+                goal.value = min(u64(double(share) * double(kept.mass)), kept.mass - 1) + 1;
+            }
+            // of a list: the border lies from `from` to before `to`, `base` before that
+            uint32_t from = 0, to = 0;
+            Sum base = {0, 0};
+            bool found = false;
+            if (!whole) {
+                const int bin = border_bin(s, goal);
+                if (bin != extra && (bin < first || bin > last)) {
+                    // all tokens up to the bin if they fit, so that further borders need no pass; else the bin's
+                    first = stage == LIST_ALL || s.bin_count[bin] <= uint32_t(LIST) ? 0 : bin;
+                    last = bin;
+                    extra = -1;
+                    if (stage == TOP_P && first == bin) {
+                        // the drawn token's as well: where it is, is known but for what this bin adds to the weight,
+                        // which moves it by a bin at most, as a rule
+                        const u64 most = c.least ? s.min_mass : ~u64(0);
+                        const u64 least = min(before_bin(s, bin).mass, most), full = min(s.bin_mass[bin], most);
+                        const int one = border_bin(s, {false, min(u64(double(share) * double(least)), full - 1) + 1});
+                        const int two = border_bin(s, {false, min(u64(double(share) * double(full)), full - 1) + 1});
+                        uint32_t held = s.bin_count[two] - before_bin(s, one).count;
+                        if (two < bin) held += s.bin_count[bin] - before_bin(s, bin).count;
+                        if (held <= uint32_t(LIST)) {
+                            first = one;
+                            last = two;
+                            extra = two < bin ? bin : -1;
+                        }
+                    }
+                    Window window = {0, 0};
+                    bool keys = false;
+                    while (true) {
+                        if (!keys) window = bin_window(row.w, first, last);
+                        gather(s, row, window, extra < 0 ? window : bin_window(row.w, extra, extra), first, last, extra);
+                        if (s.listed <= uint32_t(LIST) || stage == LIST_ALL) break;
+                        if (first < last || extra >= 0) {
+                            // the numbers of tokens were estimates: the bin alone
+                            first = last = bin;
+                            extra = -1;
+                            continue;
+                        }
+                        uint32_t low_key, high_key;
+                        base = before_bin(s, bin);
+                        first = 1;  // what is listed now is of no other border's use
+                        last = 0;
+                        found = !divide_bin(s, row, bin, base, goal, low_key, high_key);
+                        if (found) break;
+                        window = {key_value(high_key), key_value(low_key)};
+                        keys = true;
+                    }
+                    if (stage == LIST_ALL && s.listed > uint32_t(LIST)) break;
+                    if (!found) split_list(s, row, extra);
+                }
+                if (first <= last) base = before_bin(s, bin == extra ? bin : first);
+                from = bin == extra ? s.split : 0;
+                to = bin == extra ? s.listed : s.split;
+            } else {
+                __syncthreads();
+                to = s.listed;
+            }
+            if (!found && stage != LIST_ALL) search_list(s, base, goal, from, to);
+            if (stage == LIST_ALL) {
+                whole = true;
+                kept = {s.listed, s.weight[s.listed - 1]};
+                if (c.least) {
+                    for (uint32_t i = tid; i < s.listed; i += THREADS) {
+                        const u64 own = s.weight[i] - (i ? s.weight[i - 1] : 0);
+                        if (own >= c.least && (i + 1 == s.listed || s.weight[i + 1] - s.weight[i] < c.least)) s.min_mass = s.weight[i];
+                    }
+                    __syncthreads();
+                }
+            } else if (stage != DRAW) {
+                kept = s.found;
+            }
+        }
+        if (stage == LIST_ALL) counts = masses = true;
+    } while (stage < DONE);
     if (tid == 0) {
         p.token[r] = int32_t(s.found_id);
         if (p.prob) p.prob[r] = float(double(s.found_weight) / double(kept.mass));
