@@ -296,12 +296,15 @@ __global__ __launch_bounds__(256) void paged_qkv_kernel(PagedQkvParams p) {
 constexpr int ATTN_WAVES = 4;
 constexpr int ATTN_THREADS = ATTN_WAVES * 64;
 constexpr int PART_KEYS = 32 * ATTN_WAVES;  // fewest keys of a part: a tile for each wave
-// Parts aimed at over all rows and KV heads: four workgroups for each of 256 CUs.
-constexpr int ATTN_TARGET = 1024;
-
+// Parts aimed at over all rows and KV heads: as many workgroups as 256 CUs hold at once (registers: six of
+// a head of 64, four of 128, two of 256).  More begin when others end and bring more parts to join, fewer
+// leave loads out: two rows of 131,072 keys 112.8 / 87.3 / 101.1 us with 512 / 1,024 / 1,536, a window
+// of 2,048 keys in 48 rows of heads of 64 45.3 / 39.6 / 38.0 with 1,024 / 1,536 / 2,048.
+constexpr int CUS = 256;
 inline int attn_tiles(int heads, int kv_heads) { return (heads / kv_heads + 15) / 16; }
-inline int attn_target(int heads, int kv_heads) {
-    return std::max(1, ATTN_TARGET / (kv_heads * attn_tiles(heads, kv_heads)));
+inline int attn_target(int heads, int kv_heads, int head_dim) {
+    const int held = head_dim <= 64 ? 6 : head_dim <= 128 ? 4 : 2;
+    return std::max(1, CUS * held / (kv_heads * attn_tiles(heads, kv_heads)));
 }
 
 struct Row {
@@ -324,7 +327,9 @@ __device__ __forceinline__ int part_chunk(const PagedAttnParams& p) {
     long long sum = 0;
     for (int r = lane; r < p.rows; r += 64) sum += row_keys(p, r).span;
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    const long long each = (sum + p.target - 1) / p.target;  // at most the longest table's keys per row
+    // a row's last part is half empty on the average
+    const int target = max(p.target - p.rows / 2, (p.target + 1) / 2);
+    const long long each = (sum + target - 1) / target;
     return each <= PART_KEYS ? PART_KEYS : int((each + PART_KEYS - 1) / PART_KEYS * PART_KEYS);
 }
 
@@ -376,6 +381,17 @@ struct Tile {
     bool whole;     // all keys of the tile are
 };
 
+// Reads of the pages: each once, so not to stay in the caches (nt: two rows of 131,072 keys 98.6 -> 88.2 us,
+// 128 ragged rows 41.7 -> 36.8), and issued where they stand (volatile).
+__device__ __forceinline__ uint4 stream16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    const u32x4_t v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, int(0x80000002u));
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ uint2 stream8(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    const u32x2_t v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, int(0x80000002u));
+    return make_uint2(v[0], v[1]);
+}
+
 // EVEN: pages of whole half tiles (a multiple of 16 tokens), so that a half tile is one page's and
 // its page and addresses are the wave's, not the lane's.
 template <int TYPE, int D, bool EVEN>
@@ -413,17 +429,17 @@ __device__ __forceinline__ void load_tile(Tile<TYPE, D>& t, const PagedAttnParam
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int s = 0; s < X::STEPS; ++s) t.k[h][s] = buffer_prefetch16(kr[h], ks + s * 64);
+            for (int s = 0; s < X::STEPS; ++s) t.k[h][s] = stream16(kr[h], ks + s * 64);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
             for (int s = 0; s < X::SLABS; ++s) {
                 const uint32_t at = uint32_t((4 * g + (i & 3)) * int(p.slot_stride) + col * X::CHUNK * 2 + s * 256);
                 if constexpr (X::CHUNK == 8) {
-                    const uint4 w = buffer_prefetch16(vr[i >> 2], at);
+                    const uint4 w = stream16(vr[i >> 2], at);
                     t.v[i][s][0] = w.x, t.v[i][s][1] = w.y, t.v[i][s][2] = w.z, t.v[i][s][3] = w.w;
                 } else {
-                    const uint2 w = buffer_load8(vr[i >> 2], at);
+                    const uint2 w = stream8(vr[i >> 2], at);
                     t.v[i][s][0] = w.x, t.v[i][s][1] = w.y;
                 }
             }
@@ -625,52 +641,60 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void paged_attention_kernel(PagedA
     }
 }
 
-// A head of a row from its parts, in a fixed order: D / 4 lanes hold the dims, the groups of lanes
-// take every GROUPS-th part.
+// A head of a row from its parts, in a fixed order: D / 4 lanes hold the dims, the groups of lanes take
+// every GROUPS-th part, eight parts' loads at once, with a running maximum; the groups are joined in LDS.
+// Bound by latency: the row's parts, then the parts themselves.
 constexpr int MERGE_THREADS = 512;
 
 template <int TYPE, int D>
 __global__ __launch_bounds__(MERGE_THREADS) void paged_merge_kernel(PagedAttnParams p) {
-    constexpr int LANES = D / 4, GROUPS = MERGE_THREADS / LANES;
+    constexpr int LANES = D / 4, GROUPS = MERGE_THREADS / LANES, AHEAD = 8;
     __shared__ __align__(16) float s_o[GROUPS][D];
-    __shared__ float s_m[MERGE_THREADS / 64], s_l[MERGE_THREADS / 64];
+    __shared__ float s_m[GROUPS], s_l[GROUPS];
     const int row = blockIdx.x, h = blockIdx.y, heads = p.kv_heads * p.group;
     const int2 parts = p.row_parts[row];
     if (parts.y == 1) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const float2* ml = p.part_ml + int64_t(parts.x) * heads + h;
-    float m = NEG_INF;
-    for (int i = tid; i < parts.y; i += MERGE_THREADS) m = fmaxf(m, ml[int64_t(i) * heads].x);
-    m = wave_max(m);
-    if (lane == 0) s_m[wave] = m;
-    __syncthreads();
-    for (int w = 0; w < MERGE_THREADS / 64; ++w) m = fmaxf(m, s_m[w]);
-    const float from = m == NEG_INF ? 0.f : m;
-    float l = 0.f;
-    for (int i = tid; i < parts.y; i += MERGE_THREADS) {
-        const float2 v = ml[int64_t(i) * heads];
-        l += v.y * __builtin_amdgcn_exp2f(v.x - from);
-    }
-    l = wave_sum(l);
-    if (lane == 0) s_l[wave] = l;
-    const int group = tid / LANES, d = (tid % LANES) * 4;
+    const int tid = threadIdx.x, group = tid / LANES, d = (tid % LANES) * 4;
+    const int64_t first = int64_t(parts.x) * heads + h;
+    float m = NEG_INF, l = 0.f;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float* o = p.part_o + (int64_t(parts.x) * heads + h) * D + d;
-#pragma unroll 4
-    for (int i = group; i < parts.y; i += GROUPS) {
-        const float share = __builtin_amdgcn_exp2f(ml[int64_t(i) * heads].x - from);
-        const float4 v = *reinterpret_cast<const float4*>(o + int64_t(i) * heads * D);
-        sum.x += v.x * share, sum.y += v.y * share, sum.z += v.z * share, sum.w += v.w * share;
+    for (int i = group; i < parts.y; i += GROUPS * AHEAD) {
+        float2 ml[AHEAD];
+        float4 o[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            const int64_t at = first + int64_t(min(i + a * GROUPS, parts.y - 1)) * heads;
+            ml[a] = p.part_ml[at];
+            o[a] = *reinterpret_cast<const float4*>(p.part_o + at * D + d);
+        }
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            if (i + a * GROUPS >= parts.y) break;
+            const float most = fmaxf(m, ml[a].x), from = most == NEG_INF ? 0.f : most;
+            const float keep = __builtin_amdgcn_exp2f(m - from), share = __builtin_amdgcn_exp2f(ml[a].x - from);
+            m = most;
+            l = l * keep + ml[a].y * share;
+            sum.x = sum.x * keep + o[a].x * share, sum.y = sum.y * keep + o[a].y * share;
+            sum.z = sum.z * keep + o[a].z * share, sum.w = sum.w * keep + o[a].w * share;
+        }
     }
     *reinterpret_cast<float4*>(&s_o[group][d]) = sum;
+    if (d == 0) {
+        s_m[group] = m;
+        s_l[group] = l;
+    }
     __syncthreads();
-    l = 0.f;
-    for (int w = 0; w < MERGE_THREADS / 64; ++w) l += s_l[w];
     if (tid < LANES) {
+        const int live = min(GROUPS, parts.y);
+        for (int k = 0; k < live; ++k) m = fmaxf(m, s_m[k]);
+        const float from = m == NEG_INF ? 0.f : m;
+        l = 0.f;
         sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = 0; k < GROUPS; ++k) {
+        for (int k = 0; k < live; ++k) {
+            const float share = __builtin_amdgcn_exp2f(s_m[k] - from);
             const float4 v = *reinterpret_cast<const float4*>(&s_o[k][d]);
-            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+            l += s_l[k] * share;
+            sum.x += v.x * share, sum.y += v.y * share, sum.z += v.z * share, sum.w += v.w * share;
         }
         const float r = l == 0.f ? 0.f : 1.0f / l;
         *reinterpret_cast<uint2*>(p.out + row * p.out_stride + int64_t(h) * D + d) =
@@ -682,7 +706,8 @@ __global__ __launch_bounds__(MERGE_THREADS) void paged_merge_kernel(PagedAttnPar
 
 template <int TYPE, int D>
 void run_attention(const PagedAttnParams& p, hipStream_t s) {
-    // parts: at most one more than its share of the aimed ones for each row, and none of less than PART_KEYS
+    // parts: at most one more than its share of the aimed ones for each row, and none of less than PART_KEYS but a
+    // row's only one
     const int64_t most = int64_t(p.rows) * std::max<int64_t>(1, (int64_t(p.most) + 15 + PART_KEYS - 1) / PART_KEYS);
     const unsigned parts = unsigned(std::min<int64_t>(most, int64_t(p.rows) + p.target));
     const dim3 grid(parts, unsigned(p.kv_heads * p.tiles));
@@ -724,7 +749,7 @@ void launch_paged_qkv(const PagedQkvParams& p, int source, int type, int head_di
 }
 
 size_t paged_attn_workspace(int rows, int heads, int kv_heads, int head_dim) {
-    const size_t parts = size_t(rows) + size_t(attn_target(heads, kv_heads));
+    const size_t parts = size_t(rows) + size_t(attn_target(heads, kv_heads, head_dim));
     const size_t lists = (size_t(rows) * sizeof(int2) + 15) / 16 * 16 + (parts * size_t(heads) * sizeof(float2) + 15) / 16 * 16;
     return lists + parts * size_t(heads) * size_t(head_dim) * sizeof(float);
 }
@@ -732,7 +757,7 @@ size_t paged_attn_workspace(int rows, int heads, int kv_heads, int head_dim) {
 void paged_attn_bind(PagedAttnParams& p, void* workspace, int head_dim) {
     const int heads = p.kv_heads * p.group;
     p.tiles = attn_tiles(heads, p.kv_heads);
-    p.target = attn_target(heads, p.kv_heads);
+    p.target = attn_target(heads, p.kv_heads, head_dim);
     const size_t parts = size_t(p.rows) + size_t(p.target);
     char* at = static_cast<char*>(workspace);
     p.row_parts = reinterpret_cast<int2*>(at);
