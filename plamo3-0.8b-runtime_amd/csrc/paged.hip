@@ -27,50 +27,64 @@ __device__ __forceinline__ uint32_t divide(uint32_t x, Divider d) { return uint3
 
 // ------------------------------------------------------------------------------------ tables
 // One workgroup: prefix sums over the requests of pages given back, pages taken and tokens, then the
-// moves flattened over pages so that a long request's are not one thread's.  Latency-bound: at 64
-// requests the few KB move in the time of the dependent loads and barriers.
+// moves flattened over pages so that a long request's are not one thread's.  Latency-bound: a few KB move
+// in the time of some dependent loads (lengths, free pages, tables) and barriers.
 constexpr int TABLE_THREADS = 1024;
+
+// Places up to which the tables' workgroup fills in the slots too.
+constexpr int SLOTS_IN_TABLES = 2048;
 
 struct Scan3 {
     int back, take, fresh;
 };
 
-// Inclusive sums over the workgroup; `total` in every thread.
-__device__ Scan3 block_scan3(Scan3 v, Scan3* waves, Scan3& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int o = 1; o < 64; o <<= 1) {
-        const int a = __shfl_up(v.back, o, 64), b = __shfl_up(v.take, o, 64), c = __shfl_up(v.fresh, o, 64);
-        if (lane >= o) {
-            v.back += a;
-            v.take += b;
-            v.fresh += c;
-        }
-    }
+// v of the lane that a DPP control names, 0 where there is none (or the row is not in ROWS).
+template <int CONTROL, int ROWS = 0xf>
+__device__ __forceinline__ int shifted(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CONTROL, ROWS, 0xf, false);
+}
+template <int CONTROL, int ROWS = 0xf>
+__device__ __forceinline__ void add_shifted(Scan3& v) {
+    v.back += shifted<CONTROL, ROWS>(v.back);
+    v.take += shifted<CONTROL, ROWS>(v.take);
+    v.fresh += shifted<CONTROL, ROWS>(v.fresh);
+}
+
+// Inclusive sums over the workgroup; `total` in every thread.  Rows of 16 lanes by shifts of 1, 2, 4 and 8,
+// then the last lane of the row, and of the half, before; the waves' sums as one such row.
+__device__ __forceinline__ Scan3 block_scan3(Scan3 v, Scan3* waves, Scan3& total) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    add_shifted<0x111>(v);
+    add_shifted<0x112>(v);
+    add_shifted<0x114>(v);
+    add_shifted<0x118>(v);
+    add_shifted<0x142, 0xa>(v);
+    add_shifted<0x143, 0xc>(v);
     __syncthreads();  // the sums of a scan before this one have been read
     if (lane == 63) waves[wave] = v;
     __syncthreads();
-    total = {0, 0, 0};
-    for (int w = 0; w < TABLE_THREADS / 64; ++w) {
-        if (w == wave) {
-            v.back += total.back;
-            v.take += total.take;
-            v.fresh += total.fresh;
-        }
-        total.back += waves[w].back;
-        total.take += waves[w].take;
-        total.fresh += waves[w].fresh;
+    static_assert(TABLE_THREADS / 64 == 16, "a row");
+    Scan3 sum = waves[lane & 15];
+    add_shifted<0x111>(sum);
+    add_shifted<0x112>(sum);
+    add_shifted<0x114>(sum);
+    add_shifted<0x118>(sum);
+    auto of = [&](int l) -> Scan3 {
+        return {__builtin_amdgcn_readlane(sum.back, l), __builtin_amdgcn_readlane(sum.take, l), __builtin_amdgcn_readlane(sum.fresh, l)};
+    };
+    total = of(15);
+    if (wave > 0) {
+        const Scan3 before = of(wave - 1);
+        v = {v.back + before.back, v.take + before.take, v.fresh + before.fresh};
     }
     return v;
 }
 
-// What row r asks for, from its length and count (both checked).
-__device__ __forceinline__ Scan3 row_moves(const PagedTablesParams& p, int r, int& held) {
-    held = 0;
-    if (r >= p.rows) return {0, 0, 0};
-    const int64_t length = p.lengths[r], count = p.counts[r];
-    held = int((length + p.page_size - 1) / p.page_size);
+// What a request of this length and count (both checked) asks for.
+__device__ __forceinline__ Scan3 row_moves(const PagedTablesParams& p, int length, int count, int& held) {
+    held = int((int64_t(length) + p.page_size - 1) / p.page_size);
     if (count < 0) return {held, 0, 0};
-    return {0, int((length + count + p.page_size - 1) / p.page_size) - held, int(count)};
+    return {0, int((int64_t(length) + count + p.page_size - 1) / p.page_size) - held, count};
 }
 
 // The first of `n` ascending inclusive sums above x.
@@ -113,12 +127,18 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(PagedTables
         s_status = 0;
     }
     const int64_t first = *p.free_count;
+    // the first TABLE_THREADS requests' stay in registers
+    int own_length = 0, own_count = 0;
+    if (tid < p.rows) {
+        own_length = p.lengths[tid];
+        own_count = p.counts[tid];
+    }
     __syncthreads();
     // totals and checks before anything is written
     int bad = 0;
-    int64_t back = 0, take = 0, fresh = 0;
+    long long back = 0, take = 0, fresh = 0;
     for (int r = tid; r < p.rows; r += TABLE_THREADS) {
-        const int64_t length = p.lengths[r], count = p.counts[r];
+        const int64_t length = r == tid ? own_length : p.lengths[r], count = r == tid ? own_count : p.counts[r];
         if (length < 0 || count < -1) {
             bad |= 8;
             continue;
@@ -129,10 +149,18 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(PagedTables
         if (count < 0) back += held;
         else take += after - held, fresh += count;
     }
-    if (bad) atomicOr(&s_status, bad);
-    if (back) atomicAdd(&s_back, static_cast<unsigned long long>(back));
-    if (take) atomicAdd(&s_take, static_cast<unsigned long long>(take));
-    if (fresh) atomicAdd(&s_fresh, static_cast<unsigned long long>(fresh));
+    for (int o = 32; o > 0; o >>= 1) {
+        back += __shfl_xor(back, o, 64);
+        take += __shfl_xor(take, o, 64);
+        fresh += __shfl_xor(fresh, o, 64);
+        bad |= __shfl_xor(bad, o, 64);
+    }
+    if ((tid & 63) == 0) {
+        if (bad) atomicOr(&s_status, bad);
+        atomicAdd(&s_back, static_cast<unsigned long long>(back));
+        atomicAdd(&s_take, static_cast<unsigned long long>(take));
+        atomicAdd(&s_fresh, static_cast<unsigned long long>(fresh));
+    }
     __syncthreads();
     const int64_t full = first + int64_t(s_back);
     int status = s_status;
@@ -151,31 +179,36 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(PagedTables
             p.lengths_out[r] = p.lengths[r];
         }
     } else {
-        // pages given back, on top of the free ones, in row order; lengths and offsets, unless the
-        // lengths are still read by the second pass
-        Scan3 run = {0, 0, 0}, sum;
-        for (int pass = 0; pass < 2; ++pass) {
-            run = {0, 0, 0};
+        // pages given back, on top of the free ones, in row order; then pages taken, lengths and offsets
+        Scan3 sum;
+        for (int pass = s_back ? 0 : 1; pass < 2; ++pass) {
+            Scan3 run = {0, 0, 0};
             for (int base = 0; base < p.rows; base += TABLE_THREADS) {
                 const int r = base + tid;
-                int held;
-                const Scan3 own = row_moves(p, r, held);
+                int held = 0, length = own_length, count = own_count;
+                if (base > 0 && r < p.rows) {
+                    length = p.lengths[r];
+                    count = p.counts[r];
+                }
+                const Scan3 own = r < p.rows ? row_moves(p, length, count, held) : Scan3{0, 0, 0};
                 const Scan3 incl = block_scan3(own, s_waves, sum);
                 const int moved = pass ? own.take : own.back, chunk = pass ? sum.take : sum.back;
                 const int before = pass ? run.take : run.back;
-                s_sums[tid] = pass ? incl.take : incl.back;
-                s_start[tid] = s_sums[tid] - moved;
-                s_held[tid] = held;
-                __syncthreads();
-                for (int e = tid; e < chunk; e += TABLE_THREADS) {
-                    const int q = first_above(s_sums, TABLE_THREADS, e), i = e - s_start[q];
-                    int32_t* table = p.tables + int64_t(base + q) * p.width;
-                    if (pass) table[s_held[q] + i] = p.free_pages[full - 1 - (before + e)];
-                    else p.free_pages[first + before + e] = table[i];
+                if (chunk) {
+                    s_sums[tid] = pass ? incl.take : incl.back;
+                    s_start[tid] = s_sums[tid] - moved;
+                    s_held[tid] = held;
+                    __syncthreads();
+                    for (int e = tid; e < chunk; e += TABLE_THREADS) {
+                        const int q = first_above(s_sums, TABLE_THREADS, e), i = e - s_start[q];
+                        int32_t* table = p.tables + int64_t(base + q) * p.width;
+                        if (pass) table[s_held[q] + i] = p.free_pages[full - 1 - (before + e)];
+                        else p.free_pages[first + before + e] = table[i];
+                    }
                 }
                 if (pass && r < p.rows) {
                     p.offsets[r + 1] = run.fresh + incl.fresh;
-                    p.lengths_out[r] = p.counts[r] < 0 ? 0 : p.lengths[r] + p.counts[r];
+                    p.lengths_out[r] = count < 0 ? 0 : length + count;
                 }
                 run = {run.back + sum.back, run.take + sum.take, run.fresh + sum.fresh};
             }
@@ -732,9 +765,12 @@ void run_qkv(const PagedQkvParams& p, int head_dim, hipStream_t s) {
 }  // namespace
 
 void launch_paged_tables(const PagedTablesParams& p, hipStream_t s) {
+    if (p.capacity <= SLOTS_IN_TABLES) {
+        hipLaunchKernelGGL((paged_tables_kernel<true>), dim3(1), dim3(TABLE_THREADS), 0, s, p);
+        return;
+    }
     hipLaunchKernelGGL((paged_tables_kernel<false>), dim3(1), dim3(TABLE_THREADS), 0, s, p);
-    if (p.capacity > 0)
-        hipLaunchKernelGGL(paged_slots_kernel, dim3(unsigned((p.capacity + 255) / 256)), dim3(256), 0, s, p);
+    hipLaunchKernelGGL(paged_slots_kernel, dim3(unsigned((p.capacity + 255) / 256)), dim3(256), 0, s, p);
 }
 
 void launch_paged_qkv(const PagedQkvParams& p, int source, int type, int head_dim, hipStream_t s) {
