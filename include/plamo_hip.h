@@ -414,7 +414,7 @@ int plamo_kernel_paged_tables(uint64_t lengths, uint64_t counts, int32_t rows, u
  * keys, values; `type` PLAMO_F32 or the cache's, qkv_stride elements between rows).  q_norm, k_norm
  * ([head_dim], the cache's type; 0: none): x / sqrt(mean(x^2) + 1e-6) * (1 + gain).  rope (0: none;
  * [rope_rows][head_dim / 2] words as plamo_rope_table makes them): pairs (d, d + head_dim / 2) turned by
- * row positions[token].  FP32 inside, rounded once.  Queries go to q [tokens][heads * head_dim] (the
+ * row positions[token].  Rows, gains and rope are 16-byte aligned.  FP32 inside, rounded once.  Queries go to q [tokens][heads * head_dim] (the
  * cache's type; rows of that type may be overwritten in place), keys and values to slots[token].  A token
  * with a position below 0 or from rope_rows on is skipped, and one with a slot outside the cache leaves
  * the cache as it is.  Slots that are not skipped have to differ. */

@@ -951,9 +951,9 @@ int plamo_kernel_paged_qkv(const plamo_paged_cache* cache, uint64_t qkv, int32_t
                     q_stride % 8 == 0,
                 "paged qkv: row strides must hold a row and be multiples of 16 bytes");
         require(int64_t(tokens) * wide / 8 <= INT32_MAX, "paged qkv: too many rows");
-        require((tokens == 0 || (qkv && q && slots)) && aligned(qkv, 16) && aligned(q, 16) && aligned(q_norm, 8) && aligned(k_norm, 8) &&
+        require((tokens == 0 || (qkv && q && slots)) && aligned(qkv, 16) && aligned(q, 16) && aligned(q_norm, 16) && aligned(k_norm, 16) &&
                     aligned(rope, 16),
-                "paged qkv: rows and rope must be 16-byte aligned, gains 8-byte");
+                "paged qkv: rows, gains and rope must be 16-byte aligned");
         require(!rope || ((positions || tokens == 0) && rope_rows >= 1), "paged qkv: a rotation needs positions and rope_rows");
         const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
         const OnDeviceOf device(s);

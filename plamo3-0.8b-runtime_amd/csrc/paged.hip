@@ -240,59 +240,69 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
     return __builtin_bit_cast(uint32_t, h);
 }
 template <int SOURCE>
-__device__ __forceinline__ void load4(const void* base, int64_t at, float (&v)[4]) {
+__device__ __forceinline__ void load8(const void* base, int64_t at, float (&v)[8]) {
     if constexpr (SOURCE == TYPE_F32) {
-        const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
+        const float4* from = reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
+        const float4 x = from[0], y = from[1];
         v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+        v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
     } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + at);
+        const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at);
         v[0] = from16<SOURCE>(x.x), v[1] = from16<SOURCE>(x.x >> 16);
         v[2] = from16<SOURCE>(x.y), v[3] = from16<SOURCE>(x.y >> 16);
+        v[4] = from16<SOURCE>(x.z), v[5] = from16<SOURCE>(x.z >> 16);
+        v[6] = from16<SOURCE>(x.w), v[7] = from16<SOURCE>(x.w >> 16);
     }
+}
+template <int TYPE>
+__device__ __forceinline__ void store8(uint16_t* to, const float (&v)[8]) {
+    *reinterpret_cast<uint4*>(to) =
+        make_uint4(pack16<TYPE>(v[0], v[1]), pack16<TYPE>(v[2], v[3]), pack16<TYPE>(v[4], v[5]), pack16<TYPE>(v[6], v[7]));
 }
 
 // y = x / sqrt(mean(x^2) + 1e-6) (1 + g), (y_i, y_{i + D/2}) turned by the position's angle, rounded
-// once.  D / 8 lanes hold a head, each four dims of its first half and the same four of its second, so
-// that the rotation stays in a lane.  Bound by memory: each element is read and written once.
+// once.  D / 16 lanes hold a head, each eight dims of its first half and the same eight of its second, so
+// that the rotation stays in a lane and BF16 rows move in 16 bytes.  Bound by memory: each element is read
+// and written once.
 template <int SOURCE, int TYPE, int D>
 __global__ __launch_bounds__(256) void paged_qkv_kernel(PagedQkvParams p) {
-    constexpr int LANES = D / 8;
+    constexpr int LANES = D / 16;
     const int wide = p.heads + 2 * p.kv_heads;
     const int64_t item = (int64_t(blockIdx.x) * 256 + threadIdx.x) / LANES;
     if (item >= int64_t(p.tokens) * wide) return;  // whole groups of lanes
-    const int t = int(item / wide), h = int(item - int64_t(t) * wide), d = int(threadIdx.x % LANES) * 4;
+    const int t = int(item / wide), h = int(item - int64_t(t) * wide), d = int(threadIdx.x % LANES) * 8;
     const int pos = p.positions ? p.positions[t] : 0;
     if (p.rope ? uint32_t(pos) >= uint32_t(p.rope_rows) : pos < 0) return;  // a padding row
-    float a[4], b[4];
+    float a[8], b[8];
     const int64_t at = t * p.stride + int64_t(h) * D + d;
-    load4<SOURCE>(p.qkv, at, a);
-    load4<SOURCE>(p.qkv, at + D / 2, b);
+    load8<SOURCE>(p.qkv, at, a);
+    load8<SOURCE>(p.qkv, at + D / 2, b);
     const bool query = h < p.heads, value = h >= p.heads + p.kv_heads;
     const uint16_t* gain = value ? nullptr : query ? p.q_norm : p.k_norm;
     if (gain) {
         float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ss += a[i] * a[i] + b[i] * b[i];
-        if constexpr (LANES > 16) ss += xor_lane<16>(ss);
+        for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
         if constexpr (LANES > 8) ss += xor_lane<8>(ss);
-        ss += xor_lane<4>(ss);
+        if constexpr (LANES > 4) ss += xor_lane<4>(ss);
         ss += xor_lane<2>(ss);
         ss += xor_lane<1>(ss);
         const float r = 1.0f / sqrtf(ss / float(D) + 1e-6f);
-        float ga[4], gb[4];
-        load4<TYPE>(gain, d, ga);
-        load4<TYPE>(gain, d + D / 2, gb);
+        float ga[8], gb[8];
+        load8<TYPE>(gain, d, ga);
+        load8<TYPE>(gain, d + D / 2, gb);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 8; ++i) {
             a[i] = a[i] * r * (1.0f + ga[i]);
             b[i] = b[i] * r * (1.0f + gb[i]);
         }
     }
     if (p.rope && !value) {
-        const uint4 w = *reinterpret_cast<const uint4*>(p.rope + int64_t(pos) * (D / 2) + d);
-        const uint32_t cs[4] = {w.x, w.y, w.z, w.w};
+        const uint4* w = reinterpret_cast<const uint4*>(p.rope + int64_t(pos) * (D / 2) + d);
+        const uint4 u = w[0], v = w[1];
+        const uint32_t cs[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 8; ++i) {
             const float c = lo(cs[i]), s = hi(cs[i]), x = a[i], y = b[i];
             a[i] = x * c - y * s;
             b[i] = y * c + x * s;
@@ -309,8 +319,8 @@ __global__ __launch_bounds__(256) void paged_qkv_kernel(PagedQkvParams p) {
              int64_t(slot - int(page) * p.page_size) * p.slot_stride +
              int64_t(h - p.heads - (value ? p.kv_heads : 0)) * p.head_stride;
     }
-    *reinterpret_cast<uint2*>(to + d) = make_uint2(pack16<TYPE>(a[0], a[1]), pack16<TYPE>(a[2], a[3]));
-    *reinterpret_cast<uint2*>(to + d + D / 2) = make_uint2(pack16<TYPE>(b[0], b[1]), pack16<TYPE>(b[2], b[3]));
+    store8<TYPE>(to + d, a);
+    store8<TYPE>(to + d + D / 2, b);
 }
 
 // ------------------------------------------------------------------------------------ attention
@@ -755,7 +765,7 @@ void run_attention(const PagedAttnParams& p, hipStream_t s) {
 
 template <int SOURCE, int TYPE>
 void run_qkv(const PagedQkvParams& p, int head_dim, hipStream_t s) {
-    const int64_t threads = int64_t(p.tokens) * (p.heads + 2 * p.kv_heads) * (head_dim / 8);
+    const int64_t threads = int64_t(p.tokens) * (p.heads + 2 * p.kv_heads) * (head_dim / 16);
     const dim3 grid(unsigned((threads + 255) / 256));
     if (head_dim == 64) hipLaunchKernelGGL((paged_qkv_kernel<SOURCE, TYPE, 64>), grid, dim3(256), 0, s, p);
     else if (head_dim == 128) hipLaunchKernelGGL((paged_qkv_kernel<SOURCE, TYPE, 128>), grid, dim3(256), 0, s, p);

@@ -146,7 +146,7 @@ def qkv64(qkv, heads, kv, dim, positions, cos, sin, gains):
         x[:, turned, :dim // 2], x[:, turned, dim // 2:] = a * c - b * s, b * c + a * s
         both = a.abs() + b.abs()
         size[:, turned, :dim // 2], size[:, turned, dim // 2:] = both, both
-    # the sum of squares is off by 40 roundings at most (8 in a lane, 5 joins, twice for a product), half
+    # the sum of squares is off by 40 roundings at most (16 in a lane, 4 joins, twice for a product), half
     # of which reach its root; a dozen more follow
     return x, size * 32 * 2.0 ** -24
 

@@ -72,7 +72,7 @@ def test_no_cache():
     dict(type=1), dict(type=3), dict(heads=0), dict(heads=4097), dict(cache=cache(kv_heads=3)), dict(tokens=-1),
     dict(qkv_stride=18 * 128 - 4), dict(qkv_stride=18 * 128 + 1), dict(type=0, qkv_stride=18 * 128 + 4), dict(q_stride=2040),
     dict(q_stride=2050), dict(tokens=1 << 30), dict(qkv=0), dict(q=0), dict(slots=0), dict(qkv=A + 4), dict(q=A + 8),
-    dict(q_norm=A + 2), dict(k_norm=A + 4), dict(rope=A + 8), dict(positions=0), dict(rope_rows=0)])
+    dict(q_norm=A + 2), dict(k_norm=A + 8), dict(rope=A + 8), dict(positions=0), dict(rope_rows=0)])
 def test_qkv(changed):
     rc, message = call("plamo_kernel_paged_qkv", **changed)
     assert rc == 1 and message.startswith("paged qkv: ")
