@@ -364,39 +364,81 @@ __device__ __forceinline__ Row row_keys(const PagedAttnParams& p, int r) {
 }
 __device__ __forceinline__ int row_parts(int span, int chunk) { return max(1, (span + chunk - 1) / chunk); }
 
-// Keys of a part: all rows' keys divided by the parts aimed at (the same in every wave of the launch).
-__device__ __forceinline__ int part_chunk(const PagedAttnParams& p) {
-    const int lane = threadIdx.x & 63;
-    long long sum = 0;
-    for (int r = lane; r < p.rows; r += 64) sum += row_keys(p, r).span;
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    // a row's last part is half empty on the average
-    const int target = max(p.target - p.rows / 2, (p.target + 1) / 2);
-    const long long each = (sum + target - 1) / target;
-    return each <= PART_KEYS ? PART_KEYS : int((each + PART_KEYS - 1) / PART_KEYS * PART_KEYS);
+// Where the workgroups find their work: the same division in all of them, from all rows' lengths.
+struct Work {
+    int row, first, parts;  // of the part, the row's first part and number of parts
+};
+struct WorkShared {
+    long long keys[ATTN_WAVES];
+    int parts[ATTN_WAVES];
+    Work found;
+};
+
+// Inclusive sum over the wave, as in block_scan3.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += shifted<0x111>(v);
+    v += shifted<0x112>(v);
+    v += shifted<0x114>(v);
+    v += shifted<0x118>(v);
+    v += shifted<0x142, 0xa>(v);
+    v += shifted<0x143, 0xc>(v);
+    return v;
 }
 
-// The row that part `item` belongs to and the row's first part; false past the last part.
-__device__ __forceinline__ bool find_part(const PagedAttnParams& p, int chunk, int item, int& row, int& first, int& parts) {
-    const int lane = threadIdx.x & 63;
+// The row of part `item`; false past the last part.  Keys of a part: all rows' keys divided by the parts aimed
+// at, in whole tiles for each wave.  The waves look through 64 rows each at a time; up to 64 rows every wave
+// does for itself, without waiting for the others.
+__device__ __forceinline__ bool find_work(const PagedAttnParams& p, WorkShared& s, int item, Work& work) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool few = p.rows <= 64;
+    long long keys = 0;
+    for (int r = few ? lane : int(threadIdx.x); r < p.rows; r += ATTN_THREADS) keys += row_keys(p, r).span;
+    for (int o = 32; o > 0; o >>= 1) keys += __shfl_xor(keys, o, 64);
+    if (!few) {
+        if (lane == 0) s.keys[wave] = keys;
+        __syncthreads();
+        keys = 0;
+        for (int w = 0; w < ATTN_WAVES; ++w) keys += s.keys[w];
+    }
+    // a row's last part is half empty on the average
+    const int target = max(p.target - p.rows / 2, (p.target + 1) / 2);
+    const long long each = (keys + target - 1) / target;
+    const int chunk = __builtin_amdgcn_readfirstlane(each <= PART_KEYS ? PART_KEYS : int((each + PART_KEYS - 1) / PART_KEYS * PART_KEYS));
     int run = 0;
-    for (int base = 0; base < p.rows; base += 64) {
-        const int r = base + lane;
+    for (int base = 0; base < p.rows; base += few ? 64 : ATTN_THREADS) {
+        const int r = base + (few ? lane : int(threadIdx.x));
         const int own = r < p.rows ? row_parts(row_keys(p, r).span, chunk) : 0;
-        int incl = own;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(incl, o, 64);
-            if (lane >= o) incl += v;
+        const int incl = wave_scan(own), all = __builtin_amdgcn_readlane(incl, 63);
+        int before = run;
+        if (!few) {
+            __syncthreads();  // what the last rows' sums said has been read
+            if (lane == 0) s.parts[wave] = all;
+            __syncthreads();
+            for (int w = 0; w < ATTN_WAVES; ++w) {
+                before += w < wave ? s.parts[w] : 0;
+                run += s.parts[w];
+            }
+        } else {
+            run += all;
         }
-        const unsigned long long past = __ballot(run + incl > item);
-        if (past) {
-            const int l = __ffsll(past) - 1;
-            row = __builtin_amdgcn_readfirstlane(base + l);
-            parts = __builtin_amdgcn_readlane(own, l);
-            first = run + __builtin_amdgcn_readlane(incl, l) - parts;
+        if (item < run) {
+            const unsigned long long past = __ballot(before + incl > item && before <= item);
+            Work here = {0, 0, 0};
+            if (past) {
+                const int l = __ffsll(past) - 1;
+                here = {__builtin_amdgcn_readlane(r, l), 0, __builtin_amdgcn_readlane(own, l)};
+                here.first = before + __builtin_amdgcn_readlane(incl, l) - here.parts;
+            }
+            if (few) {
+                work = here;
+                return true;
+            }
+            if (past && lane == 0) s.found = here;
+            __syncthreads();
+            work = {__builtin_amdgcn_readfirstlane(s.found.row), __builtin_amdgcn_readfirstlane(s.found.first),
+                    __builtin_amdgcn_readfirstlane(s.found.parts)};
             return true;
         }
-        run += __builtin_amdgcn_readlane(incl, 63);
     }
     return false;
 }
@@ -487,34 +529,37 @@ __device__ __forceinline__ void load_tile(Tile<TYPE, D>& t, const PagedAttnParam
                 }
             }
     } else {
-        auto place = [&](int j, bool& there) {
-            int page = -1;
-            const uint32_t index = divide(uint32_t(j), p.div);
-            if (j >= lo_key && j < hi_key) page = table[index];
-            there = uint32_t(page) < uint32_t(p.pages);
-            return there ? page * p.page_stride + (j - int(index) * p.page_size) * p.slot_stride + head : int64_t(0);
-        };
+        // lane j looks key j of the tile up, for all lanes that read it; -1: not seen
+        const int key = pos + (lane & 31);
+        int64_t own = -1;
+        if (key >= lo_key && key < hi_key) {
+            const uint32_t index = divide(uint32_t(key), p.div);
+            const int page = table[index];
+            if (uint32_t(page) < uint32_t(p.pages))
+                own = page * p.page_stride + (key - int(index) * p.page_size) * p.slot_stride + head;
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            bool there;
-            const int64_t off = place(pos + 16 * h + col, there) + g * 16;
+            const int64_t off = __shfl(own, 16 * h + col, 64);
 #pragma unroll
             for (int s = 0; s < X::STEPS; ++s)
-                t.k[h][s] = there ? *reinterpret_cast<const uint4*>(p.keys + off + s * 64) : make_uint4(0, 0, 0, 0);
+                t.k[h][s] = off >= 0 ? *reinterpret_cast<const uint4*>(p.keys + off + g * 16 + s * 64) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            bool there;
-            const int64_t off = place(pos + 16 * (i >> 2) + 4 * g + (i & 3), there) + col * X::CHUNK * 2;
-            if (!there) t.seen &= ~(1u << i);
+            const int64_t off = __shfl(own, 16 * (i >> 2) + 4 * g + (i & 3), 64);
+            if (off < 0) t.seen &= ~(1u << i);
 #pragma unroll
-            for (int s = 0; s < X::SLABS; ++s)
-#pragma unroll
-                for (int w = 0; w < X::CHUNK / 2; w += 2) {
-                    const uint2 x = there ? *reinterpret_cast<const uint2*>(p.values + off + s * 256 + w * 4) : make_uint2(0, 0);
-                    t.v[i][s][w] = x.x;
-                    t.v[i][s][w + 1] = x.y;
+            for (int s = 0; s < X::SLABS; ++s) {
+                const char* from = p.values + off + col * X::CHUNK * 2 + s * 256;
+                if constexpr (X::CHUNK == 8) {
+                    const uint4 x = off >= 0 ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
+                    t.v[i][s][0] = x.x, t.v[i][s][1] = x.y, t.v[i][s][2] = x.z, t.v[i][s][3] = x.w;
+                } else {
+                    const uint2 x = off >= 0 ? *reinterpret_cast<const uint2*>(from) : make_uint2(0, 0);
+                    t.v[i][s][0] = x.x, t.v[i][s][1] = x.y;
                 }
+            }
         }
         t.whole = __all(t.seen == 0xffu);
     }
@@ -596,18 +641,22 @@ __device__ __forceinline__ void take_tile(Running<TYPE, D>& run, Tile<TYPE, D>& 
         }
 }
 
+// Waves of a SIMD whose registers hold them (uneven pages hold 64-bit addresses too).
+constexpr int attn_waves(int head_dim, bool even) { return head_dim == 64 ? (even ? 6 : 5) : head_dim == 128 ? (even ? 4 : 3) : 2; }
+
 template <int TYPE, int D, bool EVEN>
-__global__ __launch_bounds__(ATTN_THREADS, 2) void paged_attention_kernel(PagedAttnParams p) {
+__global__ __launch_bounds__(ATTN_THREADS, attn_waves(D, EVEN)) void paged_attention_kernel(PagedAttnParams p) {
     typedef Tile<TYPE, D> X;
     constexpr int PITCH = D + 4;
     __shared__ __align__(16) float s_o[ATTN_WAVES][16][PITCH];
     __shared__ float s_m[ATTN_WAVES][16], s_l[ATTN_WAVES][16];
+    __shared__ WorkShared s_work;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int item = blockIdx.x, kv = blockIdx.y / p.tiles, tile = blockIdx.y - kv * p.tiles;
-    const int chunk = __builtin_amdgcn_readfirstlane(part_chunk(p));
-    int row, first_part, parts;
-    if (!find_part(p, chunk, item, row, first_part, parts)) return;  // every wave of the workgroup
+    Work work;
+    if (!find_work(p, s_work, item, work)) return;  // every wave of the workgroup
+    const int row = work.row, first_part = work.first, parts = work.parts;
     const Row keys = row_keys(p, row);
     const int len = __builtin_amdgcn_readfirstlane(keys.len), first = __builtin_amdgcn_readfirstlane(keys.first);
     const int part = item - first_part;
@@ -684,24 +733,27 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void paged_attention_kernel(PagedA
     }
 }
 
-// A head of a row from its parts, in a fixed order: D / 4 lanes hold the dims, the groups of lanes take
-// every GROUPS-th part, eight parts' loads at once, with a running maximum; the groups are joined in LDS.
-// Bound by latency: the row's parts, then the parts themselves.
+// HEADS heads of a row from their parts, in a fixed order: D / 4 lanes hold a head's dims, its groups of
+// lanes take every GROUPS-th part, eight parts' loads at once, with a running maximum; the groups are joined
+// in LDS.  Bound by latency: the row's parts, then the parts themselves.
 constexpr int MERGE_THREADS = 512;
 
-template <int TYPE, int D>
+template <int TYPE, int D, int HEADS>
 __global__ __launch_bounds__(MERGE_THREADS) void paged_merge_kernel(PagedAttnParams p) {
-    constexpr int LANES = D / 4, GROUPS = MERGE_THREADS / LANES, AHEAD = 8;
-    __shared__ __align__(16) float s_o[GROUPS][D];
-    __shared__ float s_m[GROUPS], s_l[GROUPS];
-    const int row = blockIdx.x, h = blockIdx.y, heads = p.kv_heads * p.group;
+    constexpr int LANES = D / 4, GROUPS = MERGE_THREADS / (LANES * HEADS), AHEAD = 8;
+    __shared__ __align__(16) float s_o[HEADS][GROUPS][D];
+    __shared__ float s_m[HEADS][GROUPS], s_l[HEADS][GROUPS];
+    const int row = blockIdx.x, heads = p.kv_heads * p.group;
     const int2 parts = p.row_parts[row];
     if (parts.y == 1) return;
-    const int tid = threadIdx.x, group = tid / LANES, d = (tid % LANES) * 4;
+    const int sub = threadIdx.x / (MERGE_THREADS / HEADS), tid = threadIdx.x - sub * (MERGE_THREADS / HEADS);
+    const int group = tid / LANES, d = (tid % LANES) * 4;
+    const int h = blockIdx.y * HEADS + sub;
+    const bool live_head = h < heads;
     const int64_t first = int64_t(parts.x) * heads + h;
     float m = NEG_INF, l = 0.f;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = group; i < parts.y; i += GROUPS * AHEAD) {
+    for (int i = live_head ? group : parts.y; i < parts.y; i += GROUPS * AHEAD) {
         float2 ml[AHEAD];
         float4 o[AHEAD];
 #pragma unroll
@@ -721,22 +773,22 @@ __global__ __launch_bounds__(MERGE_THREADS) void paged_merge_kernel(PagedAttnPar
             sum.z = sum.z * keep + o[a].z * share, sum.w = sum.w * keep + o[a].w * share;
         }
     }
-    *reinterpret_cast<float4*>(&s_o[group][d]) = sum;
+    *reinterpret_cast<float4*>(&s_o[sub][group][d]) = sum;
     if (d == 0) {
-        s_m[group] = m;
-        s_l[group] = l;
+        s_m[sub][group] = m;
+        s_l[sub][group] = l;
     }
     __syncthreads();
-    if (tid < LANES) {
+    if (tid < LANES && live_head) {
         const int live = min(GROUPS, parts.y);
-        for (int k = 0; k < live; ++k) m = fmaxf(m, s_m[k]);
+        for (int k = 0; k < live; ++k) m = fmaxf(m, s_m[sub][k]);
         const float from = m == NEG_INF ? 0.f : m;
         l = 0.f;
         sum = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int k = 0; k < live; ++k) {
-            const float share = __builtin_amdgcn_exp2f(s_m[k] - from);
-            const float4 v = *reinterpret_cast<const float4*>(&s_o[k][d]);
-            l += s_l[k] * share;
+            const float share = __builtin_amdgcn_exp2f(s_m[sub][k] - from);
+            const float4 v = *reinterpret_cast<const float4*>(&s_o[sub][k][d]);
+            l += s_l[sub][k] * share;
             sum.x += v.x * share, sum.y += v.y * share, sum.z += v.z * share, sum.w += v.w * share;
         }
         const float r = l == 0.f ? 0.f : 1.0f / l;
@@ -759,8 +811,15 @@ void run_attention(const PagedAttnParams& p, hipStream_t s) {
     else
         hipLaunchKernelGGL((paged_attention_kernel<TYPE, D, false>), grid, dim3(ATTN_THREADS), 0, s, p);
     if (int64_t(parts) > p.rows)  // else no row has two
-        hipLaunchKernelGGL((paged_merge_kernel<TYPE, D>), dim3(unsigned(p.rows), unsigned(p.kv_heads * p.group)),
-                           dim3(MERGE_THREADS), 0, s, p);
+    {
+        // few rows have many parts each, many rows few: most of their workgroups would find nothing to join
+        const int heads = p.kv_heads * p.group;
+        if (int64_t(p.rows) * heads <= 4096)
+            hipLaunchKernelGGL((paged_merge_kernel<TYPE, D, 1>), dim3(unsigned(p.rows), unsigned(heads)), dim3(MERGE_THREADS), 0, s, p);
+        else
+            hipLaunchKernelGGL((paged_merge_kernel<TYPE, D, 4>), dim3(unsigned(p.rows), unsigned((heads + 3) / 4)),
+                               dim3(MERGE_THREADS), 0, s, p);
+    }
 }
 
 template <int SOURCE, int TYPE>
