@@ -155,6 +155,13 @@ int plamo_set_sampling(plamo_runtime* rt, float repetition_penalty, float freque
  * (generated tokens only, Main.swift:237-238).  Cleared by plamo_reset. */
 int plamo_sampler_observe(plamo_runtime* rt, int32_t id);
 
+/* A token drawn from the logits of output row `slot` (as plamo_logits gives them, without the controls above):
+ * temperature, top-k, top-p and min-p as for plamo_kernel_sample, by the caller's `uniform` in [0, 1).  Leaves
+ * position, logits, predictions and history alone: pass the token to plamo_forward as any other.  No
+ * counterpart in the reference, which takes the largest logit. */
+int plamo_sample(plamo_runtime* rt, int32_t slot, float temperature, int32_t top_k, float top_p, float min_p, float uniform,
+                 int32_t* token, float* prob, char* err, size_t errlen);
+
 /* The token loop of Main.swift:235-288 driven on the device: prefill `prompt`, then up to
  * `max_tokens` emitted tokens, stopping on token 1 or 16 (Main.swift:279).  Each decode
  * step is one replay of a captured hipGraph; the next token is fed back on the device.

@@ -327,6 +327,20 @@ int plamo_sampler_observe(plamo_runtime* rt, int32_t id) {
     return PLAMO_OK;
 }
 
+int plamo_sample(plamo_runtime* rt, int32_t slot, float temperature, int32_t top_k, float top_p, float min_p, float uniform,
+                 int32_t* token, float* prob, char* err, size_t errlen) {
+    return guard(err, errlen, [&] {
+        if (!rt || slot < 0 || slot >= std::max(1, rt->impl.last_output_rows))
+            throw plamo::Error(plamo::E_INVAL, "Invalid logits slot");
+        if (!std::isfinite(temperature) || std::isnan(top_p) || std::isnan(min_p))
+            throw plamo::Error(plamo::E_INVAL, "Invalid sampling controls");
+        if (!(uniform >= 0.0f && uniform < 1.0f)) throw plamo::Error(plamo::E_INVAL, "Random numbers must be in [0, 1)");
+        const auto drawn = rt->impl.sample(slot, temperature, top_k, top_p, min_p, uniform);
+        if (token) *token = drawn.token;
+        if (prob) *prob = drawn.prob;
+    });
+}
+
 int plamo_generate(plamo_runtime* rt, const int32_t* prompt, int32_t count, int32_t max_tokens, int32_t* out_ids,
                    int32_t* out_count, int32_t* stop_reason, char* err, size_t errlen) {
     return guard(err, errlen, [&] {

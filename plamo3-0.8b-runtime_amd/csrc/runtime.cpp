@@ -10,6 +10,7 @@
 
 #include "formats.h"
 #include "json.h"
+#include "paged.h"
 
 namespace plamo {
 
@@ -795,7 +796,39 @@ void Engine::prefill_heads(int n, uint16_t* slot_logits, float* slot_hidden, int
 RuntimeImpl::~RuntimeImpl() {
     eng.reset();
     model.reset();
+    if (sample_buf) (void)hipFree(sample_buf);
     if (stream) (void)hipStreamDestroy(stream);
+}
+
+RuntimeImpl::Drawn RuntimeImpl::sample(int slot, float temperature, int32_t top_k, float top_p, float min_p, float uniform) {
+    struct Block {
+        float temperature, top_p, min_p, uniform;
+        int32_t top_k;
+        Drawn drawn;
+    } block{temperature, top_p, min_p, uniform, top_k, {-1, 0.0f}};
+    constexpr size_t HEAD = 256;  // the block, and the workspace's alignment
+    static_assert(sizeof(Block) <= HEAD, "controls and results");
+    if (!sample_buf) PLAMO_HIP(hipMalloc(&sample_buf, HEAD + sample_workspace(1, VOCAB)));
+    PLAMO_HIP(hipMemcpyAsync(sample_buf, &block, sizeof(block), hipMemcpyHostToDevice, stream));
+    Block* b = static_cast<Block*>(sample_buf);
+    SampleParams p{};
+    p.logits = logits_row(slot);
+    p.stride = VOCAB;
+    p.n = VOCAB;
+    p.rows = 1;
+    p.temperature = &b->temperature;
+    p.top_k = &b->top_k;
+    p.top_p = &b->top_p;
+    p.min_p = &b->min_p;
+    p.uniform = &b->uniform;
+    p.token = &b->drawn.token;
+    p.prob = &b->drawn.prob;
+    p.workspace = static_cast<char*>(sample_buf) + HEAD;
+    launch_sample(p, TYPE_BF16, stream);
+    PLAMO_HIP(hipGetLastError());
+    PLAMO_HIP(hipMemcpyAsync(&block, sample_buf, sizeof(block), hipMemcpyDeviceToHost, stream));
+    PLAMO_HIP(hipStreamSynchronize(stream));
+    return block.drawn;
 }
 
 void RuntimeImpl::reset() {

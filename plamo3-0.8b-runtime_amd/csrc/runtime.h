@@ -213,6 +213,13 @@ struct RuntimeImpl {
     void rewind(int64_t new_position, int hidden_index);    // Runtime.rewind (Runtime.swift:527-538)
     const uint16_t* logits_row(int slot) const;             // device logits of output row `slot`
     const float* hidden_row() const;                        // device final hidden of the last row
+    // A token drawn from output row `slot` (launch_sample), and its share of what the controls leave
+    struct Drawn {
+        int32_t token;
+        float prob;
+    };
+    Drawn sample(int slot, float temperature, int32_t top_k, float top_p, float min_p, float uniform);
+    void* sample_buf = nullptr;  // its controls, results and workspace, from the first call on
     int prefill(const int32_t* tokens, int n);
     void begin_timing();
     void end_timing();

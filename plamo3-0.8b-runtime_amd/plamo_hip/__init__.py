@@ -152,6 +152,14 @@ class Runtime:
         self._lib.plamo_set_sampling(self._h, float(repetition_penalty), float(frequency_penalty),
                                      float(presence_penalty), int(no_repeat_ngram))
 
+    def sample(self, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, slot=0):
+        """A token drawn from the logits of output row `slot` by `uniform` in [0, 1) -> (token, its
+        probability among those that the controls keep)."""
+        token, prob = ctypes.c_int32(-1), ctypes.c_float()
+        native.call(self._lib.plamo_sample, self._h, int(slot), float(temperature), int(top_k), float(top_p),
+                    float(min_p), float(uniform), ctypes.byref(token), ctypes.byref(prob))
+        return token.value, prob.value
+
     def observe(self, token):
         """generated.append(token) (Main.swift:280): history the sampling controls see."""
         self._lib.plamo_sampler_observe(self._h, int(token))

@@ -80,6 +80,8 @@ _SIGNATURES = {
     "plamo_set_sampling": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_float, ctypes.c_float, ctypes.c_float,
                                           ctypes.c_int32]),
     "plamo_sampler_observe": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32]),
+    "plamo_sample": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, ctypes.c_float, ctypes.c_int32] +
+                     [ctypes.c_float] * 3 + [c_i32p, c_f32p, ctypes.c_char_p, ctypes.c_size_t]),
     "plamo_generate": (ctypes.c_int, [ctypes.c_void_p, c_i32p, ctypes.c_int32, ctypes.c_int32, c_i32p, c_i32p,
                                       c_i32p, ctypes.c_char_p, ctypes.c_size_t]),
     "plamo_bench_decode": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, ctypes.POINTER(ctypes.c_double),
