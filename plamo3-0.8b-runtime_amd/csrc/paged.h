@@ -86,6 +86,8 @@ struct PagedAttnParams {
     int64_t out_stride;
     float* lse;               // [rows][heads] or null
     int target;               // parts that all rows' keys are divided into, for one KV head's tile
+    int reach;                // most keys of a row's parts: those it can see, from a multiple of 16 on
+    int least;                // fewest keys of a part, but for a row's last
     int2* row_parts;          // [rows] first part and number of parts
     float2* part_ml;          // [parts][heads] maximum and sum
     float* part_o;            // [parts][heads][head_dim]
