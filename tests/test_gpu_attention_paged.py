@@ -219,3 +219,44 @@ def test_two_graphs_with_their_own_workspaces():
         for graph, keys, values, tables, q, _, size, out, _, _ in cases:
             eager, _ = check("bf16", keys, values, tables, q, size.tolist())
             assert torch.equal(eager, out)
+
+
+@pytest.mark.parametrize("page", [16, 20])
+def test_many_rows_in_parts(page):
+    """Enough rows that several heads' parts are joined at once, and heads that this does not divide."""
+    lengths = [(389 * r) % 1501 for r in range(240)]
+    check("bf16", *build("bf16", 64, 18, 3, page, lengths), lengths)
+
+
+@pytest.mark.parametrize("rows,kv,most", [(3, 1, 239), (3, 1, 241), (90, 3, 490), (90, 3, 500), (80, 3, 500)])
+@pytest.mark.parametrize("page", [1, 16])
+def test_rows_in_one_part(rows, kv, most, page):
+    """Beside the widths up to which a row is not divided."""
+    lengths = [most - (61 * r) % most for r in range(rows)]
+    check("fp16", *build("fp16", 64, 2 * kv, kv, page, lengths), lengths)
+
+
+@pytest.mark.parametrize("window", [239, 241, 242, 497])
+def test_windows_in_one_part(window):
+    lengths = [4000 - 133 * r for r in range(30)]
+    for kv in (1, 9):
+        check("bf16", *build("bf16", 64, kv, kv, 16, lengths, window=window), lengths, window)
+
+
+def test_nan_and_infinite_scores_are_the_formulas():
+    """NaN in a visible key, or a score of infinity, makes the rows and heads that see it NaN, no others."""
+    lengths = [700, 640, 700]
+    for page in (16, 10):
+        keys, values, tables, q = build("bf16", 64, 4, 2, page, lengths)
+        q.abs_()
+        plain = torch.zeros(3, 256, dtype=torch.bfloat16, device="cuda")
+        out = plain.clone()
+        args = describe(keys, values, "bf16"), q, 4, torch.from_numpy(tables).cuda()
+        size = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+        attend(*args, size, plain)
+        keys[int(tables[0, 320 // page]), 0, 1, 5] = math.nan
+        keys[int(tables[2, 320 // page]), 0, 0, 5] = math.inf
+        attend(*args, size, out)
+        out, plain = out.view(3, 2, 2, 64), plain.view(3, 2, 2, 64)
+        assert torch.isnan(out[0, 1]).all() and torch.isnan(out[2, 0]).all()
+        assert torch.equal(out[1], plain[1]) and torch.equal(out[0, 0], plain[0, 0]) and torch.equal(out[2, 1], plain[2, 1])

@@ -110,3 +110,35 @@ def test_slots_past_two_to_the_31_elements():
         assert torch.equal(values[slot // page, slot % page, 0], qkv[i, 2 * dim:].to(torch.bfloat16))
     del keys, values
     torch.cuda.empty_cache()
+
+
+def test_replayed_graph_and_another_stream():
+    """Replays with other rows, slots and positions between eager calls, on a stream of their own."""
+    g = torch.Generator("cuda").manual_seed(3)
+    keys, values = make_cache("bf16", 9, 16, 1, 128, fill=3.0)
+    cache = describe(keys, values, "bf16")
+    qkv = torch.randn(20, 18 * 128, generator=g, device="cuda")
+    slots = torch.arange(20, dtype=torch.int32, device="cuda")
+    positions = torch.arange(20, dtype=torch.int32, device="cuda")
+    q = torch.zeros(20, 2048, dtype=torch.bfloat16, device="cuda")
+    gains = torch.randn(2, 128, generator=g, device="cuda").to(torch.bfloat16)
+    words = rope_words(500, 64)[0].cuda()
+    call = lambda: paged_qkv(cache, "bf16", qkv, 16, slots, q, positions, gains[0], gains[1], words)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        call()
+    for _ in range(4):
+        qkv.copy_(torch.randn(20, 18 * 128, generator=g, device="cuda"))
+        slots.copy_(torch.randperm(144, generator=g, device="cuda")[:20])
+        positions.copy_(torch.randint(0, 500, (20,), generator=g, device="cuda"))
+        results = []
+        for run in (graph.replay, call):
+            q.fill_(5), keys.fill_(3), values.fill_(3)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(s):
+                run()
+            torch.cuda.synchronize()
+            results.append((q.clone(), keys.clone(), values.clone()))
+        assert all(torch.equal(a, b) for a, b in zip(*results)) and int((results[0][1] != 3).any(-1).sum()) == 20

@@ -157,3 +157,25 @@ def test_replayed_graph(capacity):
     for counts in ([1] * 6, [5, -1, 8, 1, 0, 20], [-1, 3, 1, 1, -1, 1], [capacity // 2, 0, 0, 0, 0, 1], [1] * 6):
         pool.step(counts, graph.replay)
         pool.step([1] * 6)
+
+
+def test_pools_on_two_streams():
+    """Two servers' steps in flight at once, each in the order of its own stream."""
+    pools = [Pool(40, 30, 16, 500, 700, seed=1), Pool(7, 300, 3, 900, 5000, seed=2)]
+    streams = [torch.cuda.Stream() for _ in pools]
+    wants = []
+    torch.cuda.synchronize()
+    for turn in range(6):
+        for pool, s in zip(pools, streams):
+            counts = [(turn + r) % 5 + (40 if turn == r else 0) for r in range(pool.rows)]
+            if turn == 3:
+                counts[2] = -1
+            h = pool.host
+            want = tables_step(h["lengths"], counts, h["tables"], h["free"], pool.page, pool.pages, pool.capacity)
+            with torch.cuda.stream(s):
+                pool.counts.copy_(torch.tensor(counts, dtype=torch.int32))
+                pool.call()
+            wants.append(want)
+    torch.cuda.synchronize()
+    for pool, want in zip(pools, wants[-2:]):
+        pool.check(*want)

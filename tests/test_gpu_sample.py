@@ -247,3 +247,34 @@ def test_borders_among_negative_logits():
     alone[1, 12346] = -7.0
     check(alone, [0.5, 0.5])
     check(alone, [0.5, 0.5], top_k=np.full(2, 3, np.int32))
+
+
+def test_many_rows_beyond_the_lists():
+    """Hundreds of rows whose kept tokens no list holds, among others whose it does."""
+    rng = np.random.default_rng(15)
+    x = bell(rng, 300, 9001, "bf16")
+    k = rng.integers(1, 9001, 300).astype(np.int32)
+    k[::3] = rng.integers(1, 60, 100)
+    check(x, rng.random(300), top_k=k)
+    check(x, rng.random(300), top_k=k, top_p=rng.uniform(0.1, 0.99, 300).astype(np.float32),
+          temperature=np.where(rng.random(300) < 0.2, 0, 3.0).astype(np.float32))
+
+
+def test_calls_on_two_streams_with_their_own_workspaces():
+    rng = np.random.default_rng(16)
+    cases = []
+    for rows, n in ((5, 107520), (64, 30011), (1, 700)):
+        x, u, c = bell(rng, rows, n, "bf16"), rng.random(rows).astype(np.float32), controls(rng, rows)
+        want = check(x, u, **c)
+        put = {k: torch.from_numpy(v).cuda() for k, v in c.items()}
+        work = torch.full((max(16, lib().plamo_kernel_sample_workspace(rows, n)),), 0xFF, dtype=torch.uint8, device="cuda")
+        cases.append((x, n, torch.from_numpy(u).cuda(), put, work, want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(6):
+        for x, n, u, put, work, want, s in cases:
+            with torch.cuda.stream(s):
+                got.append((sample(x, n, u, workspace=work, **put), want, x.shape[0]))
+    torch.cuda.synchronize()
+    for (token, prob), want, rows in got:
+        assert torch.equal(token[:rows], want[0]) and torch.equal(prob[:rows], want[1])
