@@ -41,6 +41,8 @@ constexpr int BIN_SHIFT = 3;         // log2 of a bin's table steps
 constexpr int BINS = 1536;           // 32 (S + 1) <= 1504 are used
 constexpr int LIST = 2048;           // tokens that are sorted at once
 constexpr int LIST_TOP_K = 1024;     // a top-k up to which its tokens' weights are summed in the list
+constexpr int BUCKETS = 2048;        // of a list's range of weights
+constexpr int BUCKET_MOST = 128;     // tokens of a bucket that are ordered by comparing all
 constexpr int SUB = 1024;            // parts that a bin is divided into again
 
 typedef unsigned long long u64;
@@ -167,6 +169,7 @@ struct Shared {
     uint32_t bin_count[BINS];
     u64 order[LIST];       // descending logit, ascending id
     u64 weight[LIST];      // inclusive sums of the list's weights
+    uint32_t bucket[BUCKETS];  // of the list's tokens: how many, then where they end
     Sum waves[WAVES];
     float wave_value[WAVES];
     uint32_t wave_id[WAVES];
@@ -174,7 +177,7 @@ struct Shared {
     Sum found;             // a border's count and mass up to and with its token
     uint32_t found_id;
     u64 found_weight;
-    int found_bin;
+    int found_bin[2];
     u64 min_mass;          // of the tokens of at least min_p
 };
 
@@ -393,43 +396,78 @@ __device__ __forceinline__ u64 exchange(u64 x, uint32_t i, uint32_t k, uint32_t 
     return x;
 }
 
-// The list's tokens (s.listed of them) in order: strides of a wave and more through LDS, shorter ones
-// between lanes.  Then inclusive sums of the weights.
-__device__ __forceinline__ void sort_list(Shared& s, const Weights& w) {
+// The list's tokens (s.listed of them) in order, from registers: by buckets of their weights' logarithms, each
+// in its place and counted by how many of its bucket are ahead.  False where a bucket has too many for that.
+__device__ __forceinline__ bool sort_by_buckets(Shared& s, const Weights& w) {
+    static_assert(BUCKETS == 2 * THREADS && LIST == 2 * THREADS, "two for each thread");
     const uint32_t tid = threadIdx.x, count = s.listed;
-    constexpr uint32_t FEW = 128, SHARE = THREADS / FEW;
-    if (count <= FEW) {
-        // each token's place and sum from those before it, counted by eight threads: the other way, a barrier or
-        // a lane exchange after the other, takes 3 us however few there are
-        u64 *weights = s.weight + FEW, *order = s.weight + 2 * FEW;  // as they were listed
-        if (tid < count) {
-            const u64 x = s.order[tid];
-            weights[tid] = w.weight_of(s.table, key_value(uint32_t(x >> 32)));
-            order[tid] = x;
-        }
-        __syncthreads();
-        const uint32_t i = tid / SHARE, part = tid % SHARE;
-        if (i < count) {
-            const u64 x = order[i];
-            Sum before = {0, 0};
-            for (uint32_t j = part; j < count; j += SHARE) {
-                const bool ahead = order[j] < x;
-                before.count += ahead;
-                before.mass += ahead ? weights[j] : 0;
-            }
+    u64 x[2];
+    uint32_t step[2], low = 0xffffffffu, high = 0;
 #pragma unroll
-            for (int o = 1; o < int(SHARE); o <<= 1) {
-                before.count += __shfl_xor(before.count, o, 64);
-                before.mass += __shfl_xor(before.mass, o, 64);
-            }
-            if (part == 0) {
-                s.order[before.count] = x;
-                s.weight[before.count] = before.mass + weights[i];
-            }
+    for (uint32_t e = 0; e < 2; ++e) {
+        const uint32_t i = tid + e * THREADS;
+        x[e] = i < count ? s.order[i] : 0;
+        double below, whole;
+        w.step(key_value(uint32_t(x[e] >> 32)), step[e], below, whole);
+        if (i < count) {
+            low = min(low, step[e]);
+            high = max(high, step[e]);
         }
-        __syncthreads();
-        return;
+        s.bucket[i] = 0;
     }
+    if (tid == 0) {
+        s.low = 0xffffffffu;
+        s.high = 0;
+    }
+    for (int o = 32; o > 0; o >>= 1) {
+        low = min(low, uint32_t(__shfl_xor(low, o, 64)));
+        high = max(high, uint32_t(__shfl_xor(high, o, 64)));
+    }
+    __syncthreads();
+    if ((tid & 63) == 0) {
+        atomicMin(&s.low, low);
+        atomicMax(&s.high, high);
+    }
+    __syncthreads();
+    low = s.low;
+    high = s.high;
+    int shift = 0;
+    while ((high - low) >> shift >= BUCKETS) ++shift;
+#pragma unroll
+    for (uint32_t e = 0; e < 2; ++e) {
+        step[e] = (step[e] - low) >> shift;
+        if (tid + e * THREADS < count) atomicAdd(&s.bucket[step[e]], 1u);
+    }
+    __syncthreads();
+    const uint32_t own[2] = {s.bucket[2 * tid], s.bucket[2 * tid + 1]};
+    if (__syncthreads_or(max(own[0], own[1]) > BUCKET_MOST)) return false;
+    Sum total;
+    const Sum incl = block_scan<THREADS>({own[0] + own[1], 0}, s.waves, total);
+    s.bucket[2 * tid] = incl.count - own[0] - own[1];
+    s.bucket[2 * tid + 1] = incl.count - own[1];
+    __syncthreads();
+#pragma unroll
+    for (uint32_t e = 0; e < 2; ++e)
+        if (tid + e * THREADS < count) s.weight[atomicAdd(&s.bucket[step[e]], 1u)] = x[e];
+    __syncthreads();
+#pragma unroll 1
+    for (uint32_t e = 0; e < 2; ++e) {
+        if (tid + e * THREADS < count) {
+            const uint32_t begin = step[0] ? s.bucket[step[0] - 1] : 0, end = s.bucket[step[0]];
+            uint32_t at = begin;
+#pragma unroll 4
+            for (uint32_t j = begin; j < end; ++j) at += s.weight[j] < x[0];
+            s.order[at] = x[0];
+        }
+        x[0] = x[1];
+        step[0] = step[1];
+    }
+    return true;
+}
+
+// The list's tokens in order: strides of a wave and more through LDS, shorter ones between lanes.
+__device__ __forceinline__ void sort_by_exchange(Shared& s) {
+    const uint32_t tid = threadIdx.x, count = s.listed;
     uint32_t size = 64;
     while (size < count) size <<= 1;
     for (uint32_t i = count + tid; i < size; i += THREADS) s.order[i] = ~u64(0);
@@ -458,6 +496,47 @@ __device__ __forceinline__ void sort_list(Shared& s, const Weights& w) {
         }
         __syncthreads();
     }
+}
+
+// The list's tokens in order, and inclusive sums of their weights.
+__device__ __forceinline__ void sort_list(Shared& s, const Weights& w) {
+    const uint32_t tid = threadIdx.x, count = s.listed;
+    constexpr uint32_t FEW = 256;
+    if (count <= FEW) {
+        // each token's place and sum from those before it, counted by four or more threads: the other ways, a barrier or
+        // a lane exchange after the other, takes 3 us however few there are
+        u64 *weights = s.weight + FEW, *order = s.weight + 2 * FEW;  // as they were listed
+        if (tid < count) {
+            const u64 x = s.order[tid];
+            weights[tid] = w.weight_of(s.table, key_value(uint32_t(x >> 32)));
+            order[tid] = x;
+        }
+        __syncthreads();
+        const uint32_t share = count <= FEW / 4 ? 16 : count <= FEW / 2 ? 8 : 4;
+        const uint32_t i = tid / share, part = tid % share;
+        if (i < count) {
+            const u64 x = order[i];
+            Sum before = {0, 0};
+#pragma unroll 4
+            for (uint32_t j = part; j < count; j += share) {
+                const bool ahead = order[j] < x;
+                before.count += ahead;
+                before.mass += ahead ? weights[j] : 0;
+            }
+            for (uint32_t o = 1; o < share; o <<= 1) {
+                before.count += __shfl_xor(before.count, int(o), 64);
+                before.mass += __shfl_xor(before.mass, int(o), 64);
+            }
+            if (part == 0) {
+                s.order[before.count] = x;
+                s.weight[before.count] = before.mass + weights[i];
+            }
+        }
+        __syncthreads();
+        return;
+    }
+    if (!sort_by_buckets(s, w)) sort_by_exchange(s);
+    __syncthreads();
     const uint32_t i = 2 * tid;
     u64 weight[2];
 #pragma unroll 1
@@ -467,7 +546,7 @@ __device__ __forceinline__ void sort_list(Shared& s, const Weights& w) {
     }
     Sum total;
     const Sum incl = block_scan<THREADS>({0, weight[0] + weight[1]}, s.waves, total);
-    if (i < size) {
+    if (i < count) {  // i + 1 is a place of the list too
         s.weight[i] = incl.mass - weight[1];
         s.weight[i + 1] = incl.mass;
     }
@@ -710,12 +789,12 @@ __device__ __forceinline__ bool divide_bin(Shared& s, const Row<TYPE>& row, int 
         const Sum upto = {base.count + incl.count, base.mass + incl.mass};
         const Sum before = {upto.count - own.count, upto.mass - own.mass};
         if (goal.reached(upto) && !goal.reached(before)) {
-            s.found_bin = tid;
+            s.found_bin[0] = tid;
             s.found = before;
             s.listed = own.count;
         }
         __syncthreads();
-        const uint32_t part = uint32_t(s.found_bin);
+        const uint32_t part = uint32_t(s.found_bin[0]);
         base = s.found;
         held = s.listed;
         high = min(high, low + (((part + 1) << shift) - 1));
@@ -775,15 +854,20 @@ struct Bins {
         return total;
     }
 
-    // The bin of a border, in every thread.
+    // The bins of two borders, or of one, in every thread.
     template <int NT>
-    __device__ __forceinline__ int border(Goal goal) const {
+    __device__ __forceinline__ int2 borders(Goal one, Goal two) const {
         __syncthreads();
-        for (int b = threadIdx.x; b < BINS; b += NT)
-            if (goal.reached(upto(b)) && !goal.reached(before(b))) *found = b;
+        for (int b = threadIdx.x; b < BINS; b += NT) {
+            const Sum until = upto(b), ahead = before(b);
+            if (one.reached(until) && !one.reached(ahead)) found[0] = b;
+            if (two.reached(until) && !two.reached(ahead)) found[1] = b;
+        }
         __syncthreads();
-        return *found;
+        return make_int2(found[0], found[1]);
     }
+    template <int NT>
+    __device__ __forceinline__ int border(Goal goal) const { return borders<NT>(goal, goal).x; }
 };
 
 __device__ __forceinline__ Goal top_p_goal(float top_p, u64 mass) {
@@ -795,21 +879,20 @@ __device__ __forceinline__ Goal draw_goal(float share, u64 mass) {
     return {false, min(u64(double(share) * double(mass)), mass - 1) + 1};
 }
 
-// Which bins a border's search lists, given its own: all up to it if they fit, so that further borders need
-// no pass; else the bin alone.  For a top-p the drawn token's as well: where it is, is known but for what the
-// top-p's bin adds to the weight, which moves it by a bin at most, as a rule.  False where the drawn token's
+// Which bins a border's search lists, given its own.  UPTO: all up to it if they fit, so that further borders
+// need no pass; else the bin alone.  For a top-p the drawn token's as well: where it is, is known but for what
+// the top-p's bin adds to the weight, which moves it by a bin at most, as a rule.  False where the drawn token's
 // may not be among them.
-template <int NT>
+template <int NT, bool UPTO>
 __device__ __forceinline__ bool choose_bins(const Bins& bins, int bin, bool top_p, u64 most, float share, int& first, int& last,
                                             int& extra) {
-    first = bins.count[bin] <= uint32_t(LIST) ? 0 : bin;
+    first = UPTO && bins.count[bin] <= uint32_t(LIST) ? 0 : bin;
     last = bin;
     extra = -1;
-    if (!top_p || first == 0) return true;
+    if (!top_p || (UPTO && first == 0)) return true;
     const u64 least = min(bins.before(bin).mass, most), full = min(bins.mass[bin], most);
-    const int one = bins.border<NT>(draw_goal(min(share, 1.0f), max(least, u64(1))));
-    __syncthreads();
-    const int two = bins.border<NT>(draw_goal(share, full));
+    const int2 drawn = bins.borders<NT>(draw_goal(share, max(least, u64(1))), draw_goal(share, full));
+    const int one = drawn.x, two = drawn.y;
     uint32_t held = bins.count[two] - bins.before(one).count;
     if (two < bin) held += bins.count[bin] - bins.before(bin).count;
     if (held > uint32_t(LIST)) return false;
@@ -931,7 +1014,7 @@ __global__ __launch_bounds__(GROUP_THREADS) void sample_list_kernel(SampleParams
     __shared__ u64 s_stage[STAGE];
     __shared__ uint32_t s_pieces[PIECES];
     __shared__ uint32_t s_queued, s_listed, s_at;
-    __shared__ int s_found;
+    __shared__ int s_found[2];
     const int r = blockIdx.y, tid = threadIdx.x;
     const Controls c(p, r);
     if (c.greedy()) return;
@@ -949,7 +1032,7 @@ __global__ __launch_bounds__(GROUP_THREADS) void sample_list_kernel(SampleParams
     }
     Weights w;
     w.set(best.value, c.temperature, p.n);
-    const Bins bins = {s_mass, s_count, &s_found};
+    const Bins bins = {s_mass, s_count, s_found};
     const u64 most = c.masses && c.least ? state.min_mass : ~u64(0);
     const float share = c.share(p, r);
     Plan plan;
@@ -972,8 +1055,14 @@ __global__ __launch_bounds__(GROUP_THREADS) void sample_list_kernel(SampleParams
     if (plan.listed) {
         const int bin = bins.border<GROUP_THREADS>(goal);
         int first, last, extra;
-        plan.listed = choose_bins<GROUP_THREADS>(bins, bin, top_p, most, share, first, last, extra);
-        if (plan.whole && first > 0) plan.listed = false;
+        if (plan.whole) {  // all up to the bin
+            first = 0;
+            last = bin;
+            extra = -1;
+            plan.listed = bins.count[bin] <= uint32_t(LIST);
+        } else {
+            plan.listed = choose_bins<GROUP_THREADS, false>(bins, bin, top_p, most, share, first, last, extra);
+        }
         plan.extra = extra;
         plan.base = bins.before(first);
         plan.extra_base = bins.before(max(extra, 0));
@@ -1005,7 +1094,7 @@ template <int TYPE>
 __device__ __forceinline__ void draw_from_row(Shared& s, const SampleParams& p, const Controls& c, Row<TYPE>& row, float share,
                                               u64& kept_mass) {
     const int tid = threadIdx.x;
-    const Bins bins = {s.bin_mass, s.bin_count, &s.found_bin};
+    const Bins bins = {s.bin_mass, s.bin_count, s.found_bin};
     // The borders one after the other: of the top-k, of the top-p, the drawn token's.  A small top-k's
     // tokens are listed first of all, with what shares the last one's bin; should too many do, weights are
     // summed after all and all begins again.
@@ -1047,7 +1136,7 @@ __device__ __forceinline__ void draw_from_row(Shared& s, const SampleParams& p, 
             if (!whole) {
                 const int bin = bins.border<THREADS>(goal);
                 if (bin != extra && (bin < first || bin > last)) {
-                    choose_bins<THREADS>(bins, bin, stage == TOP_P, c.least ? s.min_mass : ~u64(0), share, first, last, extra);
+                    choose_bins<THREADS, true>(bins, bin, stage == TOP_P, c.least ? s.min_mass : ~u64(0), share, first, last, extra);
                     if (stage == LIST_ALL) first = 0;
                     Wanted wanted;
                     wanted.bins(row.w, first, last, extra);
