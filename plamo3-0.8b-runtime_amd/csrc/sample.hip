@@ -40,9 +40,13 @@ constexpr int STEPS = 256;           // table entries for a factor of two
 constexpr int BIN_SHIFT = 3;         // log2 of a bin's table steps
 constexpr int BINS = 1536;           // 32 (S + 1) <= 1504 are used
 constexpr int LIST = 2048;           // tokens that are sorted at once
-constexpr int LIST_TOP_K = 1024;     // a top-k up to which its tokens' weights are summed in the list
+// A top-k up to which its tokens' weights are summed in the list, and no others: 64 rows of 107,520 and a top-k of
+// 1,000 take 39 us so, 73 the other way.
+constexpr int LIST_TOP_K = 1024;
 constexpr int BUCKETS = 2048;        // of a list's range of weights
-constexpr int BUCKET_MOST = 128;     // tokens of a bucket that are ordered by comparing all
+// Tokens of a bucket that are ordered by comparing all; where one has more, the list is sorted by exchanges (64 rows
+// with a top-k of 5,000 93 us, 106 with 64 for this; lists of a thousand 41 by buckets, 51 by exchanges).
+constexpr int BUCKET_MOST = 128;
 constexpr int SUB = 1024;            // parts that a bin is divided into again
 
 typedef unsigned long long u64;
@@ -941,10 +945,10 @@ template <int TYPE>
 __global__ __launch_bounds__(PART_THREADS) void sample_best_kernel(SampleParams p, int each) {
     __shared__ float s_values[PART_THREADS / 64];
     __shared__ uint32_t s_ids[PART_THREADS / 64];
-    const int r = blockIdx.y, begin = blockIdx.x * each, n = min(each, p.n - begin);
+    const int r = blockIdx.x, begin = blockIdx.y * each, n = min(each, p.n - begin);
     RowState& state = row_state(p, r);
-    for (int i = blockIdx.x * PART_THREADS + threadIdx.x; i < BINS; i += gridDim.x * PART_THREADS) state.bins[i] = 0;
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
+    for (int i = blockIdx.y * PART_THREADS + threadIdx.x; i < BINS; i += gridDim.y * PART_THREADS) state.bins[i] = 0;
+    if (blockIdx.y == 0 && threadIdx.x == 0) {
         state.min_mass = 0;
         state.listed = 0;
     }
@@ -952,7 +956,7 @@ __global__ __launch_bounds__(PART_THREADS) void sample_best_kernel(SampleParams 
     uint32_t id;
     find_best<TYPE, PART_THREADS>(segment_base<TYPE>(p, r, begin), n, Controls(p, r).greedy(), best, id);
     block_best<PART_THREADS>(best, id, s_values, s_ids);
-    if (threadIdx.x == 0) row_best(p, r, gridDim.x)[blockIdx.x] = {best, id == 0xffffffffu ? id : id + uint32_t(begin)};
+    if (threadIdx.x == 0) row_best(p, r, gridDim.y)[blockIdx.y] = {best, id == 0xffffffffu ? id : id + uint32_t(begin)};
 }
 
 // The row's largest logit from its segments', in every thread (a wave's lanes take a segment each).
@@ -977,7 +981,7 @@ __global__ __launch_bounds__(GROUP_THREADS) void sample_bins_kernel(SampleParams
     __shared__ u64 s_mass[BINS];
     __shared__ uint32_t s_count[BINS];
     __shared__ u64 s_kept;
-    const int r = blockIdx.y, tid = threadIdx.x;
+    const int r = blockIdx.x, tid = threadIdx.x;
     const Controls c(p, r);
     if (c.greedy()) return;
     for (int i = tid; i < STEPS; i += GROUP_THREADS) s_table[i] = table_entry(i, weight_scale(p.n));
@@ -991,7 +995,7 @@ __global__ __launch_bounds__(GROUP_THREADS) void sample_bins_kernel(SampleParams
     Weights w;
     w.set(best.value, c.temperature, p.n);
     __syncthreads();
-    const int begin = blockIdx.x * each, n = min(each, p.n - begin);
+    const int begin = blockIdx.y * each, n = min(each, p.n - begin);
     const u64 kept = fill_bins<TYPE, GROUP_THREADS, true>(segment_base<TYPE>(p, r, begin), n, w, s_table, false, c.masses, c.least,
                                                    s_mass, s_count);
     if (c.least && kept) atomicAdd(&s_kept, kept);
@@ -1015,7 +1019,7 @@ __global__ __launch_bounds__(GROUP_THREADS) void sample_list_kernel(SampleParams
     __shared__ uint32_t s_pieces[PIECES];
     __shared__ uint32_t s_queued, s_listed, s_at;
     __shared__ int s_found[2];
-    const int r = blockIdx.y, tid = threadIdx.x;
+    const int r = blockIdx.x, tid = threadIdx.x;
     const Controls c(p, r);
     if (c.greedy()) return;
     RowState& state = row_state(p, r);
@@ -1027,7 +1031,7 @@ __global__ __launch_bounds__(GROUP_THREADS) void sample_list_kernel(SampleParams
     const Best best = segments_best(row_best(p, r, segments), segments);
     if (best.id == 0xffffffffu) return;
     if (best.value == -NEG_INF) {
-        if (blockIdx.x == 0 && tid == 0) state.plan.listed = false;
+        if (blockIdx.y == 0 && tid == 0) state.plan.listed = false;
         return;
     }
     Weights w;
@@ -1068,9 +1072,9 @@ __global__ __launch_bounds__(GROUP_THREADS) void sample_list_kernel(SampleParams
         plan.extra_base = bins.before(max(extra, 0));
         wanted.bins(w, first, last, extra);
     }
-    if (blockIdx.x == 0 && tid == 0) state.plan = plan;
+    if (blockIdx.y == 0 && tid == 0) state.plan = plan;
     if (!plan.listed) return;
-    const int begin = blockIdx.x * each, n = min(each, p.n - begin);
+    const int begin = blockIdx.y * each, n = min(each, p.n - begin);
     if (tid == 0) s_listed = 0;
     auto append = [&](uint32_t at, u64 entry) {
         if (at < uint32_t(LIST)) state.order[at] = entry;
@@ -1251,31 +1255,33 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(SampleParams p, in
     }
 }
 
-// Segments of a row: of 4,096 logits at least, and some 2,048 in all, which fill the CUs several times;
-// 1: a workgroup does the whole row.
-int row_segments(int rows, int n) { return std::max(1, std::min((n + 4095) / 4096, 2048 / rows)); }
-constexpr int FEWEST_SEGMENTS = 3;
+// Whether a workgroup does a whole row by itself: where all rows' run at once, a CU holding one, and the row is
+// short.  256 rows of 16,000 BF16 logits take 24 to 33 us so (by what is kept), 36 to 39 in four launches, 64 rows
+// of 32,000 26 to 37 and 33 to 38; but 64 of 107,520 38 to 61 against 33 to 46, and 1,024 rows of 4,000 68 to
+// 80 against 53 to 59.
+bool row_alone(int rows, int n) { return rows <= 256 && n <= 32768; }
+// Segments of a row: of 4,096 logits at least, and some 1,024 in all, which fill the CUs.
+int row_segments(int rows, int n) { return std::max(1, std::min((n + 4095) / 4096, 1024 / rows)); }
 // Workgroups that fill histograms, and that list, over all rows: 128 FP32 rows take 18.7 and 18.0 us so, 24.8
 // and 30.3 with 2,048 of 256 threads, each of which adds its histogram to the row's and adds the row's up.
 constexpr int GROUPS = 512;
 
 template <int TYPE>
 void run_sample(const SampleParams& p, hipStream_t s) {
-    int segments = row_segments(p.rows, p.n);
-    if (segments < FEWEST_SEGMENTS) {
+    if (row_alone(p.rows, p.n)) {
         hipLaunchKernelGGL((sample_draw_kernel<TYPE, false>), dim3(unsigned(p.rows)), dim3(THREADS), 0, s, p, 0);
         return;
     }
+    int segments = row_segments(p.rows, p.n);
     const int each = (p.n + segments * 64 - 1) / (segments * 64) * 64;
     segments = (p.n + each - 1) / each;
-    const dim3 grid(unsigned(segments), unsigned(p.rows));
-    hipLaunchKernelGGL((sample_best_kernel<TYPE>), grid, dim3(PART_THREADS), 0, s, p, each);
+    hipLaunchKernelGGL((sample_best_kernel<TYPE>), dim3(unsigned(p.rows), unsigned(segments)), dim3(PART_THREADS), 0, s, p, each);
     const int bins = std::max(1, std::min(segments, GROUPS / p.rows)), part = (p.n + bins * 64 - 1) / (bins * 64) * 64;
-    hipLaunchKernelGGL((sample_bins_kernel<TYPE>), dim3(unsigned((p.n + part - 1) / part), unsigned(p.rows)), dim3(GROUP_THREADS), 0, s,
+    hipLaunchKernelGGL((sample_bins_kernel<TYPE>), dim3(unsigned(p.rows), unsigned((p.n + part - 1) / part)), dim3(GROUP_THREADS), 0, s,
                        p, segments, part);
     // each workgroup finds the bins for itself, which takes longer than a few more logits
     const int lists = std::max(1, std::min(segments, GROUPS / p.rows)), share = (p.n + lists * 64 - 1) / (lists * 64) * 64;
-    hipLaunchKernelGGL((sample_list_kernel<TYPE>), dim3(unsigned((p.n + share - 1) / share), unsigned(p.rows)), dim3(GROUP_THREADS),
+    hipLaunchKernelGGL((sample_list_kernel<TYPE>), dim3(unsigned(p.rows), unsigned((p.n + share - 1) / share)), dim3(GROUP_THREADS),
                        0, s, p, segments, share);
     hipLaunchKernelGGL((sample_draw_kernel<TYPE, true>), dim3(unsigned(p.rows)), dim3(THREADS), 0, s, p, segments);
 }
@@ -1283,8 +1289,7 @@ void run_sample(const SampleParams& p, hipStream_t s) {
 }  // namespace
 
 size_t sample_workspace(int rows, int n) {
-    const int segments = row_segments(rows, n);
-    return segments < FEWEST_SEGMENTS ? 0 : size_t(rows) * (sizeof(RowState) + size_t(segments) * sizeof(Best));
+    return row_alone(rows, n) ? 0 : size_t(rows) * (sizeof(RowState) + size_t(row_segments(rows, n)) * sizeof(Best));
 }
 
 void launch_sample(const SampleParams& p, int type, hipStream_t s) {

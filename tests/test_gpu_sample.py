@@ -278,3 +278,27 @@ def test_calls_on_two_streams_with_their_own_workspaces():
     torch.cuda.synchronize()
     for (token, prob), want, rows in got:
         assert torch.equal(token[:rows], want[0]) and torch.equal(prob[:rows], want[1])
+
+
+@pytest.mark.parametrize("n", [1, 5, 64, 1000, 4097, 9001])
+def test_short_rows_in_more_than_all_workgroups(n):
+    """The same rows among few and among many: short ones are drawn from by one workgroup or in several steps."""
+    rng = np.random.default_rng([17, n])
+    for kind in ("bf16", "fp32"):
+        wide = torch.full((300, n + 1), 1e30, dtype=TYPES[kind], device="cuda")
+        wide[:, :n] = bell(rng, 300, n, kind)
+        x, u, c = wide[:, :n], rng.random(300), controls(rng, 300)
+        token, prob = check(x, u, **c)
+        few, share = check(x[100:140], u[100:140], **{k: v[100:140] for k, v in c.items()})
+        assert torch.equal(few, token[100:140]) and torch.equal(share, prob[100:140])
+        check(x, u)
+
+
+def test_more_rows_than_a_grid_has_in_other_directions():
+    rows = 70000
+    x = torch.zeros(rows, 3, dtype=torch.bfloat16, device="cuda")
+    x[torch.arange(rows), torch.arange(rows) % 3] = 5
+    u = torch.full((rows,), 0.5, device="cuda")
+    work = torch.empty(lib().plamo_kernel_sample_workspace(rows, 3), dtype=torch.uint8, device="cuda")
+    token, prob = sample(x, 3, u, workspace=work)
+    assert torch.equal(token[:rows].long().cpu(), torch.arange(rows) % 3) and int(token[rows]) == -7
