@@ -421,10 +421,10 @@ int plamo_kernel_paged_tables(uint64_t lengths, uint64_t counts, int32_t rows, u
  * keys, values; `type` PLAMO_F32 or the cache's, qkv_stride elements between rows).  q_norm, k_norm
  * ([head_dim], the cache's type; 0: none): x / sqrt(mean(x^2) + 1e-6) * (1 + gain).  rope (0: none;
  * [rope_rows][head_dim / 2] words as plamo_rope_table makes them): pairs (d, d + head_dim / 2) turned by
- * row positions[token].  Rows, gains and rope are 16-byte aligned.  FP32 inside, rounded once.  Queries go to q [tokens][heads * head_dim] (the
- * cache's type; rows of that type may be overwritten in place), keys and values to slots[token].  A token
- * with a position below 0 or from rope_rows on is skipped, and one with a slot outside the cache leaves
- * the cache as it is.  Slots that are not skipped have to differ. */
+ * row positions[token].  Rows, gains and rope are 16-byte aligned.  FP32 inside, rounded once.  Queries go to
+ * q [tokens][heads * head_dim] (the cache's type; rows of that type may be overwritten in place), keys and values to
+ * slots[token].  A token with a position below 0 or from rope_rows on is skipped, and one with a slot outside
+ * the cache leaves the cache as it is.  Slots that are not skipped have to differ. */
 int plamo_kernel_paged_qkv(const plamo_paged_cache* cache, uint64_t qkv, int32_t type, int64_t qkv_stride, int32_t heads,
                            uint64_t q_norm, uint64_t k_norm, uint64_t rope, int32_t rope_rows, uint64_t positions,
                            uint64_t slots, int32_t tokens, uint64_t q, int64_t q_stride, uint64_t stream, char* err,
@@ -432,7 +432,7 @@ int plamo_kernel_paged_qkv(const plamo_paged_cache* cache, uint64_t qkv, int32_t
 
 /* Attention of one token per request: out[r] = softmax(scale * q[r] . k) v over keys 0 .. lengths[r] - 1
  * of tables[r][width], or the last `window` of them (window > 0); query head h reads KV head
- * h / (heads / kv_heads).  q and out: rows of heads * head_dim of the cache's type.  lse (0: none): FP32
+ * h / (heads / kv_heads).  q and out: rows of heads * head_dim of the cache's type (out may be q, row for row).  lse (0: none): FP32
  * [rows][heads], the logarithm of each sum of exponents.  Keys of a table entry outside 0 .. pages - 1 are
  * not seen, lengths past the table end with it, and a row that sees nothing gives zeros and minus
  * infinity.  `workspace` (16-byte aligned, plamo_kernel_attention_paged_workspace bytes, uninitialised) is the
@@ -452,8 +452,10 @@ int plamo_kernel_attention_paged(const plamo_paged_cache* cache, uint64_t q, int
  * top_p of the weight lies (at least one), of them those of at least min_p of the largest weight; `token`
  * (int32) is the first up to which more than `uniform` of the weight that is left lies, and prob (FP32, 0:
  * none) its share of it.  NaN counts as minus infinity, which is never drawn; a row of nothing else gives
- * -1 and 0.  Tokens below 2^-46 of the largest weight are not drawn (n > 2^17: 2^-43).  n <= 2^20.  The
- * result depends on the row and its controls alone.  Workspace as for plamo_kernel_attention_paged. */
+ * -1 and 0.  Weights are exact to 2^-42 and added without rounding; tokens below 2^-46 of the largest are not
+ * drawn (n > 2^17: 2^-43).  A temperature of NaN is 0, another control of NaN off, and a uniform number outside
+ * [0, 1) the end next to it (NaN: 0).  n <= 2^20.  The result depends on the row and its controls alone.
+ * Workspace as for plamo_kernel_attention_paged. */
 int64_t plamo_kernel_sample_workspace(int32_t rows, int32_t n);
 int plamo_kernel_sample(uint64_t logits, int32_t type, int64_t stride, int32_t n, int32_t rows, uint64_t temperature,
                         uint64_t top_k, uint64_t top_p, uint64_t min_p, uint64_t uniform, uint64_t token, uint64_t prob,

@@ -260,3 +260,12 @@ def test_nan_and_infinite_scores_are_the_formulas():
         out, plain = out.view(3, 2, 2, 64), plain.view(3, 2, 2, 64)
         assert torch.isnan(out[0, 1]).all() and torch.isnan(out[2, 0]).all()
         assert torch.equal(out[1], plain[1]) and torch.equal(out[0, 0], plain[0, 0]) and torch.equal(out[2, 1], plain[2, 1])
+
+
+@pytest.mark.parametrize("lengths", [[5000, 3, 0, 1300], [90, 200, 1]])
+def test_output_in_place_of_the_queries(lengths):
+    keys, values, tables, q = build("bf16", 128, 16, 1, 16, lengths)
+    want, _ = check("bf16", keys, values, tables, q, lengths)
+    attend(describe(keys, values, "bf16"), q, 16, torch.from_numpy(tables).cuda(),
+           torch.tensor(lengths, dtype=torch.int32, device="cuda"), q)
+    assert torch.equal(q, want)

@@ -302,3 +302,13 @@ def test_more_rows_than_a_grid_has_in_other_directions():
     work = torch.empty(lib().plamo_kernel_sample_workspace(rows, 3), dtype=torch.uint8, device="cuda")
     token, prob = sample(x, 3, u, workspace=work)
     assert torch.equal(token[:rows].long().cpu(), torch.arange(rows) % 3) and int(token[rows]) == -7
+
+
+def test_infinite_temperature_draws_evenly():
+    rng = np.random.default_rng(18)
+    for rows, n in ((5, 700), (3, 40001), (300, 900)):
+        x = bell(rng, rows, n, "bf16")
+        x[:, ::5] = -float("inf")
+        x[:, 3] = float("nan")
+        for mix in ("none", "all", "top_p"):
+            check(x, rng.random(rows), **controls(rng, rows, **MIXES[mix], temperature=np.inf))
