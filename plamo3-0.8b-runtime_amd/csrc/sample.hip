@@ -263,7 +263,7 @@ struct Weights {
     static constexpr float MOST = 3.4028234663852886e38f;
     static constexpr double ROUND = 6755399441055744.0;  // sums with it are whole numbers, in their low bits
     float top;        // largest logit
-    float cap;        // plus infinity, if that is the largest logit: only such tokens have a weight
+    float cap;        // plus infinity, if that is the largest logit: only such tokens have a weight; else minus infinity
     int scale;        // S
     double rate;      // STEPS log2(e) / T
     double end;       // ROUND and the table steps from which on nothing is weighed
@@ -272,8 +272,8 @@ struct Weights {
     __device__ __forceinline__ void set(float best, float temperature, int n) {
         scale = weight_scale(n);
         end = ROUND + (scale + 1) * STEPS;
-        // plus infinity stands for the largest finite value, next to which the others weigh nothing
-        cap = best;
+        // plus infinity's distance from the top is taken as the largest finite value's
+        cap = best == -NEG_INF ? best : NEG_INF;
         top = infinite() ? MOST : best;
         rate = infinite() ? double(MOST) : STEPS * 1.44269504088896340736 / double(temperature);
     }
@@ -286,7 +286,7 @@ struct Weights {
         const double t = fma(below, rate, ROUND);
         n = uint32_t(__double2loint(t));
         whole = t - ROUND;
-        return t < end;
+        return t < end && (FINITE || !(v < cap));
     }
     template <bool FINITE = false>
     __device__ __forceinline__ bool bin(float v, int& b) const {
@@ -403,48 +403,68 @@ __device__ __forceinline__ u64 exchange(u64 x, uint32_t i, uint32_t k, uint32_t 
     return x;
 }
 
-// The list's tokens (s.listed of them) in order, from registers: by buckets of their weights' logarithms, each
-// in its place and counted by how many of its bucket are ahead.  False where a bucket has too many for that.
-__device__ __forceinline__ bool sort_by_buckets(Shared& s, const Weights& w) {
+// The list's tokens (s.listed of them) in order, from registers: by buckets, each token in its place and counted by
+// how many of its bucket are ahead.  False where a bucket has too many for that.  Buckets are logits and, where there
+// are fewer of these, as of 16-bit types with many equal ones, ranges of ids within; else of the weights' logarithms.
+__device__ __forceinline__ bool sort_by_buckets(Shared& s, const Weights& w, int n) {
     static_assert(BUCKETS == 2 * THREADS && LIST == 2 * THREADS, "two for each thread");
     const uint32_t tid = threadIdx.x, count = s.listed;
     u64 x[2];
-    uint32_t step[2], low = 0xffffffffu, high = 0;
-#pragma unroll
-    for (uint32_t e = 0; e < 2; ++e) {
-        const uint32_t i = tid + e * THREADS;
-        x[e] = i < count ? s.order[i] : 0;
-        double below, whole;
-        w.step(key_value(uint32_t(x[e] >> 32)), step[e], below, whole);
-        if (i < count) {
-            low = min(low, step[e]);
-            high = max(high, step[e]);
-        }
-        s.bucket[i] = 0;
-    }
+    uint32_t at[2], low = 0xffffffffu, high = 0, differ = 0;
+    const uint32_t any = uint32_t(s.order[0] >> 32);
     if (tid == 0) {
         s.low = 0xffffffffu;
         s.high = 0;
+        s.queued = 0;
     }
+#pragma unroll
+    for (uint32_t e = 0; e < 2; ++e) {
+        const uint32_t i = tid + e * THREADS;
+        x[e] = i < count ? s.order[i] : s.order[0];
+        at[e] = uint32_t(x[e] >> 32);
+        low = min(low, at[e]);
+        high = max(high, at[e]);
+        differ |= at[e] ^ any;
+        s.bucket[i] = 0;
+    }
+#pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         low = min(low, uint32_t(__shfl_xor(low, o, 64)));
         high = max(high, uint32_t(__shfl_xor(high, o, 64)));
+        differ |= uint32_t(__shfl_xor(differ, o, 64));
     }
     __syncthreads();
     if ((tid & 63) == 0) {
         atomicMin(&s.low, low);
         atomicMax(&s.high, high);
+        atomicOr(&s.queued, differ);
     }
     __syncthreads();
     low = s.low;
     high = s.high;
-    int shift = 0;
-    while ((high - low) >> shift >= BUCKETS) ++shift;
+    // the bits below those in which keys differ are the same in all
+    const int same = s.queued ? __ffs(int(s.queued)) - 1 : 31;
+    const uint32_t span = (high - low) >> same;
+    if (span < uint32_t(BUCKETS)) {
+        const int id_bits = 32 - __clz(n), more = min(31 - __clz(BUCKETS / int(span + 1)), id_bits);
 #pragma unroll
-    for (uint32_t e = 0; e < 2; ++e) {
-        step[e] = (step[e] - low) >> shift;
-        if (tid + e * THREADS < count) atomicAdd(&s.bucket[step[e]], 1u);
+        for (uint32_t e = 0; e < 2; ++e) at[e] = ((at[e] - low) >> same) << more | uint32_t(x[e]) >> (id_bits - more);
+    } else {
+        auto step = [&](uint32_t key) {
+            uint32_t t;
+            double below, whole;
+            w.step(key_value(key), t, below, whole);
+            return t;
+        };
+        const uint32_t first = step(low), range = step(high) - first;
+        int shift = 0;
+        while (range >> shift >= uint32_t(BUCKETS)) ++shift;
+#pragma unroll
+        for (uint32_t e = 0; e < 2; ++e) at[e] = (step(at[e]) - first) >> shift;
     }
+#pragma unroll
+    for (uint32_t e = 0; e < 2; ++e)
+        if (tid + e * THREADS < count) atomicAdd(&s.bucket[at[e]], 1u);
     __syncthreads();
     const uint32_t own[2] = {s.bucket[2 * tid], s.bucket[2 * tid + 1]};
     if (__syncthreads_or(max(own[0], own[1]) > BUCKET_MOST)) return false;
@@ -455,19 +475,19 @@ __device__ __forceinline__ bool sort_by_buckets(Shared& s, const Weights& w) {
     __syncthreads();
 #pragma unroll
     for (uint32_t e = 0; e < 2; ++e)
-        if (tid + e * THREADS < count) s.weight[atomicAdd(&s.bucket[step[e]], 1u)] = x[e];
+        if (tid + e * THREADS < count) s.weight[atomicAdd(&s.bucket[at[e]], 1u)] = x[e];
     __syncthreads();
 #pragma unroll 1
     for (uint32_t e = 0; e < 2; ++e) {
         if (tid + e * THREADS < count) {
-            const uint32_t begin = step[0] ? s.bucket[step[0] - 1] : 0, end = s.bucket[step[0]];
-            uint32_t at = begin;
+            const uint32_t begin = at[0] ? s.bucket[at[0] - 1] : 0, end = s.bucket[at[0]];
+            uint32_t place = begin;
 #pragma unroll 4
-            for (uint32_t j = begin; j < end; ++j) at += s.weight[j] < x[0];
-            s.order[at] = x[0];
+            for (uint32_t j = begin; j < end; ++j) place += s.weight[j] < x[0];
+            s.order[place] = x[0];
         }
         x[0] = x[1];
-        step[0] = step[1];
+        at[0] = at[1];
     }
     return true;
 }
@@ -506,7 +526,7 @@ __device__ __forceinline__ void sort_by_exchange(Shared& s) {
 }
 
 // The list's tokens in order, and inclusive sums of their weights.
-__device__ __forceinline__ void sort_list(Shared& s, const Weights& w) {
+__device__ __forceinline__ void sort_list(Shared& s, const Weights& w, int n) {
     const uint32_t tid = threadIdx.x, count = s.listed;
     constexpr uint32_t FEW = 256;
     if (count <= FEW) {
@@ -542,7 +562,7 @@ __device__ __forceinline__ void sort_list(Shared& s, const Weights& w) {
         __syncthreads();
         return;
     }
-    if (!sort_by_buckets(s, w)) sort_by_exchange(s);
+    if (!sort_by_buckets(s, w, n)) sort_by_exchange(s);
     __syncthreads();
     const uint32_t i = 2 * tid;
     u64 weight[2];
@@ -695,7 +715,7 @@ __device__ __forceinline__ void list_row(Shared& s, const Row<TYPE>& row, const 
         if (threadIdx.x == 0) s.listed = LIST + 1;
         __syncthreads();
     }
-    if (s.listed <= LIST) sort_list(s, row.w);
+    if (s.listed <= LIST) sort_list(s, row.w, row.n);
 }
 
 // Where the extra bin's tokens begin in the list.
@@ -1228,7 +1248,7 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(SampleParams p, in
                 s.min_mass = state.min_mass;
             }
             __syncthreads();
-            sort_list(s, row.w);
+            sort_list(s, row.w, p.n);
             split_list(s, row.w, plan.extra);
             Sum kept = plan.whole ? list_sum(s, c.least) : plan.kept;
             // a border in the extra bin has more weight before it than there is before the bin

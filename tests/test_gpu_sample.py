@@ -312,3 +312,28 @@ def test_infinite_temperature_draws_evenly():
         x[:, 3] = float("nan")
         for mix in ("none", "all", "top_p"):
             check(x, rng.random(rows), **controls(rng, rows, **MIXES[mix], temperature=np.inf))
+
+
+def test_the_largest_finite_value_beside_infinity():
+    rng = np.random.default_rng(19)
+    for n in (900, 40001):
+        x = torch.full((6, n), torch.finfo(torch.float32).max, device="cuda")
+        x[:, 1::2] = -torch.finfo(torch.float32).max
+        x[3:, [5, 800]] = float("inf")
+        for c in ({}, {"top_k": 3}, {"top_p": 0.5}, {"min_p": 0.5}, {"temperature": 1e38}, {"temperature": 0.0}):
+            check(x, rng.random(6), **{k: np.full(6, v, np.int32 if k == "top_k" else np.float32) for k, v in c.items()})
+
+
+def test_many_equal_logits_in_a_list():
+    """Lists of a few hundred to two thousand tokens of one, two and many logits, beside each list's length."""
+    rng = np.random.default_rng(20)
+    for n in (5000, 70000):
+        for count in (255, 256, 257, 600, 2047, 2048, 2049):
+            x = torch.full((4, n), -40.0, device="cuda")
+            for r, parts in enumerate(([1.0], [1.0, 1.0078125], [1.0, 1.0000001, 1.25], rng.random(count))):
+                at = torch.from_numpy(rng.permutation(n)[:count]).cuda()
+                x[r, at] = torch.from_numpy(rng.choice(parts, count)).float().cuda()
+            for kind in ("fp32", "bf16", "fp16"):
+                check(x.to(TYPES[kind]), rng.random(4), top_k=np.full(4, min(count, 1000), np.int32))
+                check(x.to(TYPES[kind]), rng.random(4), top_p=np.full(4, 0.7, np.float32))
+                check(x.to(TYPES[kind]), rng.random(4))
