@@ -44,11 +44,11 @@ constexpr int BIN_SHIFT = 3;         // log2 of a bin's table steps
 constexpr int BINS = 1536;           // 32 (S + 1) <= 1504 are used
 constexpr int LIST = 2048;           // tokens that are sorted at once
 // A top-k up to which its tokens' weights are summed in the list, and no others: 64 rows of 107,520 and a top-k of
-// 1,000 take 39 us so, 73 the other way.
+// 1,000 take 36 us so, 73 the other way.
 constexpr int LIST_TOP_K = 1024;
 constexpr int BUCKETS = 2048;        // of a list's range of weights
-// Tokens of a bucket that are ordered by comparing all; where one has more, the list is sorted by exchanges (64 rows
-// with a top-k of 5,000 93 us, 106 with 64 for this; lists of a thousand 41 by buckets, 51 by exchanges).
+// Tokens of a bucket that are ordered by comparing all; where one has more, the list is sorted by exchanges: 64 BF16
+// rows of a top-k of 1,000 take 36 us by buckets, 48 by exchanges, of a top-p of 0.99 41 and 43 (46 with 64 for this).
 constexpr int BUCKET_MOST = 128;
 constexpr int SUB = 1024;            // parts that a bin is divided into again
 
@@ -531,7 +531,8 @@ __device__ __forceinline__ void sort_list(Shared& s, const Weights& w, int n) {
     constexpr uint32_t FEW = 256;
     if (count <= FEW) {
         // each token's place and sum from those before it, counted by four or more threads: the other ways, a barrier or
-        // a lane exchange after the other, takes 3 us however few there are
+        // a lane exchange after the other, take 3 us however few there are (64 rows of a top-p of 0.5 35.4 us, 36.1 with
+        // 128 for this; with 512, 0.9 takes 53 for 40)
         u64 *weights = s.weight + FEW, *order = s.weight + 2 * FEW;  // as they were listed
         if (tid < count) {
             const u64 x = s.order[tid];
