@@ -88,6 +88,7 @@ struct PagedAttnParams {
     int target;               // parts that all rows' keys are divided into, for one KV head's tile
     int reach;                // most keys of a row's parts: those it can see, from a multiple of 16 on
     int least;                // fewest keys of a part, but for a row's last
+    int division;             // how a workgroup finds its part
     int2* row_parts;          // [rows] first part and number of parts
     float2* part_ml;          // [parts][heads] maximum and sum
     float* part_o;            // [parts][heads][head_dim]

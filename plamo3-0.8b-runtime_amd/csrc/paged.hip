@@ -3,6 +3,7 @@
 //   paged_tables_kernel     pages taken from and given back to the free list, block tables, offsets
 //   paged_slots_kernel      slot and position of each new token
 //   paged_qkv_kernel        q and k RMS-normalised and rotated, k and v written to their slots
+//   paged_parts_kernel      how the keys of very many rows are divided
 //   paged_attention_kernel  attention of one token per request over its pages, split over the keys
 //   paged_merge_kernel      parts of a row joined
 #include <hip/hip_runtime.h>
@@ -348,9 +349,9 @@ constexpr int ATTN_WAVES = 4;
 constexpr int ATTN_THREADS = ATTN_WAVES * 64;
 constexpr int PART_KEYS = 32 * ATTN_WAVES;  // fewest keys of a part: a tile for each wave
 // Rows that can see up to so many keys, by the tables' width or the window, are one part each, which saves the
-// launch that joins parts: 64 rows of 200 keys 10.3 -> 9.8 us, 256 rows of them 18.8 -> 12.0.  Longer
-// where rows and KV heads fill the CUs by themselves (256 rows of 480 keys 24.5 -> 19.9 us), not where they
-// do not (64 rows of 480 keys 12.1 in parts, 16.0 in one).
+// search for the work and the launch that joins parts: 64 rows of 200 keys 10.3 -> 8.8 us, 256 rows of them 18.8 ->
+// 10.7.  Longer where rows and KV heads fill the CUs by themselves (256 rows of 480 keys 24.5 -> 18.5 us), not where
+// they do not (64 rows of 480 keys 12.1 in parts, 15 in one).
 constexpr int ONE_PART_KEYS = 256, ONE_PART_KEYS_FULL = 512;
 // Parts aimed at over all rows and KV heads: as many workgroups as 256 CUs hold at once (registers: six of
 // a head of 64, four of 128, two of 256).  More begin when others end and bring more parts to join, fewer
@@ -362,6 +363,12 @@ inline int attn_target(int heads, int kv_heads, int head_dim) {
     const int held = head_dim <= 64 ? 6 : head_dim <= 128 ? 4 : 2;
     return std::max(1, CUS * held / (kv_heads * attn_tiles(heads, kv_heads)));
 }
+
+// How a workgroup finds its part: it is its row; in all rows' lengths; in the list of a launch before.  The second
+// takes a time that grows with the rows, for each of as many workgroups: 1,000 rows of 700 keys take 40.6 us so, 41.8
+// with the list, 2,048 of 100 keys 29.8 and 23.0, 65,536 4,760 and 581.
+enum { DIVISION_NONE, DIVISION_FOUND, DIVISION_LISTED };
+constexpr int FOUND_ROWS = 1024;
 
 struct Row {
     int len;    // keys 0 .. len - 1
@@ -376,6 +383,14 @@ __device__ __forceinline__ Row row_keys(const PagedAttnParams& p, int r) {
     return k;
 }
 __device__ __forceinline__ int row_parts(int span, int chunk) { return max(1, (span + chunk - 1) / chunk); }
+
+// Keys of a part: all rows' keys divided by the parts aimed at, in whole tiles for each wave.
+__device__ __forceinline__ int part_keys(const PagedAttnParams& p, long long keys) {
+    // a row's last part is half empty on the average
+    const int target = max(p.target - p.rows / 2, (p.target + 1) / 2);
+    const long long each = (keys + target - 1) / target;
+    return __builtin_amdgcn_readfirstlane(each <= p.least ? p.least : int((each + PART_KEYS - 1) / PART_KEYS * PART_KEYS));
+}
 
 // Where the workgroups find their work: the same division in all of them, from all rows' lengths.
 struct Work {
@@ -398,9 +413,8 @@ __device__ __forceinline__ int wave_scan(int v) {
     return v;
 }
 
-// The row of part `item`; false past the last part.  Keys of a part: all rows' keys divided by the parts aimed
-// at, in whole tiles for each wave.  The waves look through 64 rows each at a time (1,000 rows 71.6 us, 63.4 since
-// they share the work); up to 64 rows every wave does for itself, without waiting for the others.
+// The row of part `item`; false past the last part.  The waves look through 64 rows each at a time (1,000 rows
+// 71.6 us, 63.4 since they share the work); up to 64 rows every wave does for itself, without waiting for the others.
 __device__ __forceinline__ bool find_work(const PagedAttnParams& p, WorkShared& s, int item, Work& work) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool few = p.rows <= 64;
@@ -413,10 +427,7 @@ __device__ __forceinline__ bool find_work(const PagedAttnParams& p, WorkShared& 
         keys = 0;
         for (int w = 0; w < ATTN_WAVES; ++w) keys += s.keys[w];
     }
-    // a row's last part is half empty on the average
-    const int target = max(p.target - p.rows / 2, (p.target + 1) / 2);
-    const long long each = (keys + target - 1) / target;
-    const int chunk = __builtin_amdgcn_readfirstlane(each <= p.least ? p.least : int((each + PART_KEYS - 1) / PART_KEYS * PART_KEYS));
+    const int chunk = part_keys(p, keys);
     int run = 0;
     for (int base = 0; base < p.rows; base += few ? 64 : ATTN_THREADS) {
         const int r = base + (few ? lane : int(threadIdx.x));
@@ -456,6 +467,58 @@ __device__ __forceinline__ bool find_work(const PagedAttnParams& p, WorkShared& 
     return false;
 }
 
+// The same where paged_parts_kernel has been: the last row whose first part is not past `item`, by looking at
+// 64 rows of a range at a time.
+__device__ __forceinline__ bool look_up_work(const PagedAttnParams& p, int item, Work& work) {
+    const int lane = threadIdx.x & 63;
+    int row = 0, span = p.rows;
+    while (span > 1) {
+        const int step = (span + 63) / 64, at = row + lane * step;
+        const bool upto = lane * step < span && at < p.rows && p.row_parts[at].x <= item;  // true for the first lanes
+        row += (__popcll(__ballot(upto)) - 1) * step;
+        span = step;
+    }
+    row = __builtin_amdgcn_readfirstlane(row);
+    const int2 parts = p.row_parts[row];
+    work = {row, __builtin_amdgcn_readfirstlane(parts.x), __builtin_amdgcn_readfirstlane(parts.y)};
+    return item < work.first + work.parts;
+}
+
+// First part and number of parts of every row, by one workgroup.
+constexpr int DIVIDE_THREADS = 1024;
+__global__ __launch_bounds__(DIVIDE_THREADS) void paged_parts_kernel(PagedAttnParams p) {
+    constexpr int WAVES = DIVIDE_THREADS / 64;
+    __shared__ long long s_keys[WAVES];
+    __shared__ int s_parts[WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    long long keys = 0;
+#pragma unroll 4
+    for (int r = threadIdx.x; r < p.rows; r += DIVIDE_THREADS) keys += row_keys(p, r).span;
+    for (int o = 32; o > 0; o >>= 1) keys += __shfl_xor(keys, o, 64);
+    if (lane == 0) s_keys[wave] = keys;
+    __syncthreads();
+    keys = 0;
+    for (int w = 0; w < WAVES; ++w) keys += s_keys[w];
+    const int chunk = part_keys(p, keys);
+    // a thread's rows are neighbours: sums in order
+    const int each = (p.rows + DIVIDE_THREADS - 1) / DIVIDE_THREADS;
+    const int begin = min(int(threadIdx.x) * each, p.rows), end = min(begin + each, p.rows);
+    int own = 0;
+#pragma unroll 4
+    for (int r = begin; r < end; ++r) own += row_parts(row_keys(p, r).span, chunk);
+    const int incl = wave_scan(own);
+    if (lane == 63) s_parts[wave] = incl;
+    __syncthreads();
+    int first = incl - own;
+    for (int w = 0; w < wave; ++w) first += s_parts[w];
+#pragma unroll 4
+    for (int r = begin; r < end; ++r) {
+        const int parts = row_parts(row_keys(p, r).span, chunk);
+        p.row_parts[r] = make_int2(first, parts);
+        first += parts;
+    }
+}
+
 template <int TYPE>
 __device__ __forceinline__ floatx4 mfma16(uint4 a, uint4 b, floatx4 c) {
     if constexpr (TYPE == TYPE_BF16)
@@ -490,9 +553,18 @@ __device__ __forceinline__ uint2 stream8(__amdgpu_buffer_rsrc_t r, uint32_t off)
     return make_uint2(v[0], v[1]);
 }
 
+__device__ __forceinline__ uint4 stream16(const char* at) {
+    const u32x4_t v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(at));
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ uint2 stream8(const char* at) {
+    const u32x2_t v = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(at));
+    return make_uint2(v[0], v[1]);
+}
+
 // EVEN: pages of whole half tiles (a multiple of 16 tokens), so that a half tile is one page's and
-// its page and addresses are the wave's, not the lane's.  64 rows of 2,000 to 8,000 keys take 36.1 us so, 39.1 the
-// other way, which any page size allows.
+// its page and addresses are the wave's, not the lane's.  64 rows of 5,000 keys from memory take 42.1 us so, 43.6 the
+// other way, which any page size allows; 48 of a window of 2,048, 32 heads of 64 on 8, 44.7 and 48.8.
 template <int TYPE, int D, bool EVEN>
 __device__ __forceinline__ void load_tile(Tile<TYPE, D>& t, const PagedAttnParams& p, const int32_t* table,
                                           int64_t head, int pos, int lo_key, int hi_key) {
@@ -557,7 +629,7 @@ __device__ __forceinline__ void load_tile(Tile<TYPE, D>& t, const PagedAttnParam
             const int64_t off = __shfl(own, 16 * h + col, 64);
 #pragma unroll
             for (int s = 0; s < X::STEPS; ++s)
-                t.k[h][s] = off >= 0 ? *reinterpret_cast<const uint4*>(p.keys + off + g * 16 + s * 64) : make_uint4(0, 0, 0, 0);
+                t.k[h][s] = off >= 0 ? stream16(p.keys + off + g * 16 + s * 64) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -567,10 +639,10 @@ __device__ __forceinline__ void load_tile(Tile<TYPE, D>& t, const PagedAttnParam
             for (int s = 0; s < X::SLABS; ++s) {
                 const char* from = p.values + off + col * X::CHUNK * 2 + s * 256;
                 if constexpr (X::CHUNK == 8) {
-                    const uint4 x = off >= 0 ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
+                    const uint4 x = off >= 0 ? stream16(from) : make_uint4(0, 0, 0, 0);
                     t.v[i][s][0] = x.x, t.v[i][s][1] = x.y, t.v[i][s][2] = x.z, t.v[i][s][3] = x.w;
                 } else {
-                    const uint2 x = off >= 0 ? *reinterpret_cast<const uint2*>(from) : make_uint2(0, 0);
+                    const uint2 x = off >= 0 ? stream8(from) : make_uint2(0, 0);
                     t.v[i][s][0] = x.x, t.v[i][s][1] = x.y;
                 }
             }
@@ -669,15 +741,20 @@ __global__ __launch_bounds__(ATTN_THREADS, attn_waves(D, EVEN)) void paged_atten
     const int col = lane & 15, g = lane >> 4;
     const int item = blockIdx.x, kv = blockIdx.y / p.tiles, tile = blockIdx.y - kv * p.tiles;
     Work work;
-    if (!find_work(p, s_work, item, work)) return;  // every wave of the workgroup
-    const int row = work.row, first_part = work.first, parts = work.parts;
+    bool any = true;
+    if (p.division == DIVISION_NONE) work = {item, item, 1};
+    else if (p.division == DIVISION_LISTED) any = look_up_work(p, item, work);
+    else any = find_work(p, s_work, item, work);
+    if (!any) return;  // every wave of the workgroup
+    const int row = __builtin_amdgcn_readfirstlane(work.row), first_part = __builtin_amdgcn_readfirstlane(work.first),
+              parts = __builtin_amdgcn_readfirstlane(work.parts);
     const Row keys = row_keys(p, row);
     const int len = __builtin_amdgcn_readfirstlane(keys.len), first = __builtin_amdgcn_readfirstlane(keys.first);
     const int part = item - first_part;
     const int each = __builtin_amdgcn_readfirstlane(((len - (first & ~15) + parts - 1) / parts + 31) & ~31);
     const int begin = (first & ~15) + part * each, end = min(len, begin + each);
     const int heads = p.kv_heads * p.group, head0 = kv * p.group + tile * 16, live = min(16, p.group - tile * 16);
-    if (blockIdx.y == 0 && threadIdx.x == 0 && part == 0) p.row_parts[row] = make_int2(first_part, parts);
+    if (p.division == DIVISION_FOUND && blockIdx.y == 0 && threadIdx.x == 0 && part == 0) p.row_parts[row] = make_int2(first_part, parts);
 
     uint4 q[X::STEPS];
     const uint16_t* qrow = p.q + row * p.q_stride + int64_t(head0 + min(col, live - 1)) * D;
@@ -820,12 +897,12 @@ void run_attention(const PagedAttnParams& p, hipStream_t s) {
     const int64_t most = int64_t(p.rows) * std::max<int64_t>(1, (int64_t(p.reach) + p.least - 1) / p.least);
     const unsigned parts = unsigned(std::min<int64_t>(most, int64_t(p.rows) + p.target));
     const dim3 grid(parts, unsigned(p.kv_heads * p.tiles));
+    if (p.division == DIVISION_LISTED) hipLaunchKernelGGL(paged_parts_kernel, dim3(1), dim3(DIVIDE_THREADS), 0, s, p);
     if (p.page_size % 16 == 0)
         hipLaunchKernelGGL((paged_attention_kernel<TYPE, D, true>), grid, dim3(ATTN_THREADS), 0, s, p);
     else
         hipLaunchKernelGGL((paged_attention_kernel<TYPE, D, false>), grid, dim3(ATTN_THREADS), 0, s, p);
-    if (int64_t(parts) > p.rows)  // else no row has two
-    {
+    if (p.division != DIVISION_NONE) {
         // few rows have many parts each, many rows few: most of their workgroups would find nothing to join (128 rows
         // of 16 heads 5.8 us with a head a workgroup, 6.9 with four; 1,000 rows, attention and all, 81.2 and 71.6)
         const int heads = p.kv_heads * p.group;
@@ -881,6 +958,7 @@ void paged_attn_bind(PagedAttnParams& p, void* workspace, int head_dim) {
     const int one_part = int64_t(p.rows) * p.kv_heads * p.tiles >= CUS ? ONE_PART_KEYS_FULL : ONE_PART_KEYS;
     p.reach = (p.window > 0 ? std::min(p.window, p.most) : p.most) + 15;
     p.least = p.reach <= one_part ? one_part : PART_KEYS;
+    p.division = p.reach <= p.least ? DIVISION_NONE : p.rows <= FOUND_ROWS ? DIVISION_FOUND : DIVISION_LISTED;
     const size_t parts = size_t(p.rows) + size_t(p.target);
     char* at = static_cast<char*>(workspace);
     p.row_parts = reinterpret_cast<int2*>(at);

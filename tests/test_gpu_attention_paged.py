@@ -269,3 +269,30 @@ def test_output_in_place_of_the_queries(lengths):
     attend(describe(keys, values, "bf16"), q, 16, torch.from_numpy(tables).cuda(),
            torch.tensor(lengths, dtype=torch.int32, device="cuda"), q)
     assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("rows", [1024, 1025, 2100])
+def test_more_rows_than_workgroups_search(rows):
+    lengths = [(53 * r) % 331 for r in range(rows)]
+    lengths[rows // 2], lengths[rows - 1] = 6001, 2000
+    check("bf16", *build("bf16", 64, 3, 1, 16, lengths), lengths)
+    check("fp16", *build("fp16", 64, 2, 2, 20, lengths[:1030], window=300), lengths[:1030], 300)
+
+
+def test_very_many_rows():
+    """One key each: the output is its value."""
+    rows = 70001
+    keys, values = make_cache("bf16", rows, 16, 1, 64, fill=float("nan"))
+    g = torch.Generator("cuda").manual_seed(5)
+    keys[:, 0] = torch.randn(rows, 1, 64, generator=g, device="cuda").to(torch.bfloat16)
+    values[:, 0] = torch.randn(rows, 1, 64, generator=g, device="cuda").to(torch.bfloat16)
+    pages = torch.randperm(rows, generator=g, device="cuda").to(torch.int32)
+    q = torch.randn(rows, 128, generator=g, device="cuda").to(torch.bfloat16)
+    size = torch.ones(rows, dtype=torch.int32, device="cuda")
+    for width in (1, 20):
+        tables = torch.full((rows, width), -1, dtype=torch.int32, device="cuda")
+        tables[:, 0] = pages
+        out = torch.zeros(rows, 128, dtype=torch.bfloat16, device="cuda")
+        attend(describe(keys, values, "bf16"), q, 2, tables, size, out)
+        want = values[pages.long(), 0]
+        assert torch.equal(out.view(rows, 2, 64), want.expand(rows, 2, 64))
