@@ -359,9 +359,13 @@ constexpr int ONE_PART_KEYS = 256, ONE_PART_KEYS_FULL = 512;
 // of 2,048 keys in 48 rows of heads of 64 45.3 / 39.6 / 38.0 with 1,024 / 1,536 / 2,048.
 constexpr int CUS = 256;
 inline int attn_tiles(int heads, int kv_heads) { return (heads / kv_heads + 15) / 16; }
-inline int attn_target(int heads, int kv_heads, int head_dim) {
+// Twice as many where the rows alone are as many as the CUs hold: parts of more equal lengths (128 rows of 100 to
+// 8,000 keys on 8 KV heads 267 -> 205 us, 1,024 on one 234 -> 188; all of 2,000 keys 185 -> 185 and 179 -> 184).
+constexpr int FINER = 2;
+inline int attn_target(int rows, int heads, int kv_heads, int head_dim) {
     const int held = head_dim <= 64 ? 6 : head_dim <= 128 ? 4 : 2;
-    return std::max(1, CUS * held / (kv_heads * attn_tiles(heads, kv_heads)));
+    const int64_t tiles = int64_t(kv_heads) * attn_tiles(heads, kv_heads);
+    return std::max(1, int(CUS * held * (rows * tiles >= CUS * held ? FINER : 1) / tiles));
 }
 
 // How a workgroup finds its part: it is its row; in all rows' lengths; in the list of a launch before.  The second
@@ -946,7 +950,7 @@ void launch_paged_qkv(const PagedQkvParams& p, int source, int type, int head_di
 }
 
 size_t paged_attn_workspace(int rows, int heads, int kv_heads, int head_dim) {
-    const size_t parts = size_t(rows) + size_t(attn_target(heads, kv_heads, head_dim));
+    const size_t parts = size_t(rows) + size_t(attn_target(rows, heads, kv_heads, head_dim));
     const size_t lists = (size_t(rows) * sizeof(int2) + 15) / 16 * 16 + (parts * size_t(heads) * sizeof(float2) + 15) / 16 * 16;
     return lists + parts * size_t(heads) * size_t(head_dim) * sizeof(float);
 }
@@ -954,7 +958,7 @@ size_t paged_attn_workspace(int rows, int heads, int kv_heads, int head_dim) {
 void paged_attn_bind(PagedAttnParams& p, void* workspace, int head_dim) {
     const int heads = p.kv_heads * p.group;
     p.tiles = attn_tiles(heads, p.kv_heads);
-    p.target = attn_target(heads, p.kv_heads, head_dim);
+    p.target = attn_target(p.rows, heads, p.kv_heads, head_dim);
     const int one_part = int64_t(p.rows) * p.kv_heads * p.tiles >= CUS ? ONE_PART_KEYS_FULL : ONE_PART_KEYS;
     p.reach = (p.window > 0 ? std::min(p.window, p.most) : p.most) + 15;
     p.least = p.reach <= one_part ? one_part : PART_KEYS;
