@@ -340,8 +340,8 @@ __global__ __launch_bounds__(256) void paged_qkv_kernel(PagedQkvParams p) {
 // bytes: 16 heads on one KV head cost 2 x 16 x 128 products for 512 bytes, a fifth of what the matrix
 // units do in that time.  Two rows of 131,072 keys on 4 KV heads (537 MB) take 91.3 us, 5.9 TB/s; 128 rows of 33 to
 // 16,384 keys on one (177 MB) 36.0 us, 4.9 TB/s: the start, the search for the work and the last part's end are
-// in that.  More than 16 heads of a KV head are tiles of 16, each of which reads the pages (34 heads on 2 KV
-// heads: 1.7 times the time of the same bytes on 16).
+// in that.  More than 16 heads of a KV head are tiles of 16, which take the pages from memory once and then from the
+// L2 (34 heads on 2 KV heads 80 us, 1.3 times the time of the same bytes on 32).
 // The weights are kept in two halves of the type (p = hi + lo, 2^-17 off for BF16, 2^-23 for FP16): one
 // rounding of them would be as large an error as the output's own, and the second product is hidden by the loads
 // (30.8 us without, 31.3 with).
@@ -546,30 +546,37 @@ struct Tile {
     bool whole;     // all keys of the tile are
 };
 
-// Reads of the pages: each once, so not to stay in the caches (nt: two rows of 131,072 keys 98.6 -> 88.2 us,
-// 128 ragged rows 41.7 -> 36.8), and issued where they stand (volatile).
-__device__ __forceinline__ uint4 stream16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
-    const u32x4_t v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, int(0x80000002u));
+// Reads of the pages.  Where a part is one workgroup's they are read once, so not to stay in the caches (nt: two
+// rows of 131,072 keys 98.6 -> 88.2 us, 128 ragged rows 41.7 -> 36.8), and issued where they stand (volatile).  Where
+// it is several tiles of heads' (SHARED), these are side by side on one XCD and the second finds them in
+// its L2: 64 rows of 2,000 to 8,000 keys and 32 heads on one KV head 62.6 -> 49.1 us, 64 heads 109 -> 69.
+template <bool SHARED>
+__device__ __forceinline__ uint4 read16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    const u32x4_t v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, SHARED ? 0 : int(0x80000002u));
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
-__device__ __forceinline__ uint2 stream8(__amdgpu_buffer_rsrc_t r, uint32_t off) {
-    const u32x2_t v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, int(0x80000002u));
+template <bool SHARED>
+__device__ __forceinline__ uint2 read8(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    const u32x2_t v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, SHARED ? 0 : int(0x80000002u));
     return make_uint2(v[0], v[1]);
 }
-
-__device__ __forceinline__ uint4 stream16(const char* at) {
-    const u32x4_t v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(at));
+template <bool SHARED>
+__device__ __forceinline__ uint4 read16(const char* at) {
+    const u32x4_t* from = reinterpret_cast<const u32x4_t*>(at);
+    const u32x4_t v = SHARED ? *from : __builtin_nontemporal_load(from);
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
-__device__ __forceinline__ uint2 stream8(const char* at) {
-    const u32x2_t v = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(at));
+template <bool SHARED>
+__device__ __forceinline__ uint2 read8(const char* at) {
+    const u32x2_t* from = reinterpret_cast<const u32x2_t*>(at);
+    const u32x2_t v = SHARED ? *from : __builtin_nontemporal_load(from);
     return make_uint2(v[0], v[1]);
 }
 
 // EVEN: pages of whole half tiles (a multiple of 16 tokens), so that a half tile is one page's and
 // its page and addresses are the wave's, not the lane's.  64 rows of 5,000 keys from memory take 42.1 us so, 43.6 the
 // other way, which any page size allows; 48 of a window of 2,048, 32 heads of 64 on 8, 44.7 and 48.8.
-template <int TYPE, int D, bool EVEN>
+template <int TYPE, int D, bool EVEN, bool SHARED>
 __device__ __forceinline__ void load_tile(Tile<TYPE, D>& t, const PagedAttnParams& p, const int32_t* table,
                                           int64_t head, int pos, int lo_key, int hi_key) {
     typedef Tile<TYPE, D> X;
@@ -604,17 +611,17 @@ __device__ __forceinline__ void load_tile(Tile<TYPE, D>& t, const PagedAttnParam
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int s = 0; s < X::STEPS; ++s) t.k[h][s] = stream16(kr[h], ks + s * 64);
+            for (int s = 0; s < X::STEPS; ++s) t.k[h][s] = read16<SHARED>(kr[h], ks + s * 64);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
             for (int s = 0; s < X::SLABS; ++s) {
                 const uint32_t at = uint32_t((4 * g + (i & 3)) * int(p.slot_stride) + col * X::CHUNK * 2 + s * 256);
                 if constexpr (X::CHUNK == 8) {
-                    const uint4 w = stream16(vr[i >> 2], at);
+                    const uint4 w = read16<SHARED>(vr[i >> 2], at);
                     t.v[i][s][0] = w.x, t.v[i][s][1] = w.y, t.v[i][s][2] = w.z, t.v[i][s][3] = w.w;
                 } else {
-                    const uint2 w = stream8(vr[i >> 2], at);
+                    const uint2 w = read8<SHARED>(vr[i >> 2], at);
                     t.v[i][s][0] = w.x, t.v[i][s][1] = w.y;
                 }
             }
@@ -633,7 +640,7 @@ __device__ __forceinline__ void load_tile(Tile<TYPE, D>& t, const PagedAttnParam
             const int64_t off = __shfl(own, 16 * h + col, 64);
 #pragma unroll
             for (int s = 0; s < X::STEPS; ++s)
-                t.k[h][s] = off >= 0 ? stream16(p.keys + off + g * 16 + s * 64) : make_uint4(0, 0, 0, 0);
+                t.k[h][s] = off >= 0 ? read16<SHARED>(p.keys + off + g * 16 + s * 64) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -643,10 +650,10 @@ __device__ __forceinline__ void load_tile(Tile<TYPE, D>& t, const PagedAttnParam
             for (int s = 0; s < X::SLABS; ++s) {
                 const char* from = p.values + off + col * X::CHUNK * 2 + s * 256;
                 if constexpr (X::CHUNK == 8) {
-                    const uint4 x = off >= 0 ? stream16(from) : make_uint4(0, 0, 0, 0);
+                    const uint4 x = off >= 0 ? read16<SHARED>(from) : make_uint4(0, 0, 0, 0);
                     t.v[i][s][0] = x.x, t.v[i][s][1] = x.y, t.v[i][s][2] = x.z, t.v[i][s][3] = x.w;
                 } else {
-                    const uint2 x = off >= 0 ? stream8(from) : make_uint2(0, 0);
+                    const uint2 x = off >= 0 ? read8<SHARED>(from) : make_uint2(0, 0);
                     t.v[i][s][0] = x.x, t.v[i][s][1] = x.y;
                 }
             }
@@ -734,7 +741,7 @@ __device__ __forceinline__ void take_tile(Running<TYPE, D>& run, Tile<TYPE, D>& 
 // Waves of a SIMD whose registers hold them (uneven pages hold 64-bit addresses too).
 constexpr int attn_waves(int head_dim, bool even) { return head_dim == 64 ? (even ? 6 : 5) : head_dim == 128 ? (even ? 4 : 3) : 2; }
 
-template <int TYPE, int D, bool EVEN>
+template <int TYPE, int D, bool EVEN, bool SHARED>
 __global__ __launch_bounds__(ATTN_THREADS, attn_waves(D, EVEN)) void paged_attention_kernel(PagedAttnParams p) {
     typedef Tile<TYPE, D> X;
     constexpr int PITCH = D + 4;
@@ -743,12 +750,24 @@ __global__ __launch_bounds__(ATTN_THREADS, attn_waves(D, EVEN)) void paged_atten
     __shared__ WorkShared s_work;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int item = blockIdx.x, kv = blockIdx.y / p.tiles, tile = blockIdx.y - kv * p.tiles;
+    // workgroups go to the eight XCDs in turn: eight parts' first tiles, their second ones, ...
+    const int kv = blockIdx.y;
+    int item = blockIdx.x, tile = 0;
+    if constexpr (SHARED) {
+        const int eight = int(blockIdx.x) / (8 * p.tiles), rest = int(blockIdx.x) - eight * 8 * p.tiles;
+        item = eight * 8 + (rest & 7);
+        tile = rest >> 3;
+    }
     Work work;
     bool any = true;
-    if (p.division == DIVISION_NONE) work = {item, item, 1};
-    else if (p.division == DIVISION_LISTED) any = look_up_work(p, item, work);
-    else any = find_work(p, s_work, item, work);
+    if (p.division == DIVISION_NONE) {
+        work = {item, item, 1};
+        any = !SHARED || item < p.rows;
+    } else if (p.division == DIVISION_LISTED) {
+        any = look_up_work(p, item, work);
+    } else {
+        any = find_work(p, s_work, item, work);
+    }
     if (!any) return;  // every wave of the workgroup
     const int row = __builtin_amdgcn_readfirstlane(work.row), first_part = __builtin_amdgcn_readfirstlane(work.first),
               parts = __builtin_amdgcn_readfirstlane(work.parts);
@@ -758,7 +777,7 @@ __global__ __launch_bounds__(ATTN_THREADS, attn_waves(D, EVEN)) void paged_atten
     const int each = __builtin_amdgcn_readfirstlane(((len - (first & ~15) + parts - 1) / parts + 31) & ~31);
     const int begin = (first & ~15) + part * each, end = min(len, begin + each);
     const int heads = p.kv_heads * p.group, head0 = kv * p.group + tile * 16, live = min(16, p.group - tile * 16);
-    if (p.division == DIVISION_FOUND && blockIdx.y == 0 && threadIdx.x == 0 && part == 0) p.row_parts[row] = make_int2(first_part, parts);
+    if (p.division == DIVISION_FOUND && blockIdx.y == 0 && tile == 0 && threadIdx.x == 0 && part == 0) p.row_parts[row] = make_int2(first_part, parts);
 
     uint4 q[X::STEPS];
     const uint16_t* qrow = p.q + row * p.q_stride + int64_t(head0 + min(col, live - 1)) * D;
@@ -774,7 +793,7 @@ __global__ __launch_bounds__(ATTN_THREADS, attn_waves(D, EVEN)) void paged_atten
         for (int j = 0; j < X::CHUNK; ++j) run.o[b][j] = floatx4{0.f, 0.f, 0.f, 0.f};
     for (int pos = begin + 32 * wave; pos < end; pos += PART_KEYS) {
         Tile<TYPE, D> t;
-        load_tile<TYPE, D, EVEN>(t, p, table, head, pos, first, end);
+        load_tile<TYPE, D, EVEN, SHARED>(t, p, table, head, pos, first, end);
         take_tile<TYPE, D>(run, t, q, p.scale);
     }
     run.l += xor_lane<16>(run.l);
@@ -900,12 +919,16 @@ void run_attention(const PagedAttnParams& p, hipStream_t s) {
     // row's only one
     const int64_t most = int64_t(p.rows) * std::max<int64_t>(1, (int64_t(p.reach) + p.least - 1) / p.least);
     const unsigned parts = unsigned(std::min<int64_t>(most, int64_t(p.rows) + p.target));
-    const dim3 grid(parts, unsigned(p.kv_heads * p.tiles));
+    const bool shared = p.tiles > 1;
+    // parts beside each other, KV heads one after the other: the other way two rows of 131,072 keys on 4 KV heads take
+    // 105 us for 91
+    const dim3 grid(shared ? (parts + 7) / 8 * 8 * unsigned(p.tiles) : parts, unsigned(p.kv_heads));
     if (p.division == DIVISION_LISTED) hipLaunchKernelGGL(paged_parts_kernel, dim3(1), dim3(DIVIDE_THREADS), 0, s, p);
-    if (p.page_size % 16 == 0)
-        hipLaunchKernelGGL((paged_attention_kernel<TYPE, D, true>), grid, dim3(ATTN_THREADS), 0, s, p);
-    else
-        hipLaunchKernelGGL((paged_attention_kernel<TYPE, D, false>), grid, dim3(ATTN_THREADS), 0, s, p);
+    const bool even = p.page_size % 16 == 0;
+    if (even && shared) hipLaunchKernelGGL((paged_attention_kernel<TYPE, D, true, true>), grid, dim3(ATTN_THREADS), 0, s, p);
+    else if (even) hipLaunchKernelGGL((paged_attention_kernel<TYPE, D, true, false>), grid, dim3(ATTN_THREADS), 0, s, p);
+    else if (shared) hipLaunchKernelGGL((paged_attention_kernel<TYPE, D, false, true>), grid, dim3(ATTN_THREADS), 0, s, p);
+    else hipLaunchKernelGGL((paged_attention_kernel<TYPE, D, false, false>), grid, dim3(ATTN_THREADS), 0, s, p);
     if (p.division != DIVISION_NONE) {
         // few rows have many parts each, many rows few: most of their workgroups would find nothing to join (128 rows
         // of 16 heads 5.8 us with a head a workgroup, 6.9 with four; 1,000 rows, attention and all, 81.2 and 71.6)
