@@ -30,13 +30,13 @@ __device__ __forceinline__ uint32_t divide(uint32_t x, Divider d) { return uint3
 // One workgroup: prefix sums over the requests of pages given back, pages taken and tokens, then the
 // moves flattened over pages so that a long request's are not one thread's.  Latency-bound: a few KB move
 // in the time of some dependent loads (lengths, free pages, tables) and barriers: 64 requests of one new token
-// 6.6 us with their slots, 1,000 requests that end, grow and begin 11.8, and 4.6 to 5.3 for 65,536 slots.  More
+// 6.3 us with their slots, 1,000 requests that end, grow and begin 11.7, and 4.1 for 65,536 slots.  More
 // than one workgroup would have to wait for each other between the checks of all requests and the first write.
 constexpr int TABLE_THREADS = 1024;
 
 // Places up to which the tables' workgroup fills in the slots too: each costs a search of the offsets, which
-// one CU does more slowly than all, but a launch costs 2 us (2,048 places: 7.9 us so, 9.0 in a launch of their
-// own; 4,096: 10.6 and 9.2).
+// one CU does more slowly than all, but a launch costs 2 us (2,048 places: 7.4 us so, 8.3 in a launch of their
+// own; 4,096: 9.1 and 8.6).
 constexpr int SLOTS_IN_TABLES = 2048;
 
 struct Scan3 {
@@ -107,12 +107,13 @@ __device__ __forceinline__ int first_above(const int* sums, int n, int x) {
     return lo;
 }
 
-// Token j of the step: its request by the offsets, its position behind the request's old length, its slot.
-__device__ __forceinline__ void token_slot(const PagedTablesParams& p, int j, int total) {
+// Token j of the step: its request by the ends of all requests' tokens, its position before the request's new
+// length, its slot.
+__device__ __forceinline__ void token_slot(const PagedTablesParams& p, const int* ends, const int* lengths, int j, int total) {
     int slot = -1, at = -1;
     if (j < total) {
-        const int r = first_above(p.offsets + 1, p.rows, j);
-        at = p.lengths_out[r] - (p.offsets[r + 1] - j);
+        const int r = first_above(ends, p.rows, j);
+        at = lengths[r] - (ends[r] - j);
         const uint32_t page = divide(uint32_t(at), p.div);
         slot = p.tables[int64_t(r) * p.width + page] * p.page_size + (at - int(page) * p.page_size);
     }
@@ -126,6 +127,8 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(PagedTables
     __shared__ unsigned long long s_back, s_take, s_fresh;
     __shared__ int s_status;
     __shared__ int s_sums[TABLE_THREADS], s_start[TABLE_THREADS], s_held[TABLE_THREADS];
+    // where the requests' tokens end, and their new lengths (of the last TABLE_THREADS requests)
+    __shared__ int s_ends[SLOTS ? TABLE_THREADS : 1], s_lengths[SLOTS ? TABLE_THREADS : 1];
     const int tid = threadIdx.x;
     if (tid == 0) {
         s_back = s_take = s_fresh = 0;
@@ -212,8 +215,13 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(PagedTables
                     }
                 }
                 if (pass && r < p.rows) {
-                    p.offsets[r + 1] = run.fresh + incl.fresh;
-                    p.lengths_out[r] = count < 0 ? 0 : length + count;
+                    const int end = run.fresh + incl.fresh, now = count < 0 ? 0 : length + count;
+                    p.offsets[r + 1] = end;
+                    p.lengths_out[r] = now;
+                    if constexpr (SLOTS) {
+                        s_ends[tid] = end;
+                        s_lengths[tid] = now;
+                    }
                 }
                 run = {run.back + sum.back, run.take + sum.take, run.fresh + sum.fresh};
             }
@@ -222,13 +230,27 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(PagedTables
     }
     if constexpr (SLOTS) {
         __syncthreads();
-        for (int j = tid; j < p.capacity; j += TABLE_THREADS) token_slot(p, j, total);
+        if (p.rows <= TABLE_THREADS)
+            for (int j = tid; j < p.capacity; j += TABLE_THREADS) token_slot(p, s_ends, s_lengths, j, total);
+        else
+            for (int j = tid; j < p.capacity; j += TABLE_THREADS) token_slot(p, p.offsets + 1, p.lengths_out, j, total);
     }
 }
 
+// The search is in LDS where the offsets fit: its steps wait for each other (1,000 requests, 65,536 places 4.6 us in
+// memory, 4.1 so).
+constexpr int SLOTS_ENDS = 4096;
 __global__ __launch_bounds__(256) void paged_slots_kernel(PagedTablesParams p) {
+    __shared__ int s_ends[SLOTS_ENDS];
     const int j = int(blockIdx.x * 256 + threadIdx.x);
-    if (j < p.capacity) token_slot(p, j, p.offsets[p.rows]);
+    if (p.rows <= SLOTS_ENDS) {
+#pragma unroll 4
+        for (int r = threadIdx.x; r < p.rows; r += 256) s_ends[r] = p.offsets[r + 1];
+        __syncthreads();
+        if (j < p.capacity) token_slot(p, s_ends, p.lengths_out, j, s_ends[p.rows - 1]);
+    } else if (j < p.capacity) {
+        token_slot(p, p.offsets + 1, p.lengths_out, j, p.offsets[p.rows]);
+    }
 }
 
 // ------------------------------------------------------------------------------------ qkv
