@@ -296,3 +296,13 @@ def test_very_many_rows():
         attend(describe(keys, values, "bf16"), q, 2, tables, size, out)
         want = values[pages.long(), 0]
         assert torch.equal(out.view(rows, 2, 64), want.expand(rows, 2, 64))
+
+
+@pytest.mark.parametrize("rows,most", [(1, 90), (7, 200), (9, 700), (30, 1500), (1030, 300)])
+@pytest.mark.parametrize("page", [16, 9])
+def test_several_tiles_of_heads(rows, most, page):
+    """33 heads on one KV head are three tiles of a part: alone, in parts, and of listed parts."""
+    lengths = [most - (29 * r) % most for r in range(rows)]
+    check("bf16", *build("bf16", 64, 33, 1, page, lengths), lengths)
+    if rows < 100:
+        check("fp16", *build("fp16", 128, 36, 2, page, lengths), lengths)
