@@ -409,8 +409,11 @@ typedef struct plamo_paged_cache {
  * its position and slot (page * page_size + place in the page) in positions and slots [capacity], -1
  * behind the last.  All int32, on the device.  All or nothing: with `status` (a sum of 1: too few free
  * pages, 2: a request needs more than `width` pages, 4: more than `capacity` tokens, 8: invalid lengths,
- * counts or free_count) other than 0 no length, table or free page changes and offsets are 0, slots and
- * positions -1. */
+ * counts, free_count or pages) other than 0 no length, table or free page changes and offsets are 0, slots and
+ * positions -1.  An entry outside 0 .. pages - 1 is no page, as where the caller has given the pages behind a
+ * window back itself: none goes back for it when its request ends, and a step that would take one from
+ * free_pages, or put a token into one, has status 8 (as has one that gives back more than 2^30 entries).  A page
+ * goes back with each request that ends and names it: of tables that share pages one alone may keep them then. */
 int plamo_kernel_paged_tables(uint64_t lengths, uint64_t counts, int32_t rows, uint64_t tables, int32_t width,
                               int32_t page_size, uint64_t free_pages, uint64_t free_count, int32_t pages,
                               uint64_t lengths_out, uint64_t free_out, uint64_t offsets, uint64_t slots,

@@ -30,14 +30,19 @@ __device__ __forceinline__ uint32_t divide(uint32_t x, Divider d) { return uint3
 // One workgroup: prefix sums over the requests of pages given back, pages taken and tokens, then the
 // moves flattened over pages so that a long request's are not one thread's.  Latency-bound: a few KB move
 // in the time of some dependent loads (lengths, free pages, tables) and barriers: 64 requests of one new token
-// 6.3 us with their slots, 1,000 requests that end, grow and begin 11.7, and 4.1 for 65,536 slots.  More
-// than one workgroup would have to wait for each other between the checks of all requests and the first write.
+// 7.2 us with their slots, 1,000 requests that end, grow and begin 13.2, and 4.1 for 65,536 slots.  Checking that
+// what goes back or is filled is a page is 0.9 and 1.6 us of that.  More than one workgroup would have to wait for
+// each other between the checks of all requests and the first write.
 constexpr int TABLE_THREADS = 1024;
 
 // Places up to which the tables' workgroup fills in the slots too: each costs a search of the offsets, which
 // one CU does more slowly than all, but a launch costs 2 us (2,048 places: 7.4 us so, 8.3 in a launch of their
 // own; 4,096: 9.1 and 8.6).
 constexpr int SLOTS_IN_TABLES = 2048;
+
+// Table entries that requests may give back in a step (their places are 32-bit numbers), and how many are kept in LDS
+// between the check and the move, which is then no second reading of the tables.
+constexpr int MOST_GIVEN = 1 << 30, KEPT_GIVEN = 8192;
 
 struct Scan3 {
     int back, take, fresh;
@@ -107,6 +112,41 @@ __device__ __forceinline__ int first_above(const int* sums, int n, int x) {
     return lo;
 }
 
+__device__ __forceinline__ bool is_page(const PagedTablesParams& p, int32_t entry) { return uint32_t(entry) < uint32_t(p.pages); }
+
+struct TablesShared {
+    Scan3 waves[TABLE_THREADS / 64];
+    int sums[TABLE_THREADS], start[TABLE_THREADS], held[TABLE_THREADS];
+};
+
+// f(i, entry) for the table entries of all requests that end, in the order of requests and entries: a workgroup's
+// threads side by side, those past the last one with no i (INT32_MAX) and -1.
+template <typename F>
+__device__ __forceinline__ void for_given(const PagedTablesParams& p, TablesShared& s, int own_length, int own_count, F f) {
+    const int tid = threadIdx.x;
+    int before = 0;
+    for (int base = 0; base < p.rows; base += TABLE_THREADS) {
+        const int r = base + tid;
+        int held = 0, back = 0;
+        if (r < p.rows) back = row_moves(p, base ? p.lengths[r] : own_length, base ? p.counts[r] : own_count, held).back;
+        Scan3 sum;
+        const Scan3 incl = block_scan3({back, 0, 0}, s.waves, sum);
+        s.sums[tid] = incl.back;
+        s.start[tid] = incl.back - back;
+        __syncthreads();
+        for (int at = 0; at < sum.back; at += TABLE_THREADS) {
+            const int e = at + tid;
+            int32_t entry = -1;
+            if (e < sum.back) {
+                const int q = first_above(s.sums, TABLE_THREADS, e);
+                entry = p.tables[int64_t(base + q) * p.width + (e - s.start[q])];
+            }
+            f(e < sum.back ? before + e : INT32_MAX, entry);
+        }
+        before += sum.back;
+    }
+}
+
 // Token j of the step: its request by the ends of all requests' tokens, its position before the request's new
 // length, its slot.
 __device__ __forceinline__ void token_slot(const PagedTablesParams& p, const int* ends, const int* lengths, int j, int total) {
@@ -123,18 +163,21 @@ __device__ __forceinline__ void token_slot(const PagedTablesParams& p, const int
 
 template <bool SLOTS>
 __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(PagedTablesParams p) {
-    __shared__ Scan3 s_waves[TABLE_THREADS / 64];
+    __shared__ TablesShared s;
     __shared__ unsigned long long s_back, s_take, s_fresh;
-    __shared__ int s_status;
-    __shared__ int s_sums[TABLE_THREADS], s_start[TABLE_THREADS], s_held[TABLE_THREADS];
+    __shared__ int s_status, s_given;
+    __shared__ int32_t s_entries[KEPT_GIVEN];
     // where the requests' tokens end, and their new lengths (of the last TABLE_THREADS requests)
     __shared__ int s_ends[SLOTS ? TABLE_THREADS : 1], s_lengths[SLOTS ? TABLE_THREADS : 1];
     const int tid = threadIdx.x;
     if (tid == 0) {
         s_back = s_take = s_fresh = 0;
-        s_status = 0;
+        s_status = s_given = 0;
     }
     const int64_t first = *p.free_count;
+    // the stack's top is on its way while the requests are added up
+    const int64_t own_top = first - 1 - tid;
+    const int32_t own_page = own_top >= 0 && own_top < p.pages ? p.free_pages[own_top] : -1;
     // the first TABLE_THREADS requests' stay in registers
     int own_length = 0, own_count = 0;
     if (tid < p.rows) {
@@ -154,6 +197,8 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(PagedTables
         const int64_t held = (length + p.page_size - 1) / p.page_size;
         const int64_t after = count < 0 ? 0 : (length + count + p.page_size - 1) / p.page_size;
         if (held > p.width || after > p.width || length + count > INT32_MAX) bad |= 2;
+        // a page that new tokens fill up
+        else if (count > 0 && held * p.page_size > length && !is_page(p, p.tables[r * int64_t(p.width) + held - 1])) bad |= 8;
         if (count < 0) back += held;
         else take += after - held, fresh += count;
     }
@@ -170,11 +215,33 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(PagedTables
         atomicAdd(&s_fresh, static_cast<unsigned long long>(fresh));
     }
     __syncthreads();
-    const int64_t full = first + int64_t(s_back);
     int status = s_status;
+    // entries that go back, and how many of them are pages (behind a window none may be left)
+    const int64_t entries = int64_t(s_back);
+    if (entries > MOST_GIVEN) status |= 8;
+    int64_t given = entries;
+    if (entries && !status) {
+        int own = 0;
+        for_given(p, s, own_length, own_count, [&](int i, int32_t entry) {
+            own += is_page(p, entry);
+            if (i < KEPT_GIVEN) s_entries[i] = entry;
+        });
+        for (int o = 32; o > 0; o >>= 1) own += __shfl_xor(own, o, 64);
+        if ((tid & 63) == 0) atomicAdd(&s_given, own);
+        __syncthreads();
+        given = s_given;
+    }
+    const int64_t full = first + given;
     if (first < 0 || full > p.pages) status |= 8;
     else if (int64_t(s_take) > full) status |= 1;
     if (int64_t(s_fresh) > p.capacity) status |= 4;
+    if (!status) {
+        // what is taken from the stack as it was
+        const int taken = int(max(int64_t(s_take) - given, int64_t(0)));
+        int wrong = tid < taken && !is_page(p, own_page);
+        for (int i = tid + TABLE_THREADS; i < taken; i += TABLE_THREADS) wrong |= !is_page(p, p.free_pages[first - 1 - i]);
+        if (__syncthreads_or(wrong)) status = 8;
+    }
     if (tid == 0) {
         *p.status = status;
         p.offsets[0] = 0;
@@ -187,45 +254,57 @@ __global__ __launch_bounds__(TABLE_THREADS) void paged_tables_kernel(PagedTables
             p.lengths_out[r] = p.lengths[r];
         }
     } else {
-        // pages given back, on top of the free ones, in row order; then pages taken, lengths and offsets
-        Scan3 sum;
-        for (int pass = s_back ? 0 : 1; pass < 2; ++pass) {
-            Scan3 run = {0, 0, 0};
-            for (int base = 0; base < p.rows; base += TABLE_THREADS) {
-                const int r = base + tid;
-                int held = 0, length = own_length, count = own_count;
-                if (base > 0 && r < p.rows) {
-                    length = p.lengths[r];
-                    count = p.counts[r];
-                }
-                const Scan3 own = r < p.rows ? row_moves(p, length, count, held) : Scan3{0, 0, 0};
-                const Scan3 incl = block_scan3(own, s_waves, sum);
-                const int moved = pass ? own.take : own.back, chunk = pass ? sum.take : sum.back;
-                const int before = pass ? run.take : run.back;
-                if (chunk) {
-                    s_sums[tid] = pass ? incl.take : incl.back;
-                    s_start[tid] = s_sums[tid] - moved;
-                    s_held[tid] = held;
-                    __syncthreads();
-                    for (int e = tid; e < chunk; e += TABLE_THREADS) {
-                        const int q = first_above(s_sums, TABLE_THREADS, e), i = e - s_start[q];
-                        int32_t* table = p.tables + int64_t(base + q) * p.width;
-                        if (pass) table[s_held[q] + i] = p.free_pages[full - 1 - (before + e)];
-                        else p.free_pages[first + before + e] = table[i];
-                    }
-                }
-                if (pass && r < p.rows) {
-                    const int end = run.fresh + incl.fresh, now = count < 0 ? 0 : length + count;
-                    p.offsets[r + 1] = end;
-                    p.lengths_out[r] = now;
-                    if constexpr (SLOTS) {
-                        s_ends[tid] = end;
-                        s_lengths[tid] = now;
-                    }
-                }
-                run = {run.back + sum.back, run.take + sum.take, run.fresh + sum.fresh};
+        // pages given back, on top of the free ones, in row order
+        auto for_kept = [&](auto f) {
+            if (entries > KEPT_GIVEN) return for_given(p, s, own_length, own_count, f);
+            for (int i = tid; i - tid < entries; i += TABLE_THREADS) f(i < entries ? i : INT32_MAX, i < entries ? s_entries[i] : -1);
+        };
+        if (given == entries) {
+            for_kept([&](int i, int32_t entry) {
+                if (i < given) p.free_pages[first + i] = entry;
+            });
+        } else if (given) {
+            int before = 0;
+            for_kept([&](int, int32_t entry) {
+                const int own = is_page(p, entry);
+                Scan3 sum;
+                const int at = before + block_scan3({own, 0, 0}, s.waves, sum).back - 1;
+                if (own) p.free_pages[first + at] = entry;
+                before += sum.back;
+            });
+        }
+        if (given) __syncthreads();  // they are on the stack
+        // pages taken, lengths and offsets
+        Scan3 run = {0, 0, 0}, sum;
+        for (int base = 0; base < p.rows; base += TABLE_THREADS) {
+            const int r = base + tid;
+            int held = 0, length = own_length, count = own_count;
+            if (base > 0 && r < p.rows) {
+                length = p.lengths[r];
+                count = p.counts[r];
             }
-            __syncthreads();  // the pages given back are on the stack, the tables complete
+            const Scan3 own = r < p.rows ? row_moves(p, length, count, held) : Scan3{0, 0, 0};
+            const Scan3 incl = block_scan3(own, s.waves, sum);
+            if (sum.take) {
+                s.sums[tid] = incl.take;
+                s.start[tid] = incl.take - own.take;
+                s.held[tid] = held;
+                __syncthreads();
+                for (int e = tid; e < sum.take; e += TABLE_THREADS) {
+                    const int q = first_above(s.sums, TABLE_THREADS, e);
+                    p.tables[int64_t(base + q) * p.width + s.held[q] + (e - s.start[q])] = p.free_pages[full - 1 - (run.take + e)];
+                }
+            }
+            if (r < p.rows) {
+                const int end = run.fresh + incl.fresh, now = count < 0 ? 0 : length + count;
+                p.offsets[r + 1] = end;
+                p.lengths_out[r] = now;
+                if constexpr (SLOTS) {
+                    s_ends[tid] = end;
+                    s_lengths[tid] = now;
+                }
+            }
+            run = {0, run.take + sum.take, run.fresh + sum.fresh};
         }
     }
     if constexpr (SLOTS) {
