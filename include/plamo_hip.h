@@ -157,8 +157,9 @@ int plamo_sampler_observe(plamo_runtime* rt, int32_t id);
 
 /* A token drawn from the logits of output row `slot` (as plamo_logits gives them, without the controls above):
  * temperature, top-k, top-p and min-p as for plamo_kernel_sample, by the caller's `uniform` in [0, 1).  Leaves
- * position, logits, predictions and history alone: pass the token to plamo_forward as any other.  No
- * counterpart in the reference, which takes the largest logit. */
+ * position, logits, predictions and history alone: pass the token to plamo_forward as any other.  Refused where
+ * the last call left no output row (plamo_stats.last_output_rows is 0: before any call, after plamo_reset or a
+ * plamo_forward without output).  No counterpart in the reference, which takes the largest logit. */
 int plamo_sample(plamo_runtime* rt, int32_t slot, float temperature, int32_t top_k, float top_p, float min_p, float uniform,
                  int32_t* token, float* prob, char* err, size_t errlen);
 

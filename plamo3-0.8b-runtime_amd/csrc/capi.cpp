@@ -330,7 +330,7 @@ int plamo_sampler_observe(plamo_runtime* rt, int32_t id) {
 int plamo_sample(plamo_runtime* rt, int32_t slot, float temperature, int32_t top_k, float top_p, float min_p, float uniform,
                  int32_t* token, float* prob, char* err, size_t errlen) {
     return guard(err, errlen, [&] {
-        if (!rt || slot < 0 || slot >= std::max(1, rt->impl.last_output_rows))
+        if (!rt || slot < 0 || slot >= rt->impl.last_output_rows)
             throw plamo::Error(plamo::E_INVAL, "Invalid logits slot");
         if (!std::isfinite(temperature) || std::isnan(top_p) || std::isnan(min_p))
             throw plamo::Error(plamo::E_INVAL, "Invalid sampling controls");
