@@ -14,6 +14,7 @@ Every call goes to ``lib/libplamo_hip.so``; there is no CPU fallback.
 """
 import collections
 import ctypes
+import math
 
 import numpy as np
 
@@ -156,8 +157,10 @@ class Runtime:
         """A token drawn from the logits of output row `slot` by `uniform` in [0, 1) -> (token, its
         probability among those that the controls keep)."""
         token, prob = ctypes.c_int32(-1), ctypes.c_float()
+        # the library's number is FP32, where one just below 1 is 1 and one just below 0 is 0
+        uniform = min(float(uniform), 1 - 2.0 ** -24) if 0 <= uniform < 1 else math.nan
         native.call(self._lib.plamo_sample, self._h, int(slot), float(temperature), int(top_k), float(top_p),
-                    float(min_p), float(uniform), ctypes.byref(token), ctypes.byref(prob))
+                    float(min_p), uniform, ctypes.byref(token), ctypes.byref(prob))
         return token.value, prob.value
 
     def observe(self, token):
