@@ -159,7 +159,8 @@ class Runtime:
         token, prob = ctypes.c_int32(-1), ctypes.c_float()
         # the library's number is FP32, where one just below 1 is 1 and one just below 0 is 0
         uniform = min(float(uniform), 1 - 2.0 ** -24) if 0 <= uniform < 1 else math.nan
-        native.call(self._lib.plamo_sample, self._h, int(slot), float(temperature), int(top_k), float(top_p),
+        top_k = max(-2 ** 31, min(int(top_k), 2 ** 31 - 1))
+        native.call(self._lib.plamo_sample, self._h, int(slot), float(temperature), top_k, float(top_p),
                     float(min_p), uniform, ctypes.byref(token), ctypes.byref(prob))
         return token.value, prob.value
 

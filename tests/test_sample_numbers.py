@@ -34,3 +34,11 @@ def test_numbers_below_one(runtime, uniform):
 def test_numbers_outside(runtime, uniform):
     with pytest.raises(plamo_hip.PlamoError):
         runtime.sample(uniform)
+
+
+@pytest.mark.parametrize("top_k,want", [(0, 0), (-1, -1), (5, 5), (2 ** 31 - 1, 2 ** 31 - 1), (2 ** 31, 2 ** 31 - 1),
+                                        (2 ** 32 + 1, 2 ** 31 - 1), (2 ** 63 - 1, 2 ** 31 - 1), (-2 ** 32 + 5, -2 ** 31)])
+def test_top_k_past_32_bits(runtime, top_k, want):
+    """More tokens than there are is all of them, not what is left in the low bits."""
+    runtime.sample(0.5, top_k=top_k)
+    assert runtime._lib.top_k == want
