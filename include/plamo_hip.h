@@ -408,7 +408,7 @@ typedef struct plamo_paged_cache {
  * (others are left), lengths_out and free_out (which may be lengths and free_count themselves),
  * offsets[rows + 1] (request r's new tokens are offsets[r] .. offsets[r + 1] - 1), and for each of them
  * its position and slot (page * page_size + place in the page) in positions and slots [capacity], -1
- * behind the last.  All int32, on the device.  All or nothing: with `status` (a sum of 1: too few free
+ * behind the last.  All int32, on the device; rows and capacity at most 2^30.  All or nothing: with `status` (a sum of 1: too few free
  * pages, 2: a request needs more than `width` pages, 4: more than `capacity` tokens, 8: invalid lengths,
  * counts, free_count or pages) other than 0 no length, table or free page changes and offsets are 0, slots and
  * positions -1.  An entry outside 0 .. pages - 1 is no page, as where the caller has given the pages behind a

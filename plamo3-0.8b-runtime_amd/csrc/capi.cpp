@@ -919,7 +919,8 @@ int plamo_kernel_paged_tables(uint64_t lengths, uint64_t counts, int32_t rows, u
                               uint64_t positions, int32_t capacity, uint64_t status, uint64_t stream, char* err,
                               size_t errlen) {
     return guard(err, errlen, [&] {
-        require(rows >= 1 && width >= 1 && capacity >= 0, "paged tables: rows and width must be at least 1");
+        require(rows >= 1 && rows <= (1 << 30) && width >= 1 && capacity >= 0 && capacity <= (1 << 30),
+                "paged tables: rows must be 1...2^30, width at least 1, capacity 0...2^30");
         require(page_size >= 1 && pages >= 1 && int64_t(pages) * page_size <= INT32_MAX,
                 "paged tables: pages and page_size must be at least 1, and hold less than 2^31 tokens");
         require(lengths && counts && tables && free_pages && free_count && lengths_out && free_out && offsets && status &&
