@@ -487,14 +487,21 @@ __device__ __forceinline__ Row row_keys(const PagedAttnParams& p, int r) {
     k.span = k.len - (k.first & ~15);
     return k;
 }
-__device__ __forceinline__ int row_parts(int span, int chunk) { return max(1, (span + chunk - 1) / chunk); }
+__device__ __forceinline__ int row_parts(int span, int chunk) { return (span - 1) / chunk + 1; }  // one of none
 
-// Keys of a part: all rows' keys divided by the parts aimed at, in whole tiles for each wave.
-__device__ __forceinline__ int part_keys(const PagedAttnParams& p, long long keys) {
+// Keys of a part: all rows' keys divided by the parts aimed at, in whole tiles for each wave, and a row's at most.
+__host__ __device__ constexpr int part_length(long long keys, int aim, int rows, int least, int reach) {
     // a row's last part is half empty on the average
-    const int target = max(p.target - p.rows / 2, (p.target + 1) / 2);
-    const long long each = (keys + target - 1) / target;
-    return __builtin_amdgcn_readfirstlane(each <= p.least ? p.least : int((each + PART_KEYS - 1) / PART_KEYS * PART_KEYS));
+    const int parts = aim - rows / 2 > (aim + 1) / 2 ? aim - rows / 2 : (aim + 1) / 2;
+    const long long share = (keys + parts - 1) / parts, each = share < reach ? share : reach;
+    return each <= least ? least : int((each + PART_KEYS - 1) / PART_KEYS * PART_KEYS);
+}
+// a million rows of 2^30 keys, and a share next to 2^31
+static_assert(part_length(1LL << 50, 2048, 1 << 20, PART_KEYS, (1 << 30) + 15) == (1 << 30) + PART_KEYS, "32 bits hold it");
+static_assert(part_length((1LL << 42) - 1, 2048, 4096, PART_KEYS, (1 << 30) + 15) == (1 << 30) + PART_KEYS, "32 bits hold it");
+static_assert(part_length(2 * 131072, 1024, 2, PART_KEYS, 131072 + 15) == 384, "whole tiles");
+__device__ __forceinline__ int part_keys(const PagedAttnParams& p, long long keys) {
+    return __builtin_amdgcn_readfirstlane(part_length(keys, p.target, p.rows, p.least, p.reach));
 }
 
 // Where the workgroups find their work: the same division in all of them, from all rows' lengths.
