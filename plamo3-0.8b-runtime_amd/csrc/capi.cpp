@@ -1024,8 +1024,6 @@ int plamo_kernel_attention_paged(const plamo_paged_cache* cache, uint64_t q, int
         require(workspace && aligned(workspace, 16) &&
                     workspace_bytes >= plamo_kernel_attention_paged_workspace(rows, heads, cache->kv_heads, cache->head_dim),
                 "paged attention: workspace too small or not 16-byte aligned");
-        const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-        const OnDeviceOf device(s);
         plamo::PagedAttnParams p{};
         p.keys = reinterpret_cast<const char*>(cache->keys);
         p.values = reinterpret_cast<const char*>(cache->values);
@@ -1050,6 +1048,9 @@ int plamo_kernel_attention_paged(const plamo_paged_cache* cache, uint64_t q, int
         p.out_stride = out_stride;
         p.lse = reinterpret_cast<float*>(lse);
         plamo::paged_attn_bind(p, reinterpret_cast<void*>(workspace), cache->head_dim);
+        require(plamo::paged_attn_launches(p), "paged attention: too many rows of this many query heads to a KV head");
+        const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+        const OnDeviceOf device(s);
         plamo::launch_paged_attention(p, cache->type, cache->head_dim, s);
         PLAMO_HIP(hipGetLastError());
     });

@@ -96,6 +96,7 @@ struct PagedAttnParams {
 // Workspace bytes, and the pointers of a workspace.
 size_t paged_attn_workspace(int rows, int heads, int kv_heads, int head_dim);
 void paged_attn_bind(PagedAttnParams& p, void* workspace, int head_dim);
+bool paged_attn_launches(const PagedAttnParams& p);  // a launch's threads along a direction are a 32-bit number
 void launch_paged_attention(const PagedAttnParams& p, int type, int head_dim, hipStream_t s);
 
 // Tokens drawn from logits (plamo_kernel_sample).

@@ -1021,16 +1021,21 @@ __global__ __launch_bounds__(MERGE_THREADS) void paged_merge_kernel(PagedAttnPar
     }
 }
 
-template <int TYPE, int D>
-void run_attention(const PagedAttnParams& p, hipStream_t s) {
+// Workgroups of a KV head.
+int64_t attn_workgroups(const PagedAttnParams& p) {
     // parts: at most one more than its share of the aimed ones for each row, and none of less than p.least but a
     // row's only one
     const int64_t most = int64_t(p.rows) * std::max<int64_t>(1, (int64_t(p.reach) + p.least - 1) / p.least);
-    const unsigned parts = unsigned(std::min<int64_t>(most, int64_t(p.rows) + p.target));
+    const int64_t parts = std::min<int64_t>(most, int64_t(p.rows) + p.target);
+    return p.tiles > 1 ? (parts + 7) / 8 * 8 * p.tiles : parts;
+}
+
+template <int TYPE, int D>
+void run_attention(const PagedAttnParams& p, hipStream_t s) {
     const bool shared = p.tiles > 1;
     // parts beside each other, KV heads one after the other: the other way two rows of 131,072 keys on 4 KV heads take
     // 105 us for 91
-    const dim3 grid(shared ? (parts + 7) / 8 * 8 * unsigned(p.tiles) : parts, unsigned(p.kv_heads));
+    const dim3 grid(unsigned(attn_workgroups(p)), unsigned(p.kv_heads));
     if (p.division == DIVISION_LISTED) hipLaunchKernelGGL(paged_parts_kernel, dim3(1), dim3(DIVIDE_THREADS), 0, s, p);
     const bool even = p.page_size % 16 == 0;
     if (even && shared) hipLaunchKernelGGL((paged_attention_kernel<TYPE, D, true, true>), grid, dim3(ATTN_THREADS), 0, s, p);
@@ -1102,6 +1107,8 @@ void paged_attn_bind(PagedAttnParams& p, void* workspace, int head_dim) {
     at += (parts * size_t(heads) * sizeof(float2) + 15) / 16 * 16;
     p.part_o = reinterpret_cast<float*>(at);
 }
+
+bool paged_attn_launches(const PagedAttnParams& p) { return attn_workgroups(p) * ATTN_THREADS <= UINT32_MAX; }
 
 void launch_paged_attention(const PagedAttnParams& p, int type, int head_dim, hipStream_t s) {
     if (type == TYPE_BF16) {
