@@ -457,8 +457,8 @@ int plamo_kernel_attention_paged(const plamo_paged_cache* cache, uint64_t q, int
  * top_p of the weight lies (at least one), of them those of at least min_p of the largest weight; `token`
  * (int32) is the first up to which more than `uniform` of the weight that is left lies, and prob (FP32, 0:
  * none) its share of it.  NaN counts as minus infinity, which is never drawn; a row of nothing else gives
- * -1 and 0.  Weights are exact to 2^-42 and added without rounding; tokens below 2^-46 of the largest are not
- * drawn (n > 2^17: 2^-43).  A temperature of NaN is 0, another control of NaN off, and a uniform number outside
+ * -1 and 0.  Weights are exact to 2^-42 and added without rounding; tokens below 2^-47 of the largest are not
+ * drawn (one power more for each doubling of n from 2^17 on: 2^-46 there, 2^-43 at 2^20).  A temperature of NaN is 0, another control of NaN off, and a uniform number outside
  * [0, 1) the end next to it (NaN: 0).  n <= 2^20.  The result depends on the row and its controls alone.
  * Workspace as for plamo_kernel_attention_paged. */
 int64_t plamo_kernel_sample_workspace(int32_t rows, int32_t n);
