@@ -439,7 +439,8 @@ int plamo_kernel_paged_qkv(const plamo_paged_cache* cache, uint64_t qkv, int32_t
  * h / (heads / kv_heads).  q and out: rows of heads * head_dim of the cache's type (out may be q, row for row).  lse (0: none): FP32
  * [rows][heads], the logarithm of each sum of exponents.  Keys of a table entry outside 0 .. pages - 1 are
  * not seen, lengths past the table end with it, and a row that sees nothing gives zeros and minus
- * infinity.  `workspace` (16-byte aligned, plamo_kernel_attention_paged_workspace bytes, uninitialised) is the
+ * infinity, as does one whose scores are all minus infinity.  What is not seen may hold anything; an infinite value
+ * that is seen makes its dimension infinite or NaN.  `workspace` (16-byte aligned, plamo_kernel_attention_paged_workspace bytes, uninitialised) is the
  * call's own until it has run: calls that may overlap need one each.  Results do not depend on timing;
  * how a row's keys are divided depends on all rows' lengths.  At most 2^20 rows, and 2^24 of rows and parts times
  * the sixteens of query heads on a KV head. */
