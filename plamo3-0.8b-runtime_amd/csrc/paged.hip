@@ -36,8 +36,8 @@ __device__ __forceinline__ uint32_t divide(uint32_t x, Divider d) { return uint3
 constexpr int TABLE_THREADS = 1024;
 
 // Places up to which the tables' workgroup fills in the slots too: each costs a search of the offsets, which
-// one CU does more slowly than all, but a launch costs 2 us (2,048 places: 7.4 us so, 8.3 in a launch of their
-// own; 4,096: 9.1 and 8.6).
+// one CU does more slowly than all, but a launch costs 2 us (2,048 places: 8.4 us so, 9.6 in a launch of their
+// own; 4,096: 10.1 and 9.7).
 constexpr int SLOTS_IN_TABLES = 2048;
 
 // Table entries that requests may give back in a step (their places are 32-bit numbers), and how many are kept in LDS
@@ -445,7 +445,7 @@ __global__ __launch_bounds__(256) void paged_qkv_kernel(PagedQkvParams p) {
 // L2 (34 heads on 2 KV heads 80 us, 1.3 times the time of the same bytes on 32).
 // The weights are kept in two halves of the type (p = hi + lo, 2^-17 off for BF16, 2^-23 for FP16): one
 // rounding of them would be as large an error as the output's own, and the second product is hidden by the loads
-// (30.8 us without, 31.3 with).
+// (64 rows of 2,000 to 8,000 keys 36.2 us without, 36.3 with).
 constexpr int ATTN_WAVES = 4;
 constexpr int ATTN_THREADS = ATTN_WAVES * 64;
 constexpr int PART_KEYS = 32 * ATTN_WAVES;  // fewest keys of a part: a tile for each wave
@@ -454,9 +454,9 @@ constexpr int PART_KEYS = 32 * ATTN_WAVES;  // fewest keys of a part: a tile for
 // 10.7.  Longer where rows and KV heads fill the CUs by themselves (256 rows of 480 keys 24.5 -> 18.5 us), not where
 // they do not (64 rows of 480 keys 12.1 in parts, 15 in one).
 constexpr int ONE_PART_KEYS = 256, ONE_PART_KEYS_FULL = 512;
-// Parts aimed at over all rows and KV heads: as many workgroups as 256 CUs hold at once (registers: six of
-// a head of 64, four of 128, two of 256).  More begin when others end and bring more parts to join, fewer
-// leave loads out: two rows of 131,072 keys 112.8 / 87.3 / 101.1 us with 512 / 1,024 / 1,536, a window
+// Parts aimed at over all rows and KV heads: as many workgroups as 256 CUs hold at once of the kernel for even pages
+// (registers: six of a head of 64, four of 128, two of 256; of the one for uneven pages five, three and two, which
+// get the same parts).  More begin when others end and bring more parts to join, fewer leave loads out: two rows of 131,072 keys 112.8 / 87.3 / 101.1 us with 512 / 1,024 / 1,536, a window
 // of 2,048 keys in 48 rows of heads of 64 45.3 / 39.6 / 38.0 with 1,024 / 1,536 / 2,048.
 constexpr int CUS = 256;
 inline int attn_tiles(int heads, int kv_heads) { return (heads / kv_heads + 15) / 16; }

@@ -12,11 +12,11 @@
 //      bins up to its own) are listed;
 //   4. the list is sorted in LDS and searched.  A bin of more tokens than the list holds is divided again
 //      by the bits of the logits until it is small enough or one value.
-// Each step is a launch over segments of the rows but the last: one CU draws 20 to 40 GB/s from beyond its
-// L2, so that a workgroup that read a row of 107,520 BF16 logits alone would take 5 to 7 us each time.
-// 128 FP32 rows of that length (55 MB) take 10.8, 18.3, 18.0 and 12.6 us: the first is the card's rate of
-// reading (5.1 TB/s), the second the weights' FP64 arithmetic and LDS atomics, the third reads again behind 9 us
-// of finding its bins, the last is latency.  One BF16 row takes 3.9, 4.7, 9.4 and 7.0 us, all of it latency.
+// Each step is a launch over segments of the rows but the last: one CU draws some 45 GB/s from beyond its
+// L2, so that a workgroup that read a row of 107,520 BF16 logits alone would take 5 us each time.
+// 128 FP32 rows of that length (55 MB) take 10.7, 18.2, 18.0 and 13.2 us: the first reads at 5.1 TB/s (a large read
+// reaches 6.3), the second is the weights' FP64 arithmetic and LDS atomics, the third reads again behind 8 us
+// of finding its bins, the last is latency.  One BF16 row takes 3.7, 4.6, 9.4 and 6.8 us, all of it latency.
 // Weights are whole multiples of 2^-S of the largest (S = 63 - log2 of the vocabulary, at most 46), so
 // that all sums are exact whatever their order: the token depends on the row alone, not on how it was
 // split, and sums of unsigned 64-bit atomics are the same in every run.  A token of less than 2^-(S+1)
