@@ -440,10 +440,10 @@ int plamo_kernel_paged_qkv(const plamo_paged_cache* cache, uint64_t qkv, int32_t
  * [rows][heads], the logarithm of each sum of exponents.  Keys of a table entry outside 0 .. pages - 1 are
  * not seen, lengths past the table end with it, and a row that sees nothing gives zeros and minus
  * infinity, as does one whose scores are all minus infinity.  What is not seen may hold anything; an infinite value
- * that is seen makes its dimension infinite or NaN.  `workspace` (16-byte aligned, plamo_kernel_attention_paged_workspace bytes, uninitialised) is the
- * call's own until it has run: calls that may overlap need one each.  Results do not depend on timing;
- * how a row's keys are divided depends on all rows' lengths.  At most 2^20 rows, and 2^24 of rows and parts times
- * the sixteens of query heads on a KV head. */
+ * that is seen makes its dimension infinite or NaN.  `workspace` (16-byte aligned,
+ * plamo_kernel_attention_paged_workspace bytes, uninitialised) is the call's own until it has run: calls that may
+ * overlap need one each.  Results do not depend on timing; how a row's keys are divided depends on all rows'
+ * lengths.  At most 2^20 rows, and less than 2^24 of rows and parts times the sixteens of query heads on a KV head. */
 int64_t plamo_kernel_attention_paged_workspace(int32_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim);
 int plamo_kernel_attention_paged(const plamo_paged_cache* cache, uint64_t q, int64_t q_stride, int32_t heads,
                                  uint64_t tables, int32_t width, uint64_t lengths, int32_t rows, float scale,
