@@ -11,20 +11,12 @@
 #include <algorithm>
 
 #include "common.h"
-#include "device.h"
-#include "paged.h"
+#include "paged_device.h"
 
 namespace plamo {
 using namespace dev;
 
 namespace {
-
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef float floatx4 __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ uint32_t divide(uint32_t x, Divider d) { return uint32_t((uint64_t(x) * d.mul) >> d.shift); }
 
 // ------------------------------------------------------------------------------------ tables
 // One workgroup: prefix sums over the requests of pages given back, pages taken and tokens, then the
@@ -48,11 +40,6 @@ struct Scan3 {
     int back, take, fresh;
 };
 
-// v of the lane that a DPP control names, 0 where there is none (or the row is not in ROWS).
-template <int CONTROL, int ROWS = 0xf>
-__device__ __forceinline__ int shifted(int v) {
-    return __builtin_amdgcn_update_dpp(0, v, CONTROL, ROWS, 0xf, false);
-}
 template <int CONTROL, int ROWS = 0xf>
 __device__ __forceinline__ void add_shifted(Scan3& v) {
     v.back += shifted<CONTROL, ROWS>(v.back);
@@ -333,18 +320,6 @@ __global__ __launch_bounds__(256) void paged_slots_kernel(PagedTablesParams p) {
 }
 
 // ------------------------------------------------------------------------------------ qkv
-template <int TYPE>
-__device__ __forceinline__ float from16(uint32_t h) {
-    if constexpr (TYPE == TYPE_BF16) return bf(h & 0xffffu);
-    return float(__builtin_bit_cast(_Float16, uint16_t(h)));
-}
-// Two values rounded to nearest even and packed.
-template <int TYPE>
-__device__ __forceinline__ uint32_t pack16(float a, float b) {
-    if constexpr (TYPE == TYPE_BF16) return pack_bf16(a, b);
-    const f16x2 h = {_Float16(a), _Float16(b)};
-    return __builtin_bit_cast(uint32_t, h);
-}
 template <int SOURCE>
 __device__ __forceinline__ void load8(const void* base, int64_t at, float (&v)[8]) {
     if constexpr (SOURCE == TYPE_F32) {
@@ -513,17 +488,6 @@ struct WorkShared {
     int parts[ATTN_WAVES];
     Work found;
 };
-
-// Inclusive sum over the wave, as in block_scan3.
-__device__ __forceinline__ int wave_scan(int v) {
-    v += shifted<0x111>(v);
-    v += shifted<0x112>(v);
-    v += shifted<0x114>(v);
-    v += shifted<0x118>(v);
-    v += shifted<0x142, 0xa>(v);
-    v += shifted<0x143, 0xc>(v);
-    return v;
-}
 
 // The row of part `item`; false past the last part.  The waves look through 64 rows each at a time (1,000 rows
 // 71.6 us, 63.4 since they share the work); up to 64 rows every wave does for itself, without waiting for the others.
