@@ -467,6 +467,97 @@ int plamo_kernel_sample(uint64_t logits, int32_t type, int64_t stride, int32_t n
                         uint64_t top_k, uint64_t top_p, uint64_t min_p, uint64_t uniform, uint64_t token, uint64_t prob,
                         uint64_t workspace, int64_t workspace_bytes, uint64_t stream, char* err, size_t errlen);
 
+/* ---- A speculative step over the pool: trees of drafted tokens verified at once ------------
+ * Every request brings several new tokens: its next one and drafts behind it, as a tree, or a chunk of its
+ * prompt, which is a chain.  After plamo_kernel_paged_tables has made room, plamo_kernel_paged_tree gives the nodes'
+ * positions and ancestors, plamo_kernel_paged_qkv writes them, plamo_kernel_attention_paged_tree attends,
+ * plamo_kernel_logit_controls and plamo_kernel_sample draw a token at every node, plamo_kernel_paged_accept keeps the path
+ * that these agree with, and plamo_kernel_paged_move puts its keys and values side by side in every layer.  Request r's
+ * new tokens, its nodes, are offsets[r] .. offsets[r + 1] - 1 of the step, `offsets` ascending numbers of 0 .. tokens
+ * (a request whose offsets are not has no nodes); lengths[r] counts them.  As the paged calls, these launch on `stream` and
+ * its device, allocate nothing, keep nothing and can be captured; what device arrays hold leads nowhere outside. */
+
+/* Positions and ancestors of the nodes: parents[t] is the index in its request of node t's parent, a node before it (any
+ * other number: none, the node follows the cached tokens).  positions[t] = lengths[r] - nodes + the number of ancestors.
+ * ancestors [tokens][words]: bit j (of word j / 32) says that node j of the request is t or an ancestor of it, with
+ * window > 0 only those less than `window` positions before t.  Tokens behind the last request's, and those of a request
+ * that has more than 32 * words nodes or a length below their number, get position -1 and no bits.  words 1...32,
+ * at most 2^20 rows and 2^24 tokens; int32 on the device. */
+int plamo_kernel_paged_tree(uint64_t lengths, uint64_t offsets, int32_t rows, uint64_t parents, int32_t tokens,
+                            int32_t window, uint64_t positions, uint64_t ancestors, int32_t words, uint64_t stream, char* err,
+                            size_t errlen);
+
+/* Attention of all new tokens of `rows` requests: out[t] = softmax(scale * q[t] . k) v over what token t of request r sees
+ * of keys 0 .. lengths[r] - 1 of tables[r][width]: without ancestors (0) those up to its own, its position being
+ * lengths[r] - nodes + its index; with ancestors [tokens][words] the keys before the request's nodes, and the nodes whose
+ * bits are set (words 1...32; nodes without a bit are not seen), its position being positions[t] (read only then; a
+ * negative one sees nothing).  window > 0: keys at most window - 1 positions before the token's (nodes seen by bits are not
+ * left out by it: paged_tree's window does that).  Cache, heads, q, out, lse, what is not seen, what nothing or minus
+ * infinity alone is seen of, entries that are no pages, and the workspace are as for plamo_kernel_attention_paged; rows of q and
+ * out are tokens, those behind offsets[rows] are left as they are, and a request whose length is below its number of nodes
+ * sees nothing.  At most 2^20 rows and tokens, 2^30 of tokens times heads. */
+int64_t plamo_kernel_attention_paged_tree_workspace(int32_t rows, int32_t tokens, int32_t heads, int32_t kv_heads,
+                                                    int32_t head_dim);
+int plamo_kernel_attention_paged_tree(const plamo_paged_cache* cache, uint64_t q, int64_t q_stride, int32_t heads,
+                                      uint64_t tables, int32_t width, uint64_t lengths, uint64_t offsets, int32_t rows,
+                                      int32_t tokens, uint64_t positions, uint64_t ancestors, int32_t words, float scale,
+                                      int32_t window, uint64_t out, int64_t out_stride, uint64_t lse, uint64_t workspace,
+                                      int64_t workspace_bytes, uint64_t stream, char* err, size_t errlen);
+
+/* What plamo_kernel_logit_controls does to a row (device addresses, 0: off).  Row t of the logits belongs to sequence t,
+ * or with `offsets` [sequences + 1] to the sequence r with offsets[r] <= t < offsets[r + 1] (rows of none are left as they
+ * are).  What the sequence has said is history[r][0 .. history_lengths[r]) and, with ancestors [rows][words] as
+ * paged_tree gives them without a window, the tokens of the nodes on t's path, in their order. */
+typedef struct plamo_logit_controls {
+    uint64_t history, history_lengths;                   /* int32 [sequences][history_stride], [sequences] */
+    uint64_t offsets, tokens, ancestors;                 /* int32 [sequences + 1], [rows], [rows][words] */
+    uint64_t repetition, presence, frequency;            /* FP32 [sequences] */
+    uint64_t ngram;                                      /* int32 [sequences] */
+    uint64_t bias_ids, bias;                             /* int32 and FP32 [sequences][bias_width] */
+    uint64_t masks, mask_rows;                           /* [mask_count][mask_stride] words, int32 [rows] */
+    int64_t history_stride, mask_stride;                 /* elements */
+    int32_t sequences, history_width, words, bias_width, mask_count;
+} plamo_logit_controls;
+
+/* Controls on `rows` rows of n logits (`type`, `stride` elements apart, any alignment) into out (`type` or PLAMO_F32;
+ * logits itself, of the same type and stride, or apart from it).  Of tokens that the sequence has said, in FP32 and as
+ * plamo_set_sampling's: the logit is divided by `repetition` if positive, else multiplied (1, 0 or less: off), then less
+ * `presence`, then less `frequency` times how often.  Then bias[r][i] is added to token bias_ids[r][i] (ids outside
+ * 0 .. n - 1 are skipped; of equal ids the last counts).  Minus infinity then replaces tokens that would repeat an n-gram:
+ * those that have followed the sequence's last ngram - 1 tokens before (1 or less: off), and tokens whose bit v % 32 of
+ * word v / 32 is 0 in mask mask_rows[t] (outside 0 .. mask_count - 1: no mask; mask_rows 0: mask t).  A control of NaN is off.
+ * n <= 2^20, rows <= 2^20, history_width (histories longer than it end there) <= 2^17, bias_width <= 4096, words 1...32. */
+int plamo_kernel_logit_controls(const plamo_logit_controls* controls, uint64_t logits, int32_t type, int64_t stride, int32_t n,
+                                int32_t rows, uint64_t out, int32_t out_type, int64_t out_stride, uint64_t stream, char* err,
+                                size_t errlen);
+
+/* The paths that the drawn tokens agree with.  Of request r's nodes the first given[r] (1 ... their number; `given` 0: 1)
+ * are kept whatever was drawn: its next token, or a prompt's.  From the last of these on, the first node is kept whose
+ * parent was kept last (parents as for paged_tree) and whose token is the one drawn there (drawn[t], of plamo_kernel_sample;
+ * -1 agrees with none).  accepted [rows][nodes + 1]: the drafted tokens that are kept, then the token drawn at the last
+ * node kept, -1 behind; accepted_counts [rows]: their number (0 without new tokens); last [rows]: that node, -1 for none.
+ * lengths_out: the lengths without the nodes that are not kept (may be lengths); pages that a table holds past that go on
+ * top of free_pages, in the order of requests and entries (entries that are no pages do not; tables are left as they are),
+ * and free_out counts them (may be free_count).  from, to [rows][nodes]: slots that plamo_kernel_paged_move moves, groups
+ * of `nodes`, -1 where nothing is to be.  All or nothing, as for paged_tables: with `status` (a sum of 2: a request holds
+ * more than `width` pages, 4: more than `nodes` drafts, 8: invalid offsets, lengths or free_count, or more pages than `pages`)
+ * other than 0 no length or free page changes, nothing is accepted and nothing is to be moved.  At most 2^20 rows, 2^24
+ * of capacity, 2^16 nodes; int32 on the device. */
+int plamo_kernel_paged_accept(uint64_t lengths, uint64_t offsets, int32_t rows, uint64_t parents, uint64_t tokens,
+                              uint64_t drawn, int32_t capacity, uint64_t given, uint64_t tables, int32_t width,
+                              int32_t page_size, uint64_t free_pages, uint64_t free_count, int32_t pages,
+                              uint64_t lengths_out, uint64_t free_out, uint64_t accepted, uint64_t accepted_counts,
+                              uint64_t last, int32_t nodes, uint64_t from, uint64_t to, uint64_t status, uint64_t stream,
+                              char* err, size_t errlen);
+
+/* Keys and values of slots from[g][i] to slots to[g][i], in all `layers` caches (a host array; alike but for their
+ * addresses, which must not overlap).  Moves with a slot outside the cache are skipped.  A slot that is written is
+ * written once, and read only by moves of the same group that are not behind that one, as where a request's kept tokens
+ * move up: such a move reads what was there before.  Groups of 1 are copies.  (Other slots' contents are undefined after a
+ * call that breaks this.) */
+int plamo_kernel_paged_move(const plamo_paged_cache* caches, int32_t layers, uint64_t from, uint64_t to, int32_t groups,
+                            int32_t group, uint64_t stream, char* err, size_t errlen);
+
 /* The host RoPE table builder the runtime uploads (`init_rope`, Kernels.metal:212-219; global
  * factors of `rotated`, Kernels.metal:264-267): `rows` x 64 entries of BF16 cos | sin << 16
  * from 64 inverse frequencies (config-mlx.json plamo_rope_inv_freq, Runtime.swift:268-274).

@@ -14,6 +14,7 @@
 #include "formats.h"
 #include "paged.h"
 #include "runtime.h"
+#include "speculate.h"
 #include "tokenizer.h"
 
 struct plamo_runtime {
@@ -1089,6 +1090,251 @@ int plamo_kernel_sample(uint64_t logits, int32_t type, int64_t stride, int32_t n
         p.workspace = reinterpret_cast<void*>(workspace);
         plamo::launch_sample(p, type, s);
         PLAMO_HIP(hipGetLastError());
+    });
+}
+
+int plamo_kernel_paged_tree(uint64_t lengths, uint64_t offsets, int32_t rows, uint64_t parents, int32_t tokens,
+                            int32_t window, uint64_t positions, uint64_t ancestors, int32_t words, uint64_t stream, char* err,
+                            size_t errlen) {
+    return guard(err, errlen, [&] {
+        require(rows >= 1 && rows <= (1 << 20) && tokens >= 0 && tokens <= (1 << 24),
+                "paged tree: rows must be 1...2^20, tokens 0...2^24");
+        require(words >= 1 && words <= plamo::TREE_MAX_WORDS && window >= 0, "paged tree: words must be 1...32, window not negative");
+        require(lengths && offsets && (tokens == 0 || (parents && positions && ancestors)), "paged tree: null argument");
+        const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+        const OnDeviceOf device(s);
+        plamo::TreeParams p{};
+        p.lengths = reinterpret_cast<const int32_t*>(lengths);
+        p.offsets = reinterpret_cast<const int32_t*>(offsets);
+        p.rows = rows;
+        p.parents = reinterpret_cast<const int32_t*>(parents);
+        p.tokens = tokens;
+        p.window = window;
+        p.positions = reinterpret_cast<int32_t*>(positions);
+        p.ancestors = reinterpret_cast<uint32_t*>(ancestors);
+        p.words = words;
+        plamo::launch_paged_tree(p, s);
+        PLAMO_HIP(hipGetLastError());
+    });
+}
+
+int64_t plamo_kernel_attention_paged_tree_workspace(int32_t rows, int32_t tokens, int32_t heads, int32_t kv_heads,
+                                                    int32_t head_dim) {
+    if (rows < 1 || rows > (1 << 20) || tokens < 0 || tokens > (1 << 20) || heads < 1 || heads > 4096 || kv_heads < 1 ||
+        heads % kv_heads != 0 || head_dim < 1 || head_dim > 256)
+        return -1;
+    return plamo::tree_attn_workspace(rows, tokens, heads, kv_heads, head_dim);
+}
+
+int plamo_kernel_attention_paged_tree(const plamo_paged_cache* cache, uint64_t q, int64_t q_stride, int32_t heads,
+                                      uint64_t tables, int32_t width, uint64_t lengths, uint64_t offsets, int32_t rows,
+                                      int32_t tokens, uint64_t positions, uint64_t ancestors, int32_t words, float scale,
+                                      int32_t window, uint64_t out, int64_t out_stride, uint64_t lse, uint64_t workspace,
+                                      int64_t workspace_bytes, uint64_t stream, char* err, size_t errlen) {
+    return guard(err, errlen, [&] {
+        check_cache(cache);
+        require(heads >= 1 && heads <= 4096 && heads % cache->kv_heads == 0,
+                "tree attention: heads must be a multiple of kv_heads, at most 4096");
+        require(rows >= 1 && rows <= (1 << 20) && width >= 1 && int64_t(width) * cache->page_size <= (1 << 30),
+                "tree attention: rows must be 1...2^20, width at least 1, and a row's pages hold at most 2^30 tokens");
+        require(tokens >= 0 && tokens <= (1 << 20) && int64_t(tokens) * heads <= (1 << 30),
+                "tree attention: tokens must be 0...2^20, and tokens times heads at most 2^30");
+        require(window >= 0 && std::isfinite(scale), "tree attention: window must not be negative, scale finite");
+        const int64_t wide = int64_t(heads) * cache->head_dim;
+        require(q_stride >= wide && out_stride >= wide && q_stride % 8 == 0 && out_stride % 8 == 0,
+                "tree attention: row strides must hold a row and be multiples of 16 bytes");
+        require(tables && lengths && offsets && (tokens == 0 || (q && out)) && aligned(q, 16) && aligned(out, 16),
+                "tree attention: q and out must be 16-byte aligned");
+        require(!ancestors || ((positions || tokens == 0) && words >= 1 && words <= plamo::TREE_MAX_WORDS),
+                "tree attention: ancestors need positions, and words of 1...32");
+        require(workspace && aligned(workspace, 16) &&
+                    workspace_bytes >= plamo_kernel_attention_paged_tree_workspace(rows, tokens, heads, cache->kv_heads, cache->head_dim),
+                "tree attention: workspace too small or not 16-byte aligned");
+        plamo::TreeAttnParams p{};
+        p.keys = reinterpret_cast<const char*>(cache->keys);
+        p.values = reinterpret_cast<const char*>(cache->values);
+        p.page_stride = cache->page_stride * 2;
+        p.slot_stride = cache->slot_stride * 2;
+        p.head_stride = cache->head_stride * 2;
+        p.pages = cache->pages;
+        p.page_size = cache->page_size;
+        p.div = plamo::divider(uint32_t(cache->page_size));
+        p.kv_heads = cache->kv_heads;
+        p.group = heads / cache->kv_heads;
+        p.q = reinterpret_cast<const uint16_t*>(q);
+        p.q_stride = q_stride;
+        p.tables = reinterpret_cast<const int32_t*>(tables);
+        p.width = width;
+        p.lengths = reinterpret_cast<const int32_t*>(lengths);
+        p.offsets = reinterpret_cast<const int32_t*>(offsets);
+        p.rows = rows;
+        p.tokens = tokens;
+        p.most = width * cache->page_size;
+        p.positions = reinterpret_cast<const int32_t*>(positions);
+        p.ancestors = reinterpret_cast<const uint32_t*>(ancestors);
+        p.words = words;
+        p.window = window;
+        p.scale = scale * 1.4426950408889634f;
+        p.out = reinterpret_cast<uint16_t*>(out);
+        p.out_stride = out_stride;
+        p.lse = reinterpret_cast<float*>(lse);
+        plamo::tree_attn_bind(p, reinterpret_cast<void*>(workspace), cache->head_dim);
+        const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+        const OnDeviceOf device(s);
+        plamo::launch_tree_attention(p, cache->type, cache->head_dim, s);
+        PLAMO_HIP(hipGetLastError());
+    });
+}
+
+int plamo_kernel_logit_controls(const plamo_logit_controls* c, uint64_t logits, int32_t type, int64_t stride, int32_t n,
+                                int32_t rows, uint64_t out, int32_t out_type, int64_t out_stride, uint64_t stream, char* err,
+                                size_t errlen) {
+    return guard(err, errlen, [&] {
+        require(c != nullptr, "null logit controls");
+        require((type == PLAMO_BF16 || type == PLAMO_F16 || type == PLAMO_F32) && (out_type == type || out_type == PLAMO_F32),
+                "logit controls: unknown logits type, or an output that is neither of it nor FP32");
+        require(n >= 1 && n <= plamo::SAMPLE_MAX_VOCAB && rows >= 0 && rows <= (1 << 20) && plamo::controls_launches(n, rows),
+                "logit controls: n must be 1...2^20, rows 0...2^20, and a launch hold them");
+        require((stride >= n && out_stride >= n) || rows <= 1, "logit controls: rows overlap");
+        require(rows == 0 || (logits && out && aligned(logits, type == PLAMO_F32 ? 4 : 2) && aligned(out, out_type == PLAMO_F32 ? 4 : 2)),
+                "logit controls: null or unaligned argument");
+        require(logits != out || (type == out_type && (stride == out_stride || rows <= 1)),
+                "logit controls: in place, type and stride must stay");
+        require(c->sequences >= 1 && c->sequences <= (1 << 20) && (c->offsets || c->sequences >= rows),
+                "logit controls: sequences must be 1...2^20, and one a row without offsets");
+        require(!c->history || (c->history_lengths && c->history_width >= 0 && c->history_width <= plamo::CONTROL_MAX_HISTORY &&
+                                (c->history_stride >= c->history_width || c->sequences == 1)),
+                "logit controls: histories need lengths, a width of 0...2^17, and strides that hold it");
+        require(!c->ancestors || (c->offsets && c->tokens && c->words >= 1 && c->words <= plamo::TREE_MAX_WORDS),
+                "logit controls: ancestors need offsets, tokens, and words of 1...32");
+        require(!c->bias_ids || (c->bias && c->bias_width >= 0 && c->bias_width <= plamo::CONTROL_MAX_BIAS),
+                "logit controls: bias ids need biases, and a width of 0...4096");
+        require(!c->masks || (c->mask_count >= 1 && c->mask_stride >= (int64_t(n) + 31) / 32 && aligned(c->masks, 4) &&
+                              (c->mask_rows || c->mask_count >= rows)),
+                "logit controls: masks must hold n bits a row, one for each row without mask_rows");
+        if (rows == 0) return;
+        const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+        const OnDeviceOf device(s);
+        plamo::ControlParams p{};
+        p.history = reinterpret_cast<const int32_t*>(c->history);
+        p.history_lengths = reinterpret_cast<const int32_t*>(c->history_lengths);
+        p.history_stride = c->history_stride;
+        p.sequences = c->sequences;
+        p.history_width = c->history_width;
+        p.offsets = reinterpret_cast<const int32_t*>(c->offsets);
+        p.tokens = reinterpret_cast<const int32_t*>(c->tokens);
+        p.ancestors = reinterpret_cast<const uint32_t*>(c->ancestors);
+        p.words = c->words;
+        p.repetition = reinterpret_cast<const float*>(c->repetition);
+        p.presence = reinterpret_cast<const float*>(c->presence);
+        p.frequency = reinterpret_cast<const float*>(c->frequency);
+        p.ngram = reinterpret_cast<const int32_t*>(c->ngram);
+        p.bias_ids = reinterpret_cast<const int32_t*>(c->bias_ids);
+        p.bias = reinterpret_cast<const float*>(c->bias);
+        p.bias_width = c->bias_width;
+        p.masks = reinterpret_cast<const uint32_t*>(c->masks);
+        p.mask_rows = reinterpret_cast<const int32_t*>(c->mask_rows);
+        p.mask_stride = c->mask_stride;
+        p.mask_count = c->mask_count;
+        p.logits = reinterpret_cast<const char*>(logits);
+        p.stride = stride;
+        p.n = n;
+        p.rows = rows;
+        p.out = reinterpret_cast<char*>(out);
+        p.out_stride = out_stride;
+        p.in_place = out == logits;
+        plamo::launch_logit_controls(p, type, out_type, s);
+        PLAMO_HIP(hipGetLastError());
+    });
+}
+
+int plamo_kernel_paged_accept(uint64_t lengths, uint64_t offsets, int32_t rows, uint64_t parents, uint64_t tokens,
+                              uint64_t drawn, int32_t capacity, uint64_t given, uint64_t tables, int32_t width,
+                              int32_t page_size, uint64_t free_pages, uint64_t free_count, int32_t pages,
+                              uint64_t lengths_out, uint64_t free_out, uint64_t accepted, uint64_t accepted_counts,
+                              uint64_t last, int32_t nodes, uint64_t from, uint64_t to, uint64_t status, uint64_t stream,
+                              char* err, size_t errlen) {
+    return guard(err, errlen, [&] {
+        require(rows >= 1 && rows <= (1 << 20) && capacity >= 0 && capacity <= (1 << 24) && width >= 1 && nodes >= 0 && nodes <= (1 << 16),
+                "paged accept: rows must be 1...2^20, capacity 0...2^24, width at least 1, nodes 0...2^16");
+        require(page_size >= 1 && pages >= 1 && int64_t(pages) * page_size <= INT32_MAX,
+                "paged accept: pages and page_size must be at least 1, and hold less than 2^31 tokens");
+        require(lengths && offsets && tables && free_pages && free_count && lengths_out && free_out && accepted && accepted_counts &&
+                    last && status && (capacity == 0 || (parents && tokens && drawn)) && (nodes == 0 || (from && to)),
+                "paged accept: null argument");
+        const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+        const OnDeviceOf device(s);
+        plamo::AcceptParams p{};
+        p.lengths = reinterpret_cast<const int32_t*>(lengths);
+        p.offsets = reinterpret_cast<const int32_t*>(offsets);
+        p.rows = rows;
+        p.parents = reinterpret_cast<const int32_t*>(parents);
+        p.tokens = reinterpret_cast<const int32_t*>(tokens);
+        p.drawn = reinterpret_cast<const int32_t*>(drawn);
+        p.capacity = capacity;
+        p.given = reinterpret_cast<const int32_t*>(given);
+        p.tables = reinterpret_cast<const int32_t*>(tables);
+        p.width = width;
+        p.page_size = page_size;
+        p.free_pages = reinterpret_cast<int32_t*>(free_pages);
+        p.free_count = reinterpret_cast<const int32_t*>(free_count);
+        p.pages = pages;
+        p.lengths_out = reinterpret_cast<int32_t*>(lengths_out);
+        p.free_out = reinterpret_cast<int32_t*>(free_out);
+        p.accepted = reinterpret_cast<int32_t*>(accepted);
+        p.accepted_counts = reinterpret_cast<int32_t*>(accepted_counts);
+        p.last = reinterpret_cast<int32_t*>(last);
+        p.nodes = nodes;
+        p.from = reinterpret_cast<int32_t*>(from);
+        p.to = reinterpret_cast<int32_t*>(to);
+        p.status = reinterpret_cast<int32_t*>(status);
+        p.div = plamo::divider(uint32_t(page_size));
+        plamo::launch_paged_accept(p, s);
+        PLAMO_HIP(hipGetLastError());
+    });
+}
+
+int plamo_kernel_paged_move(const plamo_paged_cache* caches, int32_t layers, uint64_t from, uint64_t to, int32_t groups,
+                            int32_t group, uint64_t stream, char* err, size_t errlen) {
+    return guard(err, errlen, [&] {
+        require(caches && layers >= 1, "paged move: no caches");
+        const plamo_paged_cache& c = caches[0];
+        for (int32_t i = 0; i < layers; ++i) {
+            const plamo_paged_cache& x = caches[i];
+            check_cache(&x);
+            require(x.page_stride == c.page_stride && x.slot_stride == c.slot_stride && x.head_stride == c.head_stride &&
+                        x.pages == c.pages && x.page_size == c.page_size && x.kv_heads == c.kv_heads && x.head_dim == c.head_dim &&
+                        x.type == c.type,
+                    "paged move: caches must be alike but for their addresses");
+        }
+        require(groups >= 0 && group >= 1 && int64_t(groups) * c.kv_heads * (c.head_dim / 8) <= UINT32_MAX - 255,
+                "paged move: groups must not be negative, of at least 1, and a launch hold them");
+        require(groups == 0 || (from && to), "paged move: null argument");
+        if (groups == 0) return;
+        const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+        const OnDeviceOf device(s);
+        plamo::MoveParams p{};
+        p.page_stride = c.page_stride * 2;
+        p.slot_stride = c.slot_stride * 2;
+        p.head_stride = c.head_stride * 2;
+        p.pages = c.pages;
+        p.page_size = c.page_size;
+        p.div = plamo::divider(uint32_t(c.page_size));
+        p.kv_heads = c.kv_heads;
+        p.chunks = c.head_dim / 8;
+        p.from = reinterpret_cast<const int32_t*>(from);
+        p.to = reinterpret_cast<const int32_t*>(to);
+        p.groups = groups;
+        p.group = group;
+        for (int32_t first = 0; first < layers; first += plamo::MOVE_LAYERS) {
+            p.layers = std::min(plamo::MOVE_LAYERS, layers - first);
+            for (int32_t i = 0; i < p.layers; ++i) {
+                p.keys[i] = caches[first + i].keys;
+                p.values[i] = caches[first + i].values;
+            }
+            plamo::launch_paged_move(p, s);
+            PLAMO_HIP(hipGetLastError());
+        }
     });
 }
 

@@ -48,6 +48,15 @@ class PagedCache(ctypes.Structure):
                 ("type", ctypes.c_int32)]
 
 
+class LogitControls(ctypes.Structure):
+    """plamo_logit_controls: what penalties, biases and masks a call has (device addresses, 0: off)."""
+    _fields_ = [(name, ctypes.c_uint64) for name in (
+        "history", "history_lengths", "offsets", "tokens", "ancestors", "repetition", "presence", "frequency", "ngram",
+        "bias_ids", "bias", "masks", "mask_rows")] + [
+            ("history_stride", ctypes.c_int64), ("mask_stride", ctypes.c_int64)] + [(name, ctypes.c_int32) for name in (
+                "sequences", "history_width", "words", "bias_width", "mask_count")]
+
+
 STEP_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, c_i32p, ctypes.c_int32, c_i32p)
 EMIT_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32)
 FINISH_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_int32, c_i32p, ctypes.c_int32, ctypes.c_int32)
@@ -157,6 +166,26 @@ _SIGNATURES = {
     "plamo_kernel_sample": (ctypes.c_int, [ctypes.c_uint64, ctypes.c_int32, ctypes.c_int64] + [ctypes.c_int32] * 2 +
                             [ctypes.c_uint64] * 8 + [ctypes.c_int64, ctypes.c_uint64, ctypes.c_char_p,
                                                      ctypes.c_size_t]),
+    "plamo_kernel_paged_tree": (ctypes.c_int, [ctypes.c_uint64] * 2 + [ctypes.c_int32, ctypes.c_uint64] +
+                                [ctypes.c_int32] * 2 + [ctypes.c_uint64] * 2 + [ctypes.c_int32, ctypes.c_uint64,
+                                                                             ctypes.c_char_p, ctypes.c_size_t]),
+    "plamo_kernel_attention_paged_tree_workspace": (ctypes.c_int64, [ctypes.c_int32] * 5),
+    "plamo_kernel_attention_paged_tree": (ctypes.c_int, [ctypes.POINTER(PagedCache), ctypes.c_uint64, ctypes.c_int64,
+                                                         ctypes.c_int32, ctypes.c_uint64, ctypes.c_int32] +
+                                          [ctypes.c_uint64] * 2 + [ctypes.c_int32] * 2 + [ctypes.c_uint64] * 2 +
+                                          [ctypes.c_int32, ctypes.c_float, ctypes.c_int32, ctypes.c_uint64,
+                                           ctypes.c_int64, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_int64,
+                                           ctypes.c_uint64, ctypes.c_char_p, ctypes.c_size_t]),
+    "plamo_kernel_logit_controls": (ctypes.c_int, [ctypes.POINTER(LogitControls), ctypes.c_uint64, ctypes.c_int32,
+                                                   ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_uint64,
+                                                   ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64, ctypes.c_char_p,
+                                                   ctypes.c_size_t]),
+    "plamo_kernel_paged_accept": (ctypes.c_int, [ctypes.c_uint64] * 2 + [ctypes.c_int32] + [ctypes.c_uint64] * 3 +
+                                  [ctypes.c_int32] + [ctypes.c_uint64] * 2 + [ctypes.c_int32] * 2 +
+                                  [ctypes.c_uint64] * 2 + [ctypes.c_int32] + [ctypes.c_uint64] * 5 + [ctypes.c_int32] +
+                                  [ctypes.c_uint64] * 4 + [ctypes.c_char_p, ctypes.c_size_t]),
+    "plamo_kernel_paged_move": (ctypes.c_int, [ctypes.POINTER(PagedCache), ctypes.c_int32] + [ctypes.c_uint64] * 2 +
+                                [ctypes.c_int32] * 2 + [ctypes.c_uint64, ctypes.c_char_p, ctypes.c_size_t]),
     "plamo_rope_table": (ctypes.c_int, [ctypes.POINTER(ctypes.c_double), ctypes.c_int32, ctypes.c_int32,
                                         ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t]),
     "plamo_version": (ctypes.c_char_p, []),

@@ -1,0 +1,228 @@
+"""Attention of several new tokens a request over its pages, against 64 bits: trees and chains, types, head layouts, page
+sizes, strides, windows, tokens that see nothing, and what lies where nobody looks."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from paged_common import TYPES, describe, half_step, make_cache, make_tables
+from speculate_common import attend_tree, attend_tree64, put, random_parents, tree64
+
+pytestmark = pytest.mark.gpu
+
+
+class Case:
+    """Requests of `before` cached and `counts` new tokens; what no token of theirs is in holds NaN."""
+
+    def __init__(self, kind, heads, kv, dim, page, before, counts, chain=False, window=0, layout="token", seed=0, spare=3, words=None):
+        rng, g = np.random.default_rng(seed), torch.Generator().manual_seed(seed)
+        self.kind, self.heads, self.window = kind, heads, window
+        self.lengths = [b + c for b, c in zip(before, counts)]
+        held = sum(-(-n // page) for n in self.lengths)
+        pages = held + spare
+        width = max(1, max(-(-n // page) for n in self.lengths)) + 1
+        self.tables = make_tables(rng, self.lengths, page, pages, width)
+        self.keys, self.values = make_cache(kind, pages, page, kv, dim, layout)
+        for r, n in enumerate(self.lengths):
+            if n:
+                p = torch.tensor([int(self.tables[r][j // page]) for j in range(n)]), torch.tensor([j % page for j in range(n)])
+                for c in (self.keys, self.values):
+                    c[p[0].cuda(), p[1].cuda()] = torch.randn(n, kv, dim, generator=g).to(TYPES[kind]).cuda()
+        self.offsets = np.concatenate([[0], np.cumsum(counts)]).tolist()
+        self.tokens = self.offsets[-1] + 2  # two of no request's behind
+        self.q = torch.randn(self.tokens, heads * dim, generator=g).to(TYPES[kind]).cuda()
+        self.positions = self.ancestors = None
+        if not chain:
+            parents = sum((random_parents(rng, c) for c in counts), []) + [0, 0]
+            self.words = words or -(-max(max(counts), 1) // 32)
+            self.positions, self.ancestors = tree64(self.lengths, self.offsets, parents, self.tokens, self.words)
+        self.scale = 1 / math.sqrt(dim)
+
+    def run(self, workspace=None):
+        t = TYPES[self.kind]
+        out = torch.full((self.tokens, self.q.shape[1] + 8), 7.0, dtype=t, device="cuda")[:, :self.q.shape[1]]
+        lse = torch.full((self.tokens, self.heads), 7.0, device="cuda")
+        tree = {} if self.ancestors is None else {"positions": put(self.positions), "ancestors": put(self.ancestors)}
+        attend_tree(describe(self.keys, self.values, self.kind), self.q, self.heads, put(self.tables), put(self.lengths),
+                    put(self.offsets), out, lse, scale=self.scale, window=self.window, workspace=workspace, **tree)
+        torch.cuda.synchronize()
+        return out, lse
+
+    def check(self):
+        out, lse = self.run()
+        want, e, slack, e_slack = attend_tree64(self.keys, self.values, self.q, self.tables, self.lengths, self.offsets, self.scale,
+                                                self.positions, self.ancestors, self.window)
+        total = self.offsets[-1]
+        got = out[:total].double().cpu()
+        off = (got - want).abs() - slack - want.abs() * half_step(self.kind) - (2.0 ** -25 if self.kind == "fp16" else 0)
+        assert torch.all(off <= 0), (off.max().item(), torch.nonzero(off > 0)[:5].tolist())
+        got = lse[:total].double().cpu()
+        assert torch.equal(got == -math.inf, e == -math.inf)
+        some = e > -math.inf
+        assert torch.all((got - e)[some].abs() <= e_slack[some]), (got - e)[some].abs().max()
+        assert torch.all(out[total:] == 7) and torch.all(lse[total:] == 7)  # as they were
+        return out, lse
+
+
+LAYOUTS = [(16, 1, 128), (8, 2, 64), (6, 2, 256), (7, 1, 64), (4, 4, 128), (40, 2, 128), (3, 1, 256)]
+
+
+@pytest.mark.parametrize("chain", [False, True])
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("heads,kv,dim", LAYOUTS)
+def test_layouts(heads, kv, dim, kind, chain):
+    Case(kind, heads, kv, dim, 16, [0, 37, 130, 300, 5], [3, 8, 1, 5, 0], chain).check()
+
+
+@pytest.mark.parametrize("page", [1, 3, 8, 16, 20, 48, 64, 256])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_pages(page, dim):
+    Case("bf16", 8, 1, dim, page, [150, 0, 63, 64], [5, 9, 2, 16], False).check()
+    Case("fp16", 4, 2, dim, page, [150, 1, 65], [5, 40, 70], True, window=33).check()
+
+
+@pytest.mark.parametrize("layout", ["head", "joined", "padded"])
+def test_strides(layout):
+    Case("bf16", 8, 2, 128, 24, [100, 7], [6, 11], False, layout=layout).check()
+    Case("fp16", 8, 2, 64, 16, [100, 7], [6, 11], True, layout=layout).check()
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(16, 1, 128), (4, 1, 64), (8, 8, 64), (2, 1, 256)])
+@pytest.mark.parametrize("count", [1, 2, 4, 8, 17, 33, 64])
+def test_numbers_of_nodes(count, heads, kv, dim):
+    """Each number of waves that share a tile, tiles that end anywhere."""
+    Case("bf16", heads, kv, dim, 16, [90, 200], [count, count], False, seed=count).check()
+
+
+@pytest.mark.parametrize("before", [0, 1, 29, 31, 32, 33, 63, 64, 65, 127, 128, 129, 257])
+def test_borders_of_tiles(before):
+    Case("bf16", 16, 1, 128, 16, [before], [13], False, seed=before).check()
+    Case("bf16", 2, 1, 128, 16, [before], [13], True, seed=before).check()
+    Case("fp16", 16, 2, 64, 16, [before] * 3, [4] * 3, False, seed=before).check()
+
+
+@pytest.mark.parametrize("window", [1, 2, 7, 64, 100])
+@pytest.mark.parametrize("chain", [False, True])
+def test_windows(window, chain):
+    Case("bf16", 16, 1, 128, 16, [0, 5, 63, 150, 400], [3, 12, 6, 8, 30], chain, window=window).check()
+
+
+@pytest.mark.parametrize("count", [33, 100, 300])
+def test_long_chains(count):
+    """More than one word of nodes, as a tree that is a chain with some branches and as a chain."""
+    Case("bf16", 4, 1, 64, 16, [70, 0], [count, 3], False, seed=count).check()
+    Case("bf16", 4, 1, 64, 16, [70, 0], [count, 3], True, seed=count).check()
+
+
+def test_nodes_past_the_words_are_not_seen():
+    case = Case("bf16", 4, 1, 64, 16, [40], [50], False, words=2)
+    case.ancestors = case.ancestors[:, :1].copy()
+    case.check()
+
+
+def test_many_parts():
+    """Few tiles over many keys: parts joined."""
+    Case("bf16", 8, 1, 64, 64, [5000], [3], False).check()
+    Case("fp16", 16, 2, 128, 64, [3000, 10, 800], [2, 9, 0], True, window=2500).check()
+    Case("bf16", 2, 1, 256, 32, [2500, 40], [5, 1], False).check()
+
+
+def test_many_requests():
+    """More than the workgroups look through for themselves, and more than a wave does."""
+    rng = np.random.default_rng(4)
+    for rows in (65, 300, 1100):
+        Case("bf16", 2, 1, 64, 16, rng.integers(0, 40, rows).tolist(), rng.integers(0, 4, rows).tolist(), False, seed=rows).check()
+    Case("bf16", 2, 1, 64, 64, [9000 if r == 700 else 3 for r in range(1030)], [2] * 1030, True).check()
+    Case("bf16", 2, 1, 64, 64, [9000 if r == 70 else 3 for r in range(80)], [2] * 80, True).check()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.09, 2.0])
+def test_scales(scale):
+    case = Case("bf16", 16, 1, 128, 16, [100, 3], [7, 20], False)
+    case.scale = scale
+    case.check()
+
+
+def test_tokens_that_see_nothing():
+    case = Case("bf16", 4, 1, 128, 16, [0, 50, 20], [4, 6, 3], False)
+    case.ancestors[1] = 0           # no cached tokens before it, and no bit
+    case.positions[6] = -1          # a token of no position
+    case.tables[2][:] = -1          # pages given back
+    out, lse = case.check()
+    assert torch.all(lse[[1, 6, 10, 11, 12]] == -math.inf) and torch.all(out[[1, 6, 10, 11, 12]] == 0)
+
+
+def test_entries_that_are_no_pages():
+    case = Case("bf16", 4, 1, 128, 16, [100, 90], [4, 6], False)
+    case.tables[0][2], case.tables[1][0], case.tables[1][3] = -1, 1 << 30, case.keys.shape[0]
+    case.check()
+    case = Case("fp16", 4, 1, 64, 12, [100, 90], [4, 6], True)
+    case.tables[0][2], case.tables[1][0], case.tables[1][3] = -1, 1 << 30, case.keys.shape[0]
+    case.check()
+
+
+def test_lengths_that_do_not_hold_the_nodes():
+    """Zeros for their tokens, keys past the table not seen, requests of invalid offsets none."""
+    case = Case("bf16", 4, 1, 128, 16, [100, 90, 30], [4, 6, 2], False)
+    case.lengths[0], case.lengths[1] = 3, -5
+    case.check()
+    case = Case("bf16", 4, 1, 128, 16, [100, 30], [4, 6], True)
+    case.tables = case.tables[:, :4].copy()
+    case.check()
+
+
+@pytest.mark.parametrize("odd", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("kind,dim", [("bf16", 128), ("fp16", 64), ("bf16", 256)])
+@pytest.mark.parametrize("chain", [False, True])
+def test_values_that_one_branch_sees(odd, kind, dim, chain):
+    """A value that is not finite reaches the tokens that see its key, and no others of its tile."""
+    case = Case(kind, 4, 1, dim, 16, [50, 20], [9, 7], chain, window=40)
+    page = case.keys.shape[1]
+    for r, node in ((0, 3), (1, 6)):
+        key = case.lengths[r] - (case.offsets[r + 1] - case.offsets[r]) + node
+        case.values[int(case.tables[r][key // page]), key % page, :, 5] = odd
+    key = 11  # outside the windows of the later tokens
+    case.values[int(case.tables[0][0]), key, :, 40] = odd
+    out, lse = case.run()
+    want, e, slack, _ = attend_tree64(case.keys, case.values, case.q, case.tables, case.lengths, case.offsets, case.scale,
+                                      case.positions, case.ancestors, case.window)
+    got = out[:case.offsets[-1]].double().cpu()
+    fine = torch.isfinite(want)
+    assert torch.equal(fine, torch.isfinite(got)) and not fine.all() and torch.equal(torch.isnan(want), torch.isnan(got))
+    assert torch.equal(got[~fine & ~torch.isnan(got)], want[~fine & ~torch.isnan(got)])
+    off = (got - want).abs() - torch.nan_to_num(slack) - want.abs() * half_step(kind) - 2.0 ** -25
+    assert torch.all(off[fine] <= 0) and torch.isfinite(lse[:case.offsets[-1]]).all()
+
+
+@pytest.mark.parametrize("odd", [math.nan, math.inf, -math.inf])
+def test_keys_that_one_branch_sees(odd):
+    """Scores of a key that is not finite reach the tokens that see it alone."""
+    case = Case("bf16", 2, 1, 128, 16, [70], [12], False)
+    key = 70 + 4
+    sees = (case.ancestors[:, 0] >> 4 & 1).astype(bool)[:12]
+    clean, _ = case.run()
+    case.keys[int(case.tables[0][key // 16]), key % 16, :, 3] = odd
+    out, _ = case.run()
+    assert sees.any() and not sees.all()
+    assert torch.equal(out[:12][~sees], clean[:12][~sees])
+
+
+def test_results_do_not_depend_on_the_workspace_or_the_call():
+    case = Case("bf16", 16, 1, 128, 16, [1000, 40, 333], [8, 3, 24], False)
+    first, e = case.run()
+    size = 1 << 27
+    for fill in (0, 0x7F):
+        again, e2 = case.run(torch.full((size,), fill, dtype=torch.uint8, device="cuda"))
+        assert torch.equal(first, again) and torch.equal(e, e2)
+
+
+def test_in_place():
+    """out may be q, row for row."""
+    case = Case("bf16", 16, 1, 128, 16, [300, 40], [8, 3], False)
+    want, _ = case.run()
+    q = case.q.clone()
+    attend_tree(describe(case.keys, case.values, "bf16"), q, 16, put(case.tables), put(case.lengths), put(case.offsets), q,
+                positions=put(case.positions), ancestors=put(case.ancestors))
+    torch.cuda.synchronize()
+    assert torch.equal(q[:11], want[:11]) and torch.equal(q[11:], case.q[11:])
