@@ -32,27 +32,28 @@ constexpr int CUS = 256;
 
 template <int D, int SHARE>
 struct Shape {
-    static constexpr int GROUPS = SHARE == 4 ? 1 : SHARE == 2 ? (D == 256 ? 1 : 2) : (D == 256 ? 2 : 4);
+    static constexpr int KEYS = SHARE == 4 || (SHARE == 2 && D == 64) ? 64 : 32;  // of a tile
+    static constexpr int GROUPS = SHARE == 4 ? 1 : SHARE == 2 || D == 256 ? 2 : 4;
     static constexpr int WAVES = SHARE * GROUPS, THREADS = 64 * WAVES;
-    static constexpr int KEYS = SHARE == 4 || (SHARE == 2 && D == 256) ? 64 : 32;  // of a tile
-    static constexpr int BLOCKS = KEYS / 32;          // of 32 keys
+    static constexpr int HELD = D == 256 || (D == 128 && SHARE == 1) ? 1 : 2;  // workgroups of a CU
+    static constexpr int OF_SIMD = HELD * WAVES > 4 ? HELD * WAVES / 4 : 1;
     static constexpr int ROW = 2 * D;                 // bytes of a key
+    static constexpr int TILE = KEYS * ROW;           // of a tile's keys, or of its values
+    static constexpr int LDS = GROUPS * 2 * 2 * TILE; // two stages
     static constexpr int PIECE_KEYS = 512 / D;        // keys of a load: 16 bytes a lane
     static constexpr int PIECES = 16 / PIECE_KEYS;    // loads of 16 keys
-    static constexpr int OWN = KEYS / 16 / SHARE;     // sixteens of keys that a wave loads
-    static constexpr int STAGE = KEYS * ROW * 2;      // keys, then values
-    static constexpr int LDS = GROUPS * 2 * STAGE;
-    static constexpr int HELD = D == 256 ? 1 : SHARE == 1 && D == 128 ? 1 : 2;  // workgroups of a CU
-    static constexpr int OF_SIMD = HELD * WAVES > 4 ? HELD * WAVES / 4 : 1;
+    static constexpr int OWN = KEYS / SHARE / 16;     // sixteens that a wave loads
+    static constexpr int BLOCKS = KEYS / 32;          // of a product
     static constexpr int STEPS = D / 16, DIMS = D / 32;
     static constexpr int SPLIT = D / 8;               // four dims each of the 64 lanes' rows
 };
-static_assert(Shape<128, 4>::LDS == 65536 && Shape<128, 1>::LDS == 131072 && Shape<256, 4>::LDS == 131072 && Shape<256, 1>::LDS == 131072, "");
+static_assert(Shape<128, 4>::LDS == 65536 && Shape<128, 2>::LDS == 65536 && Shape<128, 1>::LDS == 131072 && Shape<256, 1>::LDS == 131072 &&
+              Shape<256, 2>::LDS == 131072 && Shape<256, 4>::LDS == 131072 && Shape<64, 1>::LDS == 65536 && Shape<64, 2>::LDS == 65536, "of 160 KB");
 
 // Key of row R of sixteen in LDS: a lane's loads are of neighbouring keys.
 template <int D>
 constexpr int key_of_row(int row) { return 16 / (512 / D) * (row % (512 / D)) + row / (512 / D); }
-// The same for the rows of a lane's scores, 8 (i / 4) + 4 (l / 32) + i % 4: a constant, and what the lane's half adds.
+// The same for the rows of a lane's scores, 8 (i / 4) + 4 (lane / 32) + i % 4: a constant, and what the lane's half adds.
 template <int D>
 constexpr int score_key(int i) { return 16 * (i / 8) + key_of_row<D>(8 * (i / 4 % 2) + i % 4); }
 template <int D>
@@ -102,12 +103,14 @@ __device__ __forceinline__ Request request(const TreeAttnParams& p, int r) {
 }
 __device__ __forceinline__ int parts_of(int span, int chunk) { return span > 0 ? (span - 1) / chunk + 1 : 1; }
 
-// Keys of a part: all tiles' keys divided by the parts aimed at.
-__device__ __forceinline__ int part_keys(const TreeAttnParams& p, long long work, long long tiles) {
-    const long long half = (p.target + 1) / 2;
-    const long long parts = p.target - tiles / 2 > half ? p.target - tiles / 2 : half;  // a tile's last part is half empty
-    const long long share = (work + parts - 1) / parts, most = (long long)p.most + 8, each = share < most ? share : most;
-    return __builtin_amdgcn_readfirstlane(each <= p.least ? p.least : int((each + p.least - 1) / p.least * p.least));
+// Keys of a part: all tiles' keys, next to which FP32 is, divided by the parts aimed at, `times` eighths of that.  (A
+// little more: tiles of several parts have less than twice as many parts then as are aimed at.)
+__device__ __forceinline__ int part_keys(const TreeAttnParams& p, float work, int tiles, int times) {
+    const int parts = max(p.target - tiles / 2, (p.target + 1) / 2);  // a tile's last part is half empty
+    const float share = work * 1.0001220703125f / float(parts) * (0.125f * float(times));
+    if (share <= float(p.least)) return p.least;
+    const int each = share < float(p.most) ? int(share) + 1 : p.most;
+    return (each + p.least - 1) / p.least * p.least;
 }
 
 struct Sums {
@@ -122,6 +125,7 @@ __device__ __forceinline__ Sums at_lane(Sums v, int l) {
     return {__builtin_amdgcn_readlane(v.items, l), __builtin_amdgcn_readlane(v.slots, l), __builtin_amdgcn_readlane(v.joined, l)};
 }
 __device__ __forceinline__ Sums operator+(Sums a, Sums b) { return {a.items + b.items, a.slots + b.slots, a.joined + b.joined}; }
+__device__ __forceinline__ Sums operator-(Sums a, Sums b) { return {a.items - b.items, a.slots - b.slots, a.joined - b.joined}; }
 
 // Of an item: its request, the sums of those before, and how many parts its tiles have.
 struct Work {
@@ -129,50 +133,70 @@ struct Work {
     Sums before;
     int parts;
 };
-
-// All sums over the workgroup's waves, in every wave.
-template <int WAVES>
-__device__ __forceinline__ void total_work(const TreeAttnParams& p, long long* s_sums, long long& work, long long& tiles) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int o = 32; o > 0; o >>= 1) {
-        work += __shfl_xor(work, o, 64);
-        tiles += __shfl_xor(tiles, o, 64);
-    }
-    if (WAVES == 1) return;
-    if (lane == 0) {
-        s_sums[2 * wave] = work;
-        s_sums[2 * wave + 1] = tiles;
-    }
-    __syncthreads();
-    work = tiles = 0;
-    for (int w = 0; w < WAVES; ++w) {
-        work += s_sums[2 * w];
-        tiles += s_sums[2 * w + 1];
-    }
-}
-
 struct WorkShared {
-    long long sums[32];
+    float work[16];
+    int number[16];
     Sums waves[16];
     Work found;
 };
 
+// Sums over the workgroup's waves, in every wave and in one order.
+template <int WAVES>
+__device__ __forceinline__ void total(WorkShared& s, float& work, int& number) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    work = wave_sum(work);
+    number = __builtin_amdgcn_readlane(wave_scan(number), 63);
+    if (WAVES == 1) return;
+    __syncthreads();  // the sums before these have been read
+    if (lane == 0) {
+        s.work[wave] = work;
+        s.number[wave] = number;
+    }
+    __syncthreads();
+    work = 0.f;
+    number = 0;
+    for (int w = 0; w < WAVES; ++w) {
+        work += s.work[w];
+        number += s.number[w];
+    }
+}
+
+// A part's keys, from the requests that a thread takes: from row `first` on, every `step`-th.  More of them where
+// all parts at once would be a few too many for the CUs, and a second round had to be waited for (64 requests of 33 to 8,192 keys,
+// trees of 8 to 24 nodes 55 -> 50 us); as many as at first where that does not help.
+template <int ROWS, int WAVES>
+__device__ __forceinline__ int choose_part(const TreeAttnParams& p, WorkShared& s, int first, int step) {
+    float work = 0.f, none = 0.f;
+    int tiles = 0;
+    for (int r = first; r < p.rows; r += step) {
+        const Request q = request<ROWS>(p, r);
+        work += float(q.tiles) * float(q.span);
+        tiles += q.tiles;
+    }
+    total<WAVES>(s, work, tiles);
+    const int least = __builtin_amdgcn_readfirstlane(part_keys(p, work, tiles, 8));
+    if (least == p.least) return least;
+    for (int times = 8; times <= 16; ++times) {
+        const int chunk = __builtin_amdgcn_readfirstlane(part_keys(p, work, tiles, times));
+        int items = 0;
+        for (int r = first; r < p.rows; r += step) {
+            const Request q = request<ROWS>(p, r);
+            items += q.tiles * parts_of(q.span, chunk);
+        }
+        total<WAVES>(s, none, items);
+        if (items <= p.target) return chunk;
+    }
+    return least;
+}
+
 // The request of an item, from all requests' lengths and offsets: the same division in all workgroups.  Up to 64
-// requests every wave does for itself.  False past the last item; `joined`: tiles of several parts before that.
+// requests every wave does for itself.  False past the last item; `joined`, for the first: tiles of several parts.
 template <int ROWS, int WAVES>
 __device__ __forceinline__ bool find_work(const TreeAttnParams& p, WorkShared& s, int item, Work& work, int& joined) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool few = p.rows <= 64;
     const int step = few ? 64 : 64 * WAVES, own_row = few ? lane : int(threadIdx.x);
-    long long keys = 0, tiles = 0;
-    for (int r = own_row; r < p.rows; r += step) {
-        const Request q = request<ROWS>(p, r);
-        keys += (long long)q.tiles * q.span;
-        tiles += q.tiles;
-    }
-    if (few) total_work<1>(p, s.sums, keys, tiles);
-    else total_work<WAVES>(p, s.sums, keys, tiles);
-    const int chunk = part_keys(p, keys, tiles);
+    const int chunk = few ? choose_part<ROWS, 1>(p, s, own_row, step) : choose_part<ROWS, WAVES>(p, s, own_row, step);
     Sums run = {0, 0, 0};
     bool found = false;
     for (int base = 0; base < p.rows; base += step) {
@@ -200,11 +224,9 @@ __device__ __forceinline__ bool find_work(const TreeAttnParams& p, WorkShared& s
         const unsigned long long past = __ballot(before.items + incl.items > item && before.items + incl.items - own.items <= item);
         if (past) {
             const int l = __ffsll(past) - 1;
-            const Sums own_l = at_lane(own, l), incl_l = at_lane(incl, l);
             work.row = __builtin_amdgcn_readlane(r, l);
             work.parts = __builtin_amdgcn_readlane(parts, l);
-            work.before = {before.items + incl_l.items - own_l.items, before.slots + incl_l.slots - own_l.slots,
-                           before.joined + incl_l.joined - own_l.joined};
+            work.before = before + at_lane(incl - own, l);
             if (!few && lane == 0) s.found = work;
         }
         if (!found && item < run.items) {
@@ -244,14 +266,7 @@ __global__ __launch_bounds__(DIVIDE_THREADS) void tree_division_kernel(TreeAttnP
     constexpr int WAVES = DIVIDE_THREADS / 64;
     __shared__ WorkShared s;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    long long keys = 0, tiles = 0;
-    for (int r = threadIdx.x; r < p.rows; r += DIVIDE_THREADS) {
-        const Request q = request<ROWS>(p, r);
-        keys += (long long)q.tiles * q.span;
-        tiles += q.tiles;
-    }
-    total_work<WAVES>(p, s.sums, keys, tiles);
-    const int chunk = part_keys(p, keys, tiles);
+    const int chunk = choose_part<ROWS, WAVES>(p, s, threadIdx.x, DIVIDE_THREADS);
     // a thread's rows are neighbours: sums in order
     const int each = (p.rows + DIVIDE_THREADS - 1) / DIVIDE_THREADS;
     const int begin = min(int(threadIdx.x) * each, p.rows), end = min(begin + each, p.rows);
@@ -260,7 +275,7 @@ __global__ __launch_bounds__(DIVIDE_THREADS) void tree_division_kernel(TreeAttnP
     const Sums incl = scan(own);
     if (lane == 63) s.waves[wave] = incl;
     __syncthreads();
-    Sums run = {incl.items - own.items, incl.slots - own.slots, incl.joined - own.joined};
+    Sums run = incl - own;
     for (int w = 0; w < wave; ++w) run = run + s.waves[w];
     for (int r = begin; r < end; ++r) {
         const Request q = request<ROWS>(p, r);
@@ -298,6 +313,30 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
     return (finite16<TYPE>(w) ? w & 0xffffu : 0u) | (finite16<TYPE>(w >> 16) ? w & 0xffff0000u : 0u);
 }
 
+// Two weights rounded to the type, and what that leaves of them.
+template <int TYPE>
+__device__ __forceinline__ void split(float x, float y, uint32_t& high, uint32_t& low) {
+    high = pack16<TYPE>(x, y);
+    if constexpr (TYPE == TYPE_BF16) {
+        // the differences are exact: the pair times (-1, 0) or (0, -1) onto the value (in registers: as literals one of
+        // them would be encoded as the inline constant -1, which is no pair)
+        uint32_t first = 0x0000bf80u, second = 0xbf800000u;
+        __asm__("" : "+s"(first), "+s"(second));
+        low = pack16<TYPE>(dot2bf(high, first, x), dot2bf(high, second, y));
+    } else {
+        low = pack16<TYPE>(x - from16<TYPE>(high), y - from16<TYPE>(high >> 16));
+    }
+}
+
+// f(std::integral_constant<int, I>) for I = B .. E - 1.
+template <int B, int E, class F>
+__device__ __forceinline__ void static_for(F&& f) {
+    if constexpr (B < E) {
+        f(std::integral_constant<int, B>{});
+        static_for<B + 1, E>(f);
+    }
+}
+
 // Bits from .. to - 1 of 64 (any numbers).
 __device__ __forceinline__ uint64_t bit_range(int from, int to) {
     const uint64_t below_to = to >= 64 ? ~0ull : to <= 0 ? 0ull : (1ull << to) - 1;
@@ -311,7 +350,7 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
     constexpr int ROWS = 32 * SHARE;
     __shared__ __align__(1024) uint8_t s_ring[X::LDS];
     __shared__ float2 s_ml[X::GROUPS][ROWS];
-    __shared__ uint32_t s_there[X::GROUPS][2][X::KEYS / 16];
+    __shared__ __align__(8) uint16_t s_there[X::GROUPS][2][4];  // of a stage's tile: bits of sixteen rows each
     __shared__ WorkShared s_work;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int part_wave = wave % SHARE, set = wave / SHARE;
@@ -355,12 +394,12 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
 #pragma unroll
         for (int s = 0; s < X::STEPS; ++s) q[s] = *reinterpret_cast<const uint4*>(from + 16 * s);
     }
-    float scale = p.scale;
-    if (scale < 0.f) {  // products of the other sign, so that the largest stays the largest
-        scale = -scale;
+    // the scale is made positive, so that the largest product is the largest score: of the other sign, or of nothing
+    const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u, kept = p.scale == 0.f ? 0u : ~0u;
+    const float scale = p.scale == 0.f ? 1.0f : fabsf(p.scale);
 #pragma unroll
-        for (int s = 0; s < X::STEPS; ++s) q[s].x ^= 0x80008000u, q[s].y ^= 0x80008000u, q[s].z ^= 0x80008000u, q[s].w ^= 0x80008000u;
-    }
+    for (int s = 0; s < X::STEPS; ++s)
+        q[s] = make_uint4((q[s].x ^ flip) & kept, (q[s].y ^ flip) & kept, (q[s].z ^ flip) & kept, (q[s].w ^ flip) & kept);
     // keys low .. high - 1 before the new tokens (and in a chain up to its own), and by bits
     const uint32_t* bits = nullptr;
     int position = rq.start + token, high = min(position + 1, rq.end);
@@ -399,101 +438,174 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
     end = __builtin_amdgcn_readfirstlane(min(end, begin + each));
 
     // ---- loads: lane's row of a piece and its 16-byte chunk there
-    const uint32_t ring = lds_address(s_ring) + uint32_t(set) * 2 * X::STAGE;
     constexpr int LANES = 64 / X::PIECE_KEYS;  // of a row
-    const int group = lane / LANES, chunk = lane % LANES;
+    const int group = lane / LANES;
+    const uint32_t ring = lds_address(s_ring) + uint32_t(set) * (2 * 2 * X::TILE);  // a stage: keys, then values
     const uint64_t keys0 = reinterpret_cast<uint64_t>(p.keys) + kv * p.head_stride;
     const int64_t apart = p.values - p.keys;
     const int32_t* table = p.tables + int64_t(row) * p.width;
-    const uint64_t zeros = reinterpret_cast<uint64_t>(&ZEROS);
     constexpr int LOOK = EVEN ? 1 : X::PIECES;
-    // pages of the lane's keys of a tile
+    const int first_row = 16 * X::OWN * part_wave;  // of a tile, that the wave loads
+    // pages of the lane's keys of a tile, on their way
     int entry[X::OWN][LOOK];
     auto look_up = [&](int pos) {
 #pragma unroll
         for (int b = 0; b < X::OWN; ++b)
 #pragma unroll
             for (int l = 0; l < LOOK; ++l) {
-                const int key = pos + 16 * (part_wave * X::OWN + b) + X::PIECES * group + l;
+                const int key = pos + first_row + 16 * b + X::PIECES * group + l;
                 entry[b][l] = key < end ? table[divide(uint32_t(key), p.div)] : -1;
             }
     };
-    uint32_t own_there[X::OWN];  // bit R: row R of the sixteen is a key's
     auto request_tile = [&](int pos, int stage) {
 #pragma unroll
         for (int b = 0; b < X::OWN; ++b) {
-            const int row16 = 16 * (part_wave * X::OWN + b);
-            const uint32_t to = ring + uint32_t(stage) * X::STAGE + uint32_t(row16) * X::ROW;
-            uint32_t there = 0;
+            const int key0 = pos + first_row + 16 * b;  // of the sixteen
+            uint64_t at[LOOK];
+            bool fine = key0 + 16 <= end;
 #pragma unroll
-            for (int l = 0; l < X::PIECES; ++l) {
-                const int key = pos + row16 + X::PIECES * group + l;
-                const int page = entry[b][EVEN ? 0 : l];
-                const bool ok = key < end && uint32_t(page) < uint32_t(p.pages);
-                const int in_page = key - int(divide(uint32_t(key), p.div)) * p.page_size;
-                const uint64_t at = keys0 + uint64_t(int64_t(page) * p.page_stride + int64_t(in_page) * p.slot_stride);
-                const int r = X::PIECE_KEYS * l + group;
-                const uint64_t k_at = ok ? at + uint32_t((chunk ^ key_swizzle<D>(r)) * 16) : zeros;
-                const uint64_t v_at = ok ? at + uint64_t(apart) + uint32_t((((chunk >> 2) ^ value_swizzle<D>(r)) * 4 + (chunk & 3)) * 16) : zeros;
-                load_to_lds(to + uint32_t(l) * 1024, k_at);
-                load_to_lds(to + X::KEYS * X::ROW + uint32_t(l) * 1024, v_at);
-                const unsigned long long all = __ballot(ok);
-#pragma unroll
-                for (int g = 0; g < X::PIECE_KEYS; ++g) there |= uint32_t(all >> (g * LANES) & 1u) << (X::PIECE_KEYS * l + g);
+            for (int l = 0; l < LOOK; ++l) {
+                const int key = key0 + X::PIECES * group + l, in_page = key - int(divide(uint32_t(key), p.div)) * p.page_size;
+                at[l] = keys0 + uint64_t(int64_t(entry[b][l]) * p.page_stride + int64_t(in_page) * p.slot_stride);
+                fine = fine && uint32_t(entry[b][l]) < uint32_t(p.pages);
             }
-            own_there[b] = there;
-            if (SHARE > 1 && lane == 0) s_there[set][stage][part_wave * X::OWN + b] = there;
+            const uint32_t to = ring + uint32_t(stage) * (2 * X::TILE) + uint32_t(first_row + 16 * b) * X::ROW;
+            int own = lane;
+            __asm__ volatile("" : "+v"(own));  // (or the compiler would keep all offsets in registers)
+            const int chunk = own % LANES, own_group = own / LANES;
+            uint32_t there = 0xffffu;
+            if (__all(fine)) {
+#pragma unroll
+                for (int l = 0; l < X::PIECES; ++l) {
+                    const int r = X::PIECE_KEYS * l + own_group;
+                    const uint64_t from = at[EVEN ? 0 : l] + (EVEN ? uint64_t(l * p.slot_stride) : 0);
+                    load_to_lds(to + uint32_t(l) * 1024, from + uint32_t((chunk ^ key_swizzle<D>(r)) * 16));
+                    load_to_lds(to + X::TILE + uint32_t(l) * 1024,
+                                from + uint64_t(apart) + uint32_t((((chunk >> 2) ^ value_swizzle<D>(r)) * 4 + (chunk & 3)) * 16));
+                }
+            } else {  // rows past the last key, or of no page, are zeros
+                there = 0;
+#pragma unroll
+                for (int l = 0; l < X::PIECES; ++l) {
+                    const int r = X::PIECE_KEYS * l + own_group;
+                    const bool ok = key0 + X::PIECES * own_group + l < end && uint32_t(entry[b][EVEN ? 0 : l]) < uint32_t(p.pages);
+                    const uint64_t from = at[EVEN ? 0 : l] + (EVEN ? uint64_t(l * p.slot_stride) : 0);
+                    const uint64_t zeros = reinterpret_cast<uint64_t>(&ZEROS);
+                    load_to_lds(to + uint32_t(l) * 1024, ok ? from + uint32_t((chunk ^ key_swizzle<D>(r)) * 16) : zeros);
+                    load_to_lds(to + X::TILE + uint32_t(l) * 1024,
+                                ok ? from + uint64_t(apart) + uint32_t((((chunk >> 2) ^ value_swizzle<D>(r)) * 4 + (chunk & 3)) * 16) : zeros);
+                    const unsigned long long those = __ballot(ok);
+#pragma unroll
+                    for (int g = 0; g < X::PIECE_KEYS; ++g) there |= uint32_t(those >> (g * LANES) & 1u) << (X::PIECE_KEYS * l + g);
+                }
+            }
+            if (lane == 0) s_there[set][stage][part_wave * X::OWN + b] = uint16_t(there);
+        }
+    };
+    // the bits of the nodes in a tile, as far as they are needed: words from the first node's on
+    struct Bits {
+        uint32_t w[3];
+    };
+    Bits node_bits = {};
+    auto look_at_bits = [&](int pos) {
+        const int from = max(pos - rq.start, 0) >> 5;
+        if (p.ancestors && pos + X::KEYS > rq.start) {
+#pragma unroll
+            for (int i = 0; i <= X::BLOCKS; ++i) node_bits.w[i] = bits && from + i < p.words ? bits[from + i] : 0u;
         }
     };
 
-    // ---- a tile
+    // ---- a tile's products
     float most = NEG_INF, sum = 0.f;
     floatx16 o[X::DIMS];
 #pragma unroll
     for (int d = 0; d < X::DIMS; ++d) o[d] = floatx16{};
+    // Operands by a lane's base in a stage, exclusive-or'ed with the step: the bases are made new for each turn, or the compiler
+    // would keep all their variants in registers.
+    const uint32_t key_base = uint32_t(set * (2 * 2 * X::TILE) + col * X::ROW + (half ^ key_swizzle<D>(col)) * 16);
+    // source lane l of 16 reads 8 bytes of row 4 (lane / 32) + l / 4; lane j gets dim 16 (lane / 16 % 2) + j of the four
+    // rows, and of those 8 further (which have the same swizzle)
+    const int source_row = 4 * half + (lane >> 2 & 3);
+    const uint32_t value_base = uint32_t(set * (2 * 2 * X::TILE) + X::TILE + source_row * X::ROW + value_swizzle<D>(source_row) * 64 +
+                                         32 * (lane >> 4 & 1) + 8 * (lane & 3));
+    auto base_of = [&](uint32_t base, int stage) {
+        uint32_t x = base + uint32_t(stage) * (2 * X::TILE);
+        __asm__ volatile("" : "+v"(x));
+        return x;
+    };
     typedef short short4_t __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) short4_t* tr_ptr_t;
-    const int sl = lane & 15, grp = lane >> 4;
-    auto take = [&](int pos, int stage, uint64_t there, auto all_seen) {
-        constexpr bool whole = decltype(all_seen)::value;
-        const uint8_t* keys = s_ring + (set * 2 + stage) * X::STAGE;
-        const uint8_t* values = keys + X::KEYS * X::ROW;
+    // dims of d, keys of sixteen s
+    auto value_operand = [&](uint32_t base, int s, int d) {
+        const uint8_t* at = s_ring + (base ^ uint32_t(d * 64)) + 16 * s * X::ROW;
+        const short4_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)at);
+        const short4_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(at + 8 * X::ROW));
+        uint4 v;
+        __builtin_memcpy(&v, &x0, 8);
+        __builtin_memcpy(reinterpret_cast<char*>(&v) + 8, &x1, 8);
+        return v;
+    };
+    auto weight = [&](float x, float from) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, scale, -from)); };
+    constexpr int SIXTEENS = X::KEYS / 16;
+    // Weights in two halves of the type (2^-16 off for BF16, 2^-22 for FP16) where the products wait for memory.  With four
+    // waves a tile these and the vector arithmetic are what takes the time, and a third product and the split of the weights
+    // cost 535 us for 420 (two chunks of 999 tokens behind 28,000 and 30,720): they are rounded once there, each half a
+    // step off at most, which leaves the output 1.2 to 1.4 times as far from 64 bits as its own rounding does.
+    constexpr bool HALVES = SHARE < 4;
+
+    auto take = [&](int pos, int stage, uint64_t there, const Bits& of_nodes) {
+        constexpr int PRODUCTS = X::BLOCKS * X::STEPS, AHEAD = 4;
+        const uint32_t k_base = base_of(key_base, stage), v_base = base_of(value_base, stage);
         floatx16 s[X::BLOCKS];
+        {
+            auto operand = [&](int i) {
+                return *reinterpret_cast<const uint4*>(s_ring + (k_base ^ uint32_t(i / X::BLOCKS * 32)) + i % X::BLOCKS * 32 * X::ROW);
+            };
+            uint4 k[AHEAD];
 #pragma unroll
-        for (int b = 0; b < X::BLOCKS; ++b) {
-            s[b] = floatx16{};
-#pragma unroll
-            for (int t = 0; t < X::STEPS; ++t) {
-                const uint4 k = *reinterpret_cast<const uint4*>(keys + (32 * b + col) * X::ROW + ((2 * t + half) ^ key_swizzle<D>(col)) * 16);
-                s[b] = mfma32<TYPE>(k, q[t], s[b]);
-            }
+            for (int i = 0; i < AHEAD; ++i) k[i] = operand(i);
+            static_for<0, PRODUCTS>([&](auto n) {
+                constexpr int i = decltype(n)::value, b = i % X::BLOCKS, t = i / X::BLOCKS;
+                s[b] = mfma32<TYPE>(k[i % AHEAD], q[t], t == 0 ? floatx16{} : s[b]);
+                if constexpr (i + AHEAD < PRODUCTS) k[i % AHEAD] = operand(i + AHEAD);
+                __builtin_amdgcn_sched_barrier(0);
+            });
         }
         uint32_t seen[X::BLOCKS];
-        if constexpr (!whole) {
+        bool clean = true;
+        constexpr uint64_t ALL = X::KEYS == 64 ? ~0ull : 0xffffffffull;
+        const bool whole = pos >= all_low && pos + X::KEYS <= all_high && there == ALL;
+        if (!whole) {
             // what the lane's token sees of the keys in their order, then of its scores in theirs
             uint64_t see = bit_range(low - pos, high - pos);
-            if (bits) {
-                const int node = pos - rq.start;  // of the tile's first key
-                const int from = max(node, 0), w = from >> 5, shift = from & 31;
-                if (node > -X::KEYS && w < p.words) {
-                    const uint32_t a = bits[w], b = w + 1 < p.words ? bits[w + 1] : 0u, c = w + 2 < p.words ? bits[w + 2] : 0u;
-                    uint64_t of = (uint64_t(b) << 32 | a) >> shift;
-                    if (shift) of |= uint64_t(c) << (64 - shift);
-                    see |= node < 0 ? of << -node : of;
-                }
+            const int node = pos - rq.start;  // of the tile's first key
+            if (p.ancestors && node > -X::KEYS) {
+                const int shift = max(node, 0) & 31;
+                uint64_t of = (uint64_t(of_nodes.w[1]) << 32 | of_nodes.w[0]) >> shift;
+                if (X::BLOCKS > 1 && shift) of |= uint64_t(of_nodes.w[2]) << (64 - shift);
+                see |= node < 0 ? of << -node : of;
             }
-            see = see >> (HALF_KEY<D> * half);
+            see >>= HALF_KEY<D> * half;
             const uint64_t rows_there = there >> (4 * half);
 #pragma unroll
             for (int b = 0; b < X::BLOCKS; ++b) {
                 seen[b] = 0;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const bool yes = (see >> (32 * b + score_key<D>(i)) & 1u) && (rows_there >> (32 * b + 8 * (i / 4) + i % 4) & 1u);
-                    seen[b] |= uint32_t(yes) << i;
+                    const uint32_t yes = uint32_t(see >> (32 * b)) >> score_key<D>(i) & uint32_t(rows_there >> (32 * b)) >> (8 * (i / 4) + i % 4) & 1u;
+                    seen[b] |= yes << i;
                     s[b][i] = yes ? s[b][i] : NEG_INF;
                 }
             }
+            // Are all values finite?  An exponent of ones and a one more carry into the sign's bit.
+            constexpr uint32_t EXPONENT = TYPE == TYPE_BF16 ? 0x7f807f80u : 0x7c007c00u, ONE = TYPE == TYPE_BF16 ? 0x00800080u : 0x04000400u;
+            uint32_t carry = 0;
+#pragma unroll 4
+            for (int c = lane * 16; c < X::TILE; c += 1024) {
+                const uint4 w = *reinterpret_cast<const uint4*>(s_ring + (set * 2 + stage) * (2 * X::TILE) + X::TILE + c);
+                carry |= ((w.x & EXPONENT) + ONE) | ((w.y & EXPONENT) + ONE) | ((w.z & EXPONENT) + ONE) | ((w.w & EXPONENT) + ONE);
+            }
+            clean = !__any(carry & 0x80008000u);
         }
         float top = s[0][0];
 #pragma unroll
@@ -513,94 +625,107 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= shrink;
         }
+        if (clean) {
+            constexpr int PAIRS = X::DIMS / 2;
+            uint32_t high_w[2][4], low_w[2][HALVES ? 4 : 1];
+            uint4 v[2][2];
+            v[0][0] = value_operand(v_base, 0, 0);
+            v[0][1] = value_operand(v_base, 0, 1);
+            // sixteen n / 4: the weights of its eight scores of the lane, two at a time, beside the products of the sixteen
+            // before: a wave issues in order, and only so do the matrix units work meanwhile
+            static_for<0, 4 * (SIXTEENS + 1)>([&](auto n) {
+                constexpr int u = decltype(n)::value / 4, k = decltype(n)::value % 4;
+                if constexpr (u > 0) {
+                    constexpr int g = (u - 1) & 1;
+                    const uint4 ph = make_uint4(high_w[g][0], high_w[g][1], high_w[g][2], high_w[g][3]);
+                    uint4 pl = ph;
+                    if constexpr (HALVES) pl = make_uint4(low_w[g][0], low_w[g][1], low_w[g][2], low_w[g][3]);
+                    // products of the pairs of d: high, high (and low, low)
+                    constexpr int OF_PAIR = HALVES ? 4 : 2, ALL_OF = PAIRS * OF_PAIR;
+                    static_for<k * ALL_OF / 4, (k + 1) * ALL_OF / 4>([&](auto m) {
+                        constexpr int pair = decltype(m)::value / OF_PAIR, j = decltype(m)::value % OF_PAIR, turn = ((u - 1) * PAIRS + pair) & 1;
+                        if constexpr (j == 0 && (u < SIXTEENS || pair + 1 < PAIRS)) {  // the next pair's operands
+                            constexpr int u2 = pair + 1 < PAIRS ? u - 1 : u, p2 = pair + 1 < PAIRS ? pair + 1 : 0;
+                            v[turn ^ 1][0] = value_operand(v_base, u2, 2 * p2);
+                            v[turn ^ 1][1] = value_operand(v_base, u2, 2 * p2 + 1);
+                        }
+                        o[2 * pair + (j & 1)] = mfma32<TYPE>(v[turn][j & 1], j < 2 ? ph : pl, o[2 * pair + (j & 1)]);
+                    });
+                }
+                if constexpr (u < SIXTEENS) {
+                    constexpr int b = u / 2, i = (u & 1) * 8 + 2 * k;
+                    const float x = weight(s[b][i], from), y = weight(s[b][i + 1], from);
+                    sum += x;
+                    sum += y;
+                    if constexpr (HALVES) split<TYPE>(x, y, high_w[u & 1][k], low_w[u & 1][k]);
+                    else high_w[u & 1][k] = pack16<TYPE>(x, y);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            return;
+        }
+        // Values that are not finite reach those tokens alone that see their key: they are left out of the products (where a
+        // weight of zero would make NaN of them) and added one by one.  (`base`: or the compiler would take the weights out of
+        // both branches, and from beside the products.)
+        float base = from;
+        __asm__ volatile("" : "+v"(base));
 #pragma unroll
         for (int b = 0; b < X::BLOCKS; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], scale, -from));
-                if constexpr (!whole) s[b][i] = seen[b] >> i & 1u ? s[b][i] : 0.f;
+                s[b][i] = weight(s[b][i], base);
                 sum += s[b][i];
             }
-        // Values that are not finite reach those tokens alone that see their key: they are left out of the products
-        // (where a weight of zero would make NaN of them) and added one by one.
-        bool clean = true;
-        if constexpr (!whole) {
-            // an exponent of ones and a one more carry into the sign's bit
-            constexpr uint32_t EXPONENT = TYPE == TYPE_BF16 ? 0x7f807f80u : 0x7c007c00u, ONE = TYPE == TYPE_BF16 ? 0x00800080u : 0x04000400u;
-            uint32_t carry = 0;
-#pragma unroll 4
-            for (int c = lane * 16; c < X::KEYS * X::ROW; c += 1024) {
-                const uint4 w = *reinterpret_cast<const uint4*>(values + c);
-                carry |= ((w.x & EXPONENT) + ONE) | ((w.y & EXPONENT) + ONE) | ((w.z & EXPONENT) + ONE) | ((w.w & EXPONENT) + ONE);
+        int half = lane >> 5;
+        __asm__ volatile("" : "+v"(half));  // (as the bases)
+        const uint8_t* const values = s_ring + (set * 2 + stage) * (2 * X::TILE) + X::TILE;
+        for (int r = 0; r < X::KEYS; ++r) {
+            bool bad = false;
+            for (int c = lane * 4; c < X::ROW; c += 256) {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(values + r * X::ROW + c);
+                bad |= !(finite16<TYPE>(w) && finite16<TYPE>(w >> 16));
             }
-            uint64_t odd = 0;
-            if (__any(carry & 0x80008000u)) {
-                for (int r = 0; r < X::KEYS; ++r) {
-                    bool bad = false;
-                    for (int c = lane * 4; c < X::ROW; c += 256) {
-                        const uint32_t w = *reinterpret_cast<const uint32_t*>(values + r * X::ROW + c);
-                        bad |= !(finite16<TYPE>(w) && finite16<TYPE>(w >> 16));
-                    }
-                    if (__any(bad)) odd |= 1ull << r;
+            if (!__any(bad)) continue;
+            const int index = (r & 32) / 2 + (r & 24) / 2 + (r & 3), side = r >> 2 & 1;  // of the lane's scores, and the half
+            float w = 0.f;
+            uint32_t sees = 0;
+#pragma unroll
+            for (int b = 0; b < X::BLOCKS; ++b) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w = index == 16 * b + i ? s[b][i] : w;
+                sees = index >> 4 == b ? seen[b] >> (index & 15) & 1u : sees;
+            }
+            const float partner = xor_lane<32>(w);
+            const uint32_t partners = xor_lane<32>(sees);
+            w = side == half ? w : partner;
+            sees = side == half ? sees : partners;
+            static_for<0, X::DIMS * 4>([&](auto n) {
+                constexpr int d = decltype(n)::value / 4, i = decltype(n)::value % 4 * 4;
+                const uint2 h = *reinterpret_cast<const uint2*>(values + r * X::ROW + (d ^ value_swizzle<D>(r)) * 64 + (8 * (i / 4) + 4 * half) * 2);
+                const uint32_t of[4] = {h.x & 0xffffu, h.x >> 16, h.y & 0xffffu, h.y >> 16};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float add = w * from16<TYPE>(of[e]);
+                    o[d][i + e] += sees && !finite16<TYPE>(of[e]) ? add : 0.f;
                 }
-            }
-            clean = odd == 0;
-            while (odd) {
-                const int r = __ffsll((unsigned long long)odd) - 1;
-                odd &= odd - 1;
-                const int index = (r & 32) / 2 + (r & 24) / 2 + (r & 3), side = r >> 2 & 1;  // of the lane's scores, and the half
-                float weight = 0.f;
-                uint32_t sees = 0;
-#pragma unroll
-                for (int b = 0; b < X::BLOCKS; ++b)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        weight = index == 16 * b + i ? s[b][i] : weight;
-                        sees = index == 16 * b + i ? seen[b] >> i & 1u : sees;
-                    }
-                const float other = xor_lane<32>(weight);
-                const uint32_t others = xor_lane<32>(sees);
-                weight = side == half ? weight : other;
-                sees = side == half ? sees : others;
-#pragma unroll
-                for (int d = 0; d < X::DIMS; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int dim = 8 * (i / 4) + 4 * half + i % 4;
-                        const uint32_t h = *reinterpret_cast<const uint16_t*>(values + r * X::ROW + (d ^ value_swizzle<D>(r)) * 64 + dim * 2);
-                        if (sees && !finite16<TYPE>(h)) o[d][i] += weight * from16<TYPE>(h);
-                    }
-            }
+                __asm__ volatile("" ::: "memory");  // (a few values at a time: registers)
+            });
         }
 #pragma unroll
-        for (int b = 0; b < X::BLOCKS; ++b)
+        for (int u = 0; u < SIXTEENS; ++u) {
+            uint32_t hw[4], lw[4];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                uint32_t high_w[4], low_w[4];
+            for (int i = 0; i < 4; ++i) split<TYPE>(s[u / 2][(u & 1) * 8 + 2 * i], s[u / 2][(u & 1) * 8 + 2 * i + 1], hw[i], lw[i]);
+            const uint4 ph = make_uint4(hw[0], hw[1], hw[2], hw[3]), pl = make_uint4(lw[0], lw[1], lw[2], lw[3]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float x = s[b][8 * t + 2 * i], y = s[b][8 * t + 2 * i + 1];
-                    high_w[i] = pack16<TYPE>(x, y);
-                    low_w[i] = pack16<TYPE>(x - from16<TYPE>(high_w[i]), y - from16<TYPE>(high_w[i] >> 16));
-                }
-                const uint4 ph = make_uint4(high_w[0], high_w[1], high_w[2], high_w[3]), pl = make_uint4(low_w[0], low_w[1], low_w[2], low_w[3]);
-#pragma unroll
-                for (int d = 0; d < X::DIMS; ++d) {
-                    // source lane sl of 16-lane group grp reads 8 bytes of row 4 (grp / 2) + sl / 4; lane j gets dim
-                    // 16 (grp % 2) + j of the four rows
-                    const int r = 4 * (grp >> 1) + (sl >> 2);
-                    const uint8_t* at = values + (32 * b + 16 * t + r) * X::ROW + (d ^ value_swizzle<D>(r)) * 64 + 32 * (grp & 1) + 8 * (sl & 3);
-                    const short4_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)at);
-                    // rows 8 further: the same swizzle for D of 128 and more, the same (8 >> 1 & 1) for 64
-                    const short4_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(at + 8 * X::ROW));
-                    uint4 v;
-                    __builtin_memcpy(&v, &x0, 8);
-                    __builtin_memcpy(reinterpret_cast<char*>(&v) + 8, &x1, 8);
-                    if (!clean) v = make_uint4(finite_or_zero<TYPE>(v.x), finite_or_zero<TYPE>(v.y), finite_or_zero<TYPE>(v.z), finite_or_zero<TYPE>(v.w));
-                    o[d] = mfma32<TYPE>(v, ph, o[d]);
-                    o[d] = mfma32<TYPE>(v, pl, o[d]);
-                }
+            for (int d = 0; d < X::DIMS; ++d) {
+                uint4 v = value_operand(v_base, u, d);
+                v = make_uint4(finite_or_zero<TYPE>(v.x), finite_or_zero<TYPE>(v.y), finite_or_zero<TYPE>(v.z), finite_or_zero<TYPE>(v.w));
+                o[d] = mfma32<TYPE>(v, ph, o[d]);
+                if constexpr (HALVES) o[d] = mfma32<TYPE>(v, pl, o[d]);
+                __builtin_amdgcn_sched_barrier(0);
             }
+        }
     };
 
     // ---- the part's tiles, the next one's loads on their way
@@ -610,32 +735,23 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
         look_up(pos);
         request_tile(pos, 0);
         look_up(pos + TURN);
+        look_at_bits(pos);
     }
     for (int turn = 0; turn < turns; ++turn, pos += TURN) {
-        uint64_t there = 0;
-        if constexpr (SHARE == 1) {
-#pragma unroll
-            for (int b = 0; b < X::OWN; ++b) there |= uint64_t(own_there[b]) << (16 * b);
-        }
         __asm__ volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0070);  // the tile's loads, and LDS reads of the tile before
+        __builtin_amdgcn_s_waitcnt(0x0070);  // the wave's loads, and its LDS operations of the tile before
         if (SHARE > 1) __builtin_amdgcn_s_barrier();
         __asm__ volatile("" ::: "memory");
         const int stage = turn & 1;
-        if constexpr (SHARE > 1) {
-#pragma unroll
-            for (int b = 0; b < X::KEYS / 16; ++b) there |= uint64_t(s_there[set][stage][b]) << (16 * b);
-            there = uint64_t(__builtin_amdgcn_readfirstlane(int(there >> 32))) << 32 | uint32_t(__builtin_amdgcn_readfirstlane(int(there)));
-        }
+        uint64_t there = X::KEYS == 64 ? *reinterpret_cast<const uint64_t*>(s_there[set][stage]) : *reinterpret_cast<const uint32_t*>(s_there[set][stage]);
+        there = uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(there >> 32)))) << 32 | uint32_t(__builtin_amdgcn_readfirstlane(int(there)));
+        const Bits of_nodes = node_bits;
         if (turn + 1 < turns) {
             request_tile(pos + TURN, stage ^ 1);
             look_up(pos + 2 * TURN);
+            look_at_bits(pos + TURN);
         }
-        if (pos < end) {
-            constexpr uint64_t ALL = X::KEYS == 64 ? ~0ull : 0xffffffffull;
-            if (pos >= all_low && pos + X::KEYS <= all_high && there == ALL) take(pos, stage, there, std::true_type{});
-            else take(pos, stage, there, std::false_type{});
-        }
+        if (pos < end) take(pos, stage, there, of_nodes);
     }
     sum += xor_lane<32>(sum);
 
@@ -657,21 +773,28 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
             total += ml.x == NEG_INF ? 0.f : ml.y * __builtin_amdgcn_exp2f(ml.x - top);
         }
         const float share = exponent == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(exponent - top);
-        float4* all = reinterpret_cast<float4*>(s_ring);  // [wave][SPLIT][64]
+        auto piece = [&](int e) {
+            return make_float4(o[e >> 2][4 * (e & 3)] * share, o[e >> 2][4 * (e & 3) + 1] * share, o[e >> 2][4 * (e & 3) + 2] * share,
+                               o[e >> 2][4 * (e & 3) + 3] * share);
+        };
+        // a set gives each other one its EACH pieces of the dims: [to][from][wave of the set][EACH][64]
+        float4* all = reinterpret_cast<float4*>(s_ring);
+        static_assert((X::GROUPS - 1) * SHARE * X::SPLIT * 1024 <= X::LDS, "where the tiles were");
 #pragma unroll
-        for (int e = 0; e < X::SPLIT; ++e)
-            all[(wave * X::SPLIT + e) * 64 + lane] = make_float4(o[e >> 2][4 * (e & 3)] * share, o[e >> 2][4 * (e & 3) + 1] * share,
-                                                                o[e >> 2][4 * (e & 3) + 2] * share, o[e >> 2][4 * (e & 3) + 3] * share);
+        for (int g = 0; g < X::GROUPS; ++g)
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                if (g == set) mine[e] = piece(g * EACH + e);
+                else all[(((g * (X::GROUPS - 1) + (set < g ? set : set - 1)) * SHARE + part_wave) * EACH + e) * 64 + lane] = piece(g * EACH + e);
+            }
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-            mine[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int e = 0; e < EACH; ++e)
 #pragma unroll
-            for (int g = 0; g < X::GROUPS; ++g) {
-                const float4 v = all[((g * SHARE + part_wave) * X::SPLIT + set * EACH + e) * 64 + lane];
+            for (int g = 0; g < X::GROUPS - 1; ++g) {
+                const float4 v = all[(((set * (X::GROUPS - 1) + g) * SHARE + part_wave) * EACH + e) * 64 + lane];
                 mine[e].x += v.x, mine[e].y += v.y, mine[e].z += v.z, mine[e].w += v.w;
             }
-        }
     } else {
 #pragma unroll
         for (int e = 0; e < EACH; ++e)
@@ -770,13 +893,21 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void tree_join_kernel(TreeAttnPara
 }
 
 // ------------------------------------------------------------------------------------ launches
-// Waves that share a tile, by the rows of queries that a request has on the average.
+// Waves that share a tile, by the rows of queries that a request has on the average: few rows read the keys at the rate of
+// memory, and more rows a tile read them fewer times; many are bound by arithmetic.  64 requests of 2,000 to 4,000 keys and 16
+// heads of 128 on one, 15 / 30 / 38 / 60 / 78 rows each: 27 / 31 / 35 / 49 / 56 us with one wave, 30 / 31 / 32 / 36 / 39 with two,
+// 37 / 38 / 39 / 40 / 40 with four.  (Heads of 64 and 256 cross over at the same numbers.)
 int share_of(int rows, int tokens, int group) {
     const int64_t each = int64_t(tokens) * group / rows;
-    return each <= 32 ? 1 : each <= 64 ? 2 : 4;
+    return each <= 24 ? 1 : each <= 72 ? 2 : 4;
 }
-int held_of(int share, int head_dim) { return head_dim == 256 || (head_dim == 128 && share == 1) ? 1 : 2; }
-int target_of(int share, int kv_heads, int head_dim) { return std::max(1, CUS * held_of(share, head_dim) / kv_heads); }
+// Workgroups that the CUs hold at once.
+int target_of(int share, int kv_heads, int head_dim) {
+    return std::max(1, CUS * (head_dim == 256 || (head_dim == 128 && share == 1) ? 1 : 2) / kv_heads);
+}
+int turn_of(int share, int head_dim) {
+    return (share == 4 || (share == 2 && head_dim == 64) ? 64 : 32) * (share == 4 ? 1 : share == 2 || head_dim == 256 ? 2 : 4);
+}
 // (2^20 requests and 2^30 rows of queries are less than 2^24 workgroups: a launch holds them)
 int64_t tiles_of(const TreeAttnParams& p) { return std::min(p.rows, p.tokens) + int64_t(p.tokens) * p.group / (32 * p.share); }
 int64_t items_of(const TreeAttnParams& p) {
@@ -834,8 +965,7 @@ void tree_attn_bind(TreeAttnParams& p, void* workspace, int head_dim) {
     p.share = share_of(p.rows, p.tokens, p.group);
     p.target = target_of(p.share, p.kv_heads, head_dim);
     p.by_group = divider(uint32_t(p.group));
-    const int groups = p.share == 4 ? 1 : p.share == 2 ? (head_dim == 256 ? 1 : 2) : (head_dim == 256 ? 2 : 4);
-    p.least = groups * (p.share == 4 || (p.share == 2 && head_dim == 256) ? 64 : 32);
+    p.least = turn_of(p.share, head_dim);
     p.joins = p.most > p.least;
     p.run = int(std::min<int64_t>(16, std::max<int64_t>(1, int64_t(p.tokens) * p.group / p.rows / (32 * p.share))));
     p.listed = p.rows > FOUND_ROWS;

@@ -70,6 +70,7 @@ def attend_tree(cache, q, heads, tables, lengths, offsets, out, lse=None, positi
 def attend_tree64(keys, values, q, tables, lengths, offsets, scale, positions=None, ancestors=None, window=0):
     """-> out [tokens][heads * dim], lse [tokens][heads] of the requests' tokens, and how far a kernel with FP32 sums
     may be off them before its last rounding (for both)."""
+    weights = torch.finfo(keys.dtype).eps / 2  # of the weights' rounding to the type
     pages, page, kv, dim = keys.shape
     heads = q.shape[1] // dim
     total = int(offsets[-1])
@@ -120,9 +121,10 @@ def attend_tree64(keys, values, q, tables, lengths, offsets, scale, positions=No
                 one = float(most) * (dim + 4) * 2.0 ** -23 + 2.0 ** -21 * (1 + float(score.abs().max()))
                 # the sum of the weights is a chain of half the keys in each of two lanes (2^-24 each)
                 sums = len(score) * 2.0 ** -25 + 2.0 ** -20
-                # weights are off by twice a score's error (numerator and sum) and by two halves' rounding, 2^-16; the
-                # products' sums are chains of two steps for sixteen keys (2^-23 each: they may be truncated), and of the joins
-                s_out[t, h] = (share @ vs.abs()) * (2 * one + sums + 2.0 ** -16 + (len(score) / 8 + 64) * 2.0 ** -23)
+                # weights are off by twice a score's error (numerator and sum) and by half a step of the type where they are
+                # rounded once: sum_j (p_j (1 + e_j) - p_j) v_j is at most max |e_j| sum_j p_j |v_j|; the products' sums are
+                # chains of two steps for sixteen keys (2^-23 each: they may be truncated), and of the joins
+                s_out[t, h] = (share @ vs.abs()) * (2 * one + sums + weights + (len(score) / 8 + 64) * 2.0 ** -23)
                 s_lse[t, h] = one + sums + 2.0 ** -22 * abs(float(lse[t, h]))
     return out.view(total, -1), lse, s_out.view(total, -1), s_lse
 
