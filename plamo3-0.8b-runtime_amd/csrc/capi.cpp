@@ -1113,6 +1113,7 @@ int plamo_kernel_paged_tree(uint64_t lengths, uint64_t offsets, int32_t rows, ui
         p.positions = reinterpret_cast<int32_t*>(positions);
         p.ancestors = reinterpret_cast<uint32_t*>(ancestors);
         p.words = words;
+        p.by_words = plamo::divider(uint32_t(words));
         plamo::launch_paged_tree(p, s);
         PLAMO_HIP(hipGetLastError());
     });

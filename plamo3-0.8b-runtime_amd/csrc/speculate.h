@@ -22,6 +22,7 @@ struct TreeParams {
     int32_t* positions;       // [tokens]
     uint32_t* ancestors;      // [tokens][words]
     int words;
+    Divider by_words;
 };
 void launch_paged_tree(const TreeParams& p, hipStream_t s);
 

@@ -30,9 +30,9 @@ __device__ __forceinline__ Span new_tokens(const int32_t* offsets, int r, int mo
 
 // ------------------------------------------------------------------------------------ trees
 // Node i's bits are its parent's and its own.  All nodes at once, by doubling: after step k a node's bits hold the
-// 2^k nodes up from it, and its link the node 2^k up, so that ceil(log2(depth)) steps do.  Parents come before their
+// 2^k nodes up from it, and its link is the node 2^k up, so that ceil(log2(depth)) steps do.  Parents come before their
 // children, so a path's nodes are in the order of their depth, which is the number of bits less one, and a window
-// keeps the highest bits.  Latency-bound: some dependent loads and shuffles.
+// keeps the highest bits.  Latency-bound: some dependent loads, shuffles and barriers (64 requests of 8 nodes 2.6 us).
 constexpr int WAVE_THREADS = 256;
 
 // Tokens behind the last request's.
@@ -52,7 +52,25 @@ __device__ __forceinline__ void no_tree(const TreeParams& p, Span s, int lane, i
     }
 }
 
-// Up to 64 nodes: a wave a request, a node a lane, links followed by shuffles.
+// Among the 64 nodes from `base` on, a node a lane, links followed by shuffles: bits of these nodes alone, and the link is
+// the first ancestor before them, or none.
+__device__ __forceinline__ void wave_tree(int base, int& up, uint32_t& low, uint32_t& high) {
+    const int lane = threadIdx.x & 63;
+    low = lane < 32 ? 1u << lane : 0u;
+    high = lane < 32 ? 0u : 1u << (lane - 32);
+    while (__any(up >= base)) {
+        const int at = max(up - base, 0);
+        const uint32_t l = __shfl(low, at, 64), h = __shfl(high, at, 64);
+        const int next = __shfl(up, at, 64);
+        if (up >= base) {
+            low |= l;
+            high |= h;
+            up = next;
+        }
+    }
+}
+
+// Up to 64 nodes: a wave a request.
 __global__ __launch_bounds__(WAVE_THREADS) void tree_wave_kernel(TreeParams p) {
     const int lane = threadIdx.x & 63, r = int(blockIdx.x) * (WAVE_THREADS / 64) + int(threadIdx.x >> 6);
     pad_tokens(p, blockIdx.x, gridDim.x, WAVE_THREADS);
@@ -62,17 +80,8 @@ __global__ __launch_bounds__(WAVE_THREADS) void tree_wave_kernel(TreeParams p) {
     if (s.count > 32 * p.words || start < 0) return no_tree(p, s, lane, 64);
     int up = lane < s.count ? p.parents[s.first + lane] : -1;
     up = up >= 0 && up < lane ? up : -1;
-    uint32_t low = lane < 32 ? 1u << lane : 0u, high = lane < 32 ? 0u : 1u << (lane - 32);
-    while (__any(up >= 0)) {
-        const int at = max(up, 0);
-        const uint32_t l = __shfl(low, at, 64), h = __shfl(high, at, 64);
-        const int next = __shfl(up, at, 64);
-        if (up >= 0) {
-            low |= l;
-            high |= h;
-            up = next;
-        }
-    }
+    uint32_t low, high;
+    wave_tree(0, up, low, high);
     if (lane >= s.count) return;
     uint64_t bits = uint64_t(high) << 32 | low;
     const int depth = __popcll(bits) - 1;
@@ -84,33 +93,39 @@ __global__ __launch_bounds__(WAVE_THREADS) void tree_wave_kernel(TreeParams p) {
     if (p.words > 1) p.ancestors[t * p.words + 1] = uint32_t(bits >> 32);
 }
 
-// More: a workgroup a request, a node a thread, rows of W words in LDS.
+// More: a workgroup a request.  After each wave's own 64 nodes a link leads to an earlier wave's, so that a path has few of
+// them, and rows of words in LDS are doubled that few times (200 requests of 60 nodes, or of a chain of 500, in 16 words: all
+// steps on rows in LDS 18.7 us, so 11.3).
 template <int W>
 __global__ __launch_bounds__(32 * W) void tree_block_kernel(TreeParams p) {
     constexpr int NODES = 32 * W, PITCH = W + 1;  // banks: a row's words in those of its neighbours, one further
     __shared__ uint32_t s_bits[NODES * PITCH];
     __shared__ int s_up[NODES];
-    const int i = threadIdx.x;
+    const int i = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     pad_tokens(p, blockIdx.x, gridDim.x, NODES);
     const Span s = new_tokens(p.offsets, blockIdx.x, p.tokens);
     const int start = p.lengths[blockIdx.x] - s.count;
     if (s.count > 32 * p.words || start < 0) return no_tree(p, s, i, NODES);
-    const int used = (s.count + 31) / 32;  // words of this request's nodes
     int up = i < s.count ? p.parents[s.first + i] : -1;
     up = up >= 0 && up < i ? up : -1;
-    uint32_t bits[W];
+    uint32_t bits[W], low, high;
+    wave_tree(64 * wave, up, low, high);
 #pragma unroll
-    for (int w = 0; w < W; ++w) bits[w] = (i >> 5) == w ? 1u << (i & 31) : 0u;
+    for (int w = 0; w < W; ++w) bits[w] = w == 2 * wave ? low : w == 2 * wave + 1 ? high : 0u;
+    bool changed = true;
     while (__syncthreads_or(up >= 0)) {  // what the step before read has been read
         s_up[i] = up;
+        if (changed) {
 #pragma unroll
-        for (int w = 0; w < W; ++w)
-            if (w < used) s_bits[i * PITCH + w] = bits[w];
+            for (int w = 0; w < W; ++w)
+                if (w < 2 * wave + 2) s_bits[i * PITCH + w] = bits[w];
+        }
         __syncthreads();
+        changed = __any(up >= 0);
         if (up >= 0) {
 #pragma unroll
             for (int w = 0; w < W; ++w)
-                if (w < used) bits[w] |= s_bits[up * PITCH + w];
+                if (w < 2 * wave) bits[w] |= w < 2 * (up >> 6) + 2 ? s_bits[up * PITCH + w] : 0u;
             up = s_up[up];
         }
     }
@@ -135,8 +150,11 @@ __global__ __launch_bounds__(32 * W) void tree_block_kernel(TreeParams p) {
         if (w < p.words) s_bits[i * PITCH + w] = bits[w];
     if (i < s.count) p.positions[s.first + i] = start + depth;
     __syncthreads();
-    for (int e = i; e < s.count * p.words; e += NODES)
-        p.ancestors[int64_t(s.first) * p.words + e] = s_bits[e / p.words * PITCH + e % p.words];
+    uint32_t* to = p.ancestors + int64_t(s.first) * p.words;
+    for (int e = i; e < s.count * p.words; e += NODES) {
+        const int row = int(divide(uint32_t(e), p.by_words));
+        to[e] = s_bits[row * PITCH + e - row * p.words];
+    }
 }
 
 // ------------------------------------------------------------------------------------ accepted paths
@@ -166,47 +184,80 @@ __device__ __forceinline__ int slot_of(const AcceptParams& p, int r, int at) {
     return uint32_t(entry) < uint32_t(p.pages) ? entry * p.page_size + (at - int(page) * p.page_size) : -1;
 }
 
+// The paths of requests r, r + step, ..., EACH of them, by a wave: their loads side by side.  counts (or null): numbers of
+// accepted tokens once more, in LDS.
+template <int EACH>
+__device__ __forceinline__ void accept_walk(const AcceptParams& p, int r0, int step, int* counts) {
+    const int lane = threadIdx.x & 63;
+    Step steps[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const int r = r0 + e * step;
+        steps[e] = r < p.rows ? accept_step(p, r) : Step{{0, 0}, 0, 0, true};
+    }
+    int drawn0[EACH], parents[EACH], tokens[EACH], nexts[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const Step& s = steps[e];
+        const int i = s.span.first + s.given + lane;
+        const bool there = s.given + lane < s.span.count;
+        drawn0[e] = s.span.count > 0 ? p.drawn[s.span.first + s.given - 1] : -1;
+        parents[e] = there ? p.parents[i] : -1;
+        tokens[e] = there ? p.tokens[i] : -1;
+        nexts[e] = there ? p.drawn[i] : -1;
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const int r = r0 + e * step;
+        if (r >= p.rows) return;
+        const Step& s = steps[e];
+        const int first = s.span.first, count = s.span.count, start = s.length - count;
+        int32_t* accepted = p.accepted + int64_t(r) * (p.nodes + 1);
+        int32_t *from = p.from + int64_t(r) * p.nodes, *to = p.to + int64_t(r) * p.nodes;
+        int current = s.given - 1, kept = 0, drawn = __builtin_amdgcn_readfirstlane(drawn0[e]);
+        for (int base = s.given; base < count && drawn >= 0; base += 64) {
+            const int i = base + lane;
+            int parent = parents[e], token = tokens[e], next = nexts[e];
+            if (base > s.given) {
+                const bool there = i < count;
+                parent = there ? p.parents[first + i] : -1;
+                token = there ? p.tokens[first + i] : -1;
+                next = there ? p.drawn[first + i] : -1;
+            }
+            int place = -1;
+            while (drawn >= 0) {
+                const unsigned long long fits = __ballot(i < count && parent == current && token == drawn && i > current);
+                if (!fits) break;
+                const int l = __ffsll(fits) - 1;
+                if (lane == l) place = kept;
+                ++kept;
+                current = base + l;
+                drawn = __builtin_amdgcn_readlane(next, l);
+            }
+            if (place >= 0 && place < p.nodes) {
+                accepted[place] = token;
+                const int at = s.given + place;
+                const int source = i != at ? slot_of(p, r, start + i) : -1, target = i != at ? slot_of(p, r, start + at) : -1;
+                from[place] = source >= 0 && target >= 0 ? source : -1;
+                to[place] = source >= 0 && target >= 0 ? target : -1;
+            }
+        }
+        for (int i = kept + lane; i < p.nodes; i += 64) {
+            accepted[i + 1] = -1;
+            from[i] = to[i] = -1;
+        }
+        if (lane == 0) {
+            if (kept <= p.nodes) accepted[kept] = drawn;
+            p.accepted_counts[r] = count > 0 ? kept + 1 : 0;
+            if (counts) counts[r] = count > 0 ? kept + 1 : 0;
+            p.last[r] = count > 0 ? first + current : -1;
+        }
+    }
+}
+
 __global__ __launch_bounds__(WAVE_THREADS) void accept_walk_kernel(AcceptParams p) {
-    const int lane = threadIdx.x & 63, r = int(blockIdx.x) * (WAVE_THREADS / 64) + int(threadIdx.x >> 6);
-    if (r >= p.rows) return;
-    const Step s = accept_step(p, r);
-    const int first = s.span.first, count = s.span.count, start = s.length - count;
-    int32_t* accepted = p.accepted + int64_t(r) * (p.nodes + 1);
-    int32_t *from = p.from + int64_t(r) * p.nodes, *to = p.to + int64_t(r) * p.nodes;
-    int current = s.given - 1, kept = 0;
-    int drawn = count > 0 ? p.drawn[first + current] : -1;
-    for (int base = s.given; base < count && drawn >= 0; base += 64) {
-        const int i = base + lane;
-        const bool there = i < count;
-        const int parent = there ? p.parents[first + i] : -1, token = there ? p.tokens[first + i] : -1,
-                  next = there ? p.drawn[first + i] : -1;
-        int place = -1;
-        while (drawn >= 0) {
-            const unsigned long long fits = __ballot(there && parent == current && token == drawn && i > current);
-            if (!fits) break;
-            const int l = __ffsll(fits) - 1;
-            if (lane == l) place = kept;
-            ++kept;
-            current = base + l;
-            drawn = __builtin_amdgcn_readlane(next, l);
-        }
-        if (place >= 0 && place < p.nodes) {
-            accepted[place] = token;
-            const int at = s.given + place;
-            const int source = i != at ? slot_of(p, r, start + i) : -1, target = i != at ? slot_of(p, r, start + at) : -1;
-            from[place] = source >= 0 && target >= 0 ? source : -1;
-            to[place] = source >= 0 && target >= 0 ? target : -1;
-        }
-    }
-    for (int i = kept + lane; i < p.nodes; i += 64) {
-        accepted[i + 1] = -1;
-        from[i] = to[i] = -1;
-    }
-    if (lane == 0) {
-        if (kept <= p.nodes) accepted[kept] = drawn;
-        p.accepted_counts[r] = count > 0 ? kept + 1 : 0;
-        p.last[r] = count > 0 ? first + current : -1;
-    }
+    const int r = int(blockIdx.x) * (WAVE_THREADS / 64) + int(threadIdx.x >> 6);
+    if (r < p.rows) accept_walk<1>(p, r, 0, nullptr);
 }
 
 // One workgroup: a request a thread, sums of the pages given back in the order of requests.  A request gives back few:
@@ -226,20 +277,28 @@ __device__ __forceinline__ int block_scan(int v, int* waves, int& total) {
     return wave > 0 ? v + __builtin_amdgcn_readlane(sum, wave - 1) : v;
 }
 
+// Requests whose paths this workgroup finds by itself first, a few for each of its waves: a launch less (64 requests of 8
+// nodes 11.2 us in two, 8.4 so).
+constexpr int WALKED = 4 * PAGES_THREADS / 64;
+
+template <bool WALKS>
 __global__ __launch_bounds__(PAGES_THREADS) void accept_pages_kernel(AcceptParams p) {
     __shared__ int s_waves[PAGES_THREADS / 64];
-    __shared__ int s_status;
+    __shared__ int s_status, s_accepted[WALKS ? WALKED : 1];
     const int tid = threadIdx.x;
+    if constexpr (WALKS) {
+        accept_walk<WALKED / (PAGES_THREADS / 64)>(p, int(threadIdx.x >> 6), PAGES_THREADS / 64, s_accepted);
+    }
     if (tid == 0) s_status = 0;
     const int top = *p.free_count;
-    __syncthreads();
     // entries of request r that its length no longer reaches: columns after .. held - 1
     struct Back {
         int length, after, held, bad;
     };
     auto back_of = [&](int r) -> Back {
         const Step s = accept_step(p, r);
-        const int kept = s.span.count > 0 ? s.given + p.accepted_counts[r] - 1 : 0;
+        const int accepted = WALKS ? s_accepted[r] : p.accepted_counts[r];
+        const int kept = s.span.count > 0 ? s.given + accepted - 1 : 0;
         const int held = int((int64_t(s.length) + p.page_size - 1) / p.page_size);
         Back b;
         b.bad = s.fine ? (held > p.width ? 2 : 0) | (s.span.count - s.given > p.nodes ? 4 : 0) : 8;
@@ -248,6 +307,10 @@ __global__ __launch_bounds__(PAGES_THREADS) void accept_pages_kernel(AcceptParam
         b.held = held;
         return b;
     };
+    __syncthreads();
+    // the first PAGES_THREADS requests' stay in registers
+    Back first = {};
+    if (tid < p.rows) first = back_of(tid);
     auto pages_of = [&](const Back& b, int r, auto f) {
         for (int c = b.after; c < b.held; ++c) {
             const int entry = p.tables[int64_t(r) * p.width + c];
@@ -255,7 +318,7 @@ __global__ __launch_bounds__(PAGES_THREADS) void accept_pages_kernel(AcceptParam
         }
     };
     int bad = 0;
-    for (int r = tid; r < p.rows; r += PAGES_THREADS) bad |= back_of(r).bad;
+    for (int r = tid; r < p.rows; r += PAGES_THREADS) bad |= r == tid ? first.bad : back_of(r).bad;
     if (bad) atomicOr(&s_status, bad);
     __syncthreads();
     int status = s_status;
@@ -265,7 +328,7 @@ __global__ __launch_bounds__(PAGES_THREADS) void accept_pages_kernel(AcceptParam
         for (int base = 0; base < p.rows; base += PAGES_THREADS) {
             const int r = base + tid;
             int own = 0, sum;
-            if (r < p.rows) pages_of(back_of(r), r, [&](int) { ++own; });
+            if (r < p.rows) pages_of(base ? back_of(r) : first, r, [&](int) { ++own; });
             block_scan(own, s_waves, sum);
             total += sum;
         }
@@ -278,7 +341,7 @@ __global__ __launch_bounds__(PAGES_THREADS) void accept_pages_kernel(AcceptParam
             int own = 0, sum;
             Back b = {};
             if (r < p.rows) {
-                b = back_of(r);
+                b = base ? back_of(r) : first;
                 pages_of(b, r, [&](int) { ++own; });
             }
             int place = at + block_scan(own, s_waves, sum) - own;
@@ -305,7 +368,9 @@ __global__ __launch_bounds__(PAGES_THREADS) void accept_pages_kernel(AcceptParam
 
 // ------------------------------------------------------------------------------------ moves
 // A thread takes a 16-byte piece of a group's tokens, in their order, several loads ahead of the stores: what a move
-// of a group writes no later one of it reads.  Bound by memory, or by the latency of three accesses.
+// of a group writes no later one of it reads.  Bound by memory, which takes rows of 256 bytes from anywhere to anywhere at
+// 3.7 TB/s (20,000 tokens of one KV head in 16 layers 88 us; eight copies a thread 112, four layers' keys and values a thread 89),
+// or by the latency of three accesses (64 requests of 7 nodes 4.6 us; four moves' keys and values a thread 10).
 constexpr int MOVE_AHEAD = 8;
 
 __device__ __forceinline__ int64_t move_at(const MoveParams& p, int slot) {
@@ -343,8 +408,10 @@ __global__ __launch_bounds__(256) void move_kernel(MoveParams p) {
 
 // ------------------------------------------------------------------------------------ controls
 // A workgroup takes a segment of a row's vocabulary: a word of LDS a token counts how often the row's sequence has it,
-// and holds whether an n-gram bans it and which bias it has; then one pass over the logits.  All of the sequence is looked
-// through for each segment.
+// and holds whether an n-gram bans it and which bias it has; then one pass over the logits, which were loaded before.  All
+// of the sequence is looked through for each segment.  Bound by memory and what a workgroup waits for before it writes
+// (145 BF16 rows of 107,520, histories of up to 700 and paths, biases, masks on half of them 17.8 us, 3.5 TB/s read and
+// written; segments of 8,192 with 512 threads, and of 16,384 with 1,024, take 17.8 and 18.2).
 constexpr int CONTROL_THREADS = 256, CONTROL_SEGMENT = 4096, EACH = 8;
 constexpr uint32_t COUNT_BITS = 18, BANNED = 1u << COUNT_BITS, COUNTED = BANNED - 1;
 static_assert(CONTROL_MAX_HISTORY + 32 * TREE_MAX_WORDS < int(BANNED) && CONTROL_MAX_BIAS < (1 << (31 - COUNT_BITS)), "a word holds them");
@@ -421,7 +488,7 @@ __device__ __forceinline__ float controlled(float x, uint32_t word, bool open, c
 
 template <int TYPE, int OUT>
 __global__ __launch_bounds__(CONTROL_THREADS) void controls_kernel(ControlParams p, int segments) {
-    __shared__ uint32_t s_word[CONTROL_SEGMENT];
+    __shared__ __align__(16) uint32_t s_word[CONTROL_SEGMENT];
     __shared__ int32_t s_path[32 * TREE_MAX_WORDS];
     const int tid = threadIdx.x, lane = tid & 63;
     const int t = int(blockIdx.x) / segments, low = (int(blockIdx.x) - t * segments) * CONTROL_SEGMENT;
@@ -429,16 +496,36 @@ __global__ __launch_bounds__(CONTROL_THREADS) void controls_kernel(ControlParams
     if (r < 0) return;  // a row behind the last sequence's
     const int size = min(CONTROL_SEGMENT, p.n - low);
 
-    for (int i = tid; i < CONTROL_SEGMENT; i += CONTROL_THREADS) s_word[i] = 0;
+    // the logits and the mask's bits are on their way while the sequence is looked through
+    constexpr int ROUNDS = CONTROL_SEGMENT / (CONTROL_THREADS * EACH);
+    const char* in = p.logits + int64_t(t) * p.stride * (TYPE == TYPE_F32 ? 4 : 2);
+    const uint8_t* mask = nullptr;
+    if (p.masks) {
+        const int m = p.mask_rows ? p.mask_rows[t] : t;
+        if (uint32_t(m) < uint32_t(p.mask_count)) mask = reinterpret_cast<const uint8_t*>(p.masks + int64_t(m) * p.mask_stride) + low / 8;
+    }
+    float v[ROUNDS][EACH];
+    uint32_t open[ROUNDS];
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k) {
+        const int i = (k * CONTROL_THREADS + tid) * EACH;
+        open[k] = mask && i < size ? mask[i / 8] : 0xffu;
+        if (!p.in_place && i + EACH <= size) load8<TYPE>(in, low + i, v[k]);
+    }
+#pragma unroll
+    for (int i = 0; i < CONTROL_SEGMENT / (4 * CONTROL_THREADS); ++i)
+        *reinterpret_cast<uint4*>(&s_word[(i * CONTROL_THREADS + tid) * 4]) = make_uint4(0, 0, 0, 0);
     // the path's tokens, in the order of their bits: the same in every wave
     int path = 0;
     if (p.ancestors) {
         const int first = max(p.offsets[r], 0), count = min(min(p.offsets[r + 1], p.rows) - first, 32 * p.words);
         for (int base = 0; base < count; base += 64) {
             const int node = base + lane;
-            const bool on = node < count && (p.ancestors[int64_t(t) * p.words + node / 32] >> (node & 31) & 1u);
+            const uint32_t bits = node < count ? p.ancestors[int64_t(t) * p.words + node / 32] : 0u;
+            const int32_t token = node < count ? p.tokens[first + node] : -1;
+            const bool on = bits >> (node & 31) & 1u;
             const unsigned long long all = __ballot(on);
-            if (on && tid < 64) s_path[path + __popcll(all & ((1ull << lane) - 1))] = p.tokens[first + node];
+            if (on && tid < 64) s_path[path + __popcll(all & ((1ull << lane) - 1))] = token;
             path += __popcll(all);
         }
     }
@@ -448,55 +535,71 @@ __global__ __launch_bounds__(CONTROL_THREADS) void controls_kernel(ControlParams
     if (c.frequency != c.frequency) c.frequency = 0.0f;
     const int length = p.history ? min(max(p.history_lengths[r], 0), p.history_width) : 0, all = length + path;
     const int32_t* history = p.history + int64_t(r) * p.history_stride;
-    const int span = p.ngram && p.ngram[r] > 1 && all >= p.ngram[r] ? p.ngram[r] - 1 : 0;
+    const int ngram = p.ngram ? p.ngram[r] : 0, span = ngram > 1 && all >= ngram ? ngram - 1 : 0;
+    const bool looks = span || c.repetition != 1.0f || c.presence != 0.0f || c.frequency != 0.0f;
+    // the first tokens and biases are on their way before the counts are cleared, and the tokens before these: few follow
+    // the sequence's last one, and all but those need no look at the rest of an n-gram
+    constexpr int SOON = 4;
+    int32_t soon[SOON], before[SOON];
+#pragma unroll
+    for (int k = 0; k < SOON; ++k) {
+        const int i = k * CONTROL_THREADS + tid;
+        soon[k] = looks && i < length ? history[i] : -1;
+        before[k] = span && i > 0 && i < length ? history[i - 1] : -1;
+    }
+    int32_t last = span && path == 0 ? history[length - 1] : -1;
+    const int32_t* ids = p.bias_ids + int64_t(r) * p.bias_width;
+    const int32_t id = p.bias_ids && tid < p.bias_width ? ids[tid] : -1;
     __syncthreads();
     if (p.bias_ids) {
         for (int i = tid; i < p.bias_width; i += CONTROL_THREADS) {
-            const uint32_t at = uint32_t(p.bias_ids[int64_t(r) * p.bias_width + i] - low);
+            const uint32_t at = uint32_t(i == tid ? id : ids[i]) - uint32_t(low);
             if (at < uint32_t(size)) atomicMax(&s_word[at], uint32_t(i + 1) << (COUNT_BITS + 1));
         }
         __syncthreads();
     }
-    if (span || c.repetition != 1.0f || c.presence != 0.0f || c.frequency != 0.0f) {
+    if (span && path > 0) last = s_path[path - 1];
+    if (looks) {
         auto said = [&](int i) { return i < length ? history[i] : s_path[i - length]; };
-        for (int i = tid; i < all; i += CONTROL_THREADS) {
-            const uint32_t at = uint32_t(said(i)) - uint32_t(low);
-            if (at >= uint32_t(size)) continue;
+        auto take = [&](int i, int32_t token, int32_t previous) {
+            const uint32_t at = uint32_t(token) - uint32_t(low);
+            if (at >= uint32_t(size)) return;
             atomicAdd(&s_word[at], 1u);
-            if (span && i >= span) {
+            if (span && i >= span && previous == last) {
                 bool same = true;
-                for (int k = 1; k <= span && same; ++k) same = said(i - k) == said(all - k);
+                for (int k = 2; k <= span && same; ++k) same = said(i - k) == said(all - k);
                 if (same) atomicOr(&s_word[at], BANNED);
             }
-        }
+        };
+#pragma unroll
+        for (int k = 0; k < SOON; ++k)
+            if (k * CONTROL_THREADS + tid < length) take(k * CONTROL_THREADS + tid, soon[k], before[k]);
+        for (int i = SOON * CONTROL_THREADS + tid; i < length; i += CONTROL_THREADS) take(i, history[i], span ? history[i - 1] : -1);
+        for (int i = tid; i < path; i += CONTROL_THREADS)
+            take(length + i, s_path[i], i > 0 ? s_path[i - 1] : span && length > 0 ? history[length - 1] : -1);
     }
     __syncthreads();
-    const char* in = p.logits + int64_t(t) * p.stride * (TYPE == TYPE_F32 ? 4 : 2);
     char* out = p.out + int64_t(t) * p.out_stride * (OUT == TYPE_F32 ? 4 : 2);
     const float* bias = p.bias + int64_t(r) * p.bias_width;
-    const uint8_t* mask = nullptr;
-    if (p.masks) {
-        const int m = p.mask_rows ? p.mask_rows[t] : t;
-        if (uint32_t(m) < uint32_t(p.mask_count)) mask = reinterpret_cast<const uint8_t*>(p.masks + int64_t(m) * p.mask_stride) + low / 8;
-    }
-    for (int i = tid * EACH; i < size; i += CONTROL_THREADS * EACH) {
-        const uint32_t open = mask ? mask[i / 8] : 0xffu;
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k) {
+        const int i = (k * CONTROL_THREADS + tid) * EACH;
+        if (i >= size) break;
         uint32_t word[EACH], any = 0;
 #pragma unroll
         for (int e = 0; e < EACH; ++e) any |= word[e] = s_word[i + e];
-        if (p.in_place && !any && open == 0xffu) continue;
+        if (p.in_place && !any && open[k] == 0xffu) continue;
         if (i + EACH <= size) {
-            float v[EACH];
-            load8<TYPE>(in, low + i, v);
-            if (any || open != 0xffu) {
+            if (p.in_place) load8<TYPE>(in, low + i, v[k]);
+            if (any || open[k] != 0xffu) {
 #pragma unroll
-                for (int e = 0; e < EACH; ++e) v[e] = controlled(v[e], word[e], open >> e & 1u, c, bias);
+                for (int e = 0; e < EACH; ++e) v[k][e] = controlled(v[k][e], word[e], open[k] >> e & 1u, c, bias);
             }
-            store8<OUT>(out, low + i, v);
+            store8<OUT>(out, low + i, v[k]);
         } else {
 #pragma unroll
             for (int e = 0; e < EACH; ++e)
-                if (i + e < size) store1<OUT>(out, low + i + e, controlled(load1<TYPE>(in, low + i + e), word[e], open >> e & 1u, c, bias));
+                if (i + e < size) store1<OUT>(out, low + i + e, controlled(load1<TYPE>(in, low + i + e), word[e], open[k] >> e & 1u, c, bias));
         }
     }
 }
@@ -517,13 +620,17 @@ void launch_paged_tree(const TreeParams& p, hipStream_t s) {
 }
 
 void launch_paged_accept(const AcceptParams& p, hipStream_t s) {
+    if (p.rows <= WALKED) {
+        hipLaunchKernelGGL(accept_pages_kernel<true>, dim3(1), dim3(PAGES_THREADS), 0, s, p);
+        return;
+    }
     const int each = WAVE_THREADS / 64;
     hipLaunchKernelGGL(accept_walk_kernel, dim3(unsigned((p.rows + each - 1) / each)), dim3(WAVE_THREADS), 0, s, p);
-    hipLaunchKernelGGL(accept_pages_kernel, dim3(1), dim3(PAGES_THREADS), 0, s, p);
+    hipLaunchKernelGGL(accept_pages_kernel<false>, dim3(1), dim3(PAGES_THREADS), 0, s, p);
 }
 
 void launch_paged_move(const MoveParams& p, hipStream_t s) {
-    const int64_t items = int64_t(p.groups) * p.kv_heads * p.chunks;
+    const int64_t items = int64_t(p.groups) * p.kv_heads * p.chunks;  // (the caller's check: a launch holds them)
     hipLaunchKernelGGL(move_kernel, dim3(unsigned((items + 255) / 256), unsigned(p.layers), 2), dim3(256), 0, s, p);
 }
 

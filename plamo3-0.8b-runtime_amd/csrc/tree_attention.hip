@@ -32,10 +32,10 @@ constexpr int CUS = 256;
 
 template <int D, int SHARE>
 struct Shape {
-    static constexpr int KEYS = SHARE == 4 || (SHARE == 2 && D == 64) ? 64 : 32;  // of a tile
+    static constexpr int KEYS = SHARE == 4 ? 64 : 32;  // of a tile
     static constexpr int GROUPS = SHARE == 4 ? 1 : SHARE == 2 || D == 256 ? 2 : 4;
     static constexpr int WAVES = SHARE * GROUPS, THREADS = 64 * WAVES;
-    static constexpr int HELD = D == 256 || (D == 128 && SHARE == 1) ? 1 : 2;  // workgroups of a CU
+    static constexpr int HELD = D == 256 || (D == 128 && SHARE == 1) ? 1 : D == 64 && SHARE == 2 ? 3 : 2;  // workgroups of a CU
     static constexpr int OF_SIMD = HELD * WAVES > 4 ? HELD * WAVES / 4 : 1;
     static constexpr int ROW = 2 * D;                 // bytes of a key
     static constexpr int TILE = KEYS * ROW;           // of a tile's keys, or of its values
@@ -48,7 +48,7 @@ struct Shape {
     static constexpr int SPLIT = D / 8;               // four dims each of the 64 lanes' rows
 };
 static_assert(Shape<128, 4>::LDS == 65536 && Shape<128, 2>::LDS == 65536 && Shape<128, 1>::LDS == 131072 && Shape<256, 1>::LDS == 131072 &&
-              Shape<256, 2>::LDS == 131072 && Shape<256, 4>::LDS == 131072 && Shape<64, 1>::LDS == 65536 && Shape<64, 2>::LDS == 65536, "of 160 KB");
+              Shape<256, 2>::LDS == 131072 && Shape<256, 4>::LDS == 131072 && Shape<64, 1>::LDS == 65536 && Shape<64, 2>::LDS == 32768, "of 160 KB");
 
 // Key of row R of sixteen in LDS: a lane's loads are of neighbouring keys.
 template <int D>
@@ -903,10 +903,10 @@ int share_of(int rows, int tokens, int group) {
 }
 // Workgroups that the CUs hold at once.
 int target_of(int share, int kv_heads, int head_dim) {
-    return std::max(1, CUS * (head_dim == 256 || (head_dim == 128 && share == 1) ? 1 : 2) / kv_heads);
+    return std::max(1, CUS * (head_dim == 256 || (head_dim == 128 && share == 1) ? 1 : head_dim == 64 && share == 2 ? 3 : 2) / kv_heads);
 }
 int turn_of(int share, int head_dim) {
-    return (share == 4 || (share == 2 && head_dim == 64) ? 64 : 32) * (share == 4 ? 1 : share == 2 || head_dim == 256 ? 2 : 4);
+    return (share == 4 ? 64 : 32) * (share == 4 ? 1 : share == 2 || head_dim == 256 ? 2 : 4);
 }
 // (2^20 requests and 2^30 rows of queries are less than 2^24 workgroups: a launch holds them)
 int64_t tiles_of(const TreeAttnParams& p) { return std::min(p.rows, p.tokens) + int64_t(p.tokens) * p.group / (32 * p.share); }
