@@ -36,7 +36,7 @@ struct Shape {
     static constexpr int GROUPS = SHARE == 4 ? 1 : SHARE == 2 || D == 256 ? 2 : 4;
     static constexpr int WAVES = SHARE * GROUPS, THREADS = 64 * WAVES;
     static constexpr int HELD = D == 256 || (D == 128 && SHARE == 1) ? 1 : D == 64 && SHARE == 2 ? 3 : 2;  // workgroups of a CU
-    static constexpr int OF_SIMD = HELD * WAVES > 4 ? HELD * WAVES / 4 : 1;
+    static constexpr int OF_SIMD = HELD * WAVES <= 4 ? 1 : HELD * WAVES > 8 ? HELD * WAVES / 4 : 2;  // waves whose registers fit
     static constexpr int ROW = 2 * D;                 // bytes of a key
     static constexpr int TILE = KEYS * ROW;           // of a tile's keys, or of its values
     static constexpr int LDS = GROUPS * 2 * 2 * TILE; // two stages
@@ -83,7 +83,7 @@ struct Request {
     int first, count;  // new tokens
     int start, end;    // keys before them, keys in all
     int tiles;
-    int low, span;     // the first key that one of them sees, rounded down to 8, and the keys from it on
+    int low, span;     // the first key that one of them sees, rounded down to 16, and the keys from it on
 };
 template <int ROWS>  // of a tile
 __device__ __forceinline__ Request request(const TreeAttnParams& p, int r) {
@@ -97,7 +97,7 @@ __device__ __forceinline__ Request request(const TreeAttnParams& p, int r) {
     q.end = q.start >= 0 ? min(length, p.most) : 0;
     q.start = max(q.start, 0);
     q.tiles = (q.count * p.group + ROWS - 1) / ROWS;
-    q.low = p.window > 0 ? min(max(q.start - p.window + 1, 0), q.end) & ~7 : 0;
+    q.low = p.window > 0 ? min(max(q.start - p.window + 1, 0), q.end) & ~15 : 0;
     q.span = q.count > 0 ? q.end - q.low : 0;
     return q;
 }
@@ -299,6 +299,15 @@ __device__ __forceinline__ void load_to_lds(uint32_t lds, uint64_t at) {
                      : "s"(__builtin_amdgcn_readfirstlane(int(lds))), "v"(at)
                      : "m0", "memory");
 }
+// The same, each lane at its own offset from a wave's address.  (s_nop: the wait states between a vector instruction's write of
+// a scalar register, as where one comes back from a lane, and its use as an address.)
+__device__ __forceinline__ void load_to_lds(uint32_t lds, uint64_t at, uint32_t off) {
+    const uint64_t base = uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(at >> 32)))) << 32 | uint32_t(__builtin_amdgcn_readfirstlane(int(at)));
+    __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
+                     :
+                     : "s"(__builtin_amdgcn_readfirstlane(int(lds))), "v"(off), "s"(base)
+                     : "m0", "memory");
+}
 #pragma clang diagnostic pop
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
     return uint32_t(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)p));
@@ -423,7 +432,7 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
         first_key = p.window > 0 ? max(rq.start + token0 - p.window + 1, 0) : 0;
         end = min(rq.end, rq.start + token1 + 1);
     }
-    first_key = min(first_key, end) & ~7;
+    first_key = min(first_key, end) & ~15;
     int all_low = low, all_high = high;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -444,52 +453,81 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
     const uint64_t keys0 = reinterpret_cast<uint64_t>(p.keys) + kv * p.head_stride;
     const int64_t apart = p.values - p.keys;
     const int32_t* table = p.tables + int64_t(row) * p.width;
-    constexpr int LOOK = EVEN ? 1 : X::PIECES;
     const int first_row = 16 * X::OWN * part_wave;  // of a tile, that the wave loads
-    // pages of the lane's keys of a tile, on their way
+    // EVEN: the lane's keys of sixteen, PIECES of them, lie in one page, or with WAVEWISE all sixteen do, and their address is the
+    // wave's to find: a load is one vector instruction then, on a lane's part (its row, and its chunk, whose exclusive-or with
+    // the load's number is a constant; 16 slots of at most 2^25 bytes fit its 32 bits).  With four waves a tile arithmetic is
+    // what takes the time (16 requests of 2,000 to 9,000 keys, 78 rows of 256 each: 76 -> 64 us); with fewer memory does, and
+    // the loads would go out later (48 such requests, 8 heads of 64: 103 -> 123 us).
+    constexpr bool WAVEWISE = EVEN && SHARE == 4;
+    constexpr int LOOK = EVEN ? 1 : X::PIECES;
+    const int lane_chunk = lane % LANES;
+    const uint32_t lane_row = uint32_t(X::PIECES * group) * uint32_t(p.slot_stride);
+    const uint32_t lane_key = uint32_t(lane_chunk ^ key_swizzle<D>(group)) * 16;
+    const uint32_t lane_value = uint32_t(((lane_chunk >> 2) ^ value_swizzle<D>(group)) * 4 + (lane_chunk & 3)) * 16;
+    // pages of a tile's keys, on their way
     int entry[X::OWN][LOOK];
-    auto look_up = [&](int pos) {
+    auto look_up = [&](int pos) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < X::OWN; ++b)
 #pragma unroll
             for (int l = 0; l < LOOK; ++l) {
-                const int key = pos + first_row + 16 * b + X::PIECES * group + l;
+                const int key = pos + first_row + 16 * b + (WAVEWISE ? 0 : X::PIECES * group + l);
                 entry[b][l] = key < end ? table[divide(uint32_t(key), p.div)] : -1;
             }
     };
-    auto request_tile = [&](int pos, int stage) {
+    auto request_tile = [&](int pos, int stage) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < X::OWN; ++b) {
             const int key0 = pos + first_row + 16 * b;  // of the sixteen
-            uint64_t at[LOOK];
-            bool fine = key0 + 16 <= end;
-#pragma unroll
-            for (int l = 0; l < LOOK; ++l) {
-                const int key = key0 + X::PIECES * group + l, in_page = key - int(divide(uint32_t(key), p.div)) * p.page_size;
-                at[l] = keys0 + uint64_t(int64_t(entry[b][l]) * p.page_stride + int64_t(in_page) * p.slot_stride);
-                fine = fine && uint32_t(entry[b][l]) < uint32_t(p.pages);
-            }
             const uint32_t to = ring + uint32_t(stage) * (2 * X::TILE) + uint32_t(first_row + 16 * b) * X::ROW;
-            int own = lane;
-            __asm__ volatile("" : "+v"(own));  // (or the compiler would keep all offsets in registers)
-            const int chunk = own % LANES, own_group = own / LANES;
             uint32_t there = 0xffffu;
-            if (__all(fine)) {
-#pragma unroll
-                for (int l = 0; l < X::PIECES; ++l) {
-                    const int r = X::PIECE_KEYS * l + own_group;
-                    const uint64_t from = at[EVEN ? 0 : l] + (EVEN ? uint64_t(l * p.slot_stride) : 0);
-                    load_to_lds(to + uint32_t(l) * 1024, from + uint32_t((chunk ^ key_swizzle<D>(r)) * 16));
-                    load_to_lds(to + X::TILE + uint32_t(l) * 1024,
-                                from + uint64_t(apart) + uint32_t((((chunk >> 2) ^ value_swizzle<D>(r)) * 4 + (chunk & 3)) * 16));
+            bool all;
+            if constexpr (WAVEWISE) {
+                const int page = __builtin_amdgcn_readfirstlane(entry[b][0]);
+                all = key0 + 16 <= end && uint32_t(page) < uint32_t(p.pages);
+                if (all) {
+                    const int in_page = key0 - int(divide(uint32_t(key0), p.div)) * p.page_size;
+                    const uint64_t at = keys0 + uint64_t(page * p.page_stride + in_page * p.slot_stride);
+                    static_for<0, X::PIECES>([&](auto n) {
+                        constexpr int l = decltype(n)::value;
+                        const uint64_t row_at = at + uint64_t(l * p.slot_stride);
+                        load_to_lds(to + uint32_t(l) * 1024, row_at, (lane_key ^ uint32_t(key_swizzle<D>(X::PIECE_KEYS * l) * 16)) + lane_row);
+                        load_to_lds(to + X::TILE + uint32_t(l) * 1024, row_at + uint64_t(apart),
+                                    (lane_value ^ uint32_t(value_swizzle<D>(X::PIECE_KEYS * l) * 64)) + lane_row);
+                    });
                 }
-            } else {  // rows past the last key, or of no page, are zeros
+            } else {
+                bool fine = key0 + 16 <= end;
+                uint64_t at[LOOK];
+#pragma unroll
+                for (int l = 0; l < LOOK; ++l) {
+                    const int key = key0 + X::PIECES * group + l, in_page = key - int(divide(uint32_t(key), p.div)) * p.page_size;
+                    at[l] = keys0 + uint64_t(int64_t(entry[b][l]) * p.page_stride + int64_t(in_page) * p.slot_stride);
+                    fine = fine && uint32_t(entry[b][l]) < uint32_t(p.pages);
+                }
+                all = __all(fine);
+                if (all) {
+                    static_for<0, X::PIECES>([&](auto n) {
+                        constexpr int l = decltype(n)::value;
+                        const uint64_t from = at[EVEN ? 0 : l] + (EVEN ? uint64_t(l * p.slot_stride) : 0);
+                        load_to_lds(to + uint32_t(l) * 1024, from + (lane_key ^ uint32_t(key_swizzle<D>(X::PIECE_KEYS * l) * 16)));
+                        load_to_lds(to + X::TILE + uint32_t(l) * 1024,
+                                    from + uint64_t(apart) + (lane_value ^ uint32_t(value_swizzle<D>(X::PIECE_KEYS * l) * 64)));
+                    });
+                }
+            }
+            if (!all) {  // rows past the last key, or of no page, are zeros
                 there = 0;
+                int own = lane;
+                __asm__ volatile("" : "+v"(own));  // (or the compiler would keep all offsets in registers)
+                const int chunk = own % LANES, own_group = own / LANES;
 #pragma unroll
                 for (int l = 0; l < X::PIECES; ++l) {
-                    const int r = X::PIECE_KEYS * l + own_group;
-                    const bool ok = key0 + X::PIECES * own_group + l < end && uint32_t(entry[b][EVEN ? 0 : l]) < uint32_t(p.pages);
-                    const uint64_t from = at[EVEN ? 0 : l] + (EVEN ? uint64_t(l * p.slot_stride) : 0);
+                    const int key = key0 + X::PIECES * own_group + l, page = entry[b][EVEN ? 0 : l], r = X::PIECE_KEYS * l + own_group;
+                    const int in_page = key - int(divide(uint32_t(key), p.div)) * p.page_size;
+                    const uint64_t from = keys0 + uint64_t(int64_t(page) * p.page_stride + int64_t(in_page) * p.slot_stride);
+                    const bool ok = key < end && uint32_t(page) < uint32_t(p.pages);
                     const uint64_t zeros = reinterpret_cast<uint64_t>(&ZEROS);
                     load_to_lds(to + uint32_t(l) * 1024, ok ? from + uint32_t((chunk ^ key_swizzle<D>(r)) * 16) : zeros);
                     load_to_lds(to + X::TILE + uint32_t(l) * 1024,
@@ -507,7 +545,7 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
         uint32_t w[3];
     };
     Bits node_bits = {};
-    auto look_at_bits = [&](int pos) {
+    auto look_at_bits = [&](int pos) __attribute__((always_inline)) {
         const int from = max(pos - rq.start, 0) >> 5;
         if (p.ancestors && pos + X::KEYS > rq.start) {
 #pragma unroll
@@ -528,7 +566,7 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
     const int source_row = 4 * half + (lane >> 2 & 3);
     const uint32_t value_base = uint32_t(set * (2 * 2 * X::TILE) + X::TILE + source_row * X::ROW + value_swizzle<D>(source_row) * 64 +
                                          32 * (lane >> 4 & 1) + 8 * (lane & 3));
-    auto base_of = [&](uint32_t base, int stage) {
+    auto base_of = [&](uint32_t base, int stage) __attribute__((always_inline)) {
         uint32_t x = base + uint32_t(stage) * (2 * X::TILE);
         __asm__ volatile("" : "+v"(x));
         return x;
@@ -536,7 +574,7 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
     typedef short short4_t __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) short4_t* tr_ptr_t;
     // dims of d, keys of sixteen s
-    auto value_operand = [&](uint32_t base, int s, int d) {
+    auto value_operand = [&](uint32_t base, int s, int d) __attribute__((always_inline)) {
         const uint8_t* at = s_ring + (base ^ uint32_t(d * 64)) + 16 * s * X::ROW;
         const short4_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)at);
         const short4_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(at + 8 * X::ROW));
@@ -545,15 +583,16 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
         __builtin_memcpy(reinterpret_cast<char*>(&v) + 8, &x1, 8);
         return v;
     };
-    auto weight = [&](float x, float from) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, scale, -from)); };
+    auto weight = [&](float x, float from) __attribute__((always_inline)) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, scale, -from)); };
     constexpr int SIXTEENS = X::KEYS / 16;
     // Weights in two halves of the type (2^-16 off for BF16, 2^-22 for FP16) where the products wait for memory.  With four
     // waves a tile these and the vector arithmetic are what takes the time, and a third product and the split of the weights
-    // cost 535 us for 420 (two chunks of 999 tokens behind 28,000 and 30,720): they are rounded once there, each half a
-    // step off at most, which leaves the output 1.2 to 1.4 times as far from 64 bits as its own rounding does.
+    // are a quarter more of it (two chunks of 999 tokens 535 us for 420 when this was chosen): they are rounded once there, each
+    // half a step off at most, which leaves the output 1.2 to 1.4 times as far from 64 bits as its own rounding does.
     constexpr bool HALVES = SHARE < 4;
 
-    auto take = [&](int pos, int stage, uint64_t there, const Bits& of_nodes) {
+    bool odd = false;  // a tile that some tokens do not see whole holds values that are not finite
+    auto take = [&](int pos, int stage, uint64_t there, const Bits& of_nodes, auto with_care) __attribute__((always_inline)) {
         constexpr int PRODUCTS = X::BLOCKS * X::STEPS, AHEAD = 4;
         const uint32_t k_base = base_of(key_base, stage), v_base = base_of(value_base, stage);
         floatx16 s[X::BLOCKS];
@@ -571,8 +610,9 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
                 __builtin_amdgcn_sched_barrier(0);
             });
         }
-        uint32_t seen[X::BLOCKS];
-        bool clean = true;
+        uint32_t seen[X::BLOCKS];  // bit i: score i is one
+#pragma unroll
+        for (int b = 0; b < X::BLOCKS; ++b) seen[b] = 0xffffu;
         constexpr uint64_t ALL = X::KEYS == 64 ? ~0ull : 0xffffffffull;
         const bool whole = pos >= all_low && pos + X::KEYS <= all_high && there == ALL;
         if (!whole) {
@@ -597,7 +637,7 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
                     s[b][i] = yes ? s[b][i] : NEG_INF;
                 }
             }
-            // Are all values finite?  An exponent of ones and a one more carry into the sign's bit.
+            // are all values finite?  An exponent of ones and a one more carry into the sign's bit
             constexpr uint32_t EXPONENT = TYPE == TYPE_BF16 ? 0x7f807f80u : 0x7c007c00u, ONE = TYPE == TYPE_BF16 ? 0x00800080u : 0x04000400u;
             uint32_t carry = 0;
 #pragma unroll 4
@@ -605,7 +645,7 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
                 const uint4 w = *reinterpret_cast<const uint4*>(s_ring + (set * 2 + stage) * (2 * X::TILE) + X::TILE + c);
                 carry |= ((w.x & EXPONENT) + ONE) | ((w.y & EXPONENT) + ONE) | ((w.z & EXPONENT) + ONE) | ((w.w & EXPONENT) + ONE);
             }
-            clean = !__any(carry & 0x80008000u);
+            odd = odd || __any(carry & 0x80008000u);
         }
         float top = s[0][0];
 #pragma unroll
@@ -625,7 +665,7 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= shrink;
         }
-        if (clean) {
+        if constexpr (!decltype(with_care)::value) {
             constexpr int PAIRS = X::DIMS / 2;
             uint32_t high_w[2][4], low_w[2][HALVES ? 4 : 1];
             uint4 v[2][2];
@@ -665,15 +705,12 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
             return;
         }
         // Values that are not finite reach those tokens alone that see their key: they are left out of the products (where a
-        // weight of zero would make NaN of them) and added one by one.  (`base`: or the compiler would take the weights out of
-        // both branches, and from beside the products.)
-        float base = from;
-        __asm__ volatile("" : "+v"(base));
+        // weight of zero would make NaN of them) and added one by one.
 #pragma unroll
         for (int b = 0; b < X::BLOCKS; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[b][i] = weight(s[b][i], base);
+                s[b][i] = weight(s[b][i], from);
                 sum += s[b][i];
             }
         int half = lane >> 5;
@@ -730,28 +767,41 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
 
     // ---- the part's tiles, the next one's loads on their way
     const int turns = begin < end ? (end - begin + TURN - 1) / TURN : 0;
-    int pos = begin + set * X::KEYS;
-    if (turns > 0) {
-        look_up(pos);
-        request_tile(pos, 0);
-        look_up(pos + TURN);
-        look_at_bits(pos);
-    }
-    for (int turn = 0; turn < turns; ++turn, pos += TURN) {
-        __asm__ volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0070);  // the wave's loads, and its LDS operations of the tile before
-        if (SHARE > 1) __builtin_amdgcn_s_barrier();
-        __asm__ volatile("" ::: "memory");
-        const int stage = turn & 1;
-        uint64_t there = X::KEYS == 64 ? *reinterpret_cast<const uint64_t*>(s_there[set][stage]) : *reinterpret_cast<const uint32_t*>(s_there[set][stage]);
-        there = uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(there >> 32)))) << 32 | uint32_t(__builtin_amdgcn_readfirstlane(int(there)));
-        const Bits of_nodes = node_bits;
-        if (turn + 1 < turns) {
-            request_tile(pos + TURN, stage ^ 1);
-            look_up(pos + 2 * TURN);
-            look_at_bits(pos + TURN);
+    auto run = [&](auto with_care) __attribute__((always_inline)) {
+        int pos = begin + set * X::KEYS;
+        if (turns > 0) {
+            look_up(pos);
+            request_tile(pos, 0);
+            look_up(pos + TURN);
+            look_at_bits(pos);
         }
-        if (pos < end) take(pos, stage, there, of_nodes);
+        for (int turn = 0; turn < turns; ++turn, pos += TURN) {
+            __asm__ volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0x0070);  // the wave's loads, and its LDS operations of the tile before
+            if (SHARE > 1) __builtin_amdgcn_s_barrier();
+            __asm__ volatile("" ::: "memory");
+            const int stage = turn & 1;
+            uint64_t there = X::KEYS == 64 ? *reinterpret_cast<const uint64_t*>(s_there[set][stage]) : *reinterpret_cast<const uint32_t*>(s_there[set][stage]);
+            there = uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(there >> 32)))) << 32 | uint32_t(__builtin_amdgcn_readfirstlane(int(there)));
+            const Bits of_nodes = node_bits;
+            if (turn + 1 < turns) {
+                request_tile(pos + TURN, stage ^ 1);
+                look_up(pos + 2 * TURN);
+                look_at_bits(pos + TURN);
+            }
+            if (pos < end) take(pos, stage, there, of_nodes, with_care);
+        }
+    };
+    run(std::false_type{});
+    // once more where values need care: in the same loop their arithmetic cost every tile 64 moves of registers (two chunks of
+    // 999 tokens 412 us, so 371)
+    if (__syncthreads_or(odd)) {
+        most = NEG_INF;
+        sum = 0.f;
+#pragma unroll
+        for (int d = 0; d < X::DIMS; ++d) o[d] = floatx16{};
+        run(std::true_type{});
+        __syncthreads();
     }
     sum += xor_lane<32>(sum);
 
@@ -895,8 +945,9 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void tree_join_kernel(TreeAttnPara
 // ------------------------------------------------------------------------------------ launches
 // Waves that share a tile, by the rows of queries that a request has on the average: few rows read the keys at the rate of
 // memory, and more rows a tile read them fewer times; many are bound by arithmetic.  64 requests of 2,000 to 4,000 keys and 16
-// heads of 128 on one, 15 / 30 / 38 / 60 / 78 rows each: 27 / 31 / 35 / 49 / 56 us with one wave, 30 / 31 / 32 / 36 / 39 with two,
-// 37 / 38 / 39 / 40 / 40 with four.  (Heads of 64 and 256 cross over at the same numbers.)
+// heads of 128 on one, 15 / 22 / 29 / 36 / 58 / 73 rows each: 27 / 27 / 30 / 34 / 48 / 50 us with one wave, 29 / 30 / 31 / 31 / 35 / 38
+// with two, 36 / 36 / 37 / 37 / 39 / 39 with four.  (Heads of 256 cross over there too, 78 rows 94 / 67 / 64 us; heads of 64 later
+// between two and four: 38 rows 170 / 106 / 150.)
 int share_of(int rows, int tokens, int group) {
     const int64_t each = int64_t(tokens) * group / rows;
     return each <= 24 ? 1 : each <= 72 ? 2 : 4;
@@ -921,7 +972,7 @@ void run_shape(const TreeAttnParams& p, hipStream_t s) {
     typedef Shape<D, SHARE> X;
     if (p.listed) hipLaunchKernelGGL((tree_division_kernel<32 * SHARE>), dim3(1), dim3(DIVIDE_THREADS), 0, s, p);
     const dim3 grid(unsigned(items_of(p)), unsigned(p.kv_heads));
-    if (p.page_size % X::PIECES == 0) hipLaunchKernelGGL((tree_attention_kernel<TYPE, D, SHARE, true>), grid, dim3(X::THREADS), 0, s, p);
+    if (p.page_size % (SHARE == 4 ? 16 : X::PIECES) == 0) hipLaunchKernelGGL((tree_attention_kernel<TYPE, D, SHARE, true>), grid, dim3(X::THREADS), 0, s, p);
     else hipLaunchKernelGGL((tree_attention_kernel<TYPE, D, SHARE, false>), grid, dim3(X::THREADS), 0, s, p);
     if (p.joins)
         hipLaunchKernelGGL((tree_join_kernel<TYPE, D, SHARE>), dim3(unsigned(std::min<int64_t>(tiles_of(p), p.target)), unsigned(p.kv_heads), 4 * SHARE),

@@ -88,6 +88,19 @@ def test_strides(layout):
     Case("fp16", 8, 2, 64, 16, [100, 7], [6, 11], True, layout=layout).check()
 
 
+@pytest.mark.parametrize("count", [2, 20, 40])
+def test_slots_far_apart(count):
+    """Pages side by side and a page's slots 2^24 elements apart, the most that a cache may have."""
+    case = Case("bf16", 4, 1, 128, 16, [50, 3], [count, count], False)
+    far = []
+    for c in (case.keys, case.values):
+        room = torch.empty(15 * (1 << 24) + c.shape[0] * 128, dtype=c.dtype, device="cuda")
+        far.append(room.as_strided(c.shape, (128, 1 << 24, 128, 1)))
+        far[-1].copy_(c)
+    case.keys, case.values = far
+    case.check()
+
+
 @pytest.mark.parametrize("heads,kv,dim", [(16, 1, 128), (4, 1, 64), (8, 8, 64), (2, 1, 256)])
 @pytest.mark.parametrize("count", [1, 2, 4, 8, 17, 33, 64])
 def test_numbers_of_nodes(count, heads, kv, dim):
