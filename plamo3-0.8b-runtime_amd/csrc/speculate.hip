@@ -76,8 +76,8 @@ __global__ __launch_bounds__(WAVE_THREADS) void tree_wave_kernel(TreeParams p) {
     pad_tokens(p, blockIdx.x, gridDim.x, WAVE_THREADS);
     if (r >= p.rows) return;
     const Span s = new_tokens(p.offsets, r, p.tokens);
-    const int start = p.lengths[r] - s.count;
-    if (s.count > 32 * p.words || start < 0) return no_tree(p, s, lane, 64);
+    const int length = p.lengths[r], start = length - s.count;
+    if (s.count > 32 * p.words || length < s.count) return no_tree(p, s, lane, 64);
     int up = lane < s.count ? p.parents[s.first + lane] : -1;
     up = up >= 0 && up < lane ? up : -1;
     uint32_t low, high;
@@ -104,8 +104,8 @@ __global__ __launch_bounds__(32 * W) void tree_block_kernel(TreeParams p) {
     const int i = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     pad_tokens(p, blockIdx.x, gridDim.x, NODES);
     const Span s = new_tokens(p.offsets, blockIdx.x, p.tokens);
-    const int start = p.lengths[blockIdx.x] - s.count;
-    if (s.count > 32 * p.words || start < 0) return no_tree(p, s, i, NODES);
+    const int length = p.lengths[blockIdx.x], start = length - s.count;
+    if (s.count > 32 * p.words || length < s.count) return no_tree(p, s, i, NODES);
     int up = i < s.count ? p.parents[s.first + i] : -1;
     up = up >= 0 && up < i ? up : -1;
     uint32_t bits[W], low, high;

@@ -93,9 +93,9 @@ __device__ __forceinline__ Request request(const TreeAttnParams& p, int r) {
     const bool fine = q.first >= 0 && past >= q.first && past <= p.tokens;
     q.count = fine ? past - q.first : 0;
     q.first = fine ? q.first : 0;
-    q.start = length - q.count;
-    q.end = q.start >= 0 ? min(length, p.most) : 0;
-    q.start = max(q.start, 0);
+    const bool held = length >= q.count;  // (the difference of others may wrap)
+    q.start = held ? length - q.count : 0;
+    q.end = held ? min(length, p.most) : 0;
     q.tiles = (q.count * p.group + ROWS - 1) / ROWS;
     q.low = p.window > 0 ? min(max(q.start - p.window + 1, 0), q.end) & ~15 : 0;
     q.span = q.count > 0 ? q.end - q.low : 0;

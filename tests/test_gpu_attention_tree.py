@@ -185,6 +185,33 @@ def test_lengths_that_do_not_hold_the_nodes():
     case.check()
 
 
+@pytest.mark.parametrize("window", [0, 7])
+@pytest.mark.parametrize("chain", [False, True])
+@pytest.mark.parametrize("length", [-(1 << 31), -(1 << 31) + 1, -(1 << 31) + 2, -17, -1, 0, 2])
+def test_lengths_far_below_the_number_of_nodes(length, chain, window):
+    case = Case("bf16", 8, 2, 64, 16, [40, 20], [3, 3], chain, window=window)
+    case.lengths[0] = length
+    out, lse = case.run()
+    assert torch.all(out[:3] == 0) and torch.all(lse[:3] == -math.inf)
+    case.lengths[0] = 43
+    want, e = case.run()
+    assert torch.equal(out[3:6], want[3:6]) and torch.equal(lse[3:6], e[3:6])
+
+
+@pytest.mark.parametrize("full", [False, True])
+@pytest.mark.parametrize("heads,count", [(2, 3), (8, 3), (16, 9)])
+def test_lengths_past_the_tables(heads, count, full):
+    """All tokens see all keys of the table's pages; entries of the last column are no pages.  (Where the last page is not full
+    they see what lies behind, which is NaN here.)"""
+    case = Case("bf16", heads, 1, 64, 16, [80 - count if full else 70], [count], True)
+    case.lengths[0] = case.tables.shape[1] * 16 + count
+    out, lse = case.run()
+    case.lengths[0] = (1 << 31) - 1
+    got, e = case.run()
+    assert torch.equal(out.view(torch.int16), got.view(torch.int16)) and torch.equal(lse.view(torch.int32), e.view(torch.int32))
+    assert torch.isfinite(lse[:count]).all() if full else torch.isnan(lse[:count]).all()
+
+
 @pytest.mark.parametrize("odd", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("kind,dim", [("bf16", 128), ("fp16", 64), ("bf16", 256)])
 @pytest.mark.parametrize("chain", [False, True])

@@ -48,6 +48,11 @@ def test_too_many_nodes_and_short_lengths(words):
     check([3, n + 1, 4, 5, 200 + n], words, lengths=[10, 5000, 3, 5, 5000])
 
 
+@pytest.mark.parametrize("words", [1, 2, 6])
+def test_extreme_lengths(words):
+    check([3, 4, 2, 1], words, lengths=[-2 ** 31, -2 ** 31 + 3, 2 ** 31 - 1, 1])
+
+
 @pytest.mark.parametrize("rows", [1, 4, 5, 1000])
 def test_many_requests(rows):
     check([(r * 7) % 20 for r in range(rows)], 1, seed=rows, pad=1000)
