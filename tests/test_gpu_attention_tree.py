@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from paged_common import TYPES, describe, half_step, make_cache, make_tables
-from speculate_common import attend_tree, attend_tree64, put, random_parents, tree64
+from speculate_common import attend_tree, attend_tree64, lib, put, random_parents, tree64
 
 pytestmark = pytest.mark.gpu
 
@@ -266,3 +266,76 @@ def test_in_place():
                 positions=put(case.positions), ancestors=put(case.ancestors))
     torch.cuda.synchronize()
     assert torch.equal(q[:11], want[:11]) and torch.equal(q[11:], case.q[11:])
+
+
+def test_two_streams():
+    """Calls that run side by side, each with its own workspace, on streams that are not the current one."""
+    cases = [Case("bf16", 16, 1, 128, 16, [3000, 40, 333], [8, 3, 24], False), Case("fp16", 8, 2, 64, 16, [2000, 700], [60, 9], True)]
+    want = [c.run() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    sizes = [lib().plamo_kernel_attention_paged_tree_workspace(len(c.lengths), c.tokens, c.heads, c.keys.shape[2], c.keys.shape[3]) for c in cases]
+    rooms = [torch.full((n,), 0xFF, dtype=torch.uint8, device="cuda") for n in sizes]
+    given = []
+    for c in cases:
+        tree = {} if c.ancestors is None else {"positions": put(c.positions), "ancestors": put(c.ancestors)}
+        out = torch.full((c.tokens, c.q.shape[1]), 7.0, dtype=TYPES[c.kind], device="cuda")
+        given.append((describe(c.keys, c.values, c.kind), c.q, c.heads, put(c.tables), put(c.lengths), put(c.offsets), out,
+                      torch.full((c.tokens, c.heads), 7.0, device="cuda"), tree))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, c, g, room in zip(streams, cases, given, rooms):
+            with torch.cuda.stream(s):
+                attend_tree(*g[:-1], scale=c.scale, window=c.window, workspace=room, **g[-1])
+    torch.cuda.synchronize()
+    for g, (out, lse) in zip(given, want):
+        assert torch.equal(g[6], out) and torch.equal(g[7], lse)
+
+
+@pytest.mark.parametrize("rows", [4, 1500])
+def test_on_a_graph(rows):
+    """Lengths, tables and trees that change between replays; eager calls of the same workspace before each."""
+    cases = [Case("bf16", 8, 1, 64, 16, [(r * 37 + 900 * s) % 1100 for r in range(rows)], [(r + s) % 4 for r in range(rows)], False, seed=s)
+             for s in range(2)]
+    width, tokens = max(c.tables.shape[1] for c in cases), cases[0].tokens
+    assert cases[1].tokens == tokens
+    pages = max(c.keys.shape[0] for c in cases)
+    keys, values = make_cache("bf16", pages, 16, 1, 64, "token")
+    tables, lengths, offsets = (torch.zeros(n, dtype=torch.int32, device="cuda") for n in ((rows, width), rows, rows + 1))
+    positions, ancestors = torch.zeros(tokens, dtype=torch.int32, device="cuda"), torch.zeros(tokens, 1, dtype=torch.int32, device="cuda")
+    q, out = (torch.zeros(tokens, 8 * 64, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    lse = torch.zeros(tokens, 8, device="cuda")
+    room = torch.full((lib().plamo_kernel_attention_paged_tree_workspace(rows, tokens, 8, 1, 64),), 0xFF, dtype=torch.uint8, device="cuda")
+
+    def launch():
+        attend_tree(describe(keys, values, "bf16"), q, 8, tables, lengths, offsets, out, lse, positions, ancestors, workspace=room)
+
+    def fill(c):
+        for to, of in ((keys, c.keys), (values, c.values), (tables[:, :c.tables.shape[1]], put(c.tables)), (lengths, put(c.lengths)),
+                       (offsets, put(c.offsets)), (positions, put(c.positions)), (ancestors, put(c.ancestors)), (q, c.q)):
+            to[:of.shape[0]].copy_(of)
+        out.fill_(7.0)
+        lse.fill_(7.0)
+
+    fill(cases[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        launch()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        launch()
+    for turn in range(5):
+        c = cases[turn % 2]
+        fill(c)
+        launch()
+        torch.cuda.synchronize()
+        want, e = out.clone(), lse.clone()
+        room.fill_(0xFF)
+        out.fill_(7.0)
+        lse.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, e)
+        alone, e = c.run()  # (as many tokens: the same division of the work)
+        assert torch.equal(out, alone) and torch.equal(lse, e)
