@@ -28,6 +28,13 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 //   O^T += V^T P^T  V read from LDS by transposing reads.
 // Pages go straight into LDS, each lane from its own address: any page size and any strides.  Where a lane's keys
 // of a load are known to lie in one page (EVEN) it looks that page up once.
+// What bounds it, with what it took: arithmetic for chunks of prompts (of 999 and 333 tokens, 16 heads of 128, behind 28,000 and
+// 30,720 keys: 317 GFLOP in 367 us, 860 TFLOP/s; softmax and products of a wave take turns, two workgroups a CU fill in);
+// memory for a few nodes with a window (48 requests of up to 13 nodes, 32 heads of 64 on 8, 2,048 keys: 171 MB in 55 us); one
+// request's 343 keys the latency of its loads (9 us, then 3 to join); and many trees each a part (64 of up to 24 nodes behind 33
+// to 8,192 keys, 16 heads of 128 on one: 40 us for 53 MB) all of these: some 6 to find a part and load its first tile, five
+// more tiles of 3.5, and the parts' results, written and read once more, with a launch of 8.  (One workgroup of eight waves a CU,
+// of two sets, halves those results and took 46 for 42, and the chunks 537.)
 constexpr int CUS = 256;
 
 template <int D, int SHARE>
@@ -587,7 +594,7 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
     constexpr int SIXTEENS = X::KEYS / 16;
     // Weights in two halves of the type (2^-16 off for BF16, 2^-22 for FP16) where the products wait for memory.  With four
     // waves a tile these and the vector arithmetic are what takes the time, and a third product and the split of the weights
-    // are a quarter more of it (two chunks of 999 tokens 535 us for 420 when this was chosen): they are rounded once there, each
+    // are a quarter more of it (chunks of 999 and 333 tokens 535 us for 420 when this was chosen): they are rounded once there, each
     // half a step off at most, which leaves the output 1.2 to 1.4 times as far from 64 bits as its own rounding does.
     constexpr bool HALVES = SHARE < 4;
 
@@ -793,8 +800,8 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
         }
     };
     run(std::false_type{});
-    // once more where values need care: in the same loop their arithmetic cost every tile 64 moves of registers (two chunks of
-    // 999 tokens 412 us, so 371)
+    // once more where values need care: in the same loop their arithmetic cost every tile 64 moves of registers (chunks of
+    // 999 and 333 tokens 412 us, so 371)
     if (__syncthreads_or(odd)) {
         most = NEG_INF;
         sum = 0.f;
@@ -872,7 +879,8 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
 
 // ------------------------------------------------------------------------------------ parts joined
 // 32 rows of a tile and a quarter of their dims, in a fixed order: a workgroup's waves take every eighth part, and are
-// joined in LDS.  Pieces lie as the attention's lanes held them.
+// joined in LDS.  Pieces lie as the attention's lanes held them.  Latency-bound: a part's maximum and results, some of each on
+// their way at once, then LDS (509 parts of 128 rows of 128 8 us, 33 MB; one request's three 3 us).
 constexpr int JOIN_WAVES = 8;
 template <int TYPE, int D, int SHARE>
 __global__ __launch_bounds__(64 * JOIN_WAVES) void tree_join_kernel(TreeAttnParams p) {
@@ -1018,7 +1026,12 @@ void tree_attn_bind(TreeAttnParams& p, void* workspace, int head_dim) {
     p.by_group = divider(uint32_t(p.group));
     p.least = turn_of(p.share, head_dim);
     p.joins = p.most > p.least;
-    p.run = int(std::min<int64_t>(16, std::max<int64_t>(1, int64_t(p.tokens) * p.group / p.rows / (32 * p.share))));
+    // Neighbouring workgroups are tiles of the same keys: an XCD takes as many as a request has, as a power of two, so that the
+    // workgroups that the XCDs hold at once stay as many on each (64 requests of two tiles or so 41.9 -> 40.1 us, of three 77 -> 76;
+    // by runs of three 64 requests of one tile took 39 us for 27).
+    const int64_t tiles = (int64_t(p.tokens) * p.group / p.rows + 32 * p.share - 1) / (32 * p.share);
+    p.run = 1;
+    while (p.run < tiles && p.run < 16 && p.run * 16 <= p.target) p.run *= 2;
     p.listed = p.rows > FOUND_ROWS;
     const Layout l = layout(p.rows, p.share, p.target, p.kv_heads, head_dim);
     char* at = static_cast<char*>(workspace);
