@@ -774,6 +774,10 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
 
     // ---- the part's tiles, the next one's loads on their way
     const int turns = begin < end ? (end - begin + TURN - 1) / TURN : 0;
+    // a wave that has no rows only loads (64 trees of up to 24 nodes behind 33 to 8,192 keys 39.6 -> 38.9 us,
+    // 64 requests of 73 rows behind 2,000 to 4,000 39.0 -> 36.0)
+    const bool live = tile * ROWS + part_wave * 32 < rows;
+    const int taken = live ? end : 0;
     auto run = [&](auto with_care) __attribute__((always_inline)) {
         int pos = begin + set * X::KEYS;
         if (turns > 0) {
@@ -796,7 +800,7 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
                 look_up(pos + 2 * TURN);
                 look_at_bits(pos + TURN);
             }
-            if (pos < end) take(pos, stage, there, of_nodes, with_care);
+            if (pos < taken) take(pos, stage, there, of_nodes, with_care);
         }
     };
     run(std::false_type{});
@@ -861,8 +865,9 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
         const int64_t at = (int64_t(slot) * p.kv_heads + kv) * SHARE + part_wave;
         float4* to = reinterpret_cast<float4*>(p.part_o) + (at * X::SPLIT + set * EACH) * 64 + lane;
 #pragma unroll
-        for (int e = 0; e < EACH; ++e) to[e * 64] = mine[e];
-        if (set == 0 && half == 0) p.part_ml[at * 32 + col] = make_float2(top, total);
+        for (int e = 0; e < EACH; ++e)
+            if (live) to[e * 64] = mine[e];
+        if (live && set == 0 && half == 0) p.part_ml[at * 32 + col] = make_float2(top, total);
         return;
     }
     if (own_row >= rows) return;
@@ -953,9 +958,9 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void tree_join_kernel(TreeAttnPara
 // ------------------------------------------------------------------------------------ launches
 // Waves that share a tile, by the rows of queries that a request has on the average: few rows read the keys at the rate of
 // memory, and more rows a tile read them fewer times; many are bound by arithmetic.  64 requests of 2,000 to 4,000 keys and 16
-// heads of 128 on one, 15 / 22 / 29 / 36 / 58 / 73 rows each: 27 / 27 / 30 / 34 / 48 / 50 us with one wave, 29 / 30 / 31 / 31 / 35 / 38
-// with two, 36 / 36 / 37 / 37 / 39 / 39 with four.  (Heads of 256 cross over there too, 78 rows 94 / 67 / 64 us; heads of 64 later
-// between two and four: 38 rows 170 / 106 / 150.)
+// heads of 128 on one, 15 / 22 / 29 / 36 / 58 / 73 rows each: 27 / 27 / 31 / 32 / 45 / 51 us with one wave, 27 / 27 / 29 / 30 / 34 / 35
+// with two, 28 / 28 / 30 / 31 / 34 / 36 with four.  16 of 2,000 to 9,000 keys, 8 heads of 256 on 2, 18 / 39 / 78 rows: 47 / 62 / 98,
+// 49 / 52 / 67 and 57 / 60 / 64.  (Heads of 64 cross over later between two and four: 38 rows 164 / 105 / 146.)
 int share_of(int rows, int tokens, int group) {
     const int64_t each = int64_t(tokens) * group / rows;
     return each <= 24 ? 1 : each <= 72 ? 2 : 4;
@@ -1027,7 +1032,7 @@ void tree_attn_bind(TreeAttnParams& p, void* workspace, int head_dim) {
     p.least = turn_of(p.share, head_dim);
     p.joins = p.most > p.least;
     // Neighbouring workgroups are tiles of the same keys: an XCD takes as many as a request has, as a power of two, so that the
-    // workgroups that the XCDs hold at once stay as many on each (64 requests of two tiles or so 41.9 -> 40.1 us, of three 77 -> 76;
+    // workgroups that the XCDs hold at once stay as many on each (64 requests of two tiles or so 41.9 -> 40.1 us, of three 77.1 -> 75.6;
     // by runs of three 64 requests of one tile took 39 us for 27).
     const int64_t tiles = (int64_t(p.tokens) * p.group / p.rows + 32 * p.share - 1) / (32 * p.share);
     p.run = 1;
