@@ -592,11 +592,9 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
     };
     auto weight = [&](float x, float from) __attribute__((always_inline)) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, scale, -from)); };
     constexpr int SIXTEENS = X::KEYS / 16;
-    // Weights in two halves of the type (2^-16 off for BF16, 2^-22 for FP16) where the products wait for memory.  With four
-    // waves a tile these and the vector arithmetic are what takes the time, and a third product and the split of the weights
-    // are a quarter more of it (chunks of 999 and 333 tokens 535 us for 420 when this was chosen): they are rounded once there, each
-    // half a step off at most, which leaves the output 1.2 to 1.4 times as far from 64 bits as its own rounding does.
-    constexpr bool HALVES = SHARE < 4;
+    // Weights in two halves of the type (2^-16 off for BF16, 2^-22 for FP16), a product for each.  Rounded once they would be half
+    // a step off each, as large an error as the output's own rounding (outputs 1.2 to 1.4 times as far from 64 bits), for a third fewer products
+    // (chunks of 999 and 333 tokens 380 us for 492, 64 trees of up to 24 nodes 40 for 44).
 
     bool odd = false;  // a tile that some tokens do not see whole holds values that are not finite
     auto take = [&](int pos, int stage, uint64_t there, const Bits& of_nodes, auto with_care) __attribute__((always_inline)) {
@@ -674,7 +672,7 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
         }
         if constexpr (!decltype(with_care)::value) {
             constexpr int PAIRS = X::DIMS / 2;
-            uint32_t high_w[2][4], low_w[2][HALVES ? 4 : 1];
+            uint32_t high_w[2][4], low_w[2][4];
             uint4 v[2][2];
             v[0][0] = value_operand(v_base, 0, 0);
             v[0][1] = value_operand(v_base, 0, 1);
@@ -685,10 +683,9 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
                 if constexpr (u > 0) {
                     constexpr int g = (u - 1) & 1;
                     const uint4 ph = make_uint4(high_w[g][0], high_w[g][1], high_w[g][2], high_w[g][3]);
-                    uint4 pl = ph;
-                    if constexpr (HALVES) pl = make_uint4(low_w[g][0], low_w[g][1], low_w[g][2], low_w[g][3]);
-                    // products of the pairs of d: high, high (and low, low)
-                    constexpr int OF_PAIR = HALVES ? 4 : 2, ALL_OF = PAIRS * OF_PAIR;
+                    const uint4 pl = make_uint4(low_w[g][0], low_w[g][1], low_w[g][2], low_w[g][3]);
+                    // products of the pairs of d: high, high, low, low
+                    constexpr int OF_PAIR = 4, ALL_OF = PAIRS * OF_PAIR;
                     static_for<k * ALL_OF / 4, (k + 1) * ALL_OF / 4>([&](auto m) {
                         constexpr int pair = decltype(m)::value / OF_PAIR, j = decltype(m)::value % OF_PAIR, turn = ((u - 1) * PAIRS + pair) & 1;
                         if constexpr (j == 0 && (u < SIXTEENS || pair + 1 < PAIRS)) {  // the next pair's operands
@@ -704,8 +701,7 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
                     const float x = weight(s[b][i], from), y = weight(s[b][i + 1], from);
                     sum += x;
                     sum += y;
-                    if constexpr (HALVES) split<TYPE>(x, y, high_w[u & 1][k], low_w[u & 1][k]);
-                    else high_w[u & 1][k] = pack16<TYPE>(x, y);
+                    split<TYPE>(x, y, high_w[u & 1][k], low_w[u & 1][k]);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             });
@@ -766,7 +762,7 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
                 uint4 v = value_operand(v_base, u, d);
                 v = make_uint4(finite_or_zero<TYPE>(v.x), finite_or_zero<TYPE>(v.y), finite_or_zero<TYPE>(v.z), finite_or_zero<TYPE>(v.w));
                 o[d] = mfma32<TYPE>(v, ph, o[d]);
-                if constexpr (HALVES) o[d] = mfma32<TYPE>(v, pl, o[d]);
+                o[d] = mfma32<TYPE>(v, pl, o[d]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
