@@ -474,8 +474,9 @@ int plamo_kernel_sample(uint64_t logits, int32_t type, int64_t stride, int32_t n
  * plamo_kernel_logit_controls and plamo_kernel_sample draw a token at every node, plamo_kernel_paged_accept keeps the path
  * that these agree with, and plamo_kernel_paged_move puts its keys and values side by side in every layer.  Request r's
  * new tokens, its nodes, are offsets[r] .. offsets[r + 1] - 1 of the step, `offsets` ascending numbers of 0 .. tokens
- * (a request whose offsets are not has no nodes); lengths[r] counts them.  As the paged calls, these launch on `stream` and
- * its device, allocate nothing, keep nothing and can be captured; what device arrays hold leads nowhere outside. */
+ * (a request whose two are not has no nodes; where requests overlap, offsets descending in between, what a step gives for
+ * its tokens is undefined); lengths[r] counts them.  As the paged calls, these launch on `stream` and its device, allocate
+ * nothing, keep nothing and can be captured; what device arrays hold leads nowhere outside. */
 
 /* Positions and ancestors of the nodes: parents[t] is the index in its request of node t's parent, a node before it (any
  * other number: none, the node follows the cached tokens).  positions[t] = lengths[r] - nodes + the number of ancestors.

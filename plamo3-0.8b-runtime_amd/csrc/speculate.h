@@ -117,6 +117,7 @@ struct TreeAttnParams {
     int target;               // parts that all tiles' keys are divided into
     int least;                // fewest keys of a part, but for a tile's last
     int run;                  // neighbouring parts that are put on one XCD
+    int items;                // parts that a launch takes, for each KV head: all of requests that do not overlap
     bool joins;               // whether a tile can have several parts
     bool listed;              // rows' divisions are found by a launch before
     int* joined;              // [1] tiles of several parts

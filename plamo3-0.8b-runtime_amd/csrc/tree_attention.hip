@@ -131,7 +131,11 @@ __device__ __forceinline__ Sums scan(Sums v) { return {wave_scan(v.items), wave_
 __device__ __forceinline__ Sums at_lane(Sums v, int l) {
     return {__builtin_amdgcn_readlane(v.items, l), __builtin_amdgcn_readlane(v.slots, l), __builtin_amdgcn_readlane(v.joined, l)};
 }
-__device__ __forceinline__ Sums operator+(Sums a, Sums b) { return {a.items + b.items, a.slots + b.slots, a.joined + b.joined}; }
+// Requests overlap where offsets descend in between, and their tiles, up to 2^23 each, may then be any number of times as many as a
+// launch takes: sums of items end at MOST_ITEMS, past all that run, so that none wraps (64 requests' are less than 2^30, as are 64
+// sums that end there) and they ascend.  Slots and joined tiles come from the keys' division and stay within its bounds.
+constexpr int MOST_ITEMS = 1 << 24;
+__device__ __forceinline__ Sums operator+(Sums a, Sums b) { return {min(a.items + b.items, MOST_ITEMS), a.slots + b.slots, a.joined + b.joined}; }
 __device__ __forceinline__ Sums operator-(Sums a, Sums b) { return {a.items - b.items, a.slots - b.slots, a.joined - b.joined}; }
 
 // Of an item: its request, the sums of those before, and how many parts its tiles have.
@@ -173,12 +177,13 @@ __device__ __forceinline__ void total(WorkShared& s, float& work, int& number) {
 // trees of 8 to 24 nodes 55 -> 50 us); as many as at first where that does not help.
 template <int ROWS, int WAVES>
 __device__ __forceinline__ int choose_part(const TreeAttnParams& p, WorkShared& s, int first, int step) {
+    constexpr int ENOUGH = 1 << 20;  // more than any target; sums of 1,024 threads' do not wrap
     float work = 0.f, none = 0.f;
     int tiles = 0;
     for (int r = first; r < p.rows; r += step) {
         const Request q = request<ROWS>(p, r);
         work += float(q.tiles) * float(q.span);
-        tiles += q.tiles;
+        tiles = min(tiles + q.tiles, ENOUGH);
     }
     total<WAVES>(s, work, tiles);
     const int least = __builtin_amdgcn_readfirstlane(part_keys(p, work, tiles, 8));
@@ -188,7 +193,7 @@ __device__ __forceinline__ int choose_part(const TreeAttnParams& p, WorkShared& 
         int items = 0;
         for (int r = first; r < p.rows; r += step) {
             const Request q = request<ROWS>(p, r);
-            items += q.tiles * parts_of(q.span, chunk);
+            items = min(items + q.tiles * parts_of(q.span, chunk), ENOUGH);
         }
         total<WAVES>(s, none, items);
         if (items <= p.target) return chunk;
@@ -197,7 +202,8 @@ __device__ __forceinline__ int choose_part(const TreeAttnParams& p, WorkShared& 
 }
 
 // The request of an item, from all requests' lengths and offsets: the same division in all workgroups.  Up to 64
-// requests every wave does for itself.  False past the last item; `joined`, for the first: tiles of several parts.
+// requests every wave does for itself.  False past the last item; `joined`, for the first: tiles of several parts, none where
+// some items are not run.
 template <int ROWS, int WAVES>
 __device__ __forceinline__ bool find_work(const TreeAttnParams& p, WorkShared& s, int item, Work& work, int& joined) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -245,7 +251,7 @@ __device__ __forceinline__ bool find_work(const TreeAttnParams& p, WorkShared& s
             if (item > 0) break;  // the first item's workgroup goes on to say how many tiles have several parts
         }
     }
-    joined = run.joined;
+    joined = run.items <= p.items ? run.joined : 0;
     return found;
 }
 
@@ -283,13 +289,14 @@ __global__ __launch_bounds__(DIVIDE_THREADS) void tree_division_kernel(TreeAttnP
     if (lane == 63) s.waves[wave] = incl;
     __syncthreads();
     Sums run = incl - own;
+    run.items = min(run.items, MOST_ITEMS);
     for (int w = 0; w < wave; ++w) run = run + s.waves[w];
     for (int r = begin; r < end; ++r) {
         const Request q = request<ROWS>(p, r);
         p.row_work[r] = make_int4(run.items, run.slots, run.joined, parts_of(q.span, chunk));
         run = run + row_sums(q, chunk);
     }
-    if (threadIdx.x == DIVIDE_THREADS - 1) *p.joined = run.joined;
+    if (threadIdx.x == DIVIDE_THREADS - 1) *p.joined = run.items <= p.items ? run.joined : 0;
 }
 
 // ------------------------------------------------------------------------------------ attention
@@ -980,7 +987,7 @@ template <int TYPE, int D, int SHARE>
 void run_shape(const TreeAttnParams& p, hipStream_t s) {
     typedef Shape<D, SHARE> X;
     if (p.listed) hipLaunchKernelGGL((tree_division_kernel<32 * SHARE>), dim3(1), dim3(DIVIDE_THREADS), 0, s, p);
-    const dim3 grid(unsigned(items_of(p)), unsigned(p.kv_heads));
+    const dim3 grid(unsigned(p.items), unsigned(p.kv_heads));
     if (p.page_size % (SHARE == 4 ? 16 : X::PIECES) == 0) hipLaunchKernelGGL((tree_attention_kernel<TYPE, D, SHARE, true>), grid, dim3(X::THREADS), 0, s, p);
     else hipLaunchKernelGGL((tree_attention_kernel<TYPE, D, SHARE, false>), grid, dim3(X::THREADS), 0, s, p);
     if (p.joins)
@@ -1033,6 +1040,7 @@ void tree_attn_bind(TreeAttnParams& p, void* workspace, int head_dim) {
     const int64_t tiles = (int64_t(p.tokens) * p.group / p.rows + 32 * p.share - 1) / (32 * p.share);
     p.run = 1;
     while (p.run < tiles && p.run < 16 && p.run * 16 <= p.target) p.run *= 2;
+    p.items = int(items_of(p));
     p.listed = p.rows > FOUND_ROWS;
     const Layout l = layout(p.rows, p.share, p.target, p.kv_heads, head_dim);
     char* at = static_cast<char*>(workspace);
