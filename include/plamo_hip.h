@@ -507,7 +507,7 @@ int plamo_kernel_attention_paged_tree(const plamo_paged_cache* cache, uint64_t q
 
 /* What plamo_kernel_logit_controls does to a row (device addresses, 0: off).  Row t of the logits belongs to sequence t,
  * or with `offsets` [sequences + 1] to the sequence r with offsets[r] <= t < offsets[r + 1] (rows of none are left as they
- * are).  What the sequence has said is history[r][0 .. history_lengths[r]) and, with ancestors [rows][words] as
+ * are, as are some where offsets descend in between).  What the sequence has said is history[r][0 .. history_lengths[r]) and, with ancestors [rows][words] as
  * paged_tree gives them without a window, the tokens of the nodes on t's path, in their order. */
 typedef struct plamo_logit_controls {
     uint64_t history, history_lengths;                   /* int32 [sequences][history_stride], [sequences] */

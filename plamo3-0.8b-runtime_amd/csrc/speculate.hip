@@ -416,7 +416,8 @@ constexpr int CONTROL_THREADS = 256, CONTROL_SEGMENT = 4096, EACH = 8;
 constexpr uint32_t COUNT_BITS = 18, BANNED = 1u << COUNT_BITS, COUNTED = BANNED - 1;
 static_assert(CONTROL_MAX_HISTORY + 32 * TREE_MAX_WORDS < int(BANNED) && CONTROL_MAX_BIAS < (1 << (31 - COUNT_BITS)), "a word holds them");
 
-// The sequence of row t: the last whose first row is not past t, by looking at 64 of a range at a time; -1 behind the last.
+// The sequence of row t, offsets[r] <= t < offsets[r + 1], by looking at 64 of a range at a time; -1 for none.  (Offsets
+// that descend may lead to any sequence: it is looked at once more.)
 __device__ __forceinline__ int find_sequence(const int32_t* offsets, int sequences, int t) {
     const int lane = threadIdx.x & 63;
     int lo = 0, span = sequences, step;
@@ -427,7 +428,7 @@ __device__ __forceinline__ int find_sequence(const int32_t* offsets, int sequenc
         lo += __popcll(__ballot(before)) * step;
         span = step;
     } while (step > 1);
-    return lo < sequences && offsets[lo] <= t ? lo : -1;
+    return lo < sequences && offsets[lo] <= t && offsets[lo + 1] > t ? lo : -1;
 }
 
 template <int TYPE>
