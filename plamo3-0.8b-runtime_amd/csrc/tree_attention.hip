@@ -834,7 +834,7 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
 #pragma unroll
         for (int g = 0; g < X::GROUPS; ++g) {
             const float2 ml = s_ml[g][part_wave * 32 + col];
-            total += ml.x == NEG_INF ? 0.f : ml.y * __builtin_amdgcn_exp2f(ml.x - top);
+            total += ml.y == 0.f ? 0.f : ml.y * __builtin_amdgcn_exp2f(ml.x - top);  // (NaN alone leaves the maximum at minus infinity)
         }
         const float share = exponent == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(exponent - top);
         auto piece = [&](int e) {

@@ -1,4 +1,7 @@
-"""Attention of several new tokens a request over its pages: offsets of any kind."""
+"""Attention of several new tokens a request over its pages: offsets of any kind, scores that are
+not finite."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -63,3 +66,51 @@ def test_requests_that_overlap(rows, tokens, heads, kv, dim, long_row):
         call(rng.permutation(rows + 1) % (tokens + 1), fill)
         call(rng.integers(-3, tokens + 4, rows + 1), fill)
     assert all(torch.equal(a, b) for a, b in zip(call(ascending, 0), want))
+
+
+# heads on one KV head and new tokens: 1, 2 and 4 waves a tile, one set of waves or several
+SHAPES = [(1, 64, 3), (8, 64, 5), (16, 64, 20), (16, 128, 1), (4, 128, 12), (16, 128, 9), (4, 256, 2), (8, 256, 6), (16, 256, 8)]
+
+
+@pytest.mark.parametrize("before", [0, 24, 32, 56, 96, 160, 3000])
+@pytest.mark.parametrize("heads,dim,count", SHAPES)
+def test_nan_alone(heads, dim, count, before):
+    """The last key holds NaN, the only key of its tile that is seen or not: the token that sees it has NaN in out and lse, the
+    ones before it numbers."""
+    case = Case("bf16", heads, 1, dim, 16, [before], [count], True)
+    clean, e = case.run()
+    at = case.lengths[0] - 1
+    case.keys[int(case.tables[0][at // 16]), at % 16, :, 1] = math.nan
+    out, lse = case.run()
+    assert torch.isnan(out[count - 1]).all() and torch.isnan(lse[count - 1]).all()
+    assert torch.equal(out[:count - 1], clean[:count - 1]) and torch.equal(lse[:count - 1], e[:count - 1])
+
+
+@pytest.mark.parametrize("before", [0, 5, 40, 200, 3000])
+@pytest.mark.parametrize("heads,dim,count", SHAPES)
+def test_a_row_of_nan(heads, dim, count, before):
+    """All scores of one query row are NaN, and no other row's."""
+    case = Case("fp16", heads, 1, dim, 16, [before], [count], False)
+    clean, e = case.run()
+    token, head = count // 2, heads - 1
+    case.q[token, head * dim + 7] = math.nan
+    out, lse = case.run()
+    rows, want = out[:count].view(count, heads, dim), clean[:count].view(count, heads, dim)
+    assert torch.isnan(rows[token, head]).all() and torch.isnan(lse[token, head])
+    others = torch.ones(count, heads, dtype=torch.bool, device="cuda")
+    others[token, head] = False
+    assert torch.equal(rows[others], want[others]) and torch.equal(lse[:count][others], e[:count][others])
+
+
+@pytest.mark.parametrize("before", [0, 40, 200])
+@pytest.mark.parametrize("heads,dim,count", SHAPES)
+def test_scores_of_minus_infinity(heads, dim, count, before):
+    """A row of such scores alone gives zeros and minus infinity, beside one whose scores are numbers."""
+    case = Case("bf16", heads, 1, dim, 16, [before, 30], [count, 2], True)
+    for j in range(case.lengths[0]):
+        case.keys[int(case.tables[0][j // 16]), j % 16] = 0
+        case.keys[int(case.tables[0][j // 16]), j % 16, :, 0] = -math.inf
+    case.q.view(-1, heads, dim)[:, :, 0] = 1
+    out, lse = case.run()
+    assert torch.all(out[:count] == 0) and torch.all(lse[:count] == -math.inf)
+    assert torch.isfinite(out[count:count + 2]).all() and torch.isfinite(lse[count:count + 2]).all()
