@@ -525,7 +525,7 @@ typedef struct plamo_logit_controls {
  * plamo_set_sampling's: the logit is divided by `repetition` if positive, else multiplied (1, 0 or less: off), then less
  * `presence`, then less `frequency` times how often.  Then bias[r][i] is added to token bias_ids[r][i] (ids outside
  * 0 .. n - 1 are skipped; of equal ids the last counts).  Minus infinity then replaces tokens that would repeat an n-gram:
- * those that have followed the sequence's last ngram - 1 tokens before (1 or less: off), and tokens whose bit v % 32 of
+ * those that have followed the sequence's last ngram - 1 tokens before (1 or less, and more than 64: off), and tokens whose bit v % 32 of
  * word v / 32 is 0 in mask mask_rows[t] (outside 0 .. mask_count - 1: no mask; mask_rows 0: mask t).  A control of NaN is off.
  * n <= 2^20, rows <= 2^20, history_width (histories longer than it end there) <= 2^17, bias_width <= 4096, words 1...32. */
 int plamo_kernel_logit_controls(const plamo_logit_controls* controls, uint64_t logits, int32_t type, int64_t stride, int32_t n,

@@ -63,7 +63,7 @@ struct MoveParams {
 void launch_paged_move(const MoveParams& p, hipStream_t s);
 
 // Penalties, biases and masks on logits (plamo_kernel_logit_controls).
-constexpr int CONTROL_MAX_HISTORY = 1 << 17, CONTROL_MAX_BIAS = 4096;
+constexpr int CONTROL_MAX_HISTORY = 1 << 17, CONTROL_MAX_BIAS = 4096, CONTROL_MAX_NGRAM = 64;
 struct ControlParams {
     const int32_t *history, *history_lengths;
     int64_t history_stride;

@@ -536,7 +536,9 @@ __global__ __launch_bounds__(CONTROL_THREADS) void controls_kernel(ControlParams
     if (c.frequency != c.frequency) c.frequency = 0.0f;
     const int length = p.history ? min(max(p.history_lengths[r], 0), p.history_width) : 0, all = length + path;
     const int32_t* history = p.history + int64_t(r) * p.history_stride;
-    const int ngram = p.ngram ? p.ngram[r] : 0, span = ngram > 1 && all >= ngram ? ngram - 1 : 0;
+    // (an n-gram is compared token by token wherever the token before it fits: the longest bounds what a history of one
+    // token costs, 4.2 ms for 2^17 of it, 3-grams 0.26)
+    const int ngram = p.ngram ? p.ngram[r] : 0, span = ngram > 1 && ngram <= min(all, CONTROL_MAX_NGRAM) ? ngram - 1 : 0;
     const bool looks = span || c.repetition != 1.0f || c.presence != 0.0f || c.frequency != 0.0f;
     // the first tokens and biases are on their way before the counts are cleared, and the tokens before these: few follow
     // the sequence's last one, and all but those need no look at the rest of an n-gram
