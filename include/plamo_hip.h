@@ -496,7 +496,7 @@ int plamo_kernel_paged_tree(uint64_t lengths, uint64_t offsets, int32_t rows, ui
  * left out by it: paged_tree's window does that).  Cache, heads, q, out, lse, what is not seen, what nothing or minus
  * infinity alone is seen of, entries that are no pages, and the workspace are as for plamo_kernel_attention_paged; rows of q and
  * out are tokens, those behind offsets[rows] are left as they are, and a request whose length is below its number of nodes
- * sees nothing.  At most 2^20 rows and tokens, 2^30 of tokens times heads. */
+ * sees nothing.  A workspace is large enough for fewer rows and tokens too.  At most 2^20 rows and tokens, 2^30 of tokens times heads. */
 int64_t plamo_kernel_attention_paged_tree_workspace(int32_t rows, int32_t tokens, int32_t heads, int32_t kv_heads,
                                                     int32_t head_dim);
 int plamo_kernel_attention_paged_tree(const plamo_paged_cache* cache, uint64_t q, int64_t q_stride, int32_t heads,

@@ -1024,8 +1024,12 @@ Layout layout(int rows, int share, int target, int kv_heads, int head_dim) {
 }  // namespace
 
 int64_t tree_attn_workspace(int rows, int tokens, int heads, int kv_heads, int head_dim) {
-    const int share = share_of(rows, tokens, heads / kv_heads);
-    return layout(rows, share, target_of(share, kv_heads, head_dim), kv_heads, head_dim).bytes;
+    // enough for fewer rows and tokens too: the fewer the rows, the more waves a tile, and each number of waves that a call of
+    // them can have counts
+    int64_t bytes = 0;
+    for (int share = 1; share <= share_of(1, tokens, heads / kv_heads); share *= 2)
+        bytes = std::max(bytes, layout(rows, share, target_of(share, kv_heads, head_dim), kv_heads, head_dim).bytes);
+    return bytes;
 }
 
 void tree_attn_bind(TreeAttnParams& p, void* workspace, int head_dim) {
