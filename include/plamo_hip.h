@@ -492,8 +492,8 @@ int plamo_kernel_paged_tree(uint64_t lengths, uint64_t offsets, int32_t rows, ui
  * of keys 0 .. lengths[r] - 1 of tables[r][width]: without ancestors (0) those up to its own, its position being
  * lengths[r] - nodes + its index; with ancestors [tokens][words] the keys before the request's nodes, and the nodes whose
  * bits are set (words 1...32; nodes without a bit are not seen), its position being positions[t] (read only then; a
- * negative one sees nothing).  window > 0: keys at most window - 1 positions before the token's (nodes seen by bits are not
- * left out by it: paged_tree's window does that).  Cache, heads, q, out, lse, what is not seen, what nothing or minus
+ * negative one sees nothing).  window > 0: keys at most window - 1 positions before the token's, one before the request's nodes
+ * counting as lengths[r] - nodes (nodes seen by bits are not left out by it: paged_tree's window does that).  Cache, heads, q, out, lse, what is not seen, what nothing or minus
  * infinity alone is seen of, entries that are no pages, and the workspace are as for plamo_kernel_attention_paged; rows of q and
  * out are tokens, those behind offsets[rows] are left as they are, and a request whose length is below its number of nodes
  * sees nothing.  A workspace is large enough for fewer rows and tokens too.  At most 2^20 rows and tokens, 2^30 of tokens times heads. */

@@ -1,5 +1,5 @@
-"""Attention of several new tokens a request over its pages: offsets of any kind, scores that are
-not finite."""
+"""Attention of several new tokens a request over its pages: offsets and positions of any kind,
+scores that are not finite."""
 import math
 
 import numpy as np
@@ -114,3 +114,17 @@ def test_scores_of_minus_infinity(heads, dim, count, before):
     out, lse = case.run()
     assert torch.all(out[:count] == 0) and torch.all(lse[:count] == -math.inf)
     assert torch.isfinite(out[count:count + 2]).all() and torch.isfinite(lse[count:count + 2]).all()
+
+
+@pytest.mark.parametrize("window", [1, 20, 64, 2 ** 31 - 1])
+@pytest.mark.parametrize("heads,dim,count", SHAPES[::2])
+def test_positions_before_the_nodes(heads, dim, count, window):
+    """They count as the first node's, which sees the window's last keys before it; any position behind is its own."""
+    case = Case("bf16", heads, 1, dim, 16, [100, 70], [count, count], False, window=window)
+    first = [100] * count + [70] * count
+    case.positions[:2 * count] = first
+    want = case.run()
+    case.positions[:2 * count] = [(0, 1, p - 1, p // 2)[i % 4] for i, p in enumerate(first)]
+    assert all(torch.equal(a, b) for a, b in zip(case.run(), want))
+    case.positions[:2 * count] = [(p + 5, 2 ** 31 - 1)[i % 2] for i, p in enumerate(first)]
+    case.check()
