@@ -174,7 +174,7 @@ __device__ __forceinline__ void total(WorkShared& s, float& work, int& number) {
 
 // A part's keys, from the requests that a thread takes: from row `first` on, every `step`-th.  More of them where
 // all parts at once would be a few too many for the CUs, and a second round had to be waited for (64 requests of 33 to 8,192 keys,
-// trees of 8 to 24 nodes 55 -> 50 us); as many as at first where that does not help.
+// trees of 8 to 24 nodes 47 -> 42.5 us); as many as at first where that does not help.
 template <int ROWS, int WAVES>
 __device__ __forceinline__ int choose_part(const TreeAttnParams& p, WorkShared& s, int first, int step) {
     constexpr int ENOUGH = 1 << 20;  // more than any target; sums of 1,024 threads' do not wrap
@@ -311,15 +311,6 @@ __device__ __forceinline__ void load_to_lds(uint32_t lds, uint64_t at) {
     __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                      :
                      : "s"(__builtin_amdgcn_readfirstlane(int(lds))), "v"(at)
-                     : "m0", "memory");
-}
-// The same, each lane at its own offset from a wave's address.  (s_nop: the wait states between a vector instruction's write of
-// a scalar register, as where one comes back from a lane, and its use as an address.)
-__device__ __forceinline__ void load_to_lds(uint32_t lds, uint64_t at, uint32_t off) {
-    const uint64_t base = uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(at >> 32)))) << 32 | uint32_t(__builtin_amdgcn_readfirstlane(int(at)));
-    __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
-                     :
-                     : "s"(__builtin_amdgcn_readfirstlane(int(lds))), "v"(off), "s"(base)
                      : "m0", "memory");
 }
 #pragma clang diagnostic pop
@@ -468,15 +459,11 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
     const int64_t apart = p.values - p.keys;
     const int32_t* table = p.tables + int64_t(row) * p.width;
     const int first_row = 16 * X::OWN * part_wave;  // of a tile, that the wave loads
-    // EVEN: the lane's keys of sixteen, PIECES of them, lie in one page, or with WAVEWISE all sixteen do, and their address is the
-    // wave's to find: a load is one vector instruction then, on a lane's part (its row, and its chunk, whose exclusive-or with
-    // the load's number is a constant; 16 slots of at most 2^25 bytes fit its 32 bits).  With four waves a tile arithmetic is
-    // what takes the time (16 requests of 2,000 to 9,000 keys, 78 rows of 256 each: 76 -> 64 us); with fewer memory does, and
-    // the loads would go out later (48 such requests, 8 heads of 64: 103 -> 123 us).
-    constexpr bool WAVEWISE = EVEN && SHARE == 4;
+    // EVEN: the lane's keys of sixteen, PIECES of them, lie in one page.  (Where sixteen do, the wave could look the page up and find
+    // its address: chunks of 999 and 333 tokens 496 -> 492 us, but the loads go out later: 16 requests of 78 rows of 256 59 -> 68, 48
+    // of 38 rows of 64 with four waves 144 -> 166.)
     constexpr int LOOK = EVEN ? 1 : X::PIECES;
     const int lane_chunk = lane % LANES;
-    const uint32_t lane_row = uint32_t(X::PIECES * group) * uint32_t(p.slot_stride);
     const uint32_t lane_key = uint32_t(lane_chunk ^ key_swizzle<D>(group)) * 16;
     const uint32_t lane_value = uint32_t(((lane_chunk >> 2) ^ value_swizzle<D>(group)) * 4 + (lane_chunk & 3)) * 16;
     // pages of a tile's keys, on their way
@@ -486,7 +473,7 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
         for (int b = 0; b < X::OWN; ++b)
 #pragma unroll
             for (int l = 0; l < LOOK; ++l) {
-                const int key = pos + first_row + 16 * b + (WAVEWISE ? 0 : X::PIECES * group + l);
+                const int key = pos + first_row + 16 * b + X::PIECES * group + l;
                 entry[b][l] = key < end ? table[divide(uint32_t(key), p.div)] : -1;
             }
     };
@@ -496,42 +483,23 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
             const int key0 = pos + first_row + 16 * b;  // of the sixteen
             const uint32_t to = ring + uint32_t(stage) * (2 * X::TILE) + uint32_t(first_row + 16 * b) * X::ROW;
             uint32_t there = 0xffffu;
-            bool all;
-            if constexpr (WAVEWISE) {
-                const int page = __builtin_amdgcn_readfirstlane(entry[b][0]);
-                all = key0 + 16 <= end && uint32_t(page) < uint32_t(p.pages);
-                if (all) {
-                    const int in_page = key0 - int(divide(uint32_t(key0), p.div)) * p.page_size;
-                    const uint64_t at = keys0 + uint64_t(page * p.page_stride + in_page * p.slot_stride);
-                    static_for<0, X::PIECES>([&](auto n) {
-                        constexpr int l = decltype(n)::value;
-                        const uint64_t row_at = at + uint64_t(l * p.slot_stride);
-                        load_to_lds(to + uint32_t(l) * 1024, row_at, (lane_key ^ uint32_t(key_swizzle<D>(X::PIECE_KEYS * l) * 16)) + lane_row);
-                        load_to_lds(to + X::TILE + uint32_t(l) * 1024, row_at + uint64_t(apart),
-                                    (lane_value ^ uint32_t(value_swizzle<D>(X::PIECE_KEYS * l) * 64)) + lane_row);
-                    });
-                }
-            } else {
-                bool fine = key0 + 16 <= end;
-                uint64_t at[LOOK];
+            bool fine = key0 + 16 <= end;
+            uint64_t at[LOOK];
 #pragma unroll
-                for (int l = 0; l < LOOK; ++l) {
-                    const int key = key0 + X::PIECES * group + l, in_page = key - int(divide(uint32_t(key), p.div)) * p.page_size;
-                    at[l] = keys0 + uint64_t(int64_t(entry[b][l]) * p.page_stride + int64_t(in_page) * p.slot_stride);
-                    fine = fine && uint32_t(entry[b][l]) < uint32_t(p.pages);
-                }
-                all = __all(fine);
-                if (all) {
-                    static_for<0, X::PIECES>([&](auto n) {
-                        constexpr int l = decltype(n)::value;
-                        const uint64_t from = at[EVEN ? 0 : l] + (EVEN ? uint64_t(l * p.slot_stride) : 0);
-                        load_to_lds(to + uint32_t(l) * 1024, from + (lane_key ^ uint32_t(key_swizzle<D>(X::PIECE_KEYS * l) * 16)));
-                        load_to_lds(to + X::TILE + uint32_t(l) * 1024,
-                                    from + uint64_t(apart) + (lane_value ^ uint32_t(value_swizzle<D>(X::PIECE_KEYS * l) * 64)));
-                    });
-                }
+            for (int l = 0; l < LOOK; ++l) {
+                const int key = key0 + X::PIECES * group + l, in_page = key - int(divide(uint32_t(key), p.div)) * p.page_size;
+                at[l] = keys0 + uint64_t(int64_t(entry[b][l]) * p.page_stride + int64_t(in_page) * p.slot_stride);
+                fine = fine && uint32_t(entry[b][l]) < uint32_t(p.pages);
             }
-            if (!all) {  // rows past the last key, or of no page, are zeros
+            if (__all(fine)) {
+                static_for<0, X::PIECES>([&](auto n) {
+                    constexpr int l = decltype(n)::value;
+                    const uint64_t from = at[EVEN ? 0 : l] + (EVEN ? uint64_t(l * p.slot_stride) : 0);
+                    load_to_lds(to + uint32_t(l) * 1024, from + (lane_key ^ uint32_t(key_swizzle<D>(X::PIECE_KEYS * l) * 16)));
+                    load_to_lds(to + X::TILE + uint32_t(l) * 1024,
+                                from + uint64_t(apart) + (lane_value ^ uint32_t(value_swizzle<D>(X::PIECE_KEYS * l) * 64)));
+                });
+            } else {  // rows past the last key, or of no page, are zeros
                 there = 0;
                 int own = lane;
                 __asm__ volatile("" : "+v"(own));  // (or the compiler would keep all offsets in registers)
@@ -777,8 +745,8 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
 
     // ---- the part's tiles, the next one's loads on their way
     const int turns = begin < end ? (end - begin + TURN - 1) / TURN : 0;
-    // a wave that has no rows only loads (64 trees of up to 24 nodes behind 33 to 8,192 keys 39.6 -> 38.9 us,
-    // 64 requests of 73 rows behind 2,000 to 4,000 39.0 -> 36.0)
+    // a wave that has no rows only loads (64 trees of up to 24 nodes behind 33 to 8,192 keys 43.2 -> 42.5 us,
+    // 64 requests of 73 rows behind 2,000 to 4,000 40 -> 38.5)
     const bool live = tile * ROWS + part_wave * 32 < rows;
     const int taken = live ? end : 0;
     auto run = [&](auto with_care) __attribute__((always_inline)) {
@@ -807,8 +775,8 @@ __global__ __launch_bounds__((Shape<D, SHARE>::THREADS), (Shape<D, SHARE>::OF_SI
         }
     };
     run(std::false_type{});
-    // once more where values need care: in the same loop their arithmetic cost every tile 64 moves of registers (chunks of
-    // 999 and 333 tokens 412 us, so 371)
+    // once more where values need care: in the same loop their arithmetic cost every tile 64 moves of registers (with weights
+    // rounded once, chunks of 999 and 333 tokens 412 us, so 371)
     if (__syncthreads_or(odd)) {
         most = NEG_INF;
         sum = 0.f;
@@ -961,9 +929,10 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void tree_join_kernel(TreeAttnPara
 // ------------------------------------------------------------------------------------ launches
 // Waves that share a tile, by the rows of queries that a request has on the average: few rows read the keys at the rate of
 // memory, and more rows a tile read them fewer times; many are bound by arithmetic.  64 requests of 2,000 to 4,000 keys and 16
-// heads of 128 on one, 15 / 22 / 29 / 36 / 58 / 73 rows each: 27 / 27 / 31 / 32 / 45 / 51 us with one wave, 27 / 27 / 29 / 30 / 34 / 35
-// with two, 28 / 28 / 30 / 31 / 34 / 36 with four.  16 of 2,000 to 9,000 keys, 8 heads of 256 on 2, 18 / 39 / 78 rows: 47 / 62 / 98,
-// 49 / 52 / 67 and 57 / 60 / 64.  (Heads of 64 cross over later between two and four: 38 rows 164 / 105 / 146.)
+// heads of 128 on one, 14 / 22 / 29 / 36 / 58 / 73 / 116 / 153 rows each: 27 / 27 / 30 / 31 / 44 / 49 / 61 / 104 us with one wave,
+// 27 / 27 / 29 / 29 / 34 / 36 / 45 / 52 with two, 28 / 28 / 32 / 33 / 36 / 37 / 46 / 50 with four.  16 of 2,000 to 9,000 keys, 8 heads of
+// 256 on 2, 18 / 39 / 78 rows: 46 / 60 / 94, 48 / 51 / 65 and 53 / 56 / 59.  (Heads of 64 cross over later between two and
+// four: 48 requests, 32 heads on 8, 38 / 117 rows 105 / 252 with two and 144 / 300 with four, 4 requests of 2,000 rows 264 and 170.)
 int share_of(int rows, int tokens, int group) {
     const int64_t each = int64_t(tokens) * group / rows;
     return each <= 24 ? 1 : each <= 72 ? 2 : 4;
@@ -988,7 +957,7 @@ void run_shape(const TreeAttnParams& p, hipStream_t s) {
     typedef Shape<D, SHARE> X;
     if (p.listed) hipLaunchKernelGGL((tree_division_kernel<32 * SHARE>), dim3(1), dim3(DIVIDE_THREADS), 0, s, p);
     const dim3 grid(unsigned(p.items), unsigned(p.kv_heads));
-    if (p.page_size % (SHARE == 4 ? 16 : X::PIECES) == 0) hipLaunchKernelGGL((tree_attention_kernel<TYPE, D, SHARE, true>), grid, dim3(X::THREADS), 0, s, p);
+    if (p.page_size % X::PIECES == 0) hipLaunchKernelGGL((tree_attention_kernel<TYPE, D, SHARE, true>), grid, dim3(X::THREADS), 0, s, p);
     else hipLaunchKernelGGL((tree_attention_kernel<TYPE, D, SHARE, false>), grid, dim3(X::THREADS), 0, s, p);
     if (p.joins)
         hipLaunchKernelGGL((tree_join_kernel<TYPE, D, SHARE>), dim3(unsigned(std::min<int64_t>(tiles_of(p), p.target)), unsigned(p.kv_heads), 4 * SHARE),
@@ -1039,8 +1008,8 @@ void tree_attn_bind(TreeAttnParams& p, void* workspace, int head_dim) {
     p.least = turn_of(p.share, head_dim);
     p.joins = p.most > p.least;
     // Neighbouring workgroups are tiles of the same keys: an XCD takes as many as a request has, as a power of two, so that the
-    // workgroups that the XCDs hold at once stay as many on each (64 requests of two tiles or so 41.9 -> 40.1 us, of three 77.1 -> 75.6;
-    // by runs of three 64 requests of one tile took 39 us for 27).
+    // workgroups that the XCDs hold at once stay as many on each (chunks of 999 and 333 tokens 507 -> 496 us; 64 requests of two tiles
+    // or so 42.5 either way, but 77 MB fetched for 123; by runs of three 64 requests of one tile took 39 us for 27).
     const int64_t tiles = (int64_t(p.tokens) * p.group / p.rows + 32 * p.share - 1) / (32 * p.share);
     p.run = 1;
     while (p.run < tiles && p.run < 16 && p.run * 16 <= p.target) p.run *= 2;
