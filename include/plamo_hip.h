@@ -507,9 +507,9 @@ int plamo_kernel_attention_paged_tree(const plamo_paged_cache* cache, uint64_t q
 
 /* What plamo_kernel_logit_controls does to a row (device addresses, 0: off).  Row t of the logits belongs to sequence t,
  * or with `offsets` [sequences + 1] to the sequence r with offsets[r] <= t < offsets[r + 1] (rows of none are left as they
- * are, as are some where offsets descend in between).  What the sequence has said is history[r][0 .. history_lengths[r]) and, with ancestors [rows][words] as
- * paged_tree gives them without a window, the tokens of the nodes on t's path, in their order: a history ends before the
- * request's first node, as the token drawn last is that node of the next step. */
+ * are, as are some where offsets descend in between).  What the sequence has said is history[r][0 .. history_lengths[r])
+ * and, with ancestors [rows][words] as paged_tree gives them without a window, the tokens of the nodes on t's path, in
+ * their order: a history ends before the request's first node, as the token drawn last is that node of the next step. */
 typedef struct plamo_logit_controls {
     uint64_t history, history_lengths;                   /* int32 [sequences][history_stride], [sequences] */
     uint64_t offsets, tokens, ancestors;                 /* int32 [sequences + 1], [rows], [rows][words] */

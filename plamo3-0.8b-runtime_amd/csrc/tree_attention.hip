@@ -29,12 +29,13 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 // Pages go straight into LDS, each lane from its own address: any page size and any strides.  Where a lane's keys
 // of a load are known to lie in one page (EVEN) it looks that page up once.
 // What bounds it, with what it took: arithmetic for chunks of prompts (of 999 and 333 tokens, 16 heads of 128, behind 28,000 and
-// 30,720 keys: 317 GFLOP in 367 us, 860 TFLOP/s; softmax and products of a wave take turns, two workgroups a CU fill in);
-// memory for a few nodes with a window (48 requests of up to 13 nodes, 32 heads of 64 on 8, 2,048 keys: 171 MB in 55 us); one
-// request's 343 keys the latency of its loads (9 us, then 3 to join); and many trees each a part (64 of up to 24 nodes behind 33
-// to 8,192 keys, 16 heads of 128 on one: 40 us for 53 MB) all of these: some 6 to find a part and load its first tile, five
-// more tiles of 3.5, and the parts' results, written and read once more, with a launch of 8.  (One workgroup of eight waves a CU,
-// of two sets, halves those results and took 46 for 42, and the chunks 537.)
+// 30,720 keys: 317 GFLOP in 494 us, 640 TFLOP/s, and half as many again for the weights' second halves; softmax and products of a
+// wave take turns, two workgroups a CU fill in);
+// memory for a few nodes with a window (48 requests of up to 13 nodes, 32 heads of 64 on 8, 2,048 keys: 171 MB in 54 us); one
+// request's 343 keys the latency of its loads (9.5 us, then 3 to join); and many trees each a part (64 of up to 24 nodes behind 33
+// to 8,192 keys, 16 heads of 128 on one: 42.5 us for 53 MB) all of these: some 6 to find a part and load its first tile, five
+// more tiles of some 4.5, and the parts' results, written and read once more, with a launch of 8.  (With weights rounded once, one
+// workgroup of eight waves a CU, of two sets, halved those results and took 46 for 42, and the chunks 537 for 371.)
 constexpr int CUS = 256;
 
 template <int D, int SHARE>
