@@ -488,15 +488,16 @@ int plamo_kernel_paged_tree(uint64_t lengths, uint64_t offsets, int32_t rows, ui
                             int32_t window, uint64_t positions, uint64_t ancestors, int32_t words, uint64_t stream, char* err,
                             size_t errlen);
 
-/* Attention of all new tokens of `rows` requests: out[t] = softmax(scale * q[t] . k) v over what token t of request r sees
- * of keys 0 .. lengths[r] - 1 of tables[r][width]: without ancestors (0) those up to its own, its position being
- * lengths[r] - nodes + its index; with ancestors [tokens][words] the keys before the request's nodes, and the nodes whose
- * bits are set (words 1...32; nodes without a bit are not seen), its position being positions[t] (read only then; a
- * negative one sees nothing).  window > 0: keys at most window - 1 positions before the token's, one before the request's nodes
- * counting as lengths[r] - nodes (nodes seen by bits are not left out by it: paged_tree's window does that).  Cache, heads, q, out, lse, what is not seen, what nothing or minus
- * infinity alone is seen of, entries that are no pages, and the workspace are as for plamo_kernel_attention_paged; rows of q and
- * out are tokens, those behind offsets[rows] are left as they are, and a request whose length is below its number of nodes
- * sees nothing.  A workspace is large enough for fewer rows and tokens too.  At most 2^20 rows and tokens, 2^30 of tokens times heads. */
+/* Attention of all new tokens of `rows` requests: out[t] = softmax(scale * q[t] . k) v over what token t of request r
+ * sees of keys 0 .. lengths[r] - 1 of tables[r][width]: without ancestors (0) those up to its own, its position being
+ * lengths[r] - nodes + its index; with ancestors [tokens][words] the keys before the request's nodes, and the nodes
+ * whose bits are set (words 1...32; nodes without a bit are not seen), its position being positions[t] (read only then;
+ * a negative one sees nothing).  window > 0: keys at most window - 1 positions before the token's, one before the
+ * request's nodes counting as lengths[r] - nodes (nodes seen by bits are not left out by it: paged_tree's window does
+ * that).  Cache, heads, q, out, lse, what is not seen, what nothing or minus infinity alone is seen of, entries that are
+ * no pages, and the workspace are as for plamo_kernel_attention_paged; rows of q and out are tokens, those behind
+ * offsets[rows] are left as they are, and a request whose length is below its number of nodes sees nothing.  A workspace
+ * is large enough for fewer rows and tokens too.  At most 2^20 rows and tokens, 2^30 of tokens times heads. */
 int64_t plamo_kernel_attention_paged_tree_workspace(int32_t rows, int32_t tokens, int32_t heads, int32_t kv_heads,
                                                     int32_t head_dim);
 int plamo_kernel_attention_paged_tree(const plamo_paged_cache* cache, uint64_t q, int64_t q_stride, int32_t heads,
@@ -524,11 +525,12 @@ typedef struct plamo_logit_controls {
 /* Controls on `rows` rows of n logits (`type`, `stride` elements apart, any alignment) into out (`type` or PLAMO_F32;
  * logits itself, of the same type and stride, or apart from it).  Of tokens that the sequence has said, in FP32 and as
  * plamo_set_sampling's: the logit is divided by `repetition` if positive, else multiplied (1, 0 or less: off), then less
- * `presence`, then less `frequency` times how often.  Then bias[r][i] is added to token bias_ids[r][i] (ids outside
- * 0 .. n - 1 are skipped; of equal ids the last counts).  Minus infinity then replaces tokens that would repeat an n-gram:
- * those that have followed the sequence's last ngram - 1 tokens before (1 or less, and more than 64: off), and tokens whose bit v % 32 of
- * word v / 32 is 0 in mask mask_rows[t] (outside 0 .. mask_count - 1: no mask; mask_rows 0: mask t).  A control of NaN is off.
- * n <= 2^20, rows <= 2^20, history_width (histories longer than it end there) <= 2^17, bias_width <= 4096, words 1...32. */
+ * `presence`, then less `frequency` times how often.  Then bias[r][i] is added to token bias_ids[r][i] (ids outside 0 ..
+ * n - 1 are skipped; of equal ids the last counts).  Minus infinity then replaces tokens that would repeat an n-gram:
+ * those that have followed the sequence's last ngram - 1 tokens before (1 or less, and more than 64: off), and tokens
+ * whose bit v % 32 of word v / 32 is 0 in mask mask_rows[t] (outside 0 .. mask_count - 1: no mask; mask_rows 0: mask t).
+ * A control of NaN is off.  n <= 2^20, rows <= 2^20, history_width (histories longer than it end there) <= 2^17,
+ * bias_width <= 4096, words 1...32. */
 int plamo_kernel_logit_controls(const plamo_logit_controls* controls, uint64_t logits, int32_t type, int64_t stride, int32_t n,
                                 int32_t rows, uint64_t out, int32_t out_type, int64_t out_stride, uint64_t stream, char* err,
                                 size_t errlen);
