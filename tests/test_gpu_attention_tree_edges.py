@@ -128,3 +128,43 @@ def test_positions_before_the_nodes(heads, dim, count, window):
     assert all(torch.equal(a, b) for a, b in zip(case.run(), want))
     case.positions[:2 * count] = [(p + 5, 2 ** 31 - 1)[i % 2] for i, p in enumerate(first)]
     case.check()
+
+
+@pytest.mark.parametrize("kv,heads,dim", [(256, 256, 64), (100, 200, 128), (256, 512, 64)])
+def test_many_kv_heads(kv, heads, dim):
+    """Fewer parts aimed at than there are tiles, down to one."""
+    Case("bf16", heads, kv, dim, 16, [400, 3], [2, 1], False).check()
+    Case("fp16", heads, kv, dim, 16, [300], [3], True, window=200).check()
+
+
+def test_most_requests():
+    """2^20 requests of one token, which sees its own key alone: its value, bit for bit."""
+    rows, dim = 1 << 20, 64
+    keys, values, q = (torch.randn(rows, dim, device="cuda").to(torch.bfloat16) for _ in range(3))
+    tables = torch.randperm(rows, device="cuda").int().view(rows, 1)
+    lengths, offsets = torch.ones(rows, dtype=torch.int32, device="cuda"), torch.arange(rows + 1, dtype=torch.int32, device="cuda")
+    out, lse = torch.zeros_like(q), torch.zeros(rows, 1, device="cuda")
+    attend_tree(describe(keys.view(rows, 1, 1, dim), values.view(rows, 1, 1, dim), "bf16"), q, 1, tables, lengths, offsets, out, lse)
+    torch.cuda.synchronize()
+    page = tables[:, 0].long()
+    assert torch.equal(out, values[page])
+    score = (q.double() * keys[page].double()).sum(1) / 8
+    size = (q.double() * keys[page].double()).abs().sum(1) / 8
+    # (as in attend_tree64: sums of `dim` products, then the logarithm)
+    assert torch.all((lse[:, 0].double() - score).abs() <= size * (dim + 4) * 2.0 ** -23 + 2.0 ** -20 + score.abs() * 2.0 ** -21)
+
+
+@pytest.mark.parametrize("heads,dim", [(1, 64), (2, 128), (1, 256)])
+@pytest.mark.parametrize("before", [0, 1000])
+def test_long_chains_of_a_window_of_one(heads, dim, before):
+    """Tiles that see few of their request's keys, parts that hold none."""
+    count, page = 30000, 64
+    pages = -(-(before + count) // page)
+    keys, values = (torch.randn(pages, page, 1, dim, device="cuda").to(torch.bfloat16) for _ in range(2))
+    tables = torch.randperm(pages, device="cuda").int().view(1, pages)
+    q = torch.randn(count, heads * dim, device="cuda").to(torch.bfloat16)
+    out = torch.zeros_like(q)
+    attend_tree(describe(keys, values, "bf16"), q, heads, tables, put([before + count]), put([0, count]), out, window=1)
+    torch.cuda.synchronize()
+    own = values[tables[0].long(), :, 0].reshape(-1, dim)[before:before + count]
+    assert torch.equal(out.view(count, heads, dim), own[:, None].expand(count, heads, dim))
